@@ -379,6 +379,154 @@ typedef struct ultima_hsamp_head {
  * Allocates nothing. */
 int ultima_hsamp_lm_head(const ultima_hsamp_head* head, void* hip_stream);
 
+/* ---- Verification against the drafter's distribution --------------------------
+ * ultima_hsamp_verify_block keeps the tokens of the one-token loop: a draft
+ * survives where the loop's own sample happens to be that token. When the
+ * drafts are samples of a known distribution q, the rejection rule keeps more of
+ * them and still emits samples of the target's p. Per sequence, with drafts
+ * d[0 .. n), target distributions p[0 .. n] and the drafter's q[0 .. n):
+ *   draft i is accepted when u_accept[i] * q_i(d_i) < p_i(d_i);
+ *   m is the first rejected draft, n when there is none;
+ *   tokens[0 .. m) = d[0 .. m), and tokens[m] is drawn with u_draw from
+ *   max(p_m - q_m, 0) when m < n (from p_m when that is 0 everywhere), from p_n
+ *   when m == n: the lowest id t whose weight w(t) is above 0 and whose running
+ *   sum (id order) is >= u_draw times the sum of all weights; the highest id of
+ *   weight above 0 where rounding leaves none;
+ *   the rest of the sequence's max_draft + 1 tokens are -1, count = m + 1.
+ * A drafter that is certain of its tokens (lookup in the prompt; a greedy
+ * drafter) has q_i(d_i) = 1. Everything is evaluated in double precision.
+ * A sequence whose target row m allows nothing has no token there: tokens[m] is
+ * -1 and count m. A drafted id outside [0, vocab) has probability 0 on both
+ * sides and is rejected. n_draft outside [0, max_draft] or rows outside the
+ * arrays: count 0, every token -1.
+ * accept_prob[i] = min(1, p_i(d_i) / q_i(d_i)) (q_i(d_i) = 0: 1 if p_i(d_i) > 0,
+ * else 0) up to the first rejected draft, -1 for the drafts after it; rows of no
+ * sequence are left as they were.
+ * Row layout: target rows of sequence b start at target_start[b], its drafted
+ * rows at draft_start[b] (device int32 [seqs]), so that sequences with fewer
+ * drafts take fewer rows; NULL: b * (max_draft + 1) and b * max_draft.
+ *
+ * On logits: p = softmax(x / T) over the allowed ids, x the logits as they are
+ * (no penalties, no top-k: for those, the kept sets below). T <= 0 or NaN: all
+ * on the largest logit, the lowest id among equals. -inf and NaN logits are not
+ * allowed, +inf counts as the largest finite float. Logits of ids that a mask
+ * leaves out are not looked at. */
+#define ULTIMA_HSAMP_MAX_DRAFT 1023   /* drafted tokens per sequence */
+typedef struct ultima_hsamp_draft {
+    int32_t seqs;               /* sequences >= 1 */
+    int32_t max_draft;          /* 0 .. ULTIMA_HSAMP_MAX_DRAFT */
+    int32_t vocab;              /* V, 1 .. ULTIMA_HSAMP_MAX_VOCAB */
+    int32_t dtype;              /* ULTIMA_HSAMP_F32 or ULTIMA_HSAMP_BF16, of both logits */
+    const void* logits;         /* [logits_rows, logits_stride] the target's */
+    int64_t logits_stride;      /* elements between rows, >= vocab */
+    int32_t logits_rows;        /* rows the array holds */
+    int32_t draft_rows;         /* drafted rows the arrays below hold; 0: they may be NULL */
+    const void* draft_logits;   /* [draft_rows, draft_stride] the drafter's, or NULL: certain drafts */
+    int64_t draft_stride;       /* >= vocab */
+    const int32_t* draft;       /* [draft_rows] drafted ids */
+    const int32_t* n_draft;     /* [seqs] drafts per sequence or NULL: max_draft each */
+    const int32_t* target_start; /* [seqs] or NULL */
+    const int32_t* draft_start; /* [seqs] or NULL */
+    const float* temperature;   /* [seqs] of the target or NULL: 1 */
+    const float* draft_temperature; /* [seqs] of the drafter or NULL: 1 */
+    const uint32_t* mask;       /* [logits_rows, mask_stride] allowed-token words of the target or NULL */
+    int64_t mask_stride;        /* >= ceil(vocab / 32) */
+    const uint32_t* draft_mask; /* [draft_rows, draft_mask_stride] of the drafter or NULL */
+    int64_t draft_mask_stride;
+    const double* u_accept;     /* [draft_rows] uniforms in [0, 1) */
+    const double* u_draw;       /* [seqs] uniforms in [0, 1) */
+    void* work;                 /* ultima_hsamp_verify_draft_work_bytes() bytes, 16-byte aligned, of this call
+                                   alone until it completes; needs no initial contents */
+    int32_t* out_tokens;        /* [seqs, max_draft + 1] out */
+    int32_t* out_count;         /* [seqs] out: tokens emitted */
+    float* accept_prob;         /* [draft_rows] out or NULL */
+} ultima_hsamp_draft;
+
+/* Bytes of workspace ultima_hsamp_verify_draft needs (-1 for invalid sizes). */
+int64_t ultima_hsamp_verify_draft_work_bytes(int32_t seqs, int32_t max_draft, int32_t vocab);
+
+/* All pointers are device memory of the current device, hip_stream one of its
+ * streams; asynchronous, allocates nothing (graph-capturable). */
+int ultima_hsamp_verify_draft(const ultima_hsamp_draft* d, void* hip_stream);
+
+/* On kept sets: p and q are the sets ultima_hsamp_run() leaves (kept_idx,
+ * kept_prob, kept_count: after penalties, top-k, top-p and min-p, by ascending
+ * id), so the emitted tokens are samples of what the sampler itself draws from.
+ * Probabilities that are NaN or below 0 count as 0. A count below 0 or above its
+ * capacity (a set that was cut off) makes its sequence invalid: count 0, every
+ * token -1; an empty target set emits no token. */
+typedef struct ultima_hsamp_draft_sets {
+    int32_t seqs;               /* sequences >= 1 */
+    int32_t max_draft;          /* 0 .. ULTIMA_HSAMP_MAX_DRAFT */
+    int32_t rows;               /* target rows the arrays hold */
+    int32_t draft_rows;         /* drafted rows the arrays hold; 0: they may be NULL */
+    const int32_t* kept_idx;    /* [rows, set_cap] */
+    const float* kept_prob;     /* [rows, set_cap] */
+    const int32_t* kept_count;  /* [rows] */
+    int32_t set_cap;            /* 1 .. ULTIMA_HSAMP_MAX_VOCAB */
+    int32_t draft_cap;          /* of the drafter's sets */
+    const int32_t* draft_idx;   /* [draft_rows, draft_cap], or NULL (all three): certain drafts */
+    const float* draft_prob;
+    const int32_t* draft_count; /* [draft_rows] */
+    const int32_t* draft;       /* as in ultima_hsamp_draft, to the end */
+    const int32_t* n_draft;
+    const int32_t* target_start;
+    const int32_t* draft_start;
+    const double* u_accept;
+    const double* u_draw;
+    int32_t* out_tokens;
+    int32_t* out_count;
+    float* accept_prob;
+} ultima_hsamp_draft_sets;
+
+/* Asynchronous on hip_stream, allocates nothing, needs no workspace. */
+int ultima_hsamp_verify_sets(const ultima_hsamp_draft_sets* d, void* hip_stream);
+
+/* ---- The product with its epilogue ---------------------------------------------
+ * out = act(x W^T + bias) + residual on the matrix cores, for the layers around
+ * the logits that need not have the CPU reference's order of sums: a draft
+ * head's residual block (x + silu(W x + b) on the final hidden states), several
+ * heads in one call (groups), the vocabulary product over all positions of
+ * drafted blocks (with a logit soft cap). 16-bit inputs, sums in float, bias,
+ * activation and residual in float, rounded once to the output's type. */
+#define ULTIMA_HSAMP_F16 9           /* IEEE half (ultima_hsamp_linear) */
+#define ULTIMA_HSAMP_ACT_NONE 0
+#define ULTIMA_HSAMP_ACT_RELU 1
+#define ULTIMA_HSAMP_ACT_SILU 2      /* y / (1 + exp(-y)) */
+#define ULTIMA_HSAMP_ACT_GELU 3      /* y (1 + erf(y / sqrt 2)) / 2 */
+#define ULTIMA_HSAMP_ACT_GELU_TANH 4 /* y (1 + tanh(sqrt(2 / pi) (y + 0.044715 y^3))) / 2 */
+#define ULTIMA_HSAMP_ACT_SOFTCAP 5   /* c tanh(y / c), c = act_param > 0 */
+typedef struct ultima_hsamp_linear_args {
+    int32_t rows;               /* M >= 1 */
+    int32_t in_dim;             /* K >= 1 */
+    int32_t out_dim;            /* N >= 1 */
+    int32_t groups;             /* products in the call, >= 1 (65535 at most) */
+    int32_t dtype;              /* of x, weight, bias and residual: ULTIMA_HSAMP_BF16 or ULTIMA_HSAMP_F16 */
+    int32_t out_dtype;          /* dtype, or ULTIMA_HSAMP_F32 */
+    int32_t act;                /* ULTIMA_HSAMP_ACT_* */
+    float act_param;            /* ULTIMA_HSAMP_ACT_SOFTCAP: the cap; else ignored */
+    const void* x;              /* [M, K], rows x_stride elements apart */
+    int64_t x_stride;           /* >= K */
+    int64_t x_group;            /* elements between groups (0: one x for all) */
+    const void* weight;         /* [N, K], rows weight_stride elements apart */
+    int64_t weight_stride;      /* >= K */
+    int64_t weight_group;
+    const void* bias;           /* [N] or NULL */
+    int64_t bias_group;
+    const void* residual;       /* [M, N] or NULL; may be out itself (same type, strides and group) */
+    int64_t residual_stride;    /* >= N */
+    int64_t residual_group;
+    void* out;                  /* [M, N]; no overlap with the inputs but the one above */
+    int64_t out_stride;         /* >= N */
+    int64_t out_group;          /* groups > 1: the groups one behind the other (>= (M - 1) out_stride + N), or
+                                   side by side in each row (>= N, all of them within out_stride) */
+} ultima_hsamp_linear_args;
+
+/* All pointers are device memory of the current device, aligned to their
+ * elements; hip_stream one of its streams; asynchronous, allocates nothing
+ * (graph-capturable). */
+int ultima_hsamp_linear(const ultima_hsamp_linear_args* a, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,6 +68,8 @@ def build_all() -> None:
         "hsamp_headm.o": CSRC / "hsamp_headm.hip",
         "hsamp_history.o": CSRC / "hsamp_history.hip",
         "hsamp_callers.o": CSRC / "hsamp_callers.hip",
+        "hsamp_verify.o": CSRC / "hsamp_verify.hip",
+        "hsamp_linear.o": CSRC / "hsamp_linear.hip",
     }
     with ThreadPoolExecutor(max_workers=4) as ex:
         futs = [ex.submit(_run, [HIPCC, *HIP_FLAGS, "-x", "hip", "-c", str(src), "-o", str(BUILD / o)])

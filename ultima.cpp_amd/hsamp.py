@@ -18,7 +18,8 @@ HEADER = PKG.parent / "include" / "ultima_hsamp.h"
 NOALLOC_HEADER = PKG.parent / "include" / "ultima_hsamp_noalloc.h"
 
 OK, ERR_INVALID, ERR_HIP, ERR_UNSUPPORTED, ERR_NOMEM, ERR_CAPACITY, ERR_NO_DEVICE = 0, -1, -2, -3, -4, -5, -6
-F32, BF16 = 0, 1
+F32, BF16, F16 = 0, 1, 9
+MAX_DRAFT = 1023
 WRITEBACK, STREAM_ONLY = 1, 0x100
 NOALLOC_SCRATCH_BYTES, NOALLOC_PLAN_BYTES = 96 << 20, 2 << 20
 KERNELS_EXACT, KERNELS_GENERAL, KERNELS_FULL, KERNELS_WRITEBACK = 1, 2, 4, 8
@@ -136,6 +137,93 @@ class Verify(ctypes.Structure):
     ]
 
 
+class Draft(ctypes.Structure):
+    """ultima_hsamp_draft (include/ultima_hsamp.h)."""
+    _fields_ = [
+        ("seqs", ctypes.c_int32),
+        ("max_draft", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("logits", ctypes.c_void_p),
+        ("logits_stride", ctypes.c_int64),
+        ("logits_rows", ctypes.c_int32),
+        ("draft_rows", ctypes.c_int32),
+        ("draft_logits", ctypes.c_void_p),
+        ("draft_stride", ctypes.c_int64),
+        ("draft", ctypes.c_void_p),
+        ("n_draft", ctypes.c_void_p),
+        ("target_start", ctypes.c_void_p),
+        ("draft_start", ctypes.c_void_p),
+        ("temperature", ctypes.c_void_p),
+        ("draft_temperature", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p),
+        ("mask_stride", ctypes.c_int64),
+        ("draft_mask", ctypes.c_void_p),
+        ("draft_mask_stride", ctypes.c_int64),
+        ("u_accept", ctypes.c_void_p),
+        ("u_draw", ctypes.c_void_p),
+        ("work", ctypes.c_void_p),
+        ("out_tokens", ctypes.c_void_p),
+        ("out_count", ctypes.c_void_p),
+        ("accept_prob", ctypes.c_void_p),
+    ]
+
+
+class DraftSets(ctypes.Structure):
+    """ultima_hsamp_draft_sets (include/ultima_hsamp.h)."""
+    _fields_ = [
+        ("seqs", ctypes.c_int32),
+        ("max_draft", ctypes.c_int32),
+        ("rows", ctypes.c_int32),
+        ("draft_rows", ctypes.c_int32),
+        ("kept_idx", ctypes.c_void_p),
+        ("kept_prob", ctypes.c_void_p),
+        ("kept_count", ctypes.c_void_p),
+        ("set_cap", ctypes.c_int32),
+        ("draft_cap", ctypes.c_int32),
+        ("draft_idx", ctypes.c_void_p),
+        ("draft_prob", ctypes.c_void_p),
+        ("draft_count", ctypes.c_void_p),
+        ("draft", ctypes.c_void_p),
+        ("n_draft", ctypes.c_void_p),
+        ("target_start", ctypes.c_void_p),
+        ("draft_start", ctypes.c_void_p),
+        ("u_accept", ctypes.c_void_p),
+        ("u_draw", ctypes.c_void_p),
+        ("out_tokens", ctypes.c_void_p),
+        ("out_count", ctypes.c_void_p),
+        ("accept_prob", ctypes.c_void_p),
+    ]
+
+
+class LinearArgs(ctypes.Structure):
+    """ultima_hsamp_linear_args (include/ultima_hsamp.h)."""
+    _fields_ = [
+        ("rows", ctypes.c_int32),
+        ("in_dim", ctypes.c_int32),
+        ("out_dim", ctypes.c_int32),
+        ("groups", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("act", ctypes.c_int32),
+        ("act_param", ctypes.c_float),
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("x_group", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("weight_stride", ctypes.c_int64),
+        ("weight_group", ctypes.c_int64),
+        ("bias", ctypes.c_void_p),
+        ("bias_group", ctypes.c_int64),
+        ("residual", ctypes.c_void_p),
+        ("residual_stride", ctypes.c_int64),
+        ("residual_group", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_stride", ctypes.c_int64),
+        ("out_group", ctypes.c_int64),
+    ]
+
+
 def declared_symbols(header: Path = HEADER) -> list[str]:
     """Function names declared in a header (default include/ultima_hsamp.h)."""
     import re
@@ -197,6 +285,14 @@ def lib() -> ctypes.CDLL:
         L.ultima_hsamp_verify_work_ints.argtypes = [i32, i32]
         L.ultima_hsamp_verify_block.restype = ctypes.c_int
         L.ultima_hsamp_verify_block.argtypes = [vp, ctypes.POINTER(Verify), vp]
+        L.ultima_hsamp_verify_draft_work_bytes.restype = i64
+        L.ultima_hsamp_verify_draft_work_bytes.argtypes = [i32, i32, i32]
+        L.ultima_hsamp_verify_draft.restype = ctypes.c_int
+        L.ultima_hsamp_verify_draft.argtypes = [ctypes.POINTER(Draft), vp]
+        L.ultima_hsamp_verify_sets.restype = ctypes.c_int
+        L.ultima_hsamp_verify_sets.argtypes = [ctypes.POINTER(DraftSets), vp]
+        L.ultima_hsamp_linear.restype = ctypes.c_int
+        L.ultima_hsamp_linear.argtypes = [ctypes.POINTER(LinearArgs), vp]
         _lib = L
     return _lib
 
@@ -400,6 +496,198 @@ def lm_head(hidden, norm_scale, eps: float, weight, logit_scale: float = 1.0, lo
     s = torch.cuda.current_stream(dev) if stream is None else stream
     check(lib().ultima_hsamp_lm_head(ctypes.byref(h), ctypes.c_void_p(s.cuda_stream)), "lm_head")
     return logits, normed
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise HsampError(ERR_INVALID, what)
+
+
+def _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_start, draft_start, accept, outputs):
+    """The fields of Draft and DraftSets that say which rows are whose."""
+    import torch
+    B, K = u_draw.shape[0], int(max_draft)
+    for name, t, dt in (("draft", draft, torch.int32), ("u_accept", u_accept, torch.float64),
+                        ("u_draw", u_draw, torch.float64), ("n_draft", n_draft, torch.int32),
+                        ("target_start", target_start, torch.int32), ("draft_start", draft_start, torch.int32)):
+        if t is None:
+            continue
+        _need(t.dtype == dt and t.device == dev and t.dim() == 1 and (t.shape[0] < 2 or t.stride(0) == 1),
+              f"{what}: {name} must be a contiguous {dt} vector on {dev}")
+        if name in ("n_draft", "target_start", "draft_start"):
+            _need(t.shape[0] == B, f"{what}: {name} must have one entry per sequence")
+    _need(B >= 1 and 0 <= K <= MAX_DRAFT, f"{what}: at least one sequence, max_draft 0 .. {MAX_DRAFT}")
+    D = draft.shape[0] if draft is not None else 0
+    _need((u_accept.shape[0] if u_accept is not None else 0) == D, f"{what}: one u_accept per drafted token")
+    out = {} if outputs is None else outputs
+    for name, shape, dt in (("tokens", (B, K + 1), torch.int32), ("count", (B,), torch.int32),
+                            ("accept", (D,), torch.float32)):
+        if name not in out and (name != "accept" or accept):
+            out[name] = torch.empty(shape, dtype=dt, device=dev)
+        if name in out:
+            t = out[name]
+            _need(tuple(t.shape) == shape and t.dtype == dt and t.device == dev and t.is_contiguous(),
+                  f"{what}: output {name} must be contiguous {dt} {shape} on {dev}")
+    a.seqs, a.max_draft, a.draft_rows = B, K, D
+    a.draft = draft.data_ptr() if D else None
+    a.u_accept = u_accept.data_ptr() if D else None
+    a.u_draw = u_draw.data_ptr()
+    a.n_draft, a.target_start, a.draft_start = (None if t is None else t.data_ptr()
+                                                for t in (n_draft, target_start, draft_start))
+    a.out_tokens, a.out_count = out["tokens"].data_ptr(), out["count"].data_ptr()
+    a.accept_prob = out["accept"].data_ptr() if "accept" in out and D else None
+    return out
+
+
+def _launch(fn, a, dev, stream, what):
+    import torch
+    with torch.cuda.device(dev):
+        s = torch.cuda.current_stream(dev) if stream is None else stream
+        check(fn(ctypes.byref(a), ctypes.c_void_p(s.cuda_stream)), what)
+
+
+def verify_draft(logits, draft, u_accept, u_draw, max_draft: int, draft_logits=None, temperature=None,
+                 draft_temperature=None, mask=None, draft_mask=None, n_draft=None, target_start=None,
+                 draft_start=None, accept: bool = True, work=None, outputs=None, stream=None):
+    """ultima_hsamp_verify_draft on torch tensors of one device: drafted tokens
+    (int32 [D]) against the target's logits [R, V] and the drafter's [D, V] (None:
+    certain drafts), float32 or bfloat16, by the rejection rule. u_accept f64 [D],
+    u_draw f64 [B]; temperature, draft_temperature f32 [B] (None: 1; <= 0:
+    greedy); mask, draft_mask int32 words per row; n_draft, target_start,
+    draft_start int32 [B] for sequences of different lengths. Returns a dict:
+    tokens int32 [B, max_draft + 1], count int32 [B] and, unless accept is False,
+    accept f32 [D] (their acceptance probabilities). work: a uint8 tensor of
+    ultima_hsamp_verify_draft_work_bytes() bytes of this call alone (allocated
+    otherwise); outputs: a dict of tensors to write to."""
+    import torch
+    what = "verify_draft"
+    dev = logits.device
+    _need(logits.is_cuda and logits.dim() == 2 and logits.dtype in (torch.float32, torch.bfloat16),
+          f"{what}: logits must be a float32 or bfloat16 matrix on the GPU")
+    V = logits.shape[1]
+    a = Draft()
+    out = _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_start, draft_start, accept, outputs)
+    rows = ((logits, "logits", None, logits.dtype),) + (((draft_logits, "draft_logits", a.draft_rows, logits.dtype),)
+                                                        if draft_logits is not None else ())
+    for t, name, n, dt in rows:
+        _need(t.device == dev and t.dim() == 2 and t.dtype == dt and t.shape[1] == V and (V == 1 or t.stride(1) == 1)
+              and (n is None or t.shape[0] == n), f"{what}: {name} must be {dt} rows of {V} on {dev}")
+    words = -(-V // 32)
+    for t, name, n in ((mask, "mask", logits.shape[0]), (draft_mask, "draft_mask", a.draft_rows)):
+        _need(t is None or (t.device == dev and t.dtype in (torch.int32, torch.uint32) and t.dim() == 2 and
+                            t.shape[0] == n and t.shape[1] >= words and (t.shape[1] == 1 or t.stride(1) == 1)),
+              f"{what}: {name} must be {n} rows of at least {words} int32 words on {dev}")
+    for t, name in ((temperature, "temperature"), (draft_temperature, "draft_temperature")):
+        _need(t is None or (t.device == dev and t.dtype == torch.float32 and t.shape == (a.seqs,) and t.is_contiguous()),
+              f"{what}: {name} must be contiguous float32, one per sequence, on {dev}")
+    a.vocab, a.dtype = V, F32 if logits.dtype == torch.float32 else BF16
+    a.logits, a.logits_rows = logits.data_ptr(), logits.shape[0]
+    a.logits_stride = max(V, logits.stride(0)) if logits.shape[0] == 1 else logits.stride(0)
+    if draft_logits is not None and a.draft_rows:
+        a.draft_logits = draft_logits.data_ptr()
+        a.draft_stride = max(V, draft_logits.stride(0)) if a.draft_rows == 1 else draft_logits.stride(0)
+    if mask is not None:
+        a.mask, a.mask_stride = mask.data_ptr(), max(words, mask.stride(0)) if mask.shape[0] == 1 else mask.stride(0)
+    if draft_mask is not None and a.draft_rows:
+        _need(draft_logits is not None, f"{what}: draft_mask goes with draft_logits")
+        a.draft_mask = draft_mask.data_ptr()
+        a.draft_mask_stride = max(words, draft_mask.stride(0)) if a.draft_rows == 1 else draft_mask.stride(0)
+    a.temperature, a.draft_temperature = (None if t is None else t.data_ptr() for t in (temperature, draft_temperature))
+    need = int(lib().ultima_hsamp_verify_draft_work_bytes(a.seqs, a.max_draft, V))
+    if work is None:
+        work = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    _need(work.device == dev and work.is_contiguous() and work.numel() * work.element_size() >= need,
+          f"{what}: work must be {need} contiguous bytes on {dev}")
+    a.work = work.data_ptr()
+    _launch(lib().ultima_hsamp_verify_draft, a, dev, stream, what)
+    return out
+
+
+def verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_draft: int, draft_idx=None,
+                draft_prob=None, draft_count=None, n_draft=None, target_start=None, draft_start=None,
+                accept: bool = True, outputs=None, stream=None):
+    """ultima_hsamp_verify_sets on torch tensors of one device: drafted tokens
+    against the kept sets that run() leaves for the target's rows (kept_idx int32
+    [R, cap], kept_prob f32 [R, cap], kept_count int32 [R]) and, unless the drafts
+    are certain, for the drafter's. The other arguments and the result as in
+    verify_draft."""
+    import torch
+    what = "verify_sets"
+    dev = kept_idx.device
+    _need(kept_idx.is_cuda and kept_idx.dim() == 2, f"{what}: kept_idx must be a matrix on the GPU")
+    a = DraftSets()
+    out = _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_start, draft_start, accept, outputs)
+
+    def sets(idx, prob, count, names, rows):
+        _need(prob is not None and count is not None and idx.dim() == 2 and idx.shape[0] == rows and
+              prob.shape == idx.shape and count.shape == (rows,) and idx.dtype == torch.int32 and
+              prob.dtype == torch.float32 and count.dtype == torch.int32 and
+              all(t.device == dev and t.is_contiguous() for t in (idx, prob, count)),
+              f"{what}: {names} must be contiguous int32 [{rows}, cap], float32 [{rows}, cap], int32 [{rows}] on {dev}")
+
+    sets(kept_idx, kept_prob, kept_count, "kept_idx, kept_prob, kept_count", kept_idx.shape[0])
+    a.rows, a.set_cap = kept_idx.shape
+    a.kept_idx, a.kept_prob, a.kept_count = kept_idx.data_ptr(), kept_prob.data_ptr(), kept_count.data_ptr()
+    if draft_idx is not None:
+        sets(draft_idx, draft_prob, draft_count, "draft_idx, draft_prob, draft_count", a.draft_rows)
+        if a.draft_rows:
+            a.draft_cap = draft_idx.shape[1]
+            a.draft_idx, a.draft_prob, a.draft_count = draft_idx.data_ptr(), draft_prob.data_ptr(), draft_count.data_ptr()
+    else:
+        _need(draft_prob is None and draft_count is None, f"{what}: draft_prob and draft_count go with draft_idx")
+    _launch(lib().ultima_hsamp_verify_sets, a, dev, stream, what)
+    return out
+
+
+ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "softcap": 5}
+
+
+def linear(x, weight, bias=None, act: str = "none", act_param: float = 0.0, residual=None, out=None, out_dtype=None,
+           stream=None):
+    """ultima_hsamp_linear on torch tensors of one device: act(x weight^T + bias)
+    + residual, x [M, K] and weight [N, K], or with a leading dimension of groups
+    on all of them (expanded dimensions are fine); bfloat16 or float16, the output
+    in that type or in float32 (out_dtype; out: the tensor to write, which may be
+    the residual). act: one of ACTS; act_param: the cap of "softcap"."""
+    import torch
+    what = "linear"
+    dev = x.device
+    _need(x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and x.dim() in (2, 3) and weight.dim() == x.dim(),
+          f"{what}: x and weight must be bfloat16 or float16 matrices (or batches of them) on the GPU")
+    _need(act in ACTS, f"{what}: act must be one of {', '.join(ACTS)}")
+    one = x.dim() == 2
+    G = 1 if one else x.shape[0]
+    M, K = x.shape[-2:]
+    N = weight.shape[-2]
+    lead = () if one else (G,)
+    if out is None:
+        out = torch.empty((*lead, M, N), dtype=out_dtype or x.dtype, device=dev)
+    _need(out.dtype in (x.dtype, torch.float32) and (out_dtype is None or out.dtype == out_dtype),
+          f"{what}: the output must be {x.dtype} or torch.float32")
+    for t, name, shape, dt in ((weight, "weight", (*lead, N, K), x.dtype), (bias, "bias", (*lead, N), x.dtype),
+                               (residual, "residual", (*lead, M, N), x.dtype), (out, "out", (*lead, M, N), out.dtype)):
+        _need(t is None or (t.device == dev and tuple(t.shape) == shape and t.dtype == dt),
+              f"{what}: {name} must be {dt} {shape} on {dev}")
+    for t, name in ((x, "x"), (weight, "weight"), (bias, "bias"), (residual, "residual"), (out, "out")):
+        _need(t is None or t.shape[-1] <= 1 or t.stride(-1) == 1, f"{what}: the last dimension of {name} must be contiguous")
+
+    def row(t):
+        return t.stride(-2) if t.shape[-2] > 1 else max(t.shape[-1], t.stride(-2))
+
+    a = LinearArgs()
+    a.rows, a.in_dim, a.out_dim, a.groups = M, K, N, G
+    a.dtype = BF16 if x.dtype == torch.bfloat16 else F16
+    a.out_dtype = F32 if out.dtype == torch.float32 else a.dtype
+    a.act, a.act_param = ACTS[act], act_param
+    a.x, a.x_stride, a.x_group = x.data_ptr(), row(x), 0 if one else x.stride(0)
+    a.weight, a.weight_stride, a.weight_group = weight.data_ptr(), row(weight), 0 if one else weight.stride(0)
+    if bias is not None:
+        a.bias, a.bias_group = bias.data_ptr(), 0 if one else bias.stride(0)
+    if residual is not None:
+        a.residual, a.residual_stride, a.residual_group = residual.data_ptr(), row(residual), 0 if one else residual.stride(0)
+    a.out, a.out_stride, a.out_group = out.data_ptr(), row(out), 0 if one else out.stride(0)
+    _launch(lib().ultima_hsamp_linear, a, dev, stream, what)
+    return out
 
 
 class Sampler:
