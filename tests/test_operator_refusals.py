@@ -112,7 +112,9 @@ def test_linear_refuses_null_and_too_much(hsamp):
     assert linear(hsamp, groups=65536) == hsamp.ERR_UNSUPPORTED
     assert linear(hsamp, groups=1, in_dim=(1 << 30) + 1, x_stride=big, weight_stride=big) == hsamp.ERR_UNSUPPORTED
     assert linear(hsamp, groups=1, out_dim=(1 << 30) + 1, residual_stride=big, out_stride=big) == hsamp.ERR_UNSUPPORTED
-    assert linear(hsamp, groups=1, rows=1 << 22) == hsamp.ERR_UNSUPPORTED
+    assert linear(hsamp, groups=1, rows=(1 << 30) + 1) == hsamp.ERR_UNSUPPORTED
+    assert linear(hsamp, groups=1, rows=1 << 30, out_dim=4096, residual_stride=4096, out_stride=4096) == hsamp.ERR_UNSUPPORTED
+    assert linear(hsamp, groups=1, rows=1, out_dim=1 << 27, residual_stride=big, out_stride=big) == hsamp.ERR_UNSUPPORTED
 
 
 def test_bindings_match_the_header(hsamp):

@@ -38,23 +38,53 @@ __device__ __forceinline__ uint16_t from_f32(float f) {   // to nearest, ties to
     return __builtin_bit_cast(uint16_t, (_Float16)f);
 }
 
-// 1 / (1 + exp(-t)); exp(-t) past the largest float is infinite, the result then 0.
+// 1 / (1 + exp(-t)) by the hardware's exp2 and reciprocal (one step of 2^-23
+// each); the exponent's rounding moves exp(-t) by |t| 2^-24, at most 2^-17 of a
+// value below 2^-126. exp(-t) past the largest float is infinite, the result 0.
+// (With expf and a division the epilogue of 256 x 256 tiles took 90 of 554 us.)
 __device__ __forceinline__ float sigmoid(float t) {
-    return 1.0f / (1.0f + expf(-t));
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t * -1.44269504f));
+}
+
+// tanh: to 1/2 its Taylor series (the next term is 10^-7 of the value there),
+// from there 1 - 2 / (1 + exp(2 |t|)).
+__device__ __forceinline__ float tanh_of(float t) {
+    const float z = t * t, u = fabsf(t);
+    float p = 21844.0f / 6081075.0f;
+    p = __builtin_fmaf(p, z, -1382.0f / 155925.0f);
+    p = __builtin_fmaf(p, z, 62.0f / 2835.0f);
+    p = __builtin_fmaf(p, z, -17.0f / 315.0f);
+    p = __builtin_fmaf(p, z, 2.0f / 15.0f);
+    p = __builtin_fmaf(p, z, -1.0f / 3.0f);
+    const float low = __builtin_fmaf(t * z, p, t);
+    const float high = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * 2.88539008f)), 1.0f);
+    return u <= 0.5f ? low : __builtin_copysignf(high, t);       // (NaN: high's NaN)
 }
 
 using Args = ultima_hsamp_linear_args;
 
-// E outputs (columns n .. n + E - 1 of row m, those there are) from their finished sums.
+// The eight values of row m's columns n .. n + 7, where all of them are there.
+__device__ __forceinline__ u32x4 eight(const Args& a, const void* base, int64_t at, int m, int n) {
+    if (base == nullptr || m >= a.rows || n + 8 > a.out_dim) return u32x4{0, 0, 0, 0};
+    return *reinterpret_cast<const u32x4_a2*>(static_cast<const uint16_t*>(base) + at);
+}
+__device__ __forceinline__ u32x4 residual8(const Args& a, int g, int m, int n) {
+    return eight(a, a.residual, g * a.residual_group + m * a.residual_stride + n, m, n);
+}
+__device__ __forceinline__ u32x4 bias8(const Args& a, int g, int n) {
+    return eight(a, a.bias, g * a.bias_group + n, 0, n);
+}
+
+// E outputs (columns n .. n + E - 1 of row m, those there are) from their finished
+// sums; bias, residual: eight()'s values.
 template <bool BF, int E>
-__device__ __forceinline__ void finish(const Args& a, int g, int m, int n, float (&y)[E]) {
+__device__ __forceinline__ void finish(const Args& a, int g, int m, int n, float (&y)[E], u32x4 bias, u32x4 residual) {
     typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
     const int left = a.out_dim - n;
     if (m >= a.rows || left <= 0) return;
-    auto add = [&](const void* base, int64_t at) {
+    auto add = [&](const void* base, int64_t at, u32x4 v) {
         const uint16_t* p = static_cast<const uint16_t*>(base) + at;
         if (E == 8 && left >= 8) {
-            const u32x4 v = *reinterpret_cast<const u32x4_a2*>(p);
 #pragma unroll
             for (int e = 0; e < E; ++e) y[e] += to_f32<BF>((uint16_t)(v[e / 2 % 4] >> (16 * (e & 1))));
         } else {
@@ -63,7 +93,7 @@ __device__ __forceinline__ void finish(const Args& a, int g, int m, int n, float
                 if (e < left) y[e] += to_f32<BF>(p[e]);
         }
     };
-    if (a.bias != nullptr) add(a.bias, g * a.bias_group + n);
+    if (a.bias != nullptr) add(a.bias, g * a.bias_group + n, bias);
     switch (a.act) {
         case ULTIMA_HSAMP_ACT_RELU:
 #pragma unroll
@@ -82,12 +112,14 @@ __device__ __forceinline__ void finish(const Args& a, int g, int m, int n, float
             for (int e = 0; e < E; ++e)
                 y[e] = y[e] * sigmoid(1.59576912160573071f * (y[e] + 0.044715f * y[e] * y[e] * y[e]));
             break;
-        case ULTIMA_HSAMP_ACT_SOFTCAP:
+        case ULTIMA_HSAMP_ACT_SOFTCAP: {
+            const float inv = 1.0f / a.act_param;
 #pragma unroll
-            for (int e = 0; e < E; ++e) y[e] = a.act_param * tanhf(y[e] / a.act_param);
+            for (int e = 0; e < E; ++e) y[e] = a.act_param * tanh_of(y[e] * inv);
             break;
+        }
     }
-    if (a.residual != nullptr) add(a.residual, g * a.residual_group + m * a.residual_stride + n);
+    if (a.residual != nullptr) add(a.residual, g * a.residual_group + m * a.residual_stride + n, residual);
     const int64_t at = g * a.out_group + m * a.out_stride + n;
     if (a.out_dtype == ULTIMA_HSAMP_F32) {
         float* p = static_cast<float*>(a.out) + at;
@@ -121,154 +153,34 @@ __device__ __forceinline__ void finish(const Args& a, int g, int m, int n, float
 template <bool BF, int TN, int TM>
 __device__ __forceinline__ void store_tiles(const Args& a, int g, int m0, int n0, const f32x4 (&acc)[TN][TM], float* lds) {
     constexpr int LS = 16 * TN + 4, PR = 2 * TN;       // pieces of eight columns per row
+    constexpr int NP = TN < 2 ? 1 : TN / 2;            // pieces of one lane per 16 rows
     const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+    const int c = lane % PR * 8, row = lane / PR;
+    const bool on = row < 16;
+    u32x4 res[NP], bias = bias8(a, g, n0 + c);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) res[p] = residual8(a, g, m0 + row + 64 / PR * p, n0 + c);
 #pragma unroll
     for (int u = 0; u < TM; ++u) {
+        u32x4 next[NP] = {};
+        if (u + 1 < TM)
+#pragma unroll
+            for (int p = 0; p < NP; ++p) next[p] = residual8(a, g, m0 + 16 * (u + 1) + row + 64 / PR * p, n0 + c);
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int s = 0; s < TN; ++s) *reinterpret_cast<f32x4*>(&lds[i * LS + 16 * s + 4 * q]) = acc[s][u];
         __builtin_amdgcn_wave_barrier();
-#pragma nounroll
-        for (int o = lane; o < 16 * PR; o += 64) {
-            const int r = o / PR, c = o % PR * 8;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const int r = row + 64 / PR * p;
+            if (!on) continue;
             const f32x4 lo = *reinterpret_cast<const f32x4*>(&lds[r * LS + c]);
             const f32x4 hi = *reinterpret_cast<const f32x4*>(&lds[r * LS + c + 4]);
             float y[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            finish<BF, 8>(a, g, m0 + 16 * u + r, n0 + c, y);
+            finish<BF, 8>(a, g, m0 + 16 * u + r, n0 + c, y, bias, res[p]);
         }
-    }
-}
-
-// 64 x 64 outputs by four waves, 64 columns of x and W at a time through LDS.
-template <bool BF>
-__global__ __launch_bounds__(256) void k_linear(Args a) {
-    constexpr int BK = 64, LS = BK + 8;
-    __shared__ __attribute__((aligned(16))) uint16_t ws[64 * LS], xs[64 * LS];   // (ws: also 4 x 16 x 36 floats)
-    static_assert(sizeof(ws) + 0 >= 4 * 16 * 36 * 4);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, q = lane >> 4;
-    const int g = blockIdx.z, K = a.in_dim;
-    const int n0 = blockIdx.x * 64, m0 = blockIdx.y * 64;
-    const uint16_t* W = static_cast<const uint16_t*>(a.weight) + g * a.weight_group;
-    const uint16_t* X = static_cast<const uint16_t*>(a.x) + g * a.x_group;
-    // eight columns of a row, zeros past K and past the last row
-    auto load = [&](const uint16_t* base, int64_t stride, int row, int rows, int k) {
-        u32x4 v = {0, 0, 0, 0};
-        if (row < rows) {
-            const uint16_t* p = base + row * stride + k;
-            if (k + 8 <= K) v = *reinterpret_cast<const u32x4_a2*>(p);
-            else
-                for (int e = 0; e < 8; ++e)
-                    if (k + e < K) v[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
-        }
-        return v;
-    };
-    f32x4 acc[2][2] = {};
-    const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
-    for (int k0 = 0; k0 < K; k0 += BK) {
-        __syncthreads();
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int c = tid + 256 * t, r = c >> 3, k = (c & 7) * 8;
-            *reinterpret_cast<u32x4*>(&ws[r * LS + k]) = load(W, a.weight_stride, n0 + r, a.out_dim, k0 + k);
-            *reinterpret_cast<u32x4*>(&xs[r * LS + k]) = load(X, a.x_stride, m0 + r, a.rows, k0 + k);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < BK; k += 32) {
-            u32x4 wf[2], xf[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                wf[t] = *reinterpret_cast<const u32x4*>(&ws[(wn + 16 * t + i) * LS + k + 8 * q]);
-                xf[t] = *reinterpret_cast<const u32x4*>(&xs[(wm + 16 * t + i) * LS + k + 8 * q]);
-            }
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int s = 0; s < 2; ++s) acc[t][s] = mfma<BF>(wf[t], xf[s], acc[t][s]);
-        }
-    }
-    __syncthreads();
-    store_tiles<BF, 2, 2>(a, g, m0 + wm, n0 + wn, acc, reinterpret_cast<float*>(ws) + wave * 16 * (32 + 4));
-}
-
-// Up to 16 NT rows of x: the weights' stream. Eight waves share 16 rows of W,
-// each a part of the columns, from global memory straight into the operands'
-// layout; their sums meet in LDS.
-template <bool BF, int NT>
-__global__ __launch_bounds__(512) void k_linear_rows(Args a) {
-    constexpr int U = NT >= 4 ? 4 : 8;       // steps of 32 columns in flight, twice
-    constexpr int NN = 16, MM = 16 * NT, LS = NN + 4;
-    __shared__ __attribute__((aligned(16))) float part[8][MM * LS];
-    const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, q = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g = blockIdx.z, K = a.in_dim, n0 = blockIdx.x * NN, m0 = blockIdx.y * MM;
-    const uint16_t* wp = static_cast<const uint16_t*>(a.weight) + g * a.weight_group +
-                         min(n0 + i, a.out_dim - 1) * a.weight_stride + 8 * q;
-    const uint16_t* xp[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-        xp[t] = static_cast<const uint16_t*>(a.x) + g * a.x_group + min(m0 + 16 * t + i, a.rows - 1) * a.x_stride + 8 * q;
-    f32x4 acc[NT] = {};
-    const int steps = K / 32;
-    const int s0 = (int)((int64_t)steps * wave / 8), s1 = (int)((int64_t)steps * (wave + 1) / 8);
-    struct Group {
-        u32x4 w[U], x[U][NT];
-    };
-    // (steps past the wave's last are loaded as its last and not multiplied)
-    auto load = [&](Group& r, int s) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t k = (int64_t)min(s + u, s1 - 1) * 32;
-            r.w[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_a2*>(wp + k));
-#pragma unroll
-            for (int t = 0; t < NT; ++t) r.x[u][t] = *reinterpret_cast<const u32x4_a2*>(xp[t] + k);
-        }
-    };
-    auto multiply = [&](const Group& r, int s) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (s + u < s1)
-#pragma unroll
-                for (int v = 0; v < NT; ++v) acc[v] = mfma<BF>(r.w[u], r.x[u][v], acc[v]);
-    };
-    if (s0 < s1) {
-        Group ra, rb;
-        load(ra, s0);
-        for (int s = s0; s < s1; s += 2 * U) {
-            load(rb, s + U);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(ra, s);
-            __builtin_amdgcn_sched_barrier(0);
-            load(ra, s + 2 * U);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(rb, s + U);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-    // the columns past the last whole step
-    if (wave == 7 && K % 32 != 0) {
-        auto tail = [&](const uint16_t* p) {
-            u32x4 v = {0, 0, 0, 0};
-            for (int e = 0; e < 8; ++e)
-                if (steps * 32 + 8 * q + e < K) v[e >> 1] |= (uint32_t)p[(int64_t)steps * 32 + e] << (16 * (e & 1));
-            return v;
-        };
-        u32x4 xf[NT];
-#pragma unroll
-        for (int v = 0; v < NT; ++v) xf[v] = tail(xp[v]);
-        const u32x4 wf = tail(wp);
-#pragma unroll
-        for (int v = 0; v < NT; ++v) acc[v] = mfma<BF>(wf, xf[v], acc[v]);
-    }
-#pragma unroll
-    for (int v = 0; v < NT; ++v) *reinterpret_cast<f32x4*>(&part[wave][(16 * v + i) * LS + 4 * q]) = acc[v];
-    __syncthreads();
-    for (int o = tid; o < MM * NN; o += 512) {
-        const int m = o / NN, n = o % NN;
-        float y[1] = {};
-#pragma unroll
-        for (int w = 0; w < 8; ++w) y[0] += part[w][m * LS + n];
-        finish<BF, 1>(a, g, m0 + m, n0 + n, y);
+        for (int p = 0; p < NP; ++p) res[p] = next[p];
     }
 }
 
@@ -277,7 +189,9 @@ __global__ __launch_bounds__(512) void k_linear_rows(Args a) {
 // stages in the air or in LDS; the next step's operands are read while one is
 // multiplied. A stage is 64 columns in two steps (WK = 1), or 32 WK columns, one
 // step for each wave, whose sums meet in LDS at the end.
-template <bool BF, int WM, int WN, int WK, int TM, int TN, int ST>
+// ANY: rows at any element's address, a last piece of less than eight columns
+// (loads to LDS take neither): one stage in registers, two in LDS.
+template <bool BF, bool ANY, int WM, int WN, int WK, int TM, int TN, int ST>
 __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(Args a, int tiles_m, int tiles_n) {
 #ifdef __HIP_DEVICE_COMPILE__    // (the buffer resource's type is the device compiler's alone)
     constexpr int NW = WM * WN * WK;
@@ -289,7 +203,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(Args a, int t
     typedef __attribute__((address_space(3))) void* lds_ptr;
     constexpr int SB = (BM + BN) * BK;                   // elements per stage: by 64 columns x's rows, then W's
     constexpr int EB = WK == 1 ? NW * 16 * (16 * TN + 4) : NW * 256 * TM * TN;   // floats of the waves' sums in LDS
-    static_assert((ST & (ST - 1)) == 0 && ST * SB * 2 >= EB * 4 && ST * SB * 2 <= 160 * 1024);
+    static_assert((ST & (ST - 1)) == 0 && (!ANY || ST == 2) && ST * SB * 2 >= EB * 4 && ST * SB * 2 <= 160 * 1024);
     __shared__ __attribute__((aligned(16))) uint16_t sm[ST * SB];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -309,13 +223,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(Args a, int t
     // 12 - 15 with q = 1 of rows 4 - 11, and so on. Row r's piece p stands at
     // p ^ (r / 2 % 8), which puts each such sixteen into all 64 banks.
     uint32_t vo[NL];
+    const uint16_t* row[ANY ? NL : 1];
     int col[NL];
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
         const int c = wave + NW * j, rc = c % CR, r = (rc < CX ? rc : rc - CX) * 8 + (lane >> 3);
         col[j] = c / CR * 64 + ((lane & 7) ^ (r >> 1 & 7)) * 8;
         const bool in = rc < CX ? m0 + r < a.rows : n0 + r < a.out_dim;
-        vo[j] = in ? (uint32_t)(r * (int)(rc < CX ? a.x_stride : a.weight_stride) + col[j]) * 2u : kOutside;
+        if (ANY) row[j] = rc < CX ? X + min(r, a.rows - 1 - m0) * a.x_stride : W + min(r, a.out_dim - 1 - n0) * a.weight_stride;
+        else vo[j] = in ? (uint32_t)(r * (int)(rc < CX ? a.x_stride : a.weight_stride) + col[j]) * 2u : kOutside;
     }
     const int T = (K + BK - 1) / BK;
     const bool full = wave + NW * (NL - 1) < CT;          // this wave has NL loads a stage, not NL - 1
@@ -336,6 +252,37 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(Args a, int t
             else
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(to + c * 512), 16, v, t * BK * 2, 0, 0);
         }
+    };
+    u32x4 held[ANY ? NL : 1];
+    auto fetch = [&](int s) {
+        const int t = s + t0 < T ? s + t0 : s + t0 - T;
+        if (s >= T) return;
+        const int left = K - t * BK;
+        if (left >= BK) {
+#pragma unroll
+            for (int j = 0; j < NL; ++j)
+                if (CT % NW == 0 || j < NL - 1 || full)
+                    held[j] = *reinterpret_cast<const u32x4_a2*>(row[j] + (int64_t)t * BK + col[j]);
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+            if (CT % NW != 0 && j == NL - 1 && !full) continue;
+            const uint16_t* p = row[j] + (int64_t)t * BK + col[j];
+            u32x4 v = {0, 0, 0, 0};
+            if (col[j] + 8 <= left) v = *reinterpret_cast<const u32x4_a2*>(p);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (col[j] + e < left) v[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+            held[j] = v;
+        }
+    };
+    auto store = [&](int s) {
+#pragma unroll
+        for (int j = 0; j < NL; ++j)
+            if (CT % NW == 0 || j < NL - 1 || full)
+                *reinterpret_cast<u32x4*>(&sm[(s & 1) * SB + (wave + NW * j) * 512 + lane * 8]) = held[j];
     };
     // all but this wave's loads of the last `stages` stages are in LDS, its reads done
     auto wait = [&](auto stages) {
@@ -372,34 +319,55 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(Args a, int t
     };
     using std::integral_constant;
     Operands oa, ob;
-#pragma unroll
-    for (int t = 0; t < ST; ++t) issue(t);
-    wait(integral_constant<int, ST - 1>());
-    // (a stage past the last reads as zeros)
-    if (WK == 1) {
-        read(oa, 0, 0);
+    if constexpr (ANY) {
+        fetch(0);
+        store(0);
+        fetch(1);
+        __syncthreads();
+        if (WK == 1) read(oa, 0, 0);
         for (int t = 0; t < T; ++t) {
-            read(ob, t, 1);
+            // (the place of stage t + 1 was read before the last barrier)
+            if (t + 1 < T) store(t + 1);
+            fetch(t + 2);
+            read(WK == 1 ? ob : oa, t, WK == 1 ? 1 : wk);
             multiply(oa);
-            wait(integral_constant<int, ST - 2>());
-            issue(t + ST);
-            read(oa, t + 1, 0);
-            multiply(ob);
+            __syncthreads();
+            if (WK == 1) {
+                if (t + 1 < T) read(oa, t + 1, 0);
+                multiply(ob);
+            }
         }
+        __syncthreads();
     } else {
-        read(oa, 0, wk);
-        for (int t = 0; t < T; t += 2) {
-            wait(integral_constant<int, ST - 2>());
-            issue(t + ST);
-            read(ob, t + 1, wk);
-            multiply(oa);
-            wait(integral_constant<int, ST - 2>());
-            issue(t + 1 + ST);
-            read(oa, t + 2, wk);
-            multiply(ob);
+#pragma unroll
+        for (int t = 0; t < ST; ++t) issue(t);
+        wait(integral_constant<int, ST - 1>());
+        // (a stage past the last reads as zeros)
+        if (WK == 1) {
+            read(oa, 0, 0);
+            for (int t = 0; t < T; ++t) {
+                read(ob, t, 1);
+                multiply(oa);
+                wait(integral_constant<int, ST - 2>());
+                issue(t + ST);
+                read(oa, t + 1, 0);
+                multiply(ob);
+            }
+        } else {
+            read(oa, 0, wk);
+            for (int t = 0; t < T; t += 2) {
+                wait(integral_constant<int, ST - 2>());
+                issue(t + ST);
+                read(ob, t + 1, wk);
+                multiply(oa);
+                wait(integral_constant<int, ST - 2>());
+                issue(t + 1 + ST);
+                read(oa, t + 2, wk);
+                multiply(ob);
+            }
         }
+        wait(integral_constant<int, 0>());
     }
-    wait(integral_constant<int, 0>());
     float* sums = reinterpret_cast<float*>(sm);
     if (WK == 1) {
         store_tiles<BF, TN, TM>(a, g, m0 + wm, n0 + wn, acc, sums + wave * 16 * (16 * TN + 4));
@@ -432,7 +400,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(Args a, int t
                     for (int f = 0; f < 4; ++f) y[(e + f) % E] += v[f];
                 }
             }
-        finish<BF, E>(a, g, m0 + m, n0 + n, y);
+        finish<BF, E>(a, g, m0 + m, n0 + n, y, E == 8 ? bias8(a, g, n0 + n) : u32x4{},
+                      E == 8 ? residual8(a, g, m0 + m, n0 + n) : u32x4{});
     }
 #endif
 }
@@ -453,17 +422,24 @@ constexpr Form kForms[] = {
     {64, 64, 2, {32, 39}},  {128, 128, 1, {44, 0}},  {160, 128, 2, {62, 84}}, {256, 256, 1, {112, 0}},
 };
 
-// The form whose rounds over the 256 CUs cost least.
+// Blocks of one group.
+int64_t blocks_of(const Form& f, const Args& a) {
+    return (((int64_t)a.rows + f.bm - 1) / f.bm) * (((int64_t)a.out_dim + f.bn - 1) / f.bn);
+}
+
+// Up to 32 rows: the narrowest form that holds them (bound by W's stream at any
+// width). More: the form whose rounds over the 256 CUs cost least.
 int choose(const Args& a) {
+    if (a.rows <= 32) return a.rows <= 16 ? 0 : 1;
     int best = 0;
     float least = 0;
-    for (int f = 0; f < (int)(sizeof(kForms) / sizeof(kForms[0])); ++f) {
+    for (int f = 2; f < (int)(sizeof(kForms) / sizeof(kForms[0])); ++f) {
         const Form& v = kForms[f];
-        const int64_t blocks = (int64_t)((a.rows + v.bm - 1) / v.bm) * ((a.out_dim + v.bn - 1) / v.bn) * a.groups;
+        const int64_t blocks = blocks_of(v, a) * a.groups;
         const int64_t round = 256 * v.blocks, rest = blocks % round;
         const float cost = (float)(blocks / round) * v.one[v.blocks - 1] +
                            (rest == 0 ? 0.0f : rest <= 256 ? v.one[0] : v.one[v.blocks - 1]);
-        if (f == 0 || cost < least) {
+        if (f == 2 || cost < least) {
             best = f;
             least = cost;
         }
@@ -471,50 +447,40 @@ int choose(const Args& a) {
     return best;
 }
 
+template <bool BF, bool ANY, int WM, int WN, int WK, int TM, int TN, int ST>
+hipError_t launch_tile(const Args& a, hipStream_t s) {
+    const int tm = (a.rows + 16 * WM * TM - 1) / (16 * WM * TM), tn = (a.out_dim + 16 * WN * TN - 1) / (16 * WN * TN);
+    hipLaunchKernelGGL((k_linear_tile<BF, ANY, WM, WN, WK, TM, TN, ST>), dim3(tm * tn, 1, a.groups),
+                       dim3(64 * WM * WN * WK), 0, s, a, tm, tn);
+    return hipGetLastError();
+}
+
 template <bool BF>
 hipError_t launch_linear(const Args& a, hipStream_t s) {
-    const int M = a.rows, N = a.out_dim;
-    using std::integral_constant;
-    // 16-byte loads of every row, 32-bit offsets within a tile
-    const bool tiles = a.in_dim % 8 == 0 && a.x_stride % 8 == 0 && a.weight_stride % 8 == 0 && a.x_group % 8 == 0 &&
-                       a.weight_group % 8 == 0 &&
-                       (reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.weight)) % 16 == 0 &&
-                       std::max(a.x_stride, a.weight_stride) <= 1 << 20;
-    if (tiles) {
-        auto go = [&](auto wm, auto wn, auto wk, auto tm, auto tn, auto st) {
-            constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, WK = decltype(wk)::value;
-            constexpr int TM = decltype(tm)::value, TN = decltype(tn)::value, ST = decltype(st)::value;
-            const int tm_ = (M + 16 * WM * TM - 1) / (16 * WM * TM), tn_ = (N + 16 * WN * TN - 1) / (16 * WN * TN);
-            hipLaunchKernelGGL((k_linear_tile<BF, WM, WN, WK, TM, TN, ST>), dim3(tm_ * tn_, 1, a.groups),
-                               dim3(64 * WM * WN * WK), 0, s, a, tm_, tn_);
-            return hipGetLastError();
-        };
-        constexpr integral_constant<int, 1> c1;
-        constexpr integral_constant<int, 2> c2;
-        constexpr integral_constant<int, 4> c4;
-        constexpr integral_constant<int, 5> c5;
-        constexpr integral_constant<int, 8> c8;
-        switch (choose(a)) {
-            case 0: return go(c1, c1, c4, c1, c1, c8);
-            case 1: return go(c1, c1, c4, c2, c2, c4);
-            case 2: return go(c1, c1, c8, c4, c1, c4);
-            case 3: return go(c1, c2, c4, c4, c1, c4);
-            case 4: return go(c2, c2, c2, c2, c2, c4);
-            case 5: return go(c2, c4, c1, c4, c2, c4);
-            case 6: return go(c2, c4, c1, c5, c2, c2);
-            default: return go(c2, c4, c1, c8, c4, c2);
+    // 16-byte loads of whole pieces, 32-bit offsets within a tile
+    const bool aligned = a.in_dim % 8 == 0 && a.x_stride % 8 == 0 && a.weight_stride % 8 == 0 && a.x_group % 8 == 0 &&
+                         a.weight_group % 8 == 0 &&
+                         (reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.weight)) % 16 == 0 &&
+                         std::max(a.x_stride, a.weight_stride) <= 1 << 20;
+    const int f = choose(a);
+    if (!aligned) switch (f) {
+            case 0: return launch_tile<BF, true, 1, 1, 8, 1, 1, 2>(a, s);
+            case 1: return launch_tile<BF, true, 1, 1, 8, 2, 2, 2>(a, s);
+            case 2:
+            case 3: return launch_tile<BF, true, 1, 2, 4, 4, 1, 2>(a, s);
+            case 4: return launch_tile<BF, true, 2, 2, 2, 2, 2, 2>(a, s);
+            default: return launch_tile<BF, true, 2, 4, 1, 4, 2, 2>(a, s);
         }
+    switch (f) {
+        case 0: return launch_tile<BF, false, 1, 1, 4, 1, 1, 8>(a, s);
+        case 1: return launch_tile<BF, false, 1, 1, 4, 2, 2, 4>(a, s);
+        case 2: return launch_tile<BF, false, 1, 1, 8, 4, 1, 4>(a, s);
+        case 3: return launch_tile<BF, false, 1, 2, 4, 4, 1, 4>(a, s);
+        case 4: return launch_tile<BF, false, 2, 2, 2, 2, 2, 4>(a, s);
+        case 5: return launch_tile<BF, false, 2, 4, 1, 4, 2, 4>(a, s);
+        case 6: return launch_tile<BF, false, 2, 4, 1, 5, 2, 2>(a, s);
+        default: return launch_tile<BF, false, 2, 4, 1, 8, 4, 2>(a, s);
     }
-    auto rows = [&](auto nt) {
-        constexpr int NT = decltype(nt)::value;
-        hipLaunchKernelGGL((k_linear_rows<BF, NT>), dim3((N + 15) / 16, (M + 16 * NT - 1) / (16 * NT), a.groups),
-                           dim3(512), 0, s, a);
-        return hipGetLastError();
-    };
-    if (M <= 16) return rows(integral_constant<int, 1>());
-    if (M <= 128) return rows(integral_constant<int, 4>());
-    hipLaunchKernelGGL(k_linear<BF>, dim3((N + 63) / 64, (M + 63) / 64, a.groups), dim3(256), 0, s, a);
-    return hipGetLastError();
 }
 
 }  // namespace
@@ -547,8 +513,8 @@ extern "C" int ultima_hsamp_linear(const ultima_hsamp_linear_args* a, void* hip_
         og < (a->rows - 1) * a->out_stride + a->out_dim &&
         !(a->out_group >= a->out_dim && og < a->out_stride && (a->groups - 1) * og + a->out_dim <= a->out_stride))
         return ULTIMA_HSAMP_ERR_INVALID;
-    // 32-bit columns, grid sizes
-    if (a->groups > 65535 || a->rows >= 65535 * 64 || a->in_dim > 1 << 30 || a->out_dim > 1 << 30)
+    // 32-bit rows and columns; a launch counts its threads in 32 bits
+    if (a->groups > 65535 || std::max({a->rows, a->in_dim, a->out_dim}) > 1 << 30 || std::max(blocks_of(kForms[choose(*a)], *a), blocks_of(kForms[5], *a)) > 1 << 22)
         return ULTIMA_HSAMP_ERR_UNSUPPORTED;
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
     const hipError_t e = a->dtype == ULTIMA_HSAMP_BF16 ? launch_linear<true>(*a, s) : launch_linear<false>(*a, s);
