@@ -498,52 +498,88 @@ def lm_head(hidden, norm_scale, eps: float, weight, logit_scale: float = 1.0, lo
     return logits, normed
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise HsampError(ERR_INVALID, what)
+def _refuse(what: str):
+    raise HsampError(ERR_INVALID, what)
+
+
+class _On:
+    """The stream a call runs on and its device made current; what the call
+    allocates is allocated for that stream."""
+
+    def __init__(self, dev, stream):
+        import torch
+        self.torch = torch
+        self.stream = torch.cuda.current_stream(dev) if stream is None else stream
+        self.other = stream is not None and stream != torch.cuda.current_stream(dev)
+        self.guard = torch.cuda.stream(stream) if self.other else None
+        self.device = None if self.other or torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+    def __enter__(self):
+        for g in (self.guard, self.device):
+            if g is not None:
+                g.__enter__()
+        return self
+
+    def __exit__(self, *e):
+        for g in (self.device, self.guard):
+            if g is not None:
+                g.__exit__(*e)
+
+    def hold(self, t):
+        """A caller's scratch stays allocated until this stream is done with it."""
+        if self.other:
+            t.record_stream(self.stream)
+
+    def launch(self, fn, a, what):
+        status = fn(ctypes.byref(a), self.stream.cuda_stream)
+        if status != OK:
+            raise HsampError(status, what)
+
+
+def _vector(t, n, dtype, dev, what, name):
+    """The address of a contiguous vector of n (None: any number) elements, or None."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != dev or t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
+        _refuse(f"{what}: {name} must be a contiguous {dtype} vector{'' if n is None else f' of {n}'} on {dev}")
+    return t.data_ptr()
+
+
+def _rows(t, n, width, dtypes, dev, what, name):
+    """The address and row stride of n rows of at least `width` elements."""
+    if t.dtype not in dtypes or t.device != dev or t.dim() != 2 or t.shape[0] != n or t.shape[1] < width or \
+            (t.shape[1] > 1 and t.stride(1) != 1):
+        _refuse(f"{what}: {name} must be {n} rows of {width} {dtypes[0]} on {dev}")
+    return t.data_ptr(), t.stride(0) if n > 1 else max(width, t.stride(0))
 
 
 def _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_start, draft_start, accept, outputs):
     """The fields of Draft and DraftSets that say which rows are whose."""
     import torch
-    B, K = u_draw.shape[0], int(max_draft)
-    for name, t, dt in (("draft", draft, torch.int32), ("u_accept", u_accept, torch.float64),
-                        ("u_draw", u_draw, torch.float64), ("n_draft", n_draft, torch.int32),
-                        ("target_start", target_start, torch.int32), ("draft_start", draft_start, torch.int32)):
-        if t is None:
-            continue
-        _need(t.dtype == dt and t.device == dev and t.dim() == 1 and (t.shape[0] < 2 or t.stride(0) == 1),
-              f"{what}: {name} must be a contiguous {dt} vector on {dev}")
-        if name in ("n_draft", "target_start", "draft_start"):
-            _need(t.shape[0] == B, f"{what}: {name} must have one entry per sequence")
-    _need(B >= 1 and 0 <= K <= MAX_DRAFT, f"{what}: at least one sequence, max_draft 0 .. {MAX_DRAFT}")
-    D = draft.shape[0] if draft is not None else 0
-    _need((u_accept.shape[0] if u_accept is not None else 0) == D, f"{what}: one u_accept per drafted token")
-    out = {} if outputs is None else outputs
-    for name, shape, dt in (("tokens", (B, K + 1), torch.int32), ("count", (B,), torch.int32),
-                            ("accept", (D,), torch.float32)):
-        if name not in out and (name != "accept" or accept):
-            out[name] = torch.empty(shape, dtype=dt, device=dev)
-        if name in out:
-            t = out[name]
-            _need(tuple(t.shape) == shape and t.dtype == dt and t.device == dev and t.is_contiguous(),
-                  f"{what}: output {name} must be contiguous {dt} {shape} on {dev}")
+    i32, f64 = torch.int32, torch.float64
+    a.u_draw = _vector(u_draw, None, f64, dev, what, "u_draw")
+    B, K, D = u_draw.shape[0], int(max_draft), 0 if draft is None else draft.shape[0]
+    if B < 1 or not 0 <= K <= MAX_DRAFT or (u_accept is None) != (draft is None):
+        _refuse(f"{what}: at least one sequence, max_draft 0 .. {MAX_DRAFT}, draft and u_accept together")
+    at, u = _vector(draft, D, i32, dev, what, "draft"), _vector(u_accept, D, f64, dev, what, "u_accept")
     a.seqs, a.max_draft, a.draft_rows = B, K, D
-    a.draft = draft.data_ptr() if D else None
-    a.u_accept = u_accept.data_ptr() if D else None
-    a.u_draw = u_draw.data_ptr()
-    a.n_draft, a.target_start, a.draft_start = (None if t is None else t.data_ptr()
-                                                for t in (n_draft, target_start, draft_start))
+    if D:
+        a.draft, a.u_accept = at, u
+    a.n_draft = _vector(n_draft, B, i32, dev, what, "n_draft")
+    a.target_start = _vector(target_start, B, i32, dev, what, "target_start")
+    a.draft_start = _vector(draft_start, B, i32, dev, what, "draft_start")
+    out = {} if outputs is None else outputs
+    for name, shape, dt in (("tokens", (B, K + 1), i32), ("count", (B,), i32), ("accept", (D,), torch.float32)):
+        t = out.get(name)
+        if t is None:
+            if name != "accept" or accept:
+                out[name] = torch.empty(shape, dtype=dt, device=dev)
+        elif t.shape != shape or t.dtype != dt or t.device != dev or not t.is_contiguous():
+            _refuse(f"{what}: output {name} must be contiguous {dt} {shape} on {dev}")
     a.out_tokens, a.out_count = out["tokens"].data_ptr(), out["count"].data_ptr()
-    a.accept_prob = out["accept"].data_ptr() if "accept" in out and D else None
+    if D and "accept" in out:
+        a.accept_prob = out["accept"].data_ptr()
     return out
-
-
-def _launch(fn, a, dev, stream, what):
-    import torch
-    with torch.cuda.device(dev):
-        s = torch.cuda.current_stream(dev) if stream is None else stream
-        check(fn(ctypes.byref(a), ctypes.c_void_p(s.cuda_stream)), what)
 
 
 def verify_draft(logits, draft, u_accept, u_draw, max_draft: int, draft_logits=None, temperature=None,
@@ -560,46 +596,44 @@ def verify_draft(logits, draft, u_accept, u_draw, max_draft: int, draft_logits=N
     ultima_hsamp_verify_draft_work_bytes() bytes of this call alone (allocated
     otherwise); outputs: a dict of tensors to write to."""
     import torch
-    what = "verify_draft"
+    what, f32 = "verify_draft", torch.float32
     dev = logits.device
-    _need(logits.is_cuda and logits.dim() == 2 and logits.dtype in (torch.float32, torch.bfloat16),
-          f"{what}: logits must be a float32 or bfloat16 matrix on the GPU")
-    V = logits.shape[1]
-    a = Draft()
-    out = _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_start, draft_start, accept, outputs)
-    rows = ((logits, "logits", None, logits.dtype),) + (((draft_logits, "draft_logits", a.draft_rows, logits.dtype),)
-                                                        if draft_logits is not None else ())
-    for t, name, n, dt in rows:
-        _need(t.device == dev and t.dim() == 2 and t.dtype == dt and t.shape[1] == V and (V == 1 or t.stride(1) == 1)
-              and (n is None or t.shape[0] == n), f"{what}: {name} must be {dt} rows of {V} on {dev}")
-    words = -(-V // 32)
-    for t, name, n in ((mask, "mask", logits.shape[0]), (draft_mask, "draft_mask", a.draft_rows)):
-        _need(t is None or (t.device == dev and t.dtype in (torch.int32, torch.uint32) and t.dim() == 2 and
-                            t.shape[0] == n and t.shape[1] >= words and (t.shape[1] == 1 or t.stride(1) == 1)),
-              f"{what}: {name} must be {n} rows of at least {words} int32 words on {dev}")
-    for t, name in ((temperature, "temperature"), (draft_temperature, "draft_temperature")):
-        _need(t is None or (t.device == dev and t.dtype == torch.float32 and t.shape == (a.seqs,) and t.is_contiguous()),
-              f"{what}: {name} must be contiguous float32, one per sequence, on {dev}")
-    a.vocab, a.dtype = V, F32 if logits.dtype == torch.float32 else BF16
-    a.logits, a.logits_rows = logits.data_ptr(), logits.shape[0]
-    a.logits_stride = max(V, logits.stride(0)) if logits.shape[0] == 1 else logits.stride(0)
-    if draft_logits is not None and a.draft_rows:
-        a.draft_logits = draft_logits.data_ptr()
-        a.draft_stride = max(V, draft_logits.stride(0)) if a.draft_rows == 1 else draft_logits.stride(0)
-    if mask is not None:
-        a.mask, a.mask_stride = mask.data_ptr(), max(words, mask.stride(0)) if mask.shape[0] == 1 else mask.stride(0)
-    if draft_mask is not None and a.draft_rows:
-        _need(draft_logits is not None, f"{what}: draft_mask goes with draft_logits")
-        a.draft_mask = draft_mask.data_ptr()
-        a.draft_mask_stride = max(words, draft_mask.stride(0)) if a.draft_rows == 1 else draft_mask.stride(0)
-    a.temperature, a.draft_temperature = (None if t is None else t.data_ptr() for t in (temperature, draft_temperature))
-    need = int(lib().ultima_hsamp_verify_draft_work_bytes(a.seqs, a.max_draft, V))
-    if work is None:
-        work = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-    _need(work.device == dev and work.is_contiguous() and work.numel() * work.element_size() >= need,
-          f"{what}: work must be {need} contiguous bytes on {dev}")
-    a.work = work.data_ptr()
-    _launch(lib().ultima_hsamp_verify_draft, a, dev, stream, what)
+    if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in (f32, torch.bfloat16):
+        _refuse("verify_draft: logits must be a float32 or bfloat16 matrix on the GPU")
+    rows, V = logits.shape
+    with _On(dev, stream) as on:
+        a = Draft()
+        out = _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_start, draft_start, accept,
+                        outputs)
+        D, B = a.draft_rows, a.seqs
+        a.vocab, a.dtype, a.logits_rows = V, F32 if logits.dtype == f32 else BF16, rows
+        a.logits, a.logits_stride = _rows(logits, rows, V, (logits.dtype,), dev, what, "logits")
+        if draft_logits is not None:
+            at, stride = _rows(draft_logits, D, V, (logits.dtype,), dev, what, "draft_logits")
+            if draft_logits.shape[1] != V:
+                _refuse("verify_draft: draft_logits must have the target's vocabulary")
+            if D:
+                a.draft_logits, a.draft_stride = at, stride
+        words, kinds = -(-V // 32), (torch.int32, torch.uint32)
+        if mask is not None:
+            a.mask, a.mask_stride = _rows(mask, rows, words, kinds, dev, what, "mask")
+        if draft_mask is not None:
+            at, stride = _rows(draft_mask, D, words, kinds, dev, what, "draft_mask")
+            if draft_logits is None:
+                _refuse("verify_draft: draft_mask goes with draft_logits")
+            if D:
+                a.draft_mask, a.draft_mask_stride = at, stride
+        a.temperature = _vector(temperature, B, f32, dev, what, "temperature")
+        a.draft_temperature = _vector(draft_temperature, B, f32, dev, what, "draft_temperature")
+        need = lib().ultima_hsamp_verify_draft_work_bytes(B, a.max_draft, V)
+        if work is None:
+            work = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        elif work.device != dev or not work.is_contiguous() or work.numel() * work.element_size() < need:
+            _refuse(f"verify_draft: work must be {need} contiguous bytes on {dev}")
+        else:
+            on.hold(work)
+        a.work = work.data_ptr()
+        on.launch(lib().ultima_hsamp_verify_draft, a, what)
     return out
 
 
@@ -614,28 +648,32 @@ def verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_dr
     import torch
     what = "verify_sets"
     dev = kept_idx.device
-    _need(kept_idx.is_cuda and kept_idx.dim() == 2, f"{what}: kept_idx must be a matrix on the GPU")
-    a = DraftSets()
-    out = _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_start, draft_start, accept, outputs)
+    if not kept_idx.is_cuda or kept_idx.dim() != 2:
+        _refuse("verify_sets: kept_idx must be a matrix on the GPU")
 
-    def sets(idx, prob, count, names, rows):
-        _need(prob is not None and count is not None and idx.dim() == 2 and idx.shape[0] == rows and
-              prob.shape == idx.shape and count.shape == (rows,) and idx.dtype == torch.int32 and
-              prob.dtype == torch.float32 and count.dtype == torch.int32 and
-              all(t.device == dev and t.is_contiguous() for t in (idx, prob, count)),
-              f"{what}: {names} must be contiguous int32 [{rows}, cap], float32 [{rows}, cap], int32 [{rows}] on {dev}")
+    def sets(idx, prob, count, rows, names):
+        if prob is None or count is None or idx.dtype != torch.int32 or prob.dtype != torch.float32 or \
+                count.dtype != torch.int32 or idx.dim() != 2 or idx.shape[0] != rows or prob.shape != idx.shape or \
+                count.shape != (rows,) or not (idx.device == prob.device == count.device == dev) or \
+                not (idx.is_contiguous() and prob.is_contiguous() and count.is_contiguous()):
+            _refuse(f"{what}: {names} must be contiguous int32 [{rows}, cap], float32 [{rows}, cap], int32 [{rows}] on {dev}")
+        return idx.data_ptr(), prob.data_ptr(), count.data_ptr()
 
-    sets(kept_idx, kept_prob, kept_count, "kept_idx, kept_prob, kept_count", kept_idx.shape[0])
-    a.rows, a.set_cap = kept_idx.shape
-    a.kept_idx, a.kept_prob, a.kept_count = kept_idx.data_ptr(), kept_prob.data_ptr(), kept_count.data_ptr()
-    if draft_idx is not None:
-        sets(draft_idx, draft_prob, draft_count, "draft_idx, draft_prob, draft_count", a.draft_rows)
-        if a.draft_rows:
-            a.draft_cap = draft_idx.shape[1]
-            a.draft_idx, a.draft_prob, a.draft_count = draft_idx.data_ptr(), draft_prob.data_ptr(), draft_count.data_ptr()
-    else:
-        _need(draft_prob is None and draft_count is None, f"{what}: draft_prob and draft_count go with draft_idx")
-    _launch(lib().ultima_hsamp_verify_sets, a, dev, stream, what)
+    with _On(dev, stream) as on:
+        a = DraftSets()
+        out = _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_start, draft_start, accept,
+                        outputs)
+        a.rows, a.set_cap = kept_idx.shape
+        a.kept_idx, a.kept_prob, a.kept_count = sets(kept_idx, kept_prob, kept_count, a.rows,
+                                                     "kept_idx, kept_prob, kept_count")
+        if draft_idx is not None:
+            at = sets(draft_idx, draft_prob, draft_count, a.draft_rows, "draft_idx, draft_prob, draft_count")
+            if a.draft_rows:
+                a.draft_cap = draft_idx.shape[1]
+                a.draft_idx, a.draft_prob, a.draft_count = at
+        elif draft_prob is not None or draft_count is not None:
+            _refuse("verify_sets: draft_prob and draft_count go with draft_idx")
+        on.launch(lib().ultima_hsamp_verify_sets, a, what)
     return out
 
 
@@ -650,43 +688,43 @@ def linear(x, weight, bias=None, act: str = "none", act_param: float = 0.0, resi
     in that type or in float32 (out_dtype; out: the tensor to write, which may be
     the residual). act: one of ACTS; act_param: the cap of "softcap"."""
     import torch
-    what = "linear"
-    dev = x.device
-    _need(x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and x.dim() in (2, 3) and weight.dim() == x.dim(),
-          f"{what}: x and weight must be bfloat16 or float16 matrices (or batches of them) on the GPU")
-    _need(act in ACTS, f"{what}: act must be one of {', '.join(ACTS)}")
-    one = x.dim() == 2
-    G = 1 if one else x.shape[0]
+    dev, dt = x.device, x.dtype
+    if not x.is_cuda or dt not in (torch.bfloat16, torch.float16) or x.dim() not in (2, 3) or weight.dim() != x.dim():
+        _refuse("linear: x and weight must be bfloat16 or float16 matrices (or batches of them) on the GPU")
+    if act not in ACTS:
+        _refuse(f"linear: act must be one of {', '.join(ACTS)}")
+    lead = tuple(x.shape[:-2])
     M, K = x.shape[-2:]
     N = weight.shape[-2]
-    lead = () if one else (G,)
-    if out is None:
-        out = torch.empty((*lead, M, N), dtype=out_dtype or x.dtype, device=dev)
-    _need(out.dtype in (x.dtype, torch.float32) and (out_dtype is None or out.dtype == out_dtype),
-          f"{what}: the output must be {x.dtype} or torch.float32")
-    for t, name, shape, dt in ((weight, "weight", (*lead, N, K), x.dtype), (bias, "bias", (*lead, N), x.dtype),
-                               (residual, "residual", (*lead, M, N), x.dtype), (out, "out", (*lead, M, N), out.dtype)):
-        _need(t is None or (t.device == dev and tuple(t.shape) == shape and t.dtype == dt),
-              f"{what}: {name} must be {dt} {shape} on {dev}")
-    for t, name in ((x, "x"), (weight, "weight"), (bias, "bias"), (residual, "residual"), (out, "out")):
-        _need(t is None or t.shape[-1] <= 1 or t.stride(-1) == 1, f"{what}: the last dimension of {name} must be contiguous")
 
-    def row(t):
-        return t.stride(-2) if t.shape[-2] > 1 else max(t.shape[-1], t.stride(-2))
+    def operand(t, name, shape, dtype):
+        """The address, row stride and group stride of [.., rows, columns] or [.., columns]."""
+        if t.shape != shape or t.dtype != dtype or t.device != dev or (shape[-1] > 1 and t.stride(-1) != 1):
+            _refuse(f"linear: {name} must be {dtype} {tuple(shape)} on {dev}, contiguous in its last dimension")
+        stride = t.stride()
+        group = stride[0] if lead else 0
+        if len(shape) == len(lead) + 1:
+            return t.data_ptr(), group
+        return t.data_ptr(), (stride[-2] if shape[-2] > 1 else max(shape[-1], stride[-2])), group
 
-    a = LinearArgs()
-    a.rows, a.in_dim, a.out_dim, a.groups = M, K, N, G
-    a.dtype = BF16 if x.dtype == torch.bfloat16 else F16
-    a.out_dtype = F32 if out.dtype == torch.float32 else a.dtype
-    a.act, a.act_param = ACTS[act], act_param
-    a.x, a.x_stride, a.x_group = x.data_ptr(), row(x), 0 if one else x.stride(0)
-    a.weight, a.weight_stride, a.weight_group = weight.data_ptr(), row(weight), 0 if one else weight.stride(0)
-    if bias is not None:
-        a.bias, a.bias_group = bias.data_ptr(), 0 if one else bias.stride(0)
-    if residual is not None:
-        a.residual, a.residual_stride, a.residual_group = residual.data_ptr(), row(residual), 0 if one else residual.stride(0)
-    a.out, a.out_stride, a.out_group = out.data_ptr(), row(out), 0 if one else out.stride(0)
-    _launch(lib().ultima_hsamp_linear, a, dev, stream, what)
+    with _On(dev, stream) as on:
+        if out is None:
+            out = torch.empty((*lead, M, N), dtype=out_dtype or dt, device=dev)
+        if out.dtype not in (dt, torch.float32) or out_dtype not in (None, out.dtype):
+            _refuse(f"linear: the output must be {dt} or torch.float32")
+        a = LinearArgs()
+        a.rows, a.in_dim, a.out_dim, a.groups = M, K, N, lead[0] if lead else 1
+        a.dtype = BF16 if dt == torch.bfloat16 else F16
+        a.out_dtype = F32 if out.dtype == torch.float32 else a.dtype
+        a.act, a.act_param = ACTS[act], act_param
+        a.x, a.x_stride, a.x_group = operand(x, "x", (*lead, M, K), dt)
+        a.weight, a.weight_stride, a.weight_group = operand(weight, "weight", (*lead, N, K), dt)
+        if bias is not None:
+            a.bias, a.bias_group = operand(bias, "bias", (*lead, N), dt)
+        if residual is not None:
+            a.residual, a.residual_stride, a.residual_group = operand(residual, "residual", (*lead, M, N), dt)
+        a.out, a.out_stride, a.out_group = operand(out, "out", (*lead, M, N), out.dtype)
+        on.launch(lib().ultima_hsamp_linear, a, "linear")
     return out
 
 
