@@ -4,7 +4,11 @@ rule) against the rule in 64 bits on the host.
 Tokens and counts are equal: every decision is made in double on both sides, and
 the tests' uniforms stay 1e-11 away from the borders (checked). The acceptance
 probability is one double quotient rounded to float: half a step, 2^-24 of the
-value, and 1e-12 for the sums behind it."""
+value, and 1e-12 for the sums behind it. Large calls in bfloat16 (128 MB of logits at
+four drafts and more, as many as their shape allows) take the sums of its rows from float exponentials: each is off by at most 3e-6 of it
+(3 steps of 2^-24 of the exponent, whose mean over the weights is at most ln V < 17
+by the entropy's bound: 51 2^-24; exp2's own step 2^-23; nine float additions, 9 2^-24;
+62 2^-24 = 3.7e-6 in all), their quotient by twice that."""
 import numpy as np
 import pytest
 
@@ -13,6 +17,8 @@ import verify_reference as R
 pytestmark = pytest.mark.gpu
 
 ACCEPT_TOL = 2.0 ** -24 + 1e-12
+ACCEPT_TOL_LARGE = 2.0 ** -24 + 2 * 62 * 2.0 ** -24
+LARGE = 128 << 20
 
 
 def _torch():
@@ -39,7 +45,7 @@ def place(x, dtype, pad=0, offset=0):
     return t, t.float().cpu().numpy()
 
 
-def check(out, want, B, K, n, ds, draft_rows):
+def check(out, want, B, K, n, ds, draft_rows, tol=ACCEPT_TOL):
     tokens, count = out["tokens"].cpu().numpy(), out["count"].cpu().numpy()
     got_a = out["accept"].cpu().numpy()
     for b in range(B):
@@ -48,11 +54,11 @@ def check(out, want, B, K, n, ds, draft_rows):
         assert list(tokens[b]) == toks + [-1] * (K + 1 - len(toks)), f"sequence {b}"
         assert count[b] == len(toks), f"sequence {b}"
         full = np.array(shares + [-1.0] * (n[b] - len(shares)))
-        np.testing.assert_allclose(got_a[ds[b]:ds[b] + n[b]], full, rtol=ACCEPT_TOL, atol=1e-37)
+        np.testing.assert_allclose(got_a[ds[b]:ds[b] + n[b]], full, rtol=tol, atol=1e-37)
 
 
 def run_draft(hs, seed, B, K, V, dtype="f32", drafter=True, n=None, t=None, td=None, mask=None, dmask=None, pad=0,
-              offset=0, edit=None, near=0.5):
+              offset=0, edit=None, near=0.5, big=False):
     """One call on made-up logits; edit(x, y, d, u, v) may change them first."""
     torch, dev = _torch()
     rng = np.random.default_rng(seed)
@@ -86,7 +92,9 @@ def run_draft(hs, seed, B, K, V, dtype="f32", drafter=True, n=None, t=None, td=N
         q_of = (lambda i: R.chances(yv[ds[b] + i], TD[b], None if dmask is None else dmask[ds[b] + i])) if drafter else None  # noqa: E731,B023
         sl = slice(ds[b], ds[b] + lens[b])
         want.append(R.verify(p_of, q_of, d[sl], u[sl], v[b]))
-    check(out, want, B, K, lens, ds, D)
+    large = dtype == "bf16" and K >= 4 and (B * (K + 1) + (B * K if drafter else 0)) * V * 2 > LARGE
+    assert large == big, "the test is meant for the other size"
+    check(out, want, B, K, lens, ds, D, ACCEPT_TOL_LARGE if large else ACCEPT_TOL)
     return want
 
 
@@ -107,7 +115,7 @@ def words_of(allowed):
     (2, 4, 8192, 8, 0),
     (2, 4, 8193, 3, 3),           # a slice of one id
     (3, 7, 50257, 0, 0),
-    (1, 17, 151936, 0, 0),
+    (1, 9, 151936, 0, 0),
     (4, 5, 16385, 0, 5),
     (70, 2, 1000, 0, 0),          # more sequences than a wave
     (1, 70, 257, 0, 0),           # more drafts than a wave
@@ -120,6 +128,63 @@ def test_draft_matches_the_rule(hs, B, K, V, pad, offset, dtype):
 def test_draft_over_a_large_vocabulary(hs):
     """More slices than a wave: the slices' sums are scanned in pieces."""
     run_draft(hs, 3, 2, 1, 600011, "bf16")
+
+
+@pytest.mark.parametrize("drafter", [True, False])
+def test_draft_large_calls(hs, drafter):
+    """Float exponentials first (few of the many drafts there could be): every kind
+    of temperature, odd rows."""
+    B = 40
+    n = [i % 6 for i in range(B)]
+    t = np.resize([1.0, 0.0, 0.6, 1e-38, np.inf, 3.0, np.nan, 0.8, 0.05], B)
+    td = np.resize([0.8, 1.0, 0.0, 1.0], B)
+    run_draft(hs, 13, B, 50 if drafter else 90, 40001, "bf16", drafter=drafter, n=n, t=t, td=td, pad=3, offset=1, big=True)
+
+
+def test_draft_large_calls_with_masks(hs):
+    B, K, V = 24, 3, 40003
+    rng = np.random.default_rng(14)
+    ok = rng.random((B * (K + 1), V)) < 0.2
+    okd = rng.random((B * K, V)) < 0.5
+    ok[4] = False
+    ok[8:12] = False
+    ok[8:12, V - 1] = True
+    okd[9] = False
+
+    def edit(x, y, d, u, v):
+        for a, m in ((x, ok), (y, okd)):
+            r, c = np.nonzero(~m)
+            a[r, c] = np.resize([np.nan, np.inf, -np.inf, np.finfo(np.float32).min], r.size)
+        for i in range(B * K):
+            row = ok[i // K * (K + 1) + i % K]
+            d[i] = np.flatnonzero(row)[0] if row.any() else 7
+        x[20, 5:9] = np.nan
+        x[21, 5:9] = -np.inf
+        u[::4] = 0.0
+    want = run_draft(hs, 15, B, 80, V, "bf16", n=[K] * B, mask=words_of(ok), dmask=words_of(okd), edit=edit, big=True,
+                     t=np.full(B, 0.8))
+    assert len(want[1][0]) == 0
+
+
+def test_draft_large_calls_near_the_border(hs):
+    """u within 1e-5 of p / q on either side: the float sums cannot tell, and the rows
+    are summed again in double."""
+    import torch
+    B, K, V = 24, 4, 30001
+
+    def edit(x, y, d, u, v):
+        for a in (x, y):
+            a[:] = torch.from_numpy(a).to(torch.bfloat16).float().numpy()
+        for b in range(B):
+            for i in range(K):
+                r, s = b * (K + 1) + i, b * K + i
+                x[r] = y[s]
+                x[r, d[s]] -= 0.5        # p / q below 1
+                x[r] = torch.from_numpy(x[r]).to(torch.bfloat16).float().numpy()
+                a = R.chances(x[r])[d[s]] / R.chances(y[s])[d[s]]
+                u[s] = a * (1 + (3e-9 if (b + i) % 3 == 0 else -3e-9))
+    want = run_draft(hs, 16, B, 100, V, "bf16", n=[K] * B, edit=edit, big=True)
+    assert {len(w[0]) for w in want} == {1, 2, 3}
 
 
 @pytest.mark.parametrize("drafter", [True, False])

@@ -10,24 +10,28 @@
 //                    that completes a position's rows decides its draft, and waves
 //                    of later positions find the rejection and read nothing. What
 //                    they skip is never used, whether they see it or not.
-//   k_draft_draw     a wave per slice of each sequence's emitting row: the slice's
-//                    sum of max(p - q, 0); the wave that completes a sequence finds
-//                    the slice where the running sum reaches u_draw, then the id.
+//   k_draft_draw     a wave per quarter of a slice of each sequence's emitting row:
+//                    its sum of max(p - q, 0); the wave that completes a sequence
+//                    finds the quarter where the running sum reaches u_draw, then
+//                    the id.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cstdint>
 
+#include "hsamp_wave.h"
 #include "ultima_hsamp.h"
 
 namespace hsamp {
 namespace {
 
-using u64 = unsigned long long;
-
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kChunks = 16;                  // 16-byte loads of a lane per slice
+constexpr int kDrawThreads = 512;
+constexpr int kChunks = 16;                  // 16-byte loads of a lane per slice,
+constexpr int kStep = 4;                     // of them a step, the next step's in flight
+constexpr int kSteps = kChunks / kStep;
+constexpr int kParts = 4;                    // parts of a slice when a token is drawn
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kFltMax = 3.402823466e38f;
 
@@ -36,10 +40,10 @@ typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 
 // exp(d) in double for d <= 0 by Tang's table method: d = (k + f) ln 2 / 32, |f| <=
-// 1/2, exp(d) = 2^(k >> 5) 2^((k & 31) / 32) exp(f ln 2 / 32), the last by its series
-// to the fifth power (the sixth is below 3e-15). The 32 doubles of the table fill
-// the 64 LDS banks once, so its reads never conflict. Fourteen double operations;
-// the library's exp takes three times as long.
+// 1/2, exp(d) = 2^(k >> 5) 2^((k & 31) / 32) exp(f ln 2 / 32), the last a polynomial
+// of the fourth degree (interpolated at the Chebyshev points, off by at most 8e-14:
+// the decisions need 1e-11 or so, a float exponential's 1e-7 would move the draws).
+// The 32 doubles of the table fill the 64 LDS banks once, so its reads never conflict.
 __device__ const double kPow[32] = {
     0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
     0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
@@ -55,23 +59,51 @@ __device__ __forceinline__ void load_table(double* t) {
     __syncthreads();
 }
 
-// t = d 32 / ln 2, at most 0; below -32000 as -32000 (2^-1000).
-__device__ __forceinline__ double exp32(double t, const double* table) {
-    constexpr double kRound = 6755399441055744.0;        // 1.5 2^52: adding it rounds to a whole number
-    t = fmax(t, -32000.0);
-    const double u = t + kRound;
-    const int k = (int)__double2loint(u);
-    const double f = t - (u - kRound);
-    double p = 0x1.5d87fe78a6731p-35;
-    p = __builtin_fma(p, f, 0x1.3b2ab6fba4e77p-27);
-    p = __builtin_fma(p, f, 0x1.c6b08d704a0c0p-20);
-    p = __builtin_fma(p, f, 0x1.ebfbdff82c58fp-13);
-    p = __builtin_fma(p, f, 0x1.62e42fefa39efp-6);
+constexpr double kPerE = 46.166241308446828384;          // 32 / ln 2
+constexpr double kRound = 6755399441055744.0;            // 1.5 2^52: adding it rounds to a whole number
+
+constexpr double kPoly[4] = {0x1.62e42fef8dc67p-6, 0x1.ebfbdff82240ap-13,
+                             0x1.c6b13c3469da5p-20, 0x1.3b2b07bdf576cp-27};
+
+// exp(d c ln 2 / 32) for d <= 0, d c >= -32600.
+__device__ __forceinline__ double exp32(double d, double c, const double* table) {
+    const double u = __builtin_fma(d, c, kRound);
+    const int k = __double2loint(u);
+    const double f = __builtin_fma(d, c, kRound - u);
+    double p = __builtin_fma(kPoly[3], f, kPoly[2]);
+    p = __builtin_fma(p, f, kPoly[1]);
+    p = __builtin_fma(p, f, kPoly[0]);
     const double b = table[k & 31];
     const double v = __builtin_fma(b * f, p, b);
-    return __hiloint2double(__double2hiint(v) + ((k >> 5) << 20), __double2loint(v));
+    return __hiloint2double(__double2hiint(v) + ((k & ~31) << 15), __double2loint(v));
 }
-constexpr double kPerE = 46.166241308446828384;          // 32 / ln 2
+
+// N of them side by side, whose chains of operations overlap.
+template <int N>
+__device__ __forceinline__ void exp32n(const double (&d)[N], double c, const double* table, double (&v)[N]) {
+    double u[N], f[N], p[N], b[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) u[n] = __builtin_fma(d[n], c, kRound);
+#pragma unroll
+    for (int n = 0; n < N; ++n) b[n] = table[__double2loint(u[n]) & 31];
+#pragma unroll
+    for (int n = 0; n < N; ++n) f[n] = kRound - u[n];
+#pragma unroll
+    for (int n = 0; n < N; ++n) f[n] = __builtin_fma(d[n], c, f[n]);
+#pragma unroll
+    for (int n = 0; n < N; ++n) p[n] = __builtin_fma(kPoly[3], f[n], kPoly[2]);
+#pragma unroll
+    for (int n = 0; n < N; ++n) p[n] = __builtin_fma(p[n], f[n], kPoly[1]);
+#pragma unroll
+    for (int n = 0; n < N; ++n) p[n] = __builtin_fma(p[n], f[n], kPoly[0]);
+#pragma unroll
+    for (int n = 0; n < N; ++n) f[n] = b[n] * f[n];
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = __builtin_fma(f[n], p[n], b[n]);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+        v[n] = __hiloint2double(__double2hiint(v[n]) + ((__double2loint(u[n]) & ~31) << 15), __double2loint(v[n]));
+}
 
 struct SliceStat {
     uint32_t m;     // bits of the maximum of the allowed logits, -inf: none
@@ -79,16 +111,24 @@ struct SliceStat {
     double s;       // sum of exp((x - m) / T)
 };
 
+struct RowSum {
+    float m;
+    int at;
+    double z;       // at the maximum; greedy rows 1; 0: nothing allowed
+};
+
 struct DraftArgs {
     ultima_hsamp_draft d;
     SliceStat* stats;        // [jobs][S]
-    double* rsum;            // [seqs][S]
+    double* rsum;            // [seqs][kParts S]
+    RowSum* sums;            // [max_draft][seqs][sides] of the decided positions
     int32_t* count;          // [max_draft][seqs] slices of the position's rows that are done, then
-    int32_t* drawn;          // [seqs] slices of the emitting row, and
+    int32_t* drawn;          // [seqs] parts of the emitting row, and
     int32_t* rejected;       // [seqs] the lowest position known to be rejected
     int S;                   // slices per row
     int per;                 // slices in a row that one wave of k_draft_stats takes
     int sides;               // 2 with the drafter's logits
+    int fast;                // float exponentials first
 };
 
 // What other XCDs' waves read in the same kernel goes past the caches both ways;
@@ -110,14 +150,14 @@ __device__ __forceinline__ SliceStat get_stat(const SliceStat* p) {
     const u64 a = get(reinterpret_cast<const u64*>(p)), s = get(reinterpret_cast<const u64*>(p) + 1);
     return SliceStat{(uint32_t)a, (int32_t)(a >> 32), __longlong_as_double((long long)s)};
 }
-// Whether this wave's n parts complete the `total` counted at p.
-__device__ __forceinline__ bool completes(int32_t* p, int n, int total) {
-    int before = 0;
+// Whether the block's n parts complete the `total` counted at p: for every thread
+// of the block. One count a block: they queue at the address, 0.2 us each.
+__device__ __forceinline__ bool completes(int32_t* p, int n, int total, int32_t* lds) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if ((threadIdx.x & 63) == 0) before = __hip_atomic_fetch_add(p, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    before = __builtin_amdgcn_readfirstlane(before);
-    asm volatile("" ::: "memory");
-    return before + n == total;
+    __syncthreads();
+    if (threadIdx.x == 0) *lds = __hip_atomic_fetch_add(p, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    return *lds + n == total;
 }
 
 struct Seq {
@@ -152,9 +192,38 @@ __device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, kNegInf)
 
 // exp((x - m) / T) exactly 0 for what is not allowed, and below 2^-1000.
 __device__ __forceinline__ double weight_of(float x, float m, double c, const double* table) {
-    const double t = ((double)x - (double)m) * c;
-    return x > kNegInf && t > -32000.0 ? exp32(t, table) : 0.0;
+    const double d = (double)x - (double)m;
+    return x > kNegInf && d * c > -32000.0 ? exp32(d, c, table) : 0.0;
 }
+
+// weight_of for many logits of a row with the maximum m: they are clamped to lo,
+// 2^-1000 of the maximum, and lo's weight left out. Not for temperatures so low
+// that lo is m or its neighbour, or so high that it is beyond the floats.
+struct Scale {
+    float m, lo;
+    double md, c;
+    bool fast;
+    __device__ __forceinline__ Scale(float m_, double c_) : m(m_), md(m_), c(c_) {
+        lo = (float)(md - 32000.0 / c);
+        const double low = (md - (double)lo) * c;
+        fast = lo > -3e38f && low > 31900.0 && low < 32100.0;
+    }
+    // (2^-1000 for what is not allowed)
+    __device__ __forceinline__ double some(float x, const double* table) const {
+        return exp32((double)__builtin_amdgcn_fmed3f(x, lo, kFltMax) - md, c, table);
+    }
+    template <int N>
+    __device__ __forceinline__ void some(const float (&x)[N], const double* table, double (&v)[N]) const {
+        double d[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) d[n] = (double)__builtin_amdgcn_fmed3f(x[n], lo, kFltMax) - md;
+        exp32n(d, c, table, v);
+    }
+    __device__ __forceinline__ double of(float x, const double* table) const {
+        if (!fast) return weight_of(clean(x), m, c, table);
+        return x > lo ? some(x, table) : 0.0;
+    }
+};
 
 // A row as a wave reads it: slices of 16 KB in 16-byte chunks, chunk j of a lane
 // the (64 j + lane)-th.
@@ -203,10 +272,10 @@ struct Row {
     __device__ __forceinline__ uint32_t bits(int e0) const {
         return mask != nullptr && e0 < V ? mask[e0 >> 5] >> (e0 & 31) : 0xFFFFFFFFu;
     }
-    // id k of a chunk: its logit, -inf where it is not allowed
-    __device__ __forceinline__ static float value(const u32x4& w, uint32_t bits, int k) {
+    // id k of a chunk: its logit, -inf where it is masked
+    __device__ __forceinline__ static float raw(const u32x4& w, uint32_t bits, int k) {
         const float x = BF ? __uint_as_float(k & 1 ? w[k / 2] & 0xFFFF0000u : w[k / 2] << 16) : __uint_as_float(w[k % 4]);
-        return (bits >> k & 1u) != 0 ? clean(x) : kNegInf;
+        return (bits >> k & 1u) != 0 ? x : kNegInf;
     }
 };
 
@@ -219,20 +288,36 @@ __device__ __forceinline__ Row<BF> draft_row(const DraftArgs& a, int row) {
     return Row<BF>::of(a.d.draft_logits, a.d.draft_stride, a.d.draft_mask, a.d.draft_mask_stride, row, a.d.vocab);
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// Sums and maxima over the wave by DPP (shifts within 16 lanes, then the rows' ends
+// carried on): lane 63 has the whole, and the inclusive sums are a scan's.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xF, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xF, false);
+    return __hiloint2double(hi, lo);
+}
+__device__ __forceinline__ double wave_incl_sum(double v) {
+    v += dpp_f64<0x111, 0xF>(v);
+    v += dpp_f64<0x112, 0xF>(v);
+    v += dpp_f64<0x114, 0xF>(v);
+    v += dpp_f64<0x118, 0xF>(v);
+    v += dpp_f64<0x142, 0xA>(v);
+    v += dpp_f64<0x143, 0xC>(v);
     return v;
 }
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane),
+                            __builtin_amdgcn_readlane(__double2loint(v), lane));
 }
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-    return v;
+__device__ __forceinline__ double wave_sum(double v) { return lane_f64(wave_incl_sum(v), 63); }
+__device__ __forceinline__ float wave_max(float v) {       // (of ordered bits: signed for positives, reversed below)
+    const int b = __float_as_int(v);
+    const uint32_t key = (uint32_t)(b ^ (b >> 31 & 0x7FFFFFFF)) ^ 0x80000000u;
+    const uint32_t top = wave_max_u32(key) ^ 0x80000000u;
+    return __int_as_float((int)top ^ ((int)top >> 31 & 0x7FFFFFFF));
+}
+__device__ __forceinline__ int wave_min(int v) {           // (of values >= 0)
+    return (int)wave_min_u32((uint32_t)v);
 }
 
 // A job is one row: position i of sequence b, the target's (side 0) or the
@@ -241,31 +326,29 @@ __device__ __forceinline__ int job_of(const DraftArgs& a, int b, int i, int side
     return i < a.d.max_draft ? (i * a.d.seqs + b) * a.sides + side : a.d.max_draft * a.d.seqs * a.sides + b;
 }
 
-struct RowSum {
-    float m;
-    int at;
-    double z;       // at the maximum; greedy rows 1; 0: nothing allowed
-};
-
-// One wave: a row's maximum and sum from its slices.
-__device__ __forceinline__ RowSum row_sum(const SliceStat* st, int S, double c, const double* table) {
+// One wave: a row's maximum and sum from its slices; `first`: lane's slice of the
+// first 64, loaded ahead.
+template <class F>
+__device__ __forceinline__ RowSum row_sum(F stat, SliceStat first, int S, double c, const double* table) {
     const int lane = threadIdx.x & 63;
-    float m = kNegInf;
-    double z = 0.0;
-    int at = INT32_MAX;
+    RowSum r{kNegInf, INT32_MAX, 0.0};
     for (int s0 = 0; s0 < S; s0 += 64) {
-        SliceStat v{__float_as_uint(kNegInf), INT32_MAX, 0.0};
-        if (s0 + lane < S) v = get_stat(st + s0 + lane);
-        const float vm = __uint_as_float(v.m), top = fmaxf(m, wave_max(vm));
+        if (s0 > 0) first = stat(s0 + lane);
+        const float vm = s0 + lane < S ? __uint_as_float(first.m) : kNegInf;
+        const double vs = s0 + lane < S ? first.s : 0.0;
+        const float top = fmaxf(r.m, wave_max(vm));
         if (c > 0.0) {
-            z = z * weight_of(m, top, c, table) + wave_sum(v.s * weight_of(vm, top, c, table));
+            const double old = s0 > 0 ? r.z * weight_of(r.m, top, c, table) : 0.0;
+            r.z = old + wave_sum(vs * weight_of(vm, top, c, table));
         } else {
-            const int here = wave_min(vm == top && v.s > 0.0 ? v.at : INT32_MAX);
-            at = top > m ? here : min(at, here);
+            const int here = wave_min(vm == top && vs > 0.0 ? first.at : INT32_MAX);
+            r.at = top > r.m ? here : min(r.at, here);
         }
-        m = top;
+        r.m = top;
     }
-    return RowSum{m, at, !(m > kNegInf) ? 0.0 : c > 0.0 ? z : 1.0};
+    if (!(r.m > kNegInf)) r.z = 0.0;
+    else if (c == 0.0) r.z = 1.0;
+    return r;
 }
 
 __global__ __launch_bounds__(kThreads) void k_draft_start(DraftArgs a) {
@@ -277,38 +360,182 @@ __global__ __launch_bounds__(kThreads) void k_draft_start(DraftArgs a) {
     }
 }
 
-// Draft i of sequence b, all slices of its rows known: one wave.
+// Draft i of sequence b, all slices of its rows known: one wave. False, and nothing
+// written: its u is within `margin` (of the larger side) of the border.
+constexpr double kUnsure = 1e-5;             // both rows' sums are off by at most 3e-6
 template <bool BF>
-__device__ __forceinline__ void decide(const DraftArgs& a, const Seq& q, int b, int i, const double* table) {
+__device__ __forceinline__ bool decide(const DraftArgs& a, const Seq& q, int b, int i, double margin, const double* table) {
+    const int lane = threadIdx.x & 63;
     const double cp = inv_temperature(a.d.temperature, b), cq = inv_temperature(a.d.draft_temperature, b);
+    const SliceStat* st = a.stats + (int64_t)job_of(a, b, i, 0) * a.S;     // (the drafter's row follows)
+    auto stat = [&](int s) { return get_stat(st + min(s, a.S * a.sides - 1)); };
+    auto stat_q = [&](int s) { return stat(a.S + s); };
+    // every load that does not wait for another first
+    const SliceStat fp = stat(lane), fq = stat_q(lane);
     const int tok = a.d.draft[q.d0 + i];
+    const double u = a.d.u_accept[q.d0 + i];
     const bool in = tok >= 0 && tok < a.d.vocab;
-    auto chance = [&](const RowSum& r, double c, const Row<BF>& row) {
+    const float xp = in ? target_row<BF>(a, q.t0 + i).at(tok) : kNegInf;
+    const float xq = in && a.sides == 2 ? draft_row<BF>(a, q.d0 + i).at(tok) : kNegInf;
+    auto chance = [&](const RowSum& r, double c, float x) {
         if (!in || !(r.z > 0.0)) return 0.0;
-        return c == 0.0 ? (tok == r.at ? 1.0 : 0.0) : weight_of(row.at(tok), r.m, c, table) / r.z;
+        return c == 0.0 ? (tok == r.at ? 1.0 : 0.0) : weight_of(x, r.m, c, table) / r.z;
     };
-    const double p = chance(row_sum(a.stats + (int64_t)job_of(a, b, i, 0) * a.S, a.S, cp, table), cp,
-                            target_row<BF>(a, q.t0 + i));
-    double qd = in ? 1.0 : 0.0;
-    if (a.sides == 2)
-        qd = chance(row_sum(a.stats + (int64_t)job_of(a, b, i, 1) * a.S, a.S, cq, table), cq, draft_row<BF>(a, q.d0 + i));
-    if ((threadIdx.x & 63) != 0) return;
-    if (!(a.d.u_accept[q.d0 + i] * qd < p))
-        __hip_atomic_fetch_min(&a.rejected[b], i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const RowSum rp = row_sum(stat, fp, a.S, cp, table);
+    RowSum rq{};
+    if (a.sides == 2) rq = row_sum(stat_q, fq, a.S, cq, table);
+    const double p = chance(rp, cp, xp);
+    const double qd = a.sides == 2 ? chance(rq, cq, xq) : in ? 1.0 : 0.0;
+    if (fabs(u * qd - p) < margin * fmax(u * qd, p)) return false;
+    if (lane != 0) return true;
+    RowSum* left = a.sums + (int64_t)(i * a.d.seqs + b) * a.sides;
+    left[0] = rp;
+    if (a.sides == 2) left[1] = rq;
+    if (!(u * qd < p)) __hip_atomic_fetch_min(&a.rejected[b], i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (a.d.accept_prob != nullptr) a.d.accept_prob[q.d0 + i] = p < qd ? (float)(p / qd) : p > 0.0 ? 1.0f : 0.0f;
+    return true;
 }
 
-template <bool BF, bool MASK>
-__global__ __launch_bounds__(kThreads) void k_draft_stats(DraftArgs a) {
+// One wave: slices s0 .. s1 - 1 of a row, each slice's statistics to to[s]. A step at
+// a time, the next one's loads in flight.
+//
+// FAST: exponentials in float (twice the rate of those in double, which bound the
+// pass: 2304 + 2048 bf16 rows of 151936 525 us against 230). A slice's sum is then off
+// by at most 3e-6 of it: per term 3 |z| 2^-24 from the exponent z = (x - m) / T and 2^-23
+// from exp2, where the terms' mean |z| is at most ln V < 17 (the entropy's bound);
+// 9 2^-24 from the float additions. Enough to decide most drafts (kUnsure below), not
+// to draw a token.
+template <bool BF, bool MASK, bool FAST>
+__device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, int s1, const double* table, SliceStat* to) {
+    using R = Row<BF>;
+    const int lane = threadIdx.x & 63;
+    struct Step {
+        u32x4 x[kStep];
+        uint32_t bits[MASK ? kStep : 1];
+    };
+    auto load = [&](Step& h, int n) {
+        const int e0 = n * (R::SLICE / kSteps) + lane * R::VEC;
+        if ((n + 1) * (R::SLICE / kSteps) <= r.V) {
+#pragma unroll
+            for (int j = 0; j < kStep; ++j) {
+                if (BF) h.x[j] = *reinterpret_cast<const u32x4_a2*>(static_cast<const uint16_t*>(r.row) + e0 + j * 64 * R::VEC);
+                else h.x[j] = *reinterpret_cast<const u32x4_a4*>(static_cast<const float*>(r.row) + e0 + j * 64 * R::VEC);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kStep; ++j) h.x[j] = r.chunk(e0 + j * 64 * R::VEC);
+        }
+        if (MASK)
+#pragma unroll
+            for (int j = 0; j < kStep; ++j) h.bits[MASK ? j : 0] = r.bits(e0 + j * 64 * R::VEC);
+    };
+    float m = kNegInf;       // of the slice so far
+    double sum = 0.0;        // the lane's, at m
+    int at = INT32_MAX;
+    auto add = [&](Step& h, int n) {
+        auto value = [&](int j, int k) { return R::raw(h.x[j], MASK ? h.bits[MASK ? j : 0] : 0xFFFFFFFFu, k); };
+        float top = kNegInf;
+#pragma unroll
+        for (int j = 0; j < kStep; ++j)
+#pragma unroll
+            for (int k = 0; k < R::VEC; ++k) top = fmaxf(top, value(j, k));
+        top = fminf(wave_max(top), kFltMax);
+        // (the values are unpacked again below: kept, they take twice the registers)
+#pragma unroll
+        for (int j = 0; j < kStep; ++j) asm volatile("" : "+v"(h.x[j]));
+        if (c == 0.0) {
+            if (!(top > m)) return;      // (the lowest id: the earlier step's)
+            int here = INT32_MAX;
+#pragma unroll
+            for (int j = 0; j < kStep; ++j)
+#pragma unroll
+                for (int k = 0; k < R::VEC; ++k)
+                    if (fminf(value(j, k), kFltMax) == top) here = min(here, n * (R::SLICE / kSteps) + (j * 64 + lane) * R::VEC + k);
+            at = wave_min(here);
+            m = top;
+            return;
+        }
+        if (top > m) {
+            sum *= weight_of(m, top, c, table);
+            m = top;
+        }
+        if (!(m > kNegInf)) return;
+        const double per2 = c * 0.03125;             // log2 e / T
+        const float flo = (float)((double)m - 160.0 / per2);
+        const double flow = ((double)m - (double)flo) * per2;
+        if (FAST && flo > -3e38f && flow > 150.0 && flow < 170.0) {
+            // float exponentials, the factor in two floats; logits clamped to flo, whose
+            // weight is 0 (not for the temperatures that Scale leaves out either); the
+            // lane's four at a time in float, then in double
+            const float ch = (float)per2, cl = (float)(per2 - (double)ch);
+            float part = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kStep; ++j)
+#pragma unroll
+                for (int k = 0; k < R::VEC; k += 4) {
+                    float v[4];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const float d = __builtin_amdgcn_fmed3f(value(j, k + n), flo, kFltMax) - m;
+                        v[n] = __builtin_amdgcn_exp2f(__builtin_fmaf(d, ch, d * cl));
+                    }
+                    part += (v[0] + v[1]) + (v[2] + v[3]);
+                }
+            sum += (double)part;
+            return;
+        }
+        const Scale e(m, c);
+        if (e.fast) {
+            // (what is not allowed adds 2^-1000 here)
+#pragma unroll
+            for (int j = 0; j < kStep; ++j)
+#pragma unroll
+                for (int k = 0; k < R::VEC; k += 4) {
+                    float x[4];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) x[n] = value(j, k + n);
+                    double v[4];
+                    e.some(x, table, v);
+                    sum += (v[0] + v[1]) + (v[2] + v[3]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        } else {
+#pragma nounroll
+            for (int j = 0; j < kStep * R::VEC; ++j) {
+                const int id = n * (R::SLICE / kSteps) + j * 64 + lane;
+                if (id < r.V) sum += weight_of(r.at(id), m, c, table);
+            }
+        }
+    };
+    Step h0, h1;
+    if (s0 < s1) load(h0, kSteps * s0);
+    for (int s = s0; s < s1; ++s) {
+        for (int n = kSteps * s; n < kSteps * (s + 1); n += 2) {
+            load(h1, n + 1);
+            add(h0, n);
+            load(h0, min(n + 2, kSteps * s1 - 2));
+            add(h1, n + 1);
+        }
+        const double z = wave_sum(sum);
+        if (lane == 0)
+            put_stat(to + s,
+                     SliceStat{__float_as_uint(m), at, !(m > kNegInf) ? 0.0 : c > 0.0 ? z : 1.0});
+        m = kNegInf;
+        sum = 0.0;
+        at = INT32_MAX;
+    }
+}
+
+template <bool BF, bool MASK, bool FAST>
+__global__ __launch_bounds__(kThreads, 4) void k_draft_stats(DraftArgs a) {
     using R = Row<BF>;
     __shared__ double table[32];
-    load_table(table);
-    const int lane = threadIdx.x & 63;
-    const int groups = (a.S + a.per - 1) / a.per;        // waves per row
-    const int w = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
-    const int job = w / groups, s0 = w % groups * a.per, s1 = min(a.S, s0 + a.per);
+    __shared__ int32_t shared;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int take = a.per * kWaves, groups = (a.S + take - 1) / take;       // slices per block, blocks per row
+    const int job = blockIdx.x / groups, b0 = blockIdx.x % groups * take;
+    const int s0 = min(a.S, b0 + wave * a.per), s1 = min(a.S, s0 + a.per);
     const int drafted = a.d.max_draft * a.d.seqs * a.sides;
-    if (job >= drafted + a.d.seqs) return;
     const int side = job < drafted ? job % a.sides : 0;
     const int i = job < drafted ? job / a.sides / a.d.seqs : a.d.max_draft;
     const int b = job < drafted ? job / a.sides % a.d.seqs : job - drafted;
@@ -317,96 +544,114 @@ __global__ __launch_bounds__(kThreads) void k_draft_stats(DraftArgs a) {
     // max_draft for every sequence
     const int pos = job < drafted ? i : q.n;
     if (!q.ok || (job < drafted && i >= q.n)) return;
-    if (pos > 0 && get(&a.rejected[b]) < pos) return;
+    if (threadIdx.x == 0) shared = pos > 0 ? get(&a.rejected[b]) : INT32_MAX;
+    load_table(table);
+    if (shared < pos) return;
     const R r = side == 0 ? target_row<BF>(a, q.t0 + pos) : draft_row<BF>(a, q.d0 + pos);
     const double c = inv_temperature(side == 0 ? a.d.temperature : a.d.draft_temperature, b);
-    for (int s = s0; s < s1; ++s) {
-        const int e0 = s * R::SLICE + lane * R::VEC;
-        u32x4 x[kChunks];
-        uint32_t bits[MASK ? kChunks : 1];
-        if ((s + 1) * R::SLICE <= a.d.vocab) {
-#pragma unroll
-            for (int j = 0; j < kChunks; ++j) {
-                if (BF) x[j] = *reinterpret_cast<const u32x4_a2*>(static_cast<const uint16_t*>(r.row) + e0 + j * 64 * R::VEC);
-                else x[j] = *reinterpret_cast<const u32x4_a4*>(static_cast<const float*>(r.row) + e0 + j * 64 * R::VEC);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < kChunks; ++j) x[j] = r.chunk(e0 + j * 64 * R::VEC);
-        }
-        if (MASK)
-#pragma unroll
-            for (int j = 0; j < kChunks; ++j) bits[MASK ? j : 0] = r.bits(e0 + j * 64 * R::VEC);
-        auto value = [&](int j, int k) { return R::value(x[j], MASK ? bits[MASK ? j : 0] : 0xFFFFFFFFu, k); };
-        float m = kNegInf;
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-            for (int k = 0; k < R::VEC; ++k) m = fmaxf(m, value(j, k));
-        m = wave_max(m);
-        // (the values are unpacked again below: kept, they take twice the registers)
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j) asm volatile("" : "+v"(x[j]));
-        SliceStat st{__float_as_uint(m), INT32_MAX, 0.0};
-        if (m > kNegInf) {
-            if (c > 0.0) {
-                // (what is not allowed adds 2^-1000 here)
-                double sum = 0.0;
-                const double md = m;
-#pragma unroll
-                for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-                    for (int k = 0; k < R::VEC; ++k) sum += exp32(((double)value(j, k) - md) * c, table);
-                st.s = wave_sum(sum);
-            } else {
-                int at = INT32_MAX;
-#pragma unroll
-                for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-                    for (int k = 0; k < R::VEC; ++k)
-                        if (value(j, k) == m) at = min(at, e0 + j * 64 * R::VEC + k);
-                st.at = wave_min(at);
-                st.s = 1.0;
-            }
-        }
-        if (lane == 0) put_stat(a.stats + (int64_t)job * a.S + s, st);
+    row_slices<BF, MASK, FAST>(r, c, s0, s1, table, a.stats + (int64_t)job * a.S);
+    if (job >= drafted || !completes(a.count + i * a.d.seqs + b, min(take, a.S - b0), a.sides * a.S, &shared)) return;
+    __shared__ int32_t unsure;
+    if (wave == 0) {
+        const bool far = decide<BF>(a, q, b, i, FAST ? kUnsure : 0.0, table);
+        if (lane == 0) unsure = far ? 0 : 1;
     }
-    if (job < drafted && completes(a.count + i * a.d.seqs + b, s1 - s0, a.sides * a.S)) decide<BF>(a, q, b, i, table);
+    if (!FAST) return;
+    __syncthreads();
+    if (unsure == 0) return;
+    // too near to tell (once in 50 000 drafts): both rows again in double
+    for (int sd = 0; sd < a.sides; ++sd) {
+        const R row = sd == 0 ? target_row<BF>(a, q.t0 + i) : draft_row<BF>(a, q.d0 + i);
+        const double cs = inv_temperature(sd == 0 ? a.d.temperature : a.d.draft_temperature, b);
+        const int each = (a.S + kWaves - 1) / kWaves, from = min(a.S, wave * each);
+        row_slices<BF, MASK, false>(row, cs, from, min(a.S, from + each), table, a.stats + (int64_t)job_of(a, b, i, sd) * a.S);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (wave == 0) decide<BF>(a, q, b, i, 0.0, table);
 }
 
-// The weights of a chunk's ids: max(p - q, 0), or p; q on the drafter's row or on
-// one id.
+// FAST calls: the emitting rows' slices in double. (Greedy rows need none.)
+template <bool BF, bool MASK>
+__global__ __launch_bounds__(kThreads, 4) void k_draft_exact(DraftArgs a) {
+    __shared__ double table[32];
+    load_table(table);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int groups = (a.S + kWaves - 1) / kWaves;
+    const int row = blockIdx.x / groups, s0 = blockIdx.x % groups * kWaves + wave;
+    const int b = row / a.sides, side = row % a.sides;
+    const Seq q = seq_of(a, b);
+    if (!q.ok || s0 >= a.S) return;
+    const int m = min(a.rejected[b], q.n);
+    const double cp = inv_temperature(a.d.temperature, b), cq = inv_temperature(a.d.draft_temperature, b);
+    if (cp == 0.0 || (side == 1 && (m == q.n || cq == 0.0))) return;
+    const Row<BF> r = side == 0 ? target_row<BF>(a, q.t0 + m) : draft_row<BF>(a, q.d0 + m);
+    row_slices<BF, MASK, false>(r, side == 0 ? cp : cq, s0, s0 + 1, table,
+                                a.stats + (int64_t)job_of(a, b, m < q.n ? m : a.d.max_draft, side) * a.S);
+}
+
+// The weights of a chunk's ids, in units of 1 / the target's Z: max(p - q, 0), or p;
+// q on the drafter's row or on one id.
 template <bool BF>
 struct Weights {
     using R = Row<BF>;
     R p, q;
-    RowSum sp, sq;
-    double cp, cq;
+    Scale ep, eq;
+    double share;       // Z of the target over Z of the drafter
     int point;
     bool two;
-    __device__ __forceinline__ void load(int e0, const double* table, double (&w)[R::VEC]) const {
-        const u32x4 x = p.chunk(e0);
-        u32x4 y = x;
-        if (two) y = q.chunk(e0);
-        const uint32_t bx = p.bits(e0), by = two ? q.bits(e0) : 0u;
+    struct Chunk {
+        u32x4 x, y;
+        uint32_t bx, by;
+        __device__ __forceinline__ void load(const R& p, const R& q, bool two, int e0) {
+            x = y = p.chunk(e0);
+            bx = by = p.bits(e0);
+            if (two) {
+                y = q.chunk(e0);
+                by = q.bits(e0);
+            }
+        }
+    };
+    __device__ __forceinline__ Chunk load(int e0) const {
+        Chunk c;
+        c.load(p, q, two, e0);
+        return c;
+    }
+    // a chunk's weights
+    __device__ __forceinline__ void all(const Chunk& c, int e0, const double* table, double (&w)[R::VEC]) const {
+        if (!ep.fast || !eq.fast) {
 #pragma unroll
-        for (int k = 0; k < R::VEC; ++k) {
-            w[k] = weight_of(R::value(x, bx, k), sp.m, cp, table) / sp.z;
-            if (two) w[k] = fmax(w[k] - weight_of(R::value(y, by, k), sq.m, cq, table) / sq.z, 0.0);
-            if (e0 + k == point) w[k] = 0.0;
+            for (int k = 0; k < R::VEC; ++k) w[k] = of(c, e0, k, table);
+            return;
+        }
+#pragma unroll
+        for (int k0 = 0; k0 < R::VEC; k0 += 4) {
+            float x[4];
+            double v[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) x[n] = R::raw(c.x, c.bx, k0 + n);
+            ep.some(x, table, v);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) v[n] = x[n] > ep.lo ? v[n] : 0.0;
+            if (two) {
+                float y[4];
+                double q[4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) y[n] = R::raw(c.y, c.by, k0 + n);
+                eq.some(y, table, q);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) v[n] = fmax(__builtin_fma(-share, y[n] > eq.lo ? q[n] : 0.0, v[n]), 0.0);
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) w[k0 + n] = e0 + k0 + n == point ? 0.0 : v[n];
         }
     }
-};
-
-__device__ __forceinline__ double wave_incl_sum(double v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double t = __shfl_up(v, o, 64);
-        if (lane >= o) v += t;
+    __device__ __forceinline__ double of(const Chunk& c, int e0, int k, const double* table) const {
+        double w = ep.of(R::raw(c.x, c.bx, k), table);
+        if (two) w = fmax(__builtin_fma(-share, eq.of(R::raw(c.y, c.by, k), table), w), 0.0);
+        return e0 + k == point ? 0.0 : w;
     }
-    return v;
-}
+};
 
 // One wave: the first of n values above 0 where the running sum (from `base`)
 // reaches `want`, else the last above 0 (-1: none); `before`: the sum before it.
@@ -423,134 +668,175 @@ __device__ __forceinline__ int first_reaching(F value, int n, double base, doubl
         const int at = hit != 0 ? __ffsll((long long)hit) - 1 : some != 0 ? 63 - __clzll((long long)some) : -1;
         if (at >= 0) {
             last = s0 + at;
-            last_before = __shfl(c - v, at, 64);
+            last_before = lane_f64(c - v, at);
         }
         if (hit != 0) break;
-        run = __shfl(c, 63, 64);
+        run = lane_f64(c, 63);
     }
     before = last_before;
     return last;
 }
 
 template <bool BF>
-__global__ __launch_bounds__(kThreads) void k_draft_draw(DraftArgs a) {
+__global__ __launch_bounds__(kDrawThreads) void k_draft_draw(DraftArgs a) {
     using R = Row<BF>;
     __shared__ double table[32];
+    __shared__ int32_t shared;
     load_table(table);
-    const int lane = threadIdx.x & 63, S = a.S, K = a.d.max_draft;
-    const int wv = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
-    const int b = wv / S, slice = wv % S;
-    if (b >= a.d.seqs) return;
+    constexpr int PART = R::SLICE / kParts, CH = kChunks / kParts;       // ids and chunks of a lane per part
+    const int lane = threadIdx.x & 63, S = a.S, P = a.S * kParts, K = a.d.max_draft;
+    constexpr int NW = kDrawThreads / 64;
+    const int groups = (P + NW - 1) / NW;
+    const int b = blockIdx.x / groups, first = blockIdx.x % groups * NW;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = first + wave;
     const Seq q = seq_of(a, b);
     int32_t* out = a.d.out_tokens + (int64_t)b * (K + 1);
     const int m = q.ok ? min(a.rejected[b], q.n) : 0;
-    if (slice == 0) {
+    if (part == 0) {
         // all but the drawn token
         for (int i = lane; i <= K; i += 64)
             if (i != m) out[i] = q.ok && i < m ? a.d.draft[q.d0 + i] : -1;
         if (q.ok && a.d.accept_prob != nullptr)
             for (int i = m + 1 + lane; i < q.n; i += 64) a.d.accept_prob[q.d0 + i] = -1.0f;
     }
-    Weights<BF> w;
-    w.cp = inv_temperature(a.d.temperature, b);
-    w.cq = inv_temperature(a.d.draft_temperature, b);
-    const SliceStat* st = a.stats + (int64_t)job_of(a, b, m < q.n ? m : K, 0) * S;
-    if (q.ok) w.sp = row_sum(st, S, w.cp, table);
-    if (!q.ok || !(w.sp.z > 0.0) || w.cp == 0.0) {
+    const double cp = inv_temperature(a.d.temperature, b), cq = inv_temperature(a.d.draft_temperature, b);
+    // a rejected position's rows, their loads ahead of everything else
+    const bool reject = q.ok && m < q.n, drafter = reject && a.sides == 2;
+    Row<BF> pr{}, qr{};
+    if (q.ok) pr = qr = target_row<BF>(a, q.t0 + m);
+    if (drafter) qr = draft_row<BF>(a, q.d0 + m);
+    typename Weights<BF>::Chunk c[CH];
+    if (reject && cp > 0.0)
+#pragma unroll
+        for (int j = 0; j < CH; ++j) c[j].load(pr, qr, drafter, part * PART + (j * 64 + lane) * R::VEC);
+    RowSum sp{kNegInf, INT32_MAX, 0.0}, sq = sp;
+    const SliceStat* st = a.stats + (int64_t)job_of(a, b, K, 0) * S;      // of the row after the last draft
+    if (reject) {
+        st = a.stats + (int64_t)job_of(a, b, m, 0) * S;                   // (the drafter's row follows)
+    }
+    if (reject && !a.fast) {
+        const RowSum* left = a.sums + (int64_t)(m * a.d.seqs + b) * a.sides;
+        sp = left[0];
+        if (drafter) sq = left[1];
+    } else if (q.ok) {
+        auto stat = [&](int s) { return st[min(s, S - 1)]; };
+        auto stat_q = [&](int s) { return st[S + min(s, S - 1)]; };
+        const SliceStat fp = stat(lane), fq = drafter ? stat_q(lane) : fp;
+        sp = row_sum(stat, fp, S, cp, table);
+        if (drafter) sq = row_sum(stat_q, fq, S, cq, table);
+    }
+    if (!(sp.z > 0.0) || cp == 0.0) {
         // no token, or a greedy one: max(p - q, 0) is 0 but there, and p is all there
-        const bool some = q.ok && w.sp.z > 0.0;
-        if (slice == 0 && lane == 0) {
-            out[m] = some ? w.sp.at : -1;
+        const bool some = sp.z > 0.0;
+        if (part == 0 && lane == 0) {
+            out[m] = some ? sp.at : -1;
             a.d.out_count[b] = m + (some ? 1 : 0);
         }
         return;
     }
-    w.point = -1;
-    w.two = false;
-    w.p = w.q = target_row<BF>(a, q.t0 + m);
-    w.sq = w.sp;
-    if (m < q.n) {
-        if (a.sides == 1) w.point = a.d.draft[q.d0 + m];
-        else {
-            w.sq = row_sum(a.stats + (int64_t)job_of(a, b, m, 1) * S, S, w.cq, table);
-            if (w.sq.z > 0.0 && w.cq == 0.0) w.point = w.sq.at;
-            w.two = w.sq.z > 0.0 && w.cq > 0.0;
-            if (w.two) w.q = draft_row<BF>(a, q.d0 + m);
-        }
-    }
-    auto p_slice = [&](int s) {
-        const SliceStat v = get_stat(st + s);
-        return v.s * weight_of(__uint_as_float(v.m), w.sp.m, w.cp, table) / w.sp.z;
-    };
+    const bool two = drafter && sq.z > 0.0 && cq > 0.0;
+    Weights<BF> w{pr, qr, Scale(sp.m, cp), Scale(two ? sq.m : sp.m, two ? cq : cp), two ? sp.z / sq.z : 0.0, -1, two};
+    if (reject && a.sides == 1) w.point = a.d.draft[q.d0 + m];
+    else if (drafter && sq.z > 0.0 && !two) w.point = sq.at;
     // where the weights are p's, the slices' sums are known
-    bool whole = !w.two && w.point < 0;
-    double* rs = a.rsum + (int64_t)b * S;
+    bool whole = !two && w.point < 0;
+    double* rs = a.rsum + (int64_t)b * P;
     if (!whole) {
         double s = 0.0;
-#pragma unroll 4
-        for (int j = 0; j < kChunks; ++j) {
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
             double v[R::VEC];
-            w.load(slice * R::SLICE + (j * 64 + lane) * R::VEC, table, v);
+            w.all(c[j], part * PART + (j * 64 + lane) * R::VEC, table, v);
 #pragma unroll
             for (int k = 0; k < R::VEC; ++k) s += v[k];
         }
         s = wave_sum(s);
-        if (lane == 0) put(reinterpret_cast<u64*>(rs + slice), (u64)__double_as_longlong(s));
-        if (!completes(&a.drawn[b], 1, S)) return;
-    } else if (slice != 0) {
+        if (lane == 0 && part < P) put(reinterpret_cast<u64*>(rs + part), (u64)__double_as_longlong(s));
+        if (!completes(&a.drawn[b], min(NW, P - first), P, &shared)) return;
+    } else if (first != 0) {
         return;
     }
-    double total = whole ? 1.0 : 0.0;
+    // one block of the sequence is left
+    auto r_part = [&](int s) { return __longlong_as_double((long long)get(reinterpret_cast<const u64*>(rs + s))); };
+    auto p_slice = [&](int s) { return st[s].s * weight_of(__uint_as_float(st[s].m), sp.m, cp, table); };
+    // the first parts' sums, a few a lane, loaded once
+    constexpr int HELD = 4;
+    double held[HELD] = {}, total = 0.0;
     if (!whole) {
-        for (int s = lane; s < S; s += 64) total += __longlong_as_double((long long)get(reinterpret_cast<const u64*>(rs + s)));
+#pragma unroll
+        for (int n = 0; n < HELD; ++n) held[n] = n * 64 + lane < P ? r_part(n * 64 + lane) : 0.0;
+#pragma unroll
+        for (int n = 0; n < HELD; ++n) total += held[n];
+        for (int n = HELD * 64 + lane; n < P; n += 64) total += r_part(n);
         total = wave_sum(total);
-        if (!(total > 0.0)) {        // p = q to the last bit: the weights are p's
-            whole = true;
-            w.two = false;
-            w.point = -1;
-            total = 1.0;
-        }
+    }
+    if (!(total > 0.0)) {        // p's weights; also where p = q to the last bit
+        whole = true;
+        w.two = false;
+        w.point = -1;
+        total = sp.z;
     }
     const double want = a.d.u_draw[b] * total;
-    double before;
-    const int at = max(0, first_reaching(
-                              [&](int s) {
-                                  return whole ? p_slice(s)
-                                               : __longlong_as_double((long long)get(reinterpret_cast<const u64*>(rs + s)));
-                              },
-                              S, 0.0, want, before));
-    // the slice's 64-chunk lines in id order, then the chunk, then the id
-    int chunk = 0;
-    double run = before;
-    for (int j = 0; j < kChunks; ++j) {
-        double v[R::VEC], s = 0.0;
-        w.load(at * R::SLICE + (j * 64 + lane) * R::VEC, table, v);
+    double run;
+    auto r_held = [&](int s) {
+        const int n = s >> 6;
+        return n == 0 ? held[0] : n == 1 ? held[1] : n == 2 ? held[2] : n == 3 ? held[3] : r_part(s);
+    };
+    // the part: of the parts' sums, or of the slice's that the known sums lead to
+    int at;
+    if (whole) {
+        const int slice = max(0, first_reaching(p_slice, S, 0.0, want, run));
+        __shared__ double sums[kParts];
+        if (wave < kParts) {
+            double v = 0.0;
 #pragma unroll
-        for (int k = 0; k < R::VEC; ++k) s += v[k];
-        const double c = run + wave_incl_sum(s);
-        const u64 hit = __ballot(s > 0.0 && c >= want), some = __ballot(s > 0.0);
-        const int l = hit != 0 ? __ffsll((long long)hit) - 1 : some != 0 ? 63 - __clzll((long long)some) : -1;
-        if (l >= 0) {
-            chunk = j * 64 + l;
-            before = __shfl(c - s, l, 64);
-        }
-        if (hit != 0) break;
-        run = __shfl(c, 63, 64);
-    }
-    double v[R::VEC], c = before;
-    w.load(at * R::SLICE + chunk * R::VEC, table, v);
-    int found = 0;
-    bool done = false;
+            for (int j = 0; j < CH; ++j) c[j] = w.load((slice * kParts + wave) * PART + (j * 64 + lane) * R::VEC);
 #pragma unroll
-    for (int k = 0; k < R::VEC; ++k) {
-        c += v[k];
-        if (!done && v[k] > 0.0) {
-            found = k;
-            done = c >= want;
+            for (int j = 0; j < CH; ++j) {
+                double x[R::VEC];
+                w.all(c[j], (slice * kParts + wave) * PART + (j * 64 + lane) * R::VEC, table, x);
+#pragma unroll
+                for (int k = 0; k < R::VEC; ++k) v += x[k];
+            }
+            v = wave_sum(v);
+            if (lane == 0) sums[wave] = v;
+        }
+        __syncthreads();
+        at = slice * kParts + max(0, first_reaching([&](int n) { return sums[n]; }, kParts, run, want, run));
+    } else {
+        at = max(0, first_reaching(r_held, P, 0.0, want, run));
+    }
+    if (wave != 0) return;
+    // the part again, each lane CH chunks in a row: the lane, then the id among its
+    // weights, a lane each
+    constexpr int IDS = CH * R::VEC;
+    static_assert(IDS <= 64);
+    __shared__ double weights[64][IDS + 1];
+    const int e0 = at * PART + lane * IDS;
+    double s = 0.0;
+#pragma unroll
+    for (int j = 0; j < CH; ++j) c[j] = w.load(e0 + j * R::VEC);
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+        double v[R::VEC];
+        w.all(c[j], e0 + j * R::VEC, table, v);
+#pragma unroll
+        for (int k = 0; k < R::VEC; ++k) {
+            weights[lane][j * R::VEC + k] = v[k];
+            s += v[k];
         }
     }
+    const double cum = run + wave_incl_sum(s);
+    const u64 hit = __ballot(s > 0.0 && cum >= want), some = __ballot(s > 0.0);
+    const int l = hit != 0 ? __ffsll((long long)hit) - 1 : some != 0 ? 63 - __clzll((long long)some) : 0;
+    run = lane_f64(cum - s, l);
+    __builtin_amdgcn_wave_barrier();
+    const double mine = lane < IDS ? weights[l][lane] : 0.0;
+    const double sum = run + wave_incl_sum(mine);
+    const u64 reach = __ballot(mine > 0.0 && sum >= want), any = __ballot(mine > 0.0);
+    const int id = reach != 0 ? __ffsll((long long)reach) - 1 : any != 0 ? 63 - __clzll((long long)any) : 0;
     if (lane == 0) {
-        out[m] = at * R::SLICE + chunk * R::VEC + found;
+        out[m] = at * PART + l * IDS + id;
         a.d.out_count[b] = m + 1;
     }
 }
@@ -559,28 +845,59 @@ __global__ __launch_bounds__(kThreads) void k_draft_draw(DraftArgs a) {
 
 __device__ __forceinline__ double set_prob(float p) { return p > 0.0f ? (double)p : 0.0; }
 
-// The place of id among n ascending ids, -1: not among them.
-__device__ __forceinline__ int find_id(const int32_t* ids, int n, int id) {
-    int lo = 0, hi = n;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (ids[mid] < id) lo = mid + 1;
-        else hi = mid;
+// One wave: the places of id among the ascending ids of both sets, -1: not among
+// them. Each step reads 64 of a set's ids, evenly spread over what is left, and both
+// sets' reads are in flight together.
+__device__ __forceinline__ void find_id(const int32_t* const (&ids)[2], int (&n)[2], int id, int (&at)[2]) {
+    const int lane = threadIdx.x & 63;
+    int from[2] = {};
+    while (n[0] > 64 || n[1] > 64) {
+        int piece[2], v[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            // the ends of pieces of n / 64 ids, rounded up
+            piece[s] = (n[s] + 63) >> 6;
+            v[s] = n[s] > 64 ? ids[s][from[s] + min(n[s], (lane + 1) * piece[s]) - 1] : id;
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int skip = min(n[s], __popcll(__ballot(v[s] < id)) * piece[s]);      // pieces wholly below id
+            from[s] += skip;
+            n[s] = n[s] > 64 ? min(piece[s], n[s] - skip) : n[s];
+        }
     }
-    return lo < n && ids[lo] == id ? lo : -1;
+    int v[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) v[s] = lane < n[s] ? ids[s][from[s] + lane] : 0;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const u64 hit = __ballot(lane < n[s] && v[s] == id);
+        at[s] = hit != 0 ? from[s] + __ffsll((long long)hit) - 1 : -1;
+    }
 }
 
-// One block per sequence.
-__global__ __launch_bounds__(kThreads) void k_verify_sets(ultima_hsamp_draft_sets d) {
-    __shared__ int lm[kThreads / 64];
-    __shared__ double sums[kThreads];
-    const int b = blockIdx.x, tid = threadIdx.x, K = d.max_draft;
+constexpr int kEach = 8;       // entries of a thread per tile
+constexpr int kTiles = ULTIMA_HSAMP_MAX_VOCAB / (1024 * kEach);
+
+// One block per sequence. The drafts' probabilities by a wave per position; then the
+// emitting set in tiles of eight entries per thread, the drafter's entries of the
+// tile's ids through LDS, where each entry of the target's looks for its own.
+template <int TH>
+__global__ __launch_bounds__(TH) void k_verify_sets(ultima_hsamp_draft_sets d) {
+    constexpr int TILE = TH * kEach, NW = TH / 64, NT = TH == 1024 ? kTiles : 1;
+    __shared__ int32_t lq[TILE];
+    __shared__ float lp[TILE];
+    __shared__ double tiles[NT], waves[NW];
+    __shared__ int32_t starts[NT], first;
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, K = d.max_draft;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Seq q = seq_of(d.n_draft, d.target_start, d.draft_start, b, K, d.rows, d.draft_rows);
     int32_t* out = d.out_tokens + (int64_t)b * (K + 1);
     const bool certain = d.draft_idx == nullptr;
+    if (tid == 0) first = INT32_MAX;
     bool bad = !q.ok;
     if (!bad)
-        for (int i = tid; i <= q.n; i += kThreads) {
+        for (int i = tid; i <= q.n; i += TH) {
             const int cp = d.kept_count[q.t0 + i];
             bad = bad || cp < 0 || cp > d.set_cap;
             if (!certain && i < q.n) {
@@ -589,93 +906,187 @@ __global__ __launch_bounds__(kThreads) void k_verify_sets(ultima_hsamp_draft_set
             }
         }
     if (__syncthreads_or(bad)) {
-        for (int i = tid; i <= K; i += kThreads) out[i] = -1;
+        for (int i = tid; i <= K; i += TH) out[i] = -1;
         if (tid == 0) d.out_count[b] = 0;
         return;
     }
-    int m = q.n;
-    for (int i = tid; i < q.n; i += kThreads) {
+    for (int i = wave; i < q.n; i += NW) {
         const int tok = d.draft[q.d0 + i];
+        const double u = d.u_accept[q.d0 + i];
         const int64_t tr = (int64_t)(q.t0 + i) * d.set_cap, dr = (int64_t)(q.d0 + i) * d.draft_cap;
-        const int at = find_id(d.kept_idx + tr, d.kept_count[q.t0 + i], tok);
-        const double p = at >= 0 ? set_prob(d.kept_prob[tr + at]) : 0.0;
-        double qq = 1.0;
-        if (!certain) {
-            const int aq = find_id(d.draft_idx + dr, d.draft_count[q.d0 + i], tok);
-            qq = aq >= 0 ? set_prob(d.draft_prob[dr + aq]) : 0.0;
+        const int32_t* const ids[2] = {d.kept_idx + tr, certain ? d.kept_idx : d.draft_idx + dr};
+        int n[2] = {d.kept_count[q.t0 + i], certain ? 0 : d.draft_count[q.d0 + i]}, at[2];
+        find_id(ids, n, tok, at);
+        const double p = at[0] >= 0 ? set_prob(d.kept_prob[tr + at[0]]) : 0.0;
+        const double qd = certain ? 1.0 : at[1] >= 0 ? set_prob(d.draft_prob[dr + at[1]]) : 0.0;
+        if (lane == 0) {
+            if (!(u * qd < p)) atomicMin(&first, i);
+            if (d.accept_prob != nullptr) d.accept_prob[q.d0 + i] = p < qd ? (float)(p / qd) : p > 0.0 ? 1.0f : 0.0f;
         }
-        if (!(d.u_accept[q.d0 + i] * qq < p)) m = min(m, i);
-        if (d.accept_prob != nullptr) d.accept_prob[q.d0 + i] = p < qq ? (float)(p / qq) : p > 0.0 ? 1.0f : 0.0f;
     }
-    m = wave_min(m);
-    if ((tid & 63) == 0) lm[tid >> 6] = m;
     __syncthreads();
-    for (int w = 0; w < kThreads / 64; ++w) m = min(m, lm[w]);
+    const int m = min(first, q.n);
     if (d.accept_prob != nullptr)
-        for (int i = tid; i < q.n; i += kThreads)
-            if (i > m) d.accept_prob[q.d0 + i] = -1.0f;
-    // the emitting set: each thread a run of its entries
+        for (int i = m + 1 + tid; i < q.n; i += TH) d.accept_prob[q.d0 + i] = -1.0f;
+    for (int i = tid; i <= K; i += TH)
+        if (i != m) out[i] = i < m ? d.draft[q.d0 + i] : -1;
     const int n = d.kept_count[q.t0 + m];
     const int32_t* pi = d.kept_idx + (int64_t)(q.t0 + m) * d.set_cap;
     const float* pp = d.kept_prob + (int64_t)(q.t0 + m) * d.set_cap;
-    const bool reject = m < q.n;
+    const bool reject = m < q.n, two = reject && !certain;
     const int point = reject && certain ? d.draft[q.d0 + m] : -1;
-    const bool two = reject && !certain;
-    const int64_t dr = two ? (int64_t)(q.d0 + m) * d.draft_cap : 0;
+    const int32_t* qi = two ? d.draft_idx + (int64_t)(q.d0 + m) * d.draft_cap : nullptr;
+    const float* qp = two ? d.draft_prob + (int64_t)(q.d0 + m) * d.draft_cap : nullptr;
     const int nq = two ? d.draft_count[q.d0 + m] : 0;
-    bool residual = true;
-    auto weight = [&](int k) {
-        double w = set_prob(pp[k]);
-        if (!residual) return w;
-        const int id = pi[k];
-        if (reject && certain && id == point) return 0.0;
-        if (two) {
-            const int at = find_id(d.draft_idx + dr, nq, id);
-            if (at >= 0) w = fmax(w - set_prob(d.draft_prob[dr + at]), 0.0);
+
+    // A tile's weights, the thread's eight consecutive entries; q0: the drafter's
+    // first entry that may matter, left at the first that may for the next tile.
+    int id[kEach];
+    double w[kEach];
+    auto tile = [&](int t, int& q0, bool residual) {
+        const int e0 = t * TILE + tid * kEach;
+        if (e0 + kEach <= n) {
+#pragma unroll
+            for (int k = 0; k < kEach; k += 4) {
+                const u32x4 i4 = *reinterpret_cast<const u32x4_a4*>(pi + e0 + k);
+                const u32x4 p4 = *reinterpret_cast<const u32x4_a4*>(pp + e0 + k);
+#pragma unroll
+                for (int f = 0; f < 4; ++f) {
+                    id[k + f] = (int)i4[f];
+                    w[k + f] = set_prob(__uint_as_float(p4[f]));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                const int e = min(e0 + k, n - 1);
+                id[k] = pi[e];
+                w[k] = e0 + k < n ? set_prob(pp[e]) : 0.0;
+            }
         }
-        return w;
+        if (residual && reject && certain)
+#pragma unroll
+            for (int k = 0; k < kEach; ++k)
+                if (id[k] == point) w[k] = 0.0;
+        if (!residual || !two) return;
+        const int last = pi[min(t * TILE + TILE, n) - 1];
+        for (;;) {
+            const int c = min(TILE, nq - q0);
+            if (c <= 0) break;
+            __syncthreads();
+            for (int k = tid; k < c; k += TH) {
+                lq[k] = qi[q0 + k];
+                lp[k] = qp[q0 + k];
+            }
+            __syncthreads();
+            // the number of the drafter's ids below each entry: of the first and the
+            // last in step, then of those between within these bounds
+            int lo[kEach] = {};
+            for (int half = TILE; half > 0; half >>= 1)
+#pragma unroll
+                for (int k = 0; k < kEach; k += kEach - 1) {
+                    const int mid = lo[k] + half;
+                    if (mid <= c && lq[mid - 1] < id[k]) lo[k] = mid;
+                }
+            const int span = lo[kEach - 1] - lo[0];
+#pragma unroll
+            for (int k = 1; k < kEach - 1; ++k) lo[k] = lo[0];
+            for (int half = span > 0 ? 1 << (31 - __clz(span)) : 0; __any(half > 0); half >>= 1)
+#pragma unroll
+                for (int k = 1; k < kEach - 1; ++k) {
+                    const int mid = lo[k] + half;
+                    if (half > 0 && mid <= lo[kEach - 1] && lq[mid - 1] < id[k]) lo[k] = mid;
+                }
+#pragma unroll
+            for (int k = 0; k < kEach; ++k)
+                if (lo[k] < c && lq[lo[k]] == id[k]) w[k] = fmax(w[k] - set_prob(lp[lo[k]]), 0.0);
+            if (lq[c - 1] >= last) break;          // (what follows is beyond the tile)
+            q0 += c;
+        }
     };
-    const int run = (n + kThreads - 1) / kThreads;
-    const int from = min(n, tid * run), to = min(n, from + run);
-    double total = 0.0;
-    for (int pass = 0; pass < 2; ++pass) {
+    const int T = (n + TILE - 1) / TILE;
+    auto tile_sum = [&]() {
         double s = 0.0;
-        for (int k = from; k < to; ++k) s += weight(k);
-        __syncthreads();
-        sums[tid] = s;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) s += w[k];
+        return s;
+    };
+    bool residual = true;
+    double total = 0.0;
+    for (int pass = 0; pass < 2 && n > 0; ++pass) {
+        int q0 = 0;
+        for (int t = 0; t < T; ++t) {
+            const int begin = q0;
+            tile(t, q0, residual);
+            const double s = wave_sum(tile_sum());
+            __syncthreads();
+            if (lane == 0) waves[wave] = s;
+            __syncthreads();
+            if (tid == 0) {
+                double v = 0.0;
+                for (int k = 0; k < NW; ++k) v += waves[k];
+                tiles[min(t, NT - 1)] = v;
+                starts[min(t, NT - 1)] = begin;
+            }
+        }
         __syncthreads();
         total = 0.0;
-        for (int k = tid & 63; k < kThreads; k += 64) total += sums[k];
+        for (int t = lane; t < T; t += 64) total += tiles[t];
         total = wave_sum(total);
         if (total > 0.0) break;
         residual = false;     // p = q to the last bit: the weights are p's
     }
-    int token = -1;
-    if (total > 0.0 && tid < 64) {
-        const double want = d.u_draw[b] * total;
-        double before;
-        const int at = max(0, first_reaching([&](int k) { return sums[k]; }, kThreads, 0.0, want, before));
-        double c = before;
-        for (int k = min(n, at * run); k < min(n, at * run + run); ++k) {
-            const double w = weight(k);
-            c += w;
-            if (w > 0.0) {
-                token = pi[k];
-                if (c >= want) break;
+    if (!(total > 0.0)) {
+        if (tid == 0) {
+            out[m] = -1;
+            d.out_count[b] = m;
+        }
+        return;
+    }
+    const double want = d.u_draw[b] * total;
+    double run;
+    const int at = max(0, first_reaching([&](int t) { return tiles[t]; }, T, 0.0, want, run));
+    if (T > 1) {
+        int q0 = starts[at];
+        tile(at, q0, residual);
+    }
+    // the wave, the thread, the entry
+    const double mine = tile_sum(), s = wave_sum(mine);
+    __syncthreads();
+    if (lane == 0) waves[wave] = s;
+    __syncthreads();
+    const int hit = max(0, first_reaching([&](int k) { return waves[k]; }, NW, run, want, run));
+    if (wave != hit) return;
+    const double cum = run + wave_incl_sum(mine);
+    const u64 reach = __ballot(mine > 0.0 && cum >= want), any = __ballot(mine > 0.0);
+    const int l = reach != 0 ? __ffsll((long long)reach) - 1 : any != 0 ? 63 - __clzll((long long)any) : 0;
+    if (lane == l) {
+        double c = cum - mine;
+        int token = id[0];
+        bool done = false;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            c += w[k];
+            if (!done && w[k] > 0.0) {
+                token = id[k];
+                done = c >= want;
             }
         }
-    }
-    for (int i = tid; i <= K; i += kThreads)
-        if (i != m) out[i] = i < m ? d.draft[q.d0 + i] : -1;
-    if (tid == 0) {
         out[m] = token;
-        d.out_count[b] = m + (total > 0.0 ? 1 : 0);
+        d.out_count[b] = m + 1;
     }
 }
 
+// Float exponentials first, and the emitting rows (one or two of the 2 max_draft + 1)
+// again in double: for bf16 rows, whose doubles take longer than their bytes, where
+// that is more than a launch. 256 sequences of 8 drafts over 151936 ids: 203 + 66 us
+// against 357; of 4 drafts in f32 64 + 22 against 74; 37 of 7 over 50257 in bf16
+// (26 MB) 21 + 15 against 30.
+constexpr int64_t kFastBytes = (int64_t)128 << 20;
+
 struct Layout {
     int S;
-    int64_t jobs, stats, rsum, counts, bytes;
+    int64_t jobs, stats, sums, rsum, counts, bytes;
 };
 
 int slices_of(int32_t vocab, bool bf) {
@@ -690,8 +1101,9 @@ bool layout_of(int32_t seqs, int32_t max_draft, int32_t vocab, Layout& l) {
     l.S = slices_of(vocab, false);
     l.jobs = (int64_t)seqs * (2 * max_draft + 1);
     l.stats = 0;
-    l.rsum = l.jobs * l.S * (int64_t)sizeof(SliceStat);
-    l.counts = l.rsum + (int64_t)seqs * l.S * 8;
+    l.sums = l.jobs * l.S * (int64_t)sizeof(SliceStat);
+    l.rsum = l.sums + l.jobs * (int64_t)sizeof(RowSum);
+    l.counts = l.rsum + (int64_t)seqs * l.S * kParts * 8;
     l.bytes = l.counts + (int64_t)seqs * (max_draft + 2) * 4;
     return true;
 }
@@ -699,15 +1111,20 @@ bool layout_of(int32_t seqs, int32_t max_draft, int32_t vocab, Layout& l) {
 template <bool BF>
 hipError_t launch_draft(const DraftArgs& a, hipStream_t s) {
     const int64_t jobs = (int64_t)a.d.seqs * (a.sides * (int64_t)a.d.max_draft + 1);
-    const int64_t waves = jobs * ((a.S + a.per - 1) / a.per), draws = (int64_t)a.d.seqs * a.S;
-    const int64_t clear = std::max<int64_t>(1, (int64_t)a.d.max_draft) * a.d.seqs;
-    auto blocks = [](int64_t n, int per) { return dim3((uint32_t)((n + per - 1) / per)); };
-    hipLaunchKernelGGL(k_draft_start, blocks(clear, kThreads), dim3(kThreads), 0, s, a);
-    if (a.d.mask != nullptr || a.d.draft_mask != nullptr)
-        hipLaunchKernelGGL((k_draft_stats<BF, true>), blocks(waves, kWaves), dim3(kThreads), 0, s, a);
-    else
-        hipLaunchKernelGGL((k_draft_stats<BF, false>), blocks(waves, kWaves), dim3(kThreads), 0, s, a);
-    hipLaunchKernelGGL(k_draft_draw<BF>, blocks(draws, kWaves), dim3(kThreads), 0, s, a);
+    auto blocks = [](int64_t n, int per) { return (n + per - 1) / per; };
+    const dim3 rows((uint32_t)(jobs * blocks(a.S, a.per * kWaves)));
+    hipLaunchKernelGGL(k_draft_start, dim3((uint32_t)blocks(std::max<int64_t>(1, a.d.max_draft) * a.d.seqs, kThreads)),
+                       dim3(kThreads), 0, s, a);
+    const bool mask = a.d.mask != nullptr || a.d.draft_mask != nullptr;
+    const dim3 emitting((uint32_t)((int64_t)a.d.seqs * a.sides * blocks(a.S, kWaves)));
+    if (mask && a.fast) hipLaunchKernelGGL((k_draft_stats<BF, true, true>), rows, dim3(kThreads), 0, s, a);
+    else if (mask) hipLaunchKernelGGL((k_draft_stats<BF, true, false>), rows, dim3(kThreads), 0, s, a);
+    else if (a.fast) hipLaunchKernelGGL((k_draft_stats<BF, false, true>), rows, dim3(kThreads), 0, s, a);
+    else hipLaunchKernelGGL((k_draft_stats<BF, false, false>), rows, dim3(kThreads), 0, s, a);
+    if (mask && a.fast) hipLaunchKernelGGL((k_draft_exact<BF, true>), emitting, dim3(kThreads), 0, s, a);
+    else if (a.fast) hipLaunchKernelGGL((k_draft_exact<BF, false>), emitting, dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL(k_draft_draw<BF>, dim3((uint32_t)(a.d.seqs * blocks((int64_t)a.S * kParts, kDrawThreads / 64))),
+                       dim3(kDrawThreads), 0, s, a);
     return hipGetLastError();
 }
 
@@ -750,9 +1167,12 @@ extern "C" int ultima_hsamp_verify_draft(const ultima_hsamp_draft* d, void* hip_
     a.per = (int)std::clamp<int64_t>((int64_t)d->seqs * a.sides * a.S / 4096, 1, a.S);
     const int64_t jobs = (int64_t)d->seqs * (a.sides * (int64_t)d->max_draft + 1);
     // a wave per slice of a row, numbered in 32 bits by their threads
-    if (jobs * a.S > ((int64_t)1 << 32) / 64 - kWaves) return ULTIMA_HSAMP_ERR_UNSUPPORTED;
+    // (up to a block's waves more per row)
+    if (std::max(jobs, (int64_t)d->seqs * kParts) * (a.S + 8) > ((int64_t)1 << 32) / 64) return ULTIMA_HSAMP_ERR_UNSUPPORTED;
+    a.fast = d->dtype == ULTIMA_HSAMP_BF16 && d->max_draft >= 4 && jobs * d->vocab * (int64_t)es > kFastBytes;
     unsigned char* w = static_cast<unsigned char*>(d->work);
     a.stats = reinterpret_cast<SliceStat*>(w + l.stats);
+    a.sums = reinterpret_cast<RowSum*>(w + l.sums);
     a.rsum = reinterpret_cast<double*>(w + l.rsum);
     a.count = reinterpret_cast<int32_t*>(w + l.counts);
     a.drawn = a.count + (int64_t)d->seqs * d->max_draft;
@@ -778,6 +1198,10 @@ extern "C" int ultima_hsamp_verify_sets(const ultima_hsamp_draft_sets* d, void* 
         return ULTIMA_HSAMP_ERR_INVALID;
     if (d->target_start == nullptr && (int64_t)d->seqs * (d->max_draft + 1) > d->rows) return ULTIMA_HSAMP_ERR_INVALID;
     if (d->draft_start == nullptr && (int64_t)d->seqs * d->max_draft > d->draft_rows) return ULTIMA_HSAMP_ERR_INVALID;
-    hipLaunchKernelGGL(k_verify_sets, dim3(d->seqs), dim3(kThreads), 0, static_cast<hipStream_t>(hip_stream), *d);
+    // sets of one tile of 4096, or of tiles of 8192
+    if (d->set_cap <= 512 * kEach)
+        hipLaunchKernelGGL(k_verify_sets<512>, dim3(d->seqs), dim3(512), 0, static_cast<hipStream_t>(hip_stream), *d);
+    else
+        hipLaunchKernelGGL(k_verify_sets<1024>, dim3(d->seqs), dim3(1024), 0, static_cast<hipStream_t>(hip_stream), *d);
     return hipGetLastError() == hipSuccess ? ULTIMA_HSAMP_OK : ULTIMA_HSAMP_ERR_HIP;
 }
