@@ -502,38 +502,20 @@ def _refuse(what: str):
     raise HsampError(ERR_INVALID, what)
 
 
-class _On:
-    """The stream a call runs on and its device made current; what the call
-    allocates is allocated for that stream."""
+def _elsewhere(dev, stream):
+    """The context that makes `stream` (None: the device's current one) and its device
+    current, or None where they are: the call, and what it allocates, then go there."""
+    import torch
+    if stream is not None:
+        return torch.cuda.stream(stream)
+    return None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
-    def __init__(self, dev, stream):
-        import torch
-        self.torch = torch
-        self.stream = torch.cuda.current_stream(dev) if stream is None else stream
-        self.other = stream is not None and stream != torch.cuda.current_stream(dev)
-        self.guard = torch.cuda.stream(stream) if self.other else None
-        self.device = None if self.other or torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
-    def __enter__(self):
-        for g in (self.guard, self.device):
-            if g is not None:
-                g.__enter__()
-        return self
-
-    def __exit__(self, *e):
-        for g in (self.device, self.guard):
-            if g is not None:
-                g.__exit__(*e)
-
-    def hold(self, t):
-        """A caller's scratch stays allocated until this stream is done with it."""
-        if self.other:
-            t.record_stream(self.stream)
-
-    def launch(self, fn, a, what):
-        status = fn(ctypes.byref(a), self.stream.cuda_stream)
-        if status != OK:
-            raise HsampError(status, what)
+def _launch(fn, a, dev, what):
+    import torch
+    status = fn(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev.index))
+    if status != OK:
+        raise HsampError(status, what)
 
 
 def _vector(t, n, dtype, dev, what, name):
@@ -600,40 +582,44 @@ def verify_draft(logits, draft, u_accept, u_draw, max_draft: int, draft_logits=N
     dev = logits.device
     if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in (f32, torch.bfloat16):
         _refuse("verify_draft: logits must be a float32 or bfloat16 matrix on the GPU")
+    there = _elsewhere(dev, stream)
+    if there is not None:
+        with there:
+            if work is not None and stream is not None:
+                work.record_stream(stream)       # the caller's scratch lives until this stream is done with it
+            return verify_draft(logits, draft, u_accept, u_draw, max_draft, draft_logits, temperature, draft_temperature,
+                                mask, draft_mask, n_draft, target_start, draft_start, accept, work, outputs)
     rows, V = logits.shape
-    with _On(dev, stream) as on:
-        a = Draft()
-        out = _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_start, draft_start, accept,
-                        outputs)
-        D, B = a.draft_rows, a.seqs
-        a.vocab, a.dtype, a.logits_rows = V, F32 if logits.dtype == f32 else BF16, rows
-        a.logits, a.logits_stride = _rows(logits, rows, V, (logits.dtype,), dev, what, "logits")
-        if draft_logits is not None:
-            at, stride = _rows(draft_logits, D, V, (logits.dtype,), dev, what, "draft_logits")
-            if draft_logits.shape[1] != V:
-                _refuse("verify_draft: draft_logits must have the target's vocabulary")
-            if D:
-                a.draft_logits, a.draft_stride = at, stride
-        words, kinds = -(-V // 32), (torch.int32, torch.uint32)
-        if mask is not None:
-            a.mask, a.mask_stride = _rows(mask, rows, words, kinds, dev, what, "mask")
-        if draft_mask is not None:
-            at, stride = _rows(draft_mask, D, words, kinds, dev, what, "draft_mask")
-            if draft_logits is None:
-                _refuse("verify_draft: draft_mask goes with draft_logits")
-            if D:
-                a.draft_mask, a.draft_mask_stride = at, stride
-        a.temperature = _vector(temperature, B, f32, dev, what, "temperature")
-        a.draft_temperature = _vector(draft_temperature, B, f32, dev, what, "draft_temperature")
-        need = lib().ultima_hsamp_verify_draft_work_bytes(B, a.max_draft, V)
-        if work is None:
-            work = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-        elif work.device != dev or not work.is_contiguous() or work.numel() * work.element_size() < need:
-            _refuse(f"verify_draft: work must be {need} contiguous bytes on {dev}")
-        else:
-            on.hold(work)
-        a.work = work.data_ptr()
-        on.launch(lib().ultima_hsamp_verify_draft, a, what)
+    a = Draft()
+    out = _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_start, draft_start, accept,
+                    outputs)
+    D, B = a.draft_rows, a.seqs
+    a.vocab, a.dtype, a.logits_rows = V, F32 if logits.dtype == f32 else BF16, rows
+    a.logits, a.logits_stride = _rows(logits, rows, V, (logits.dtype,), dev, what, "logits")
+    if draft_logits is not None:
+        at, stride = _rows(draft_logits, D, V, (logits.dtype,), dev, what, "draft_logits")
+        if draft_logits.shape[1] != V:
+            _refuse("verify_draft: draft_logits must have the target's vocabulary")
+        if D:
+            a.draft_logits, a.draft_stride = at, stride
+    words, kinds = -(-V // 32), (torch.int32, torch.uint32)
+    if mask is not None:
+        a.mask, a.mask_stride = _rows(mask, rows, words, kinds, dev, what, "mask")
+    if draft_mask is not None:
+        at, stride = _rows(draft_mask, D, words, kinds, dev, what, "draft_mask")
+        if draft_logits is None:
+            _refuse("verify_draft: draft_mask goes with draft_logits")
+        if D:
+            a.draft_mask, a.draft_mask_stride = at, stride
+    a.temperature = _vector(temperature, B, f32, dev, what, "temperature")
+    a.draft_temperature = _vector(draft_temperature, B, f32, dev, what, "draft_temperature")
+    need = lib().ultima_hsamp_verify_draft_work_bytes(B, a.max_draft, V)
+    if work is None:
+        work = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    elif work.device != dev or not work.is_contiguous() or work.numel() * work.element_size() < need:
+        _refuse(f"verify_draft: work must be {need} contiguous bytes on {dev}")
+    a.work = work.data_ptr()
+    _launch(lib().ultima_hsamp_verify_draft, a, dev, what)
     return out
 
 
@@ -650,6 +636,11 @@ def verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_dr
     dev = kept_idx.device
     if not kept_idx.is_cuda or kept_idx.dim() != 2:
         _refuse("verify_sets: kept_idx must be a matrix on the GPU")
+    there = _elsewhere(dev, stream)
+    if there is not None:
+        with there:
+            return verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_draft, draft_idx, draft_prob,
+                               draft_count, n_draft, target_start, draft_start, accept, outputs)
 
     def sets(idx, prob, count, rows, names):
         if prob is None or count is None or idx.dtype != torch.int32 or prob.dtype != torch.float32 or \
@@ -659,25 +650,33 @@ def verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_dr
             _refuse(f"{what}: {names} must be contiguous int32 [{rows}, cap], float32 [{rows}, cap], int32 [{rows}] on {dev}")
         return idx.data_ptr(), prob.data_ptr(), count.data_ptr()
 
-    with _On(dev, stream) as on:
-        a = DraftSets()
-        out = _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_start, draft_start, accept,
-                        outputs)
-        a.rows, a.set_cap = kept_idx.shape
-        a.kept_idx, a.kept_prob, a.kept_count = sets(kept_idx, kept_prob, kept_count, a.rows,
-                                                     "kept_idx, kept_prob, kept_count")
-        if draft_idx is not None:
-            at = sets(draft_idx, draft_prob, draft_count, a.draft_rows, "draft_idx, draft_prob, draft_count")
-            if a.draft_rows:
-                a.draft_cap = draft_idx.shape[1]
-                a.draft_idx, a.draft_prob, a.draft_count = at
-        elif draft_prob is not None or draft_count is not None:
-            _refuse("verify_sets: draft_prob and draft_count go with draft_idx")
-        on.launch(lib().ultima_hsamp_verify_sets, a, what)
+    a = DraftSets()
+    out = _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_start, draft_start, accept,
+                    outputs)
+    a.rows, a.set_cap = kept_idx.shape
+    a.kept_idx, a.kept_prob, a.kept_count = sets(kept_idx, kept_prob, kept_count, a.rows,
+                                                 "kept_idx, kept_prob, kept_count")
+    if draft_idx is not None:
+        at = sets(draft_idx, draft_prob, draft_count, a.draft_rows, "draft_idx, draft_prob, draft_count")
+        if a.draft_rows:
+            a.draft_cap = draft_idx.shape[1]
+            a.draft_idx, a.draft_prob, a.draft_count = at
+    elif draft_prob is not None or draft_count is not None:
+        _refuse("verify_sets: draft_prob and draft_count go with draft_idx")
+    _launch(lib().ultima_hsamp_verify_sets, a, dev, what)
     return out
 
 
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "softcap": 5}
+
+
+def _matrix(t, lead, rows, columns, dtype, dev, name):
+    """The address, row stride and group stride of a [*lead, rows, columns] operand."""
+    shape, stride = t.shape, t.stride()
+    if shape[:-2] != lead or len(shape) < 2 or shape[-2] != rows or shape[-1] != columns or t.dtype != dtype or \
+            t.device != dev or (columns > 1 and stride[-1] != 1):
+        _refuse(f"linear: {name} must be {dtype} {(*lead, rows, columns)} on {dev}, contiguous in its last dimension")
+    return t.data_ptr(), stride[-2] if rows > 1 else max(columns, stride[-2]), stride[0] if lead else 0
 
 
 def linear(x, weight, bias=None, act: str = "none", act_param: float = 0.0, residual=None, out=None, out_dtype=None,
@@ -693,38 +692,30 @@ def linear(x, weight, bias=None, act: str = "none", act_param: float = 0.0, resi
         _refuse("linear: x and weight must be bfloat16 or float16 matrices (or batches of them) on the GPU")
     if act not in ACTS:
         _refuse(f"linear: act must be one of {', '.join(ACTS)}")
-    lead = tuple(x.shape[:-2])
+    there = _elsewhere(dev, stream)
+    if there is not None:
+        with there:
+            return linear(x, weight, bias, act, act_param, residual, out, out_dtype)
+    lead = x.shape[:-2]
     M, K = x.shape[-2:]
     N = weight.shape[-2]
-
-    def operand(t, name, shape, dtype):
-        """The address, row stride and group stride of [.., rows, columns] or [.., columns]."""
-        if t.shape != shape or t.dtype != dtype or t.device != dev or (shape[-1] > 1 and t.stride(-1) != 1):
-            _refuse(f"linear: {name} must be {dtype} {tuple(shape)} on {dev}, contiguous in its last dimension")
-        stride = t.stride()
-        group = stride[0] if lead else 0
-        if len(shape) == len(lead) + 1:
-            return t.data_ptr(), group
-        return t.data_ptr(), (stride[-2] if shape[-2] > 1 else max(shape[-1], stride[-2])), group
-
-    with _On(dev, stream) as on:
-        if out is None:
-            out = torch.empty((*lead, M, N), dtype=out_dtype or dt, device=dev)
-        if out.dtype not in (dt, torch.float32) or out_dtype not in (None, out.dtype):
-            _refuse(f"linear: the output must be {dt} or torch.float32")
-        a = LinearArgs()
-        a.rows, a.in_dim, a.out_dim, a.groups = M, K, N, lead[0] if lead else 1
-        a.dtype = BF16 if dt == torch.bfloat16 else F16
-        a.out_dtype = F32 if out.dtype == torch.float32 else a.dtype
-        a.act, a.act_param = ACTS[act], act_param
-        a.x, a.x_stride, a.x_group = operand(x, "x", (*lead, M, K), dt)
-        a.weight, a.weight_stride, a.weight_group = operand(weight, "weight", (*lead, N, K), dt)
-        if bias is not None:
-            a.bias, a.bias_group = operand(bias, "bias", (*lead, N), dt)
-        if residual is not None:
-            a.residual, a.residual_stride, a.residual_group = operand(residual, "residual", (*lead, M, N), dt)
-        a.out, a.out_stride, a.out_group = operand(out, "out", (*lead, M, N), out.dtype)
-        on.launch(lib().ultima_hsamp_linear, a, "linear")
+    if out is None:
+        out = torch.empty((*lead, M, N), dtype=out_dtype or dt, device=dev)
+    odt = out.dtype
+    if odt not in (dt, torch.float32) or out_dtype not in (None, odt):
+        _refuse(f"linear: the output must be {dt} or torch.float32")
+    kind = BF16 if dt == torch.bfloat16 else F16
+    a = LinearArgs(M, K, N, lead[0] if lead else 1, kind, F32 if odt == torch.float32 else kind, ACTS[act], act_param)
+    a.x, a.x_stride, a.x_group = _matrix(x, lead, M, K, dt, dev, "x")
+    a.weight, a.weight_stride, a.weight_group = _matrix(weight, lead, N, K, dt, dev, "weight")
+    if bias is not None:
+        if bias.shape != (*lead, N) or bias.dtype != dt or bias.device != dev or (N > 1 and bias.stride(-1) != 1):
+            _refuse(f"linear: bias must be {dt} {(*lead, N)} on {dev}, contiguous in its last dimension")
+        a.bias, a.bias_group = bias.data_ptr(), bias.stride(0) if lead else 0
+    if residual is not None:
+        a.residual, a.residual_stride, a.residual_group = _matrix(residual, lead, M, N, dt, dev, "residual")
+    a.out, a.out_stride, a.out_group = _matrix(out, lead, M, N, odt, dev, "out")
+    _launch(lib().ultima_hsamp_linear, a, dev, "linear")
     return out
 
 
