@@ -394,14 +394,17 @@ int ultima_hsamp_lm_head(const ultima_hsamp_head* head, void* hip_stream);
  *   weight above 0 where rounding leaves none;
  *   the rest of the sequence's max_draft + 1 tokens are -1, count = m + 1.
  * A drafter that is certain of its tokens (lookup in the prompt; a greedy
- * drafter) has q_i(d_i) = 1. Everything is evaluated in double precision.
+ * drafter) has q_i(d_i) = 1. Every decision is made in double precision; weights
+ * below 2^-1000 of their row's largest count as 0.
  * A sequence whose target row m allows nothing has no token there: tokens[m] is
  * -1 and count m. A drafted id outside [0, vocab) has probability 0 on both
  * sides and is rejected. n_draft outside [0, max_draft] or rows outside the
  * arrays: count 0, every token -1.
  * accept_prob[i] = min(1, p_i(d_i) / q_i(d_i)) (q_i(d_i) = 0: 1 if p_i(d_i) > 0,
  * else 0) up to the first rejected draft, -1 for the drafts after it; rows of no
- * sequence are left as they were.
+ * sequence are left as they were. (In bfloat16 calls of more than 128 MB of logits
+ * and four drafts or more it may be off by 1e-5 of its value; else it is the
+ * rounded double.)
  * Row layout: target rows of sequence b start at target_start[b], its drafted
  * rows at draft_start[b] (device int32 [seqs]), so that sequences with fewer
  * drafts take fewer rows; NULL: b * (max_draft + 1) and b * max_draft.

@@ -2,22 +2,25 @@
 // (ultima_hsamp_verify_draft) and on kept sets (ultima_hsamp_verify_sets). The
 // formulas stand at their declarations.
 //
-// On logits, three kernels:
+// On logits:
 //   k_draft_start    clears the call's counters
 //   k_draft_stats    a wave per slice of a row (16 KB of logits): its maximum m_s
 //                    and sum of exp((x - m_s) / T) in double, a greedy row's lowest
-//                    id of the maximum. Positions first, sequences second: the wave
-//                    that completes a position's rows decides its draft, and waves
+//                    id of the maximum. Positions first, sequences second: the block
+//                    that completes a position's rows decides its draft, and blocks
 //                    of later positions find the rejection and read nothing. What
 //                    they skip is never used, whether they see it or not.
-//   k_draft_draw     a wave per quarter of a slice of each sequence's emitting row:
-//                    its sum of max(p - q, 0); the wave that completes a sequence
-//                    finds the quarter where the running sum reaches u_draw, then
-//                    the id.
+//   k_draft_exact    large bf16 calls only, whose sums above come from float
+//                    exponentials: the emitting rows' slices again in double
+//   k_draft_draw     a wave per part of a slice of each sequence's emitting row: its
+//                    sum of max(p - q, 0); the block that completes a sequence
+//                    finds the part where the running sum reaches u_draw, then the
+//                    id.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "hsamp_wave.h"
 #include "ultima_hsamp.h"
@@ -27,11 +30,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kDrawThreads = 512;
 constexpr int kChunks = 16;                  // 16-byte loads of a lane per slice,
 constexpr int kStep = 4;                     // of them a step, the next step's in flight
 constexpr int kSteps = kChunks / kStep;
-constexpr int kParts = 4;                    // parts of a slice when a token is drawn
+constexpr int kMaxParts = 8;                 // parts of a slice when a token is drawn
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kFltMax = 3.402823466e38f;
 
@@ -41,7 +43,7 @@ typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 
 // exp(d) in double for d <= 0 by Tang's table method: d = (k + f) ln 2 / 32, |f| <=
 // 1/2, exp(d) = 2^(k >> 5) 2^((k & 31) / 32) exp(f ln 2 / 32), the last a polynomial
-// of the fourth degree (interpolated at the Chebyshev points, off by at most 8e-14:
+// of the fourth degree (interpolated at the Chebyshev points, off by at most 1.6e-13:
 // the decisions need 1e-11 or so, a float exponential's 1e-7 would move the draws).
 // The 32 doubles of the table fill the 64 LDS banks once, so its reads never conflict.
 __device__ const double kPow[32] = {
@@ -120,7 +122,7 @@ struct RowSum {
 struct DraftArgs {
     ultima_hsamp_draft d;
     SliceStat* stats;        // [jobs][S]
-    double* rsum;            // [seqs][kParts S]
+    double* rsum;            // [seqs][parts of the row]
     RowSum* sums;            // [max_draft][seqs][sides] of the decided positions
     int32_t* count;          // [max_draft][seqs] slices of the position's rows that are done, then
     int32_t* drawn;          // [seqs] parts of the emitting row, and
@@ -677,15 +679,17 @@ __device__ __forceinline__ int first_reaching(F value, int n, double base, doubl
     return last;
 }
 
-template <bool BF>
-__global__ __launch_bounds__(kDrawThreads) void k_draft_draw(DraftArgs a) {
+// TH threads a block, a wave per part of a slice (PARTS of them).
+template <bool BF, int TH, int PARTS>
+__global__ __launch_bounds__(TH) void k_draft_draw(DraftArgs a) {
     using R = Row<BF>;
     __shared__ double table[32];
     __shared__ int32_t shared;
     load_table(table);
-    constexpr int PART = R::SLICE / kParts, CH = kChunks / kParts;       // ids and chunks of a lane per part
-    const int lane = threadIdx.x & 63, S = a.S, P = a.S * kParts, K = a.d.max_draft;
-    constexpr int NW = kDrawThreads / 64;
+    constexpr int PART = R::SLICE / PARTS, CH = kChunks / PARTS;       // ids and chunks of a lane per part
+    const int lane = threadIdx.x & 63, S = a.S, P = a.S * PARTS, K = a.d.max_draft;
+    constexpr int NW = TH / 64;
+    static_assert(NW >= PARTS && PARTS <= kMaxParts);
     const int groups = (P + NW - 1) / NW;
     const int b = blockIdx.x / groups, first = blockIdx.x % groups * NW;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = first + wave;
@@ -786,15 +790,15 @@ __global__ __launch_bounds__(kDrawThreads) void k_draft_draw(DraftArgs a) {
     int at;
     if (whole) {
         const int slice = max(0, first_reaching(p_slice, S, 0.0, want, run));
-        __shared__ double sums[kParts];
-        if (wave < kParts) {
+        __shared__ double sums[PARTS];
+        if (wave < PARTS) {
             double v = 0.0;
 #pragma unroll
-            for (int j = 0; j < CH; ++j) c[j] = w.load((slice * kParts + wave) * PART + (j * 64 + lane) * R::VEC);
+            for (int j = 0; j < CH; ++j) c[j] = w.load((slice * PARTS + wave) * PART + (j * 64 + lane) * R::VEC);
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 double x[R::VEC];
-                w.all(c[j], (slice * kParts + wave) * PART + (j * 64 + lane) * R::VEC, table, x);
+                w.all(c[j], (slice * PARTS + wave) * PART + (j * 64 + lane) * R::VEC, table, x);
 #pragma unroll
                 for (int k = 0; k < R::VEC; ++k) v += x[k];
             }
@@ -802,7 +806,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_draft_draw(DraftArgs a) {
             if (lane == 0) sums[wave] = v;
         }
         __syncthreads();
-        at = slice * kParts + max(0, first_reaching([&](int n) { return sums[n]; }, kParts, run, want, run));
+        at = slice * PARTS + max(0, first_reaching([&](int n) { return sums[n]; }, PARTS, run, want, run));
     } else {
         at = max(0, first_reaching(r_held, P, 0.0, want, run));
     }
@@ -1103,7 +1107,7 @@ bool layout_of(int32_t seqs, int32_t max_draft, int32_t vocab, Layout& l) {
     l.stats = 0;
     l.sums = l.jobs * l.S * (int64_t)sizeof(SliceStat);
     l.rsum = l.sums + l.jobs * (int64_t)sizeof(RowSum);
-    l.counts = l.rsum + (int64_t)seqs * l.S * kParts * 8;
+    l.counts = l.rsum + (int64_t)seqs * l.S * kMaxParts * 8;
     l.bytes = l.counts + (int64_t)seqs * (max_draft + 2) * 4;
     return true;
 }
@@ -1123,8 +1127,16 @@ hipError_t launch_draft(const DraftArgs& a, hipStream_t s) {
     else hipLaunchKernelGGL((k_draft_stats<BF, false, false>), rows, dim3(kThreads), 0, s, a);
     if (mask && a.fast) hipLaunchKernelGGL((k_draft_exact<BF, true>), emitting, dim3(kThreads), 0, s, a);
     else if (a.fast) hipLaunchKernelGGL((k_draft_exact<BF, false>), emitting, dim3(kThreads), 0, s, a);
-    hipLaunchKernelGGL(k_draft_draw<BF>, dim3((uint32_t)(a.d.seqs * blocks((int64_t)a.S * kParts, kDrawThreads / 64))),
-                       dim3(kDrawThreads), 0, s, a);
+    auto draw = [&](auto th, auto parts) {
+        constexpr int TH = decltype(th)::value, PARTS = decltype(parts)::value;
+        hipLaunchKernelGGL((k_draft_draw<BF, TH, PARTS>), dim3((uint32_t)(a.d.seqs * blocks((int64_t)a.S * PARTS, TH / 64))),
+                           dim3(TH), 0, s, a);
+    };
+    // few rows: more waves a slice, for its latency; many: fewer (each starts with the
+    // sequence's own data), in smaller blocks. 8 of 512 threads against 4 of 256: one
+    // sequence 8.9 and 12.2 us, 64 (f32) 32 and 30, 256 (bf16) 112 and 94.
+    if ((int64_t)a.d.seqs * a.S < 4096) draw(std::integral_constant<int, 512>(), std::integral_constant<int, 8>());
+    else draw(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
     return hipGetLastError();
 }
 
@@ -1168,7 +1180,7 @@ extern "C" int ultima_hsamp_verify_draft(const ultima_hsamp_draft* d, void* hip_
     const int64_t jobs = (int64_t)d->seqs * (a.sides * (int64_t)d->max_draft + 1);
     // a wave per slice of a row, numbered in 32 bits by their threads
     // (up to a block's waves more per row)
-    if (std::max(jobs, (int64_t)d->seqs * kParts) * (a.S + 8) > ((int64_t)1 << 32) / 64) return ULTIMA_HSAMP_ERR_UNSUPPORTED;
+    if (std::max(jobs, (int64_t)d->seqs * kMaxParts) * (a.S + 8) > ((int64_t)1 << 32) / 64) return ULTIMA_HSAMP_ERR_UNSUPPORTED;
     a.fast = d->dtype == ULTIMA_HSAMP_BF16 && d->max_draft >= 4 && jobs * d->vocab * (int64_t)es > kFastBytes;
     unsigned char* w = static_cast<unsigned char*>(d->work);
     a.stats = reinterpret_cast<SliceStat*>(w + l.stats);
