@@ -521,3 +521,81 @@ def test_sets_from_the_sampler(hs, sampler, wl):
                              lambda i: R.dense(*(a[b * K + i] for a in Q), V), d[sl], u[sl], v[b]))
     check(out, want, B, K, [K] * B, [b * K for b in range(B)], B * K)
     assert any(len(w[0]) > 1 for w in want)
+
+
+def test_large_draft_and_sets_captured(hs):
+    """A large bfloat16 call (float exponentials, then double) and a call on sets in one
+    graph, replayed with new contents and eager work between; every replay the
+    eager calls' results."""
+    torch, dev = _torch()
+    B, K, V, cap = 16, 6, 40009, 200
+    pitch = 64                        # many drafts could be: the call counts as large
+
+    def inputs(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        n = torch.randint(0, K + 1, (B,), generator=g, device=dev, dtype=torch.int32)
+        ts = (torch.arange(B, device=dev) * (K + 1)).to(torch.int32)
+        ds = (torch.arange(B, device=dev) * K).to(torch.int32)
+        x = (torch.randn((B * (K + 1), V), generator=g, device=dev) * 3).to(torch.bfloat16)
+        y = (x.view(B, K + 1, V)[:, :K].reshape(B * K, V).float() + torch.randn((B * K, V), generator=g, device=dev) * 0.5).to(torch.bfloat16)
+        d = y.argmax(1).to(torch.int32)
+        u = torch.rand(B * K, generator=g, device=dev, dtype=torch.float64)
+        v = torch.rand(B, generator=g, device=dev, dtype=torch.float64)
+
+        def top(z):
+            p, i = torch.topk(torch.softmax(z.float(), 1), cap, dim=1)
+            i, order = torch.sort(i, dim=1)
+            return [i.to(torch.int32), p.gather(1, order).contiguous(),
+                    torch.full((z.shape[0],), cap, dtype=torch.int32, device=dev)]
+        return [x, d, u, v, y, n, ts, ds] + top(x) + top(y)
+
+    def call(i, out=({}, {}), work=None):
+        a = hs.verify_draft(*i[:4], pitch, draft_logits=i[4], n_draft=i[5], target_start=i[6], draft_start=i[7],
+                            outputs=out[0], work=work)
+        b = hs.verify_sets(*i[8:11], *i[1:4], pitch, draft_idx=i[11], draft_prob=i[12], draft_count=i[13], n_draft=i[5],
+                           target_start=i[6], draft_start=i[7], outputs=out[1])
+        return a, b
+
+    assert B * (2 * pitch + 1) * V * 2 > LARGE
+    held = inputs(0)
+    work = torch.full((hs.lib().ultima_hsamp_verify_draft_work_bytes(B, pitch, V),), 255, dtype=torch.uint8, device=dev)
+    accept = [torch.zeros(B * K, device=dev) for _ in range(2)]
+    out = ({"accept": accept[0]}, {"accept": accept[1]})
+    call(held, out, work)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(held, out, work)
+    for seed in range(1, 5):
+        new = inputs(seed)
+        want = call(new, ({"accept": torch.zeros(B * K, device=dev)}, {"accept": torch.zeros(B * K, device=dev)}))
+        for h, t in zip(held, new):
+            h.copy_(t)
+        for a in accept:
+            a.zero_()
+        work.fill_(255)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(out, want):
+            for k in w:
+                assert torch.equal(o[k], w[k]), (seed, k)
+
+
+def test_draft_sequences_that_share_rows(hs):
+    """Two sequences on the same target rows with uniforms of their own (two samples
+    of one continuation): each as if alone."""
+    torch, dev = _torch()
+    rng = np.random.default_rng(91)
+    V, K = 7001, 2
+    x, y = logits(rng, 3, V), logits(rng, 4, V)
+    d = rng.integers(0, V, 4).astype(np.int32)
+    u, v = rng.random(4) * 1e-3, rng.random(2)
+    to = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(dev)  # noqa: E731
+    out = hs.verify_draft(to(x), to(d), to(u), to(v), K, draft_logits=to(y), target_start=to(np.zeros(2, np.int32)),
+                          draft_start=to(np.array([0, 2], np.int32)))
+    tokens, count = out["tokens"].cpu().numpy(), out["count"].cpu().numpy()
+    for b in range(2):
+        w, _, near = R.verify(lambda i: R.chances(x[i]), lambda i: R.chances(y[2 * b + i]), d[2 * b:2 * b + 2],
+                              u[2 * b:2 * b + 2], v[b])
+        assert near > R.NEAR and list(tokens[b][:count[b]]) == w
