@@ -477,12 +477,17 @@ typedef struct ultima_hsamp_draft_sets {
     const int32_t* draft_start;
     const double* u_accept;
     const double* u_draw;
+    void* work;                 /* ultima_hsamp_verify_sets_work_bytes() bytes as in ultima_hsamp_draft; 0: may be NULL */
     int32_t* out_tokens;
     int32_t* out_count;
     float* accept_prob;
 } ultima_hsamp_draft_sets;
 
-/* Asynchronous on hip_stream, allocates nothing, needs no workspace. */
+/* Bytes of workspace ultima_hsamp_verify_sets needs, 0 for sets of up to 4096 ids
+ * (-1 for invalid sizes). */
+int64_t ultima_hsamp_verify_sets_work_bytes(int32_t seqs, int32_t set_cap);
+
+/* Asynchronous on hip_stream, allocates nothing (graph-capturable). */
 int ultima_hsamp_verify_sets(const ultima_hsamp_draft_sets* d, void* hip_stream);
 
 /* ---- The product with its epilogue ---------------------------------------------

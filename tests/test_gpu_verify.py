@@ -453,6 +453,101 @@ def test_sets_match_the_rule(hs, B, K, cap, V, drafter):
     check(out, want, B, K, n, ds, D)
 
 
+@pytest.mark.parametrize("B,cap", [(300, 9000), (600, 9000), (2, 70000)])
+def test_sets_of_several_tiles(hs, B, cap):
+    """Sets of 0 to cap ids whose tiles go to several blocks of a sequence or to one;
+    the workspace holds anything. Every third sequence's drafter has the target's set
+    and a draft outside it: the weights are then the target's."""
+    torch, dev = _torch()
+    rng = np.random.default_rng(B + cap)
+    K, V = 1, cap + 500
+    counts = np.minimum(cap, (rng.random(2 * B) ** 3 * (cap + 1)).astype(np.int32))
+    counts[:2] = cap
+    P = make_sets(rng, 2 * B, cap, V, counts)
+    Q = make_sets(rng, B, cap, V, np.minimum(cap, (rng.random(B) ** 2 * (cap + 1)).astype(np.int32)))
+    d = rng.integers(0, V, B).astype(np.int32)
+    for b in range(B):
+        if b % 3 == 0:
+            for q, t in zip(Q, P):
+                q[b] = t[2 * b]
+            d[b] = np.setdiff1d(np.arange(V), Q[0][b, :Q[2][b]])[0]
+        elif Q[2][b]:
+            d[b] = Q[0][b, rng.integers(0, Q[2][b])]
+    u, v = rng.random(B), rng.random(B)
+    to = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(dev)  # noqa: E731
+    need = hs.lib().ultima_hsamp_verify_sets_work_bytes(B, cap)
+    args = [to(t) for t in (*P, d, u, v)] + [K]
+    kw = dict(draft_idx=to(Q[0]), draft_prob=to(Q[1]), draft_count=to(Q[2]))
+    out = hs.verify_sets(*args, **kw, work=torch.full((need,), 255, dtype=torch.uint8, device=dev))
+    torch.cuda.synchronize()
+    want = [R.verify(lambda i: R.dense(*(a[2 * b + i] for a in P), V), lambda i: R.dense(*(a[b] for a in Q), V),  # noqa: B023
+                     d[b:b + 1], u[b:b + 1], v[b]) for b in range(B)]
+    check(out, want, B, K, [1] * B, np.arange(B), B)
+    with pytest.raises(hs.HsampError):
+        hs.verify_sets(*args, **kw, work=torch.empty(need - 1, dtype=torch.uint8, device=dev))
+
+
+@pytest.mark.parametrize("cap,draft_cap,V", [(64, 60000, 61000), (60000, 64, 61000), (3, 200000, 250000), (4097, 4096, 9000),
+                                             (9000, 50001, 50001)])
+def test_sets_of_different_capacities(hs, cap, draft_cap, V):
+    """A target's few ids among many of the drafter's, and the other way round."""
+    torch, dev = _torch()
+    rng = np.random.default_rng(cap + draft_cap)
+    B, K = 12, 1
+    P = make_sets(rng, 2 * B, cap, V, [max(1, cap - r % 3) for r in range(2 * B)])
+    Q = make_sets(rng, B, draft_cap, V, [max(1, draft_cap - r % 5) for r in range(B)])
+    for b in range(B):
+        few, many = (P, Q) if cap < draft_cap else (Q, P)
+        rf, rm = (2 * b, b) if few is P else (b, 2 * b)
+        if b % 2:             # the few among the many, some of them likelier
+            ids = np.sort(rng.choice(many[0][rm, :many[2][rm]], few[2][rf], replace=False))
+            few[0][rf, :few[2][rf]] = ids
+            at = np.searchsorted(many[0][rm, :many[2][rm]], ids)
+            many[1][rm, at] = few[1][rf, :few[2][rf]] * rng.choice([0.5, 1.0, 2.0], ids.size).astype(np.float32)
+    d = np.array([Q[0][r, rng.integers(0, Q[2][r])] for r in range(B)], np.int32)
+    u, v = rng.random(B) * 0.5 + 0.5, rng.random(B)
+    to = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(dev)  # noqa: E731
+    out = hs.verify_sets(*[to(t) for t in (*P, d, u, v)], K, draft_idx=to(Q[0]), draft_prob=to(Q[1]), draft_count=to(Q[2]))
+    torch.cuda.synchronize()
+    want = [R.verify(lambda i: R.dense(*(a[2 * b + i] for a in P), V), lambda i: R.dense(*(a[b] for a in Q), V),  # noqa: B023
+                     d[b:b + 1], u[b:b + 1], v[b]) for b in range(B)]
+    check(out, want, B, K, [1] * B, np.arange(B), B)
+    assert any(len(w[0]) == 1 for w in want)
+
+
+def test_sets_of_several_tiles_captured(hs):
+    """Replays of a captured call with new contents give the eager call's tokens."""
+    torch, dev = _torch()
+    B, K, cap, V = 5, 3, 12000, 20000
+    to = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(dev)  # noqa: E731
+
+    def inputs(seed):
+        rng = np.random.default_rng(seed)
+        P, Q = make_sets(rng, B * (K + 1), cap, V), make_sets(rng, B * K, cap, V)
+        d = np.array([Q[0][r, rng.integers(0, Q[2][r])] for r in range(B * K)], np.int32)
+        return [to(t) for t in (*P, d, rng.random(B * K), rng.random(B), *Q)]
+
+    def call(i, out):
+        return hs.verify_sets(*i[:6], K, draft_idx=i[6], draft_prob=i[7], draft_count=i[8], outputs=out)
+
+    held, out = inputs(0), {}
+    call(held, out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(held, out)
+    for seed in range(1, 5):
+        new = inputs(seed)
+        want = call(new, {})
+        for h, t in zip(held, new):
+            h.copy_(t)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for k in want:
+            assert torch.equal(out[k], want[k]), (seed, k)
+
+
 def test_sets_that_are_no_sets(hs):
     """Counts outside the capacity and rows outside the arrays: count 0 and -1
     everywhere; an empty target set: no token; an empty drafter's set: q = 0; NaN

@@ -69,10 +69,21 @@ def sets(hsamp, **kw):
     dict(draft_rows=-1), dict(set_cap=0), dict(set_cap=(1 << 24) + 1), dict(draft_cap=0), dict(draft_cap=(1 << 24) + 1),
     dict(kept_idx=None), dict(kept_prob=None), dict(kept_count=None), dict(draft_idx=None), dict(draft_prob=None),
     dict(draft_count=None), dict(draft=None), dict(u_accept=None), dict(u_draw=None), dict(out_tokens=None),
-    dict(out_count=None),
+    dict(out_count=None), dict(set_cap=4097), dict(set_cap=4097, work=OK_PTR + 8),
 ])
 def test_sets_refuse(hsamp, kw):
     assert sets(hsamp, **kw) == hsamp.ERR_INVALID
+
+
+def test_sets_work_bytes(hsamp):
+    f = hsamp.lib().ultima_hsamp_verify_sets_work_bytes
+    assert f(0, 1) == -1 and f(1, 0) == -1 and f(1, (1 << 24) + 1) == -1
+    assert f(1, 1) == f(5, 4096) == 0 < f(1, 4097) < f(2, 4097) < f(2, 151936)
+    assert f(2**31 - 1, 1 << 24) > 2**40      # no 32-bit overflow
+
+
+def test_sets_refuse_too_many(hsamp):
+    assert sets(hsamp, seqs=(1 << 21) + 1, target_start=OK_PTR, draft_start=OK_PTR) == hsamp.ERR_UNSUPPORTED
 
 
 def test_sets_refuse_null(hsamp):
@@ -97,7 +108,7 @@ def linear(hsamp, **kw):
     dict(act=5, act_param=float("nan")), dict(act=5, act_param=float("inf")), dict(x=None), dict(weight=None),
     dict(out=None), dict(x_stride=63), dict(weight_stride=63), dict(out_stride=31), dict(residual_stride=31),
     dict(x=OK_PTR + 1), dict(weight=OK_PTR + 1), dict(bias=OK_PTR + 1), dict(residual=OK_PTR + 1), dict(out=OK_PTR + 1),
-    dict(out_dtype=0, out=OK_PTR + 2),
+    dict(out_dtype=0, out=OK_PTR + 2), dict(out=OK_PTR), dict(out=2 * OK_PTR), dict(out=3 * OK_PTR),
     dict(residual=OK_PTR * 5, out_stride=33), dict(residual=OK_PTR * 5, out_dtype=0), dict(residual=OK_PTR * 5, out_group=256),
     dict(out_group=0), dict(out_group=64), dict(out_group=-1), dict(out_group=-64), dict(out_group=31, out_stride=64),
     dict(out_group=40, out_stride=64), dict(out_group=1 << 62, groups=0),

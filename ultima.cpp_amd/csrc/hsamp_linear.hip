@@ -124,7 +124,7 @@ __device__ __forceinline__ void finish(const Args& a, int g, int m, int n, float
     if (a.out_dtype == ULTIMA_HSAMP_F32) {
         float* p = static_cast<float*>(a.out) + at;
         if (E == 8 && left >= 8) {
-            #pragma unroll
+#pragma unroll
             for (int e = 0; e < E; e += 4)
                 *reinterpret_cast<f32x4_a4*>(p + e) = f32x4{y[e], y[(e + 1) % E], y[(e + 2) % E], y[(e + 3) % E]};
         } else {
@@ -189,6 +189,16 @@ __device__ __forceinline__ void store_tiles(const Args& a, int g, int m0, int n0
 // stages in the air or in LDS; the next step's operands are read while one is
 // multiplied. A stage is 64 columns in two steps (WK = 1), or 32 WK columns, one
 // step for each wave, whose sums meet in LDS at the end.
+//
+// Few rows: W's stream bounds it (one row of 4096 x 4096 8.3 us, 4.0 TB/s with the
+// launch and the ramp in it; four groups of 64 rows 37 us, 134 MB at 3.6 TB/s): hence
+// narrow tiles, whose waves share K instead of columns, and many loads in the air.
+// Many: per stage the loads to LDS and the LDS reads beside the products: hence the
+// widest tile that the accumulators allow, whose operands are read least often
+// (4096 rows of 4096 x 16384 462 us, 1190 TFLOP/s, where 8192 cubed reaches 1215 in
+// the library; with bias, tanh and residual 519). 320 rows of 4096 x 151936: 440 us
+// (with the soft cap in float 458), 905 TFLOP/s: 190 MB are written, and two and a
+// half tiles of rows need 160 of 128.
 // ANY: rows at any element's address, a last piece of less than eight columns
 // (loads to LDS take neither): one stage in registers, two in LDS.
 template <bool BF, bool ANY, int WM, int WN, int WK, int TM, int TN, int ST>
@@ -305,9 +315,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(Args a, int t
         for (int s = 0; s < TN; ++s) o.w[s] = *reinterpret_cast<const u32x4*>(from + (BM + wn + 16 * s + i) * 64);
 #pragma unroll
         for (int s = 0; s < TM; ++s) o.x[s] = *reinterpret_cast<const u32x4*>(from + (wm + 16 * s + i) * 64);
-#ifndef NOSB
         __builtin_amdgcn_sched_barrier(0);      // (and the reads ahead of the products)
-#endif
     };
     f32x4 acc[TN][TM] = {};
     auto multiply = [&](const Operands& o) {
@@ -489,6 +497,7 @@ hipError_t launch_linear(const Args& a, hipStream_t s) {
 extern "C" int ultima_hsamp_linear(const ultima_hsamp_linear_args* a, void* hip_stream) {
     using namespace hsamp;
     if (a == nullptr || a->x == nullptr || a->weight == nullptr || a->out == nullptr) return ULTIMA_HSAMP_ERR_INVALID;
+    if (a->out == a->x || a->out == a->weight || a->out == a->bias) return ULTIMA_HSAMP_ERR_INVALID;
     if (a->rows < 1 || a->in_dim < 1 || a->out_dim < 1 || a->groups < 1) return ULTIMA_HSAMP_ERR_INVALID;
     if (a->dtype != ULTIMA_HSAMP_BF16 && a->dtype != ULTIMA_HSAMP_F16) return ULTIMA_HSAMP_ERR_INVALID;
     if (a->out_dtype != a->dtype && a->out_dtype != ULTIMA_HSAMP_F32) return ULTIMA_HSAMP_ERR_INVALID;
@@ -514,7 +523,8 @@ extern "C" int ultima_hsamp_linear(const ultima_hsamp_linear_args* a, void* hip_
         !(a->out_group >= a->out_dim && og < a->out_stride && (a->groups - 1) * og + a->out_dim <= a->out_stride))
         return ULTIMA_HSAMP_ERR_INVALID;
     // 32-bit rows and columns; a launch counts its threads in 32 bits
-    if (a->groups > 65535 || std::max({a->rows, a->in_dim, a->out_dim}) > 1 << 30 || std::max(blocks_of(kForms[choose(*a)], *a), blocks_of(kForms[5], *a)) > 1 << 22)
+    if (a->groups > 65535 || std::max({a->rows, a->in_dim, a->out_dim}) > 1 << 30 ||
+        std::max(blocks_of(kForms[choose(*a)], *a), blocks_of(kForms[5], *a)) > 1 << 22)
         return ULTIMA_HSAMP_ERR_UNSUPPORTED;
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
     const hipError_t e = a->dtype == ULTIMA_HSAMP_BF16 ? launch_linear<true>(*a, s) : launch_linear<false>(*a, s);

@@ -4,7 +4,7 @@
 //
 // On logits:
 //   k_draft_start    clears the call's counters
-//   k_draft_stats    a wave per slice of a row (16 KB of logits): its maximum m_s
+//   k_draft_stats    a wave per slice of a row (8 KB of logits): its maximum m_s
 //                    and sum of exp((x - m_s) / T) in double, a greedy row's lowest
 //                    id of the maximum. Positions first, sequences second: the block
 //                    that completes a position's rows decides its draft, and blocks
@@ -16,6 +16,8 @@
 //                    sum of max(p - q, 0); the block that completes a sequence
 //                    finds the part where the running sum reaches u_draw, then the
 //                    id.
+//
+// On kept sets: k_verify_sets, one launch or two.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -30,14 +32,15 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kChunks = 16;                  // 16-byte loads of a lane per slice,
+constexpr int kChunks = 8;                   // 16-byte loads of a lane per slice,
 constexpr int kStep = 4;                     // of them a step, the next step's in flight
 constexpr int kSteps = kChunks / kStep;
-constexpr int kMaxParts = 8;                 // parts of a slice when a token is drawn
+constexpr int kMaxParts = 4;                 // parts of a slice when a token is drawn
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kFltMax = 3.402823466e38f;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 
@@ -227,7 +230,7 @@ struct Scale {
     }
 };
 
-// A row as a wave reads it: slices of 16 KB in 16-byte chunks, chunk j of a lane
+// A row as a wave reads it: slices of 8 KB in 16-byte chunks, chunk j of a lane
 // the (64 j + lane)-th.
 template <bool BF>
 struct Row {
@@ -528,6 +531,12 @@ __device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, i
     }
 }
 
+// Bound by the bytes of the rows that are read and, as much, by the exponentials beside
+// them: 64 sequences of 4 drafts over 151936 f32 logits 74 us, 283 MB at 3.8 TB/s (350 MB
+// are there, the drafts up to the rejected ones need 224); 256 of 8 in bf16 207 us, 758 MB
+// (1.3 GB there, 690 needed). One sequence of 4: 12 us, its start, one slice a wave and the
+// decisions one after the other. Four waves a SIMD: their registers; with more (5, 6, 8)
+// the large call takes 233, 284, 525 us, spills.
 template <bool BF, bool MASK, bool FAST>
 __global__ __launch_bounds__(kThreads, 4) void k_draft_stats(DraftArgs a) {
     using R = Row<BF>;
@@ -573,7 +582,8 @@ __global__ __launch_bounds__(kThreads, 4) void k_draft_stats(DraftArgs a) {
     if (wave == 0) decide<BF>(a, q, b, i, 0.0, table);
 }
 
-// FAST calls: the emitting rows' slices in double. (Greedy rows need none.)
+// FAST calls: the emitting rows' slices in double. (Greedy rows need none.) Bound by the
+// exponentials: 256 sequences, 155 MB, 59 us.
 template <bool BF, bool MASK>
 __global__ __launch_bounds__(kThreads, 4) void k_draft_exact(DraftArgs a) {
     __shared__ double table[32];
@@ -679,7 +689,9 @@ __device__ __forceinline__ int first_reaching(F value, int n, double base, doubl
     return last;
 }
 
-// TH threads a block, a wave per part of a slice (PARTS of them).
+// TH threads a block, a wave per part of a slice (PARTS of them). Few sequences: bound by
+// what waits for each other (statistics, part, count, parts' sums, the part again): one
+// 9 us. Many: two exponentials an id: 256 over 151936 92 us.
 template <bool BF, int TH, int PARTS>
 __global__ __launch_bounds__(TH) void k_draft_draw(DraftArgs a) {
     using R = Row<BF>;
@@ -880,60 +892,140 @@ __device__ __forceinline__ void find_id(const int32_t* const (&ids)[2], int (&n)
     }
 }
 
-constexpr int kEach = 8;       // entries of a thread per tile
-constexpr int kTiles = ULTIMA_HSAMP_MAX_VOCAB / (1024 * kEach);
+// One wave: where among the n ascending ids those from `low` to `high` begin and end.
+__device__ __forceinline__ void range_of(const int32_t* ids, int n, int low, int high, int& begin, int& end) {
+    const int lane = threadIdx.x & 63, key[2] = {low, high};
+    int from[2] = {}, left[2] = {n, n};
+    auto below = [&](int s, int v) { return s == 0 ? v < key[s] : v <= key[s]; };
+    while (left[0] > 64 || left[1] > 64) {
+        int piece[2], v[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            piece[s] = (left[s] + 63) >> 6;
+            v[s] = left[s] > 0 ? ids[from[s] + min(left[s], (lane + 1) * piece[s]) - 1] : 0;
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int skip = min(left[s], __popcll(__ballot(below(s, v[s]))) * piece[s]);
+            from[s] += skip;
+            left[s] = min(piece[s], left[s] - skip);
+        }
+    }
+    int v[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) v[s] = lane < left[s] ? ids[from[s] + lane] : 0;
+    begin = from[0] + __popcll(__ballot(lane < left[0] && below(0, v[0])));
+    end = from[1] + __popcll(__ballot(lane < left[1] && below(1, v[1])));
+}
 
-// One block per sequence. The drafts' probabilities by a wave per position; then the
-// emitting set in tiles of eight entries per thread, the drafter's entries of the
-// tile's ids through LDS, where each entry of the target's looks for its own.
-template <int TH>
-__global__ __launch_bounds__(TH) void k_verify_sets(ultima_hsamp_draft_sets d) {
-    constexpr int TILE = TH * kEach, NW = TH / 64, NT = TH == 1024 ? kTiles : 1;
-    __shared__ int32_t lq[TILE];
-    __shared__ float lp[TILE];
-    __shared__ double tiles[NT], waves[NW];
-    __shared__ int32_t starts[NT], first;
-    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, K = d.max_draft;
+constexpr int kEach = 8;                       // entries of a thread per tile
+constexpr int kSetThreads = 512;
+constexpr int kSetTile = kSetThreads * kEach;
+
+// A thread's eight entries at e of a set of n >= 1 (the last one's past the end).
+__device__ __forceinline__ void eight_of(const int32_t* ids, const float* probs, int e, int n, int (&id)[kEach], float (&p)[kEach]) {
+    if (e + kEach <= n) {
+#pragma unroll
+        for (int k = 0; k < kEach; k += 4) {
+            const u32x4 i4 = *reinterpret_cast<const u32x4_a4*>(ids + e + k), p4 = *reinterpret_cast<const u32x4_a4*>(probs + e + k);
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                id[k + f] = (int)i4[f];
+                p[k + f] = __uint_as_float(p4[f]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            id[k] = ids[min(e + k, n - 1)];
+            p[k] = probs[min(e + k, n - 1)];
+        }
+    }
+}
+
+struct SetsArgs {
+    ultima_hsamp_draft_sets d;
+    double* sums;            // [seqs][T] of the emitting set's tiles, and
+    int32_t* emits;          // [seqs] its position, -1: none (sets of several tiles)
+    int T;                   // tiles that set_cap holds
+    int blocks;              // per sequence
+};
+
+enum SetsPart { kSetsWhole, kSetsTiles, kSetsPick };
+
+// The drafts' probabilities by a wave per position; then the emitting set in tiles of
+// eight entries per thread, the drafter's entries of the tile's ids through LDS, where
+// each entry of the target's looks for its own. What bounds it are the chains of reads
+// that wait for each other (rows, counts, three or four steps of a search, a tile): 8 us
+// for one sequence of sets up to 64, 11 for 64 of up to 1024. Larger sets would follow
+// one block's tiles one after the other: 32 of up to 32768 ids 62 us, as here 24 + 16.
+//   kSetsWhole: sets of one tile, one block per sequence
+//   kSetsTiles: the tiles' sums, tiles shared out to a sequence's blocks (each finds
+//               the emitting position by itself)
+//   kSetsPick:  from these sums the tile, from it the token, one block per sequence
+template <int PART>
+__global__ __launch_bounds__(kSetThreads) void k_verify_sets(SetsArgs a) {
+    const ultima_hsamp_draft_sets& d = a.d;
+    constexpr int TILE = kSetTile, TH = kSetThreads, NW = TH / 64;
+    __shared__ __attribute__((aligned(16))) int32_t lq[TILE];
+    __shared__ __attribute__((aligned(16))) float lp[TILE];
+    __shared__ double waves[NW];
+    __shared__ int32_t first;
+    const int b = PART == kSetsTiles ? blockIdx.x / a.blocks : blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const int t0 = PART == kSetsTiles ? blockIdx.x % a.blocks : 0, K = d.max_draft;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Seq q = seq_of(d.n_draft, d.target_start, d.draft_start, b, K, d.rows, d.draft_rows);
     int32_t* out = d.out_tokens + (int64_t)b * (K + 1);
-    const bool certain = d.draft_idx == nullptr;
-    if (tid == 0) first = INT32_MAX;
-    bool bad = !q.ok;
-    if (!bad)
-        for (int i = tid; i <= q.n; i += TH) {
-            const int cp = d.kept_count[q.t0 + i];
-            bad = bad || cp < 0 || cp > d.set_cap;
-            if (!certain && i < q.n) {
-                const int cq = d.draft_count[q.d0 + i];
-                bad = bad || cq < 0 || cq > d.draft_cap;
+    const bool certain = d.draft_idx == nullptr, writes = PART != kSetsTiles || t0 == 0;
+    int m;
+    if (PART != kSetsPick) {
+        if (tid == 0) first = INT32_MAX;
+        bool bad = !q.ok, more = false;
+        if (!bad)
+            for (int i = tid; i <= q.n; i += TH) {
+                const int cp = d.kept_count[q.t0 + i];
+                bad = bad || cp < 0 || cp > d.set_cap;
+                more = more || cp > t0 * TILE;
+                if (!certain && i < q.n) {
+                    const int cq = d.draft_count[q.d0 + i];
+                    bad = bad || cq < 0 || cq > d.draft_cap;
+                }
+            }
+        if (__syncthreads_or(bad)) {
+            if (!writes) return;
+            for (int i = tid; i <= K; i += TH) out[i] = -1;
+            if (tid == 0) d.out_count[b] = 0;
+            if (PART == kSetsTiles && tid == 0) a.emits[b] = -1;
+            return;
+        }
+        if (!writes && !__syncthreads_or(more)) return;        // (no set of the sequence has this tile)
+        for (int i = wave; i < q.n; i += NW) {
+            const int tok = d.draft[q.d0 + i];
+            const double u = d.u_accept[q.d0 + i];
+            const int64_t tr = (int64_t)(q.t0 + i) * d.set_cap, dr = (int64_t)(q.d0 + i) * d.draft_cap;
+            const int32_t* const ids[2] = {d.kept_idx + tr, certain ? d.kept_idx : d.draft_idx + dr};
+            int n[2] = {d.kept_count[q.t0 + i], certain ? 0 : d.draft_count[q.d0 + i]}, at[2];
+            find_id(ids, n, tok, at);
+            const double p = at[0] >= 0 ? set_prob(d.kept_prob[tr + at[0]]) : 0.0;
+            const double qd = certain ? 1.0 : at[1] >= 0 ? set_prob(d.draft_prob[dr + at[1]]) : 0.0;
+            if (lane == 0) {
+                if (!(u * qd < p)) atomicMin(&first, i);
+                if (writes && d.accept_prob != nullptr)
+                    d.accept_prob[q.d0 + i] = p < qd ? (float)(p / qd) : p > 0.0 ? 1.0f : 0.0f;
             }
         }
-    if (__syncthreads_or(bad)) {
-        for (int i = tid; i <= K; i += TH) out[i] = -1;
-        if (tid == 0) d.out_count[b] = 0;
-        return;
+        __syncthreads();
+        m = min(first, q.n);
+        if (writes && d.accept_prob != nullptr)
+            for (int i = m + 1 + tid; i < q.n; i += TH) d.accept_prob[q.d0 + i] = -1.0f;
+        if (writes)
+            for (int i = tid; i <= K; i += TH)
+                if (i != m) out[i] = i < m ? d.draft[q.d0 + i] : -1;
+        if (PART == kSetsTiles && writes && tid == 0) a.emits[b] = m;
+    } else {
+        m = a.emits[b];
+        if (m < 0) return;
     }
-    for (int i = wave; i < q.n; i += NW) {
-        const int tok = d.draft[q.d0 + i];
-        const double u = d.u_accept[q.d0 + i];
-        const int64_t tr = (int64_t)(q.t0 + i) * d.set_cap, dr = (int64_t)(q.d0 + i) * d.draft_cap;
-        const int32_t* const ids[2] = {d.kept_idx + tr, certain ? d.kept_idx : d.draft_idx + dr};
-        int n[2] = {d.kept_count[q.t0 + i], certain ? 0 : d.draft_count[q.d0 + i]}, at[2];
-        find_id(ids, n, tok, at);
-        const double p = at[0] >= 0 ? set_prob(d.kept_prob[tr + at[0]]) : 0.0;
-        const double qd = certain ? 1.0 : at[1] >= 0 ? set_prob(d.draft_prob[dr + at[1]]) : 0.0;
-        if (lane == 0) {
-            if (!(u * qd < p)) atomicMin(&first, i);
-            if (d.accept_prob != nullptr) d.accept_prob[q.d0 + i] = p < qd ? (float)(p / qd) : p > 0.0 ? 1.0f : 0.0f;
-        }
-    }
-    __syncthreads();
-    const int m = min(first, q.n);
-    if (d.accept_prob != nullptr)
-        for (int i = m + 1 + tid; i < q.n; i += TH) d.accept_prob[q.d0 + i] = -1.0f;
-    for (int i = tid; i <= K; i += TH)
-        if (i != m) out[i] = i < m ? d.draft[q.d0 + i] : -1;
     const int n = d.kept_count[q.t0 + m];
     const int32_t* pi = d.kept_idx + (int64_t)(q.t0 + m) * d.set_cap;
     const float* pp = d.kept_prob + (int64_t)(q.t0 + m) * d.set_cap;
@@ -943,102 +1035,129 @@ __global__ __launch_bounds__(TH) void k_verify_sets(ultima_hsamp_draft_sets d) {
     const float* qp = two ? d.draft_prob + (int64_t)(q.d0 + m) * d.draft_cap : nullptr;
     const int nq = two ? d.draft_count[q.d0 + m] : 0;
 
-    // A tile's weights, the thread's eight consecutive entries; q0: the drafter's
-    // first entry that may matter, left at the first that may for the next tile.
+    // A tile's weights, the thread's eight consecutive entries.
     int id[kEach];
     double w[kEach];
-    auto tile = [&](int t, int& q0, bool residual) {
-        const int e0 = t * TILE + tid * kEach;
-        if (e0 + kEach <= n) {
+    auto tile = [&](int t, bool residual) {
+        float p[kEach];
+        eight_of(pi, pp, t * TILE + tid * kEach, n, id, p);
 #pragma unroll
-            for (int k = 0; k < kEach; k += 4) {
-                const u32x4 i4 = *reinterpret_cast<const u32x4_a4*>(pi + e0 + k);
-                const u32x4 p4 = *reinterpret_cast<const u32x4_a4*>(pp + e0 + k);
-#pragma unroll
-                for (int f = 0; f < 4; ++f) {
-                    id[k + f] = (int)i4[f];
-                    w[k + f] = set_prob(__uint_as_float(p4[f]));
-                }
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < kEach; ++k) {
-                const int e = min(e0 + k, n - 1);
-                id[k] = pi[e];
-                w[k] = e0 + k < n ? set_prob(pp[e]) : 0.0;
-            }
-        }
+        for (int k = 0; k < kEach; ++k) w[k] = t * TILE + tid * kEach + k < n ? set_prob(p[k]) : 0.0;
         if (residual && reject && certain)
 #pragma unroll
             for (int k = 0; k < kEach; ++k)
                 if (id[k] == point) w[k] = 0.0;
         if (!residual || !two) return;
-        const int last = pi[min(t * TILE + TILE, n) - 1];
-        for (;;) {
-            const int c = min(TILE, nq - q0);
-            if (c <= 0) break;
-            __syncthreads();
-            for (int k = tid; k < c; k += TH) {
-                lq[k] = qi[q0 + k];
-                lp[k] = qp[q0 + k];
+        // the drafter's ids of the tile's range: all of them in LDS, or the ends of as
+        // many pieces as it holds, whose ids are looked through where they are
+        int begin = 0, end = nq;
+        if (nq > TILE) range_of(qi, nq, pi[t * TILE], pi[min(t * TILE + TILE, n) - 1], begin, end);
+        const int in = max(0, end - begin), step = (in + TILE - 1) / TILE;
+        if (in == 0) return;
+        const int c = (in + step - 1) / step;
+        int qid[kEach];
+        if (step == 1) {
+            eight_of(qi, qp, begin + tid * kEach, nq, qid, p);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) qid[k] = qi[begin + (int)min((int64_t)in, (int64_t)(tid * kEach + k + 1) * step) - 1];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kEach; k += 4) {
+            *reinterpret_cast<u32x4*>(&lq[tid * kEach + k]) =
+                u32x4{(uint32_t)qid[k], (uint32_t)qid[k + 1], (uint32_t)qid[k + 2], (uint32_t)qid[k + 3]};
+            *reinterpret_cast<f32x4*>(&lp[tid * kEach + k]) = f32x4{p[k], p[k + 1], p[k + 2], p[k + 3]};
+        }
+        __syncthreads();
+        // the number of the LDS ids below each entry: of the first and the last in
+        // step, then of those between within these bounds
+        int lo[kEach] = {};
+        for (int half = TILE; half > 0; half >>= 1)
+#pragma unroll
+            for (int k = 0; k < kEach; k += kEach - 1) {
+                const int mid = lo[k] + half;
+                if (mid <= c && lq[mid - 1] < id[k]) lo[k] = mid;
             }
-            __syncthreads();
-            // the number of the drafter's ids below each entry: of the first and the
-            // last in step, then of those between within these bounds
-            int lo[kEach] = {};
-            for (int half = TILE; half > 0; half >>= 1)
+        const int span = lo[kEach - 1] - lo[0];
 #pragma unroll
-                for (int k = 0; k < kEach; k += kEach - 1) {
-                    const int mid = lo[k] + half;
-                    if (mid <= c && lq[mid - 1] < id[k]) lo[k] = mid;
-                }
-            const int span = lo[kEach - 1] - lo[0];
+        for (int k = 1; k < kEach - 1; ++k) lo[k] = lo[0];
+        for (int half = span > 0 ? 1 << (31 - __clz(span)) : 0; __any(half > 0); half >>= 1)
 #pragma unroll
-            for (int k = 1; k < kEach - 1; ++k) lo[k] = lo[0];
-            for (int half = span > 0 ? 1 << (31 - __clz(span)) : 0; __any(half > 0); half >>= 1)
-#pragma unroll
-                for (int k = 1; k < kEach - 1; ++k) {
-                    const int mid = lo[k] + half;
-                    if (half > 0 && mid <= lo[kEach - 1] && lq[mid - 1] < id[k]) lo[k] = mid;
-                }
+            for (int k = 1; k < kEach - 1; ++k) {
+                const int mid = lo[k] + half;
+                if (half > 0 && mid <= lo[kEach - 1] && lq[mid - 1] < id[k]) lo[k] = mid;
+            }
+        if (step == 1) {
 #pragma unroll
             for (int k = 0; k < kEach; ++k)
                 if (lo[k] < c && lq[lo[k]] == id[k]) w[k] = fmax(w[k] - set_prob(lp[lo[k]]), 0.0);
-            if (lq[c - 1] >= last) break;          // (what follows is beyond the tile)
-            q0 += c;
+            return;
         }
+        int base[kEach], at[kEach];
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            base[k] = begin + min(lo[k], c - 1) * step;
+            at[k] = 0;
+        }
+        for (int half = 1 << (31 - __clz(step - 1)); half > 0; half >>= 1)
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                const int mid = at[k] + half;
+                if (qi[min(base[k] + mid, end) - 1] < id[k] && base[k] + mid < end) at[k] = mid;
+            }
+#pragma unroll
+        for (int k = 0; k < kEach; ++k)
+            if (qi[base[k] + at[k]] == id[k]) w[k] = fmax(w[k] - set_prob(qp[base[k] + at[k]]), 0.0);
     };
-    const int T = (n + TILE - 1) / TILE;
-    auto tile_sum = [&]() {
+    auto mine = [&]() {
         double s = 0.0;
 #pragma unroll
         for (int k = 0; k < kEach; ++k) s += w[k];
         return s;
     };
-    bool residual = true;
-    double total = 0.0;
-    for (int pass = 0; pass < 2 && n > 0; ++pass) {
-        int q0 = 0;
-        for (int t = 0; t < T; ++t) {
-            const int begin = q0;
-            tile(t, q0, residual);
-            const double s = wave_sum(tile_sum());
-            __syncthreads();
-            if (lane == 0) waves[wave] = s;
-            __syncthreads();
-            if (tid == 0) {
-                double v = 0.0;
-                for (int k = 0; k < NW; ++k) v += waves[k];
-                tiles[min(t, NT - 1)] = v;
-                starts[min(t, NT - 1)] = begin;
-            }
-        }
+    // a tile's sum, the waves' in LDS; for every thread
+    auto tile_sum = [&](int t, bool residual) {
+        tile(t, residual);
+        const double s = wave_sum(mine());
         __syncthreads();
+        if (lane == 0) waves[wave] = s;
+        __syncthreads();
+        double v = 0.0;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) v += waves[k];
+        return v;
+    };
+    const int T = (n + TILE - 1) / TILE;
+    double* sums = a.sums + (int64_t)b * a.T;
+    auto all_tiles = [&](int from, int step, bool residual) {
+        for (int t = from; t < T; t += step) {
+            const double s = tile_sum(t, residual);
+            if (tid == 0) sums[t] = s;
+        }
+    };
+    if (PART == kSetsTiles) {
+        all_tiles(t0, a.blocks, true);
+        return;
+    }
+    double total = 0.0, run = 0.0;
+    int at = 0;
+    // (p = q to the last bit: the weights are p's)
+    for (int pass = 0; pass < 2 && n > 0 && !(total > 0.0); ++pass) {
+        if (PART == kSetsWhole) {
+            total = tile_sum(0, pass == 0);
+            continue;
+        }
+        if (pass > 0) {
+            all_tiles(0, 1, false);
+            __syncthreads();
+        }
         total = 0.0;
-        for (int t = lane; t < T; t += 64) total += tiles[t];
+        for (int t = lane; t < T; t += 64) total += sums[t];
         total = wave_sum(total);
-        if (total > 0.0) break;
-        residual = false;     // p = q to the last bit: the weights are p's
+        if (!(total > 0.0)) continue;
+        at = max(0, first_reaching([&](int t) { return sums[t]; }, T, 0.0, d.u_draw[b] * total, run));
+        tile_sum(at, pass == 0);
     }
     if (!(total > 0.0)) {
         if (tid == 0) {
@@ -1048,24 +1167,14 @@ __global__ __launch_bounds__(TH) void k_verify_sets(ultima_hsamp_draft_sets d) {
         return;
     }
     const double want = d.u_draw[b] * total;
-    double run;
-    const int at = max(0, first_reaching([&](int t) { return tiles[t]; }, T, 0.0, want, run));
-    if (T > 1) {
-        int q0 = starts[at];
-        tile(at, q0, residual);
-    }
     // the wave, the thread, the entry
-    const double mine = tile_sum(), s = wave_sum(mine);
-    __syncthreads();
-    if (lane == 0) waves[wave] = s;
-    __syncthreads();
     const int hit = max(0, first_reaching([&](int k) { return waves[k]; }, NW, run, want, run));
     if (wave != hit) return;
-    const double cum = run + wave_incl_sum(mine);
-    const u64 reach = __ballot(mine > 0.0 && cum >= want), any = __ballot(mine > 0.0);
+    const double own = mine(), cum = run + wave_incl_sum(own);
+    const u64 reach = __ballot(own > 0.0 && cum >= want), any = __ballot(own > 0.0);
     const int l = reach != 0 ? __ffsll((long long)reach) - 1 : any != 0 ? 63 - __clzll((long long)any) : 0;
     if (lane == l) {
-        double c = cum - mine;
+        double c = cum - own;
         int token = id[0];
         bool done = false;
 #pragma unroll
@@ -1083,9 +1192,9 @@ __global__ __launch_bounds__(TH) void k_verify_sets(ultima_hsamp_draft_sets d) {
 
 // Float exponentials first, and the emitting rows (one or two of the 2 max_draft + 1)
 // again in double: for bf16 rows, whose doubles take longer than their bytes, where
-// that is more than a launch. 256 sequences of 8 drafts over 151936 ids: 203 + 66 us
-// against 357; of 4 drafts in f32 64 + 22 against 74; 37 of 7 over 50257 in bf16
-// (26 MB) 21 + 15 against 30.
+// that is more than a launch. 256 sequences of 8 drafts over 151936 ids: 207 + 60 us
+// against 357; of 4 drafts in f32 66 + 19 against 74; 37 of 7 over 50257 in bf16
+// (26 MB) 20 + 9 against 26.
 constexpr int64_t kFastBytes = (int64_t)128 << 20;
 
 struct Layout {
@@ -1121,22 +1230,31 @@ hipError_t launch_draft(const DraftArgs& a, hipStream_t s) {
                        dim3(kThreads), 0, s, a);
     const bool mask = a.d.mask != nullptr || a.d.draft_mask != nullptr;
     const dim3 emitting((uint32_t)((int64_t)a.d.seqs * a.sides * blocks(a.S, kWaves)));
-    if (mask && a.fast) hipLaunchKernelGGL((k_draft_stats<BF, true, true>), rows, dim3(kThreads), 0, s, a);
-    else if (mask) hipLaunchKernelGGL((k_draft_stats<BF, true, false>), rows, dim3(kThreads), 0, s, a);
-    else if (a.fast) hipLaunchKernelGGL((k_draft_stats<BF, false, true>), rows, dim3(kThreads), 0, s, a);
-    else hipLaunchKernelGGL((k_draft_stats<BF, false, false>), rows, dim3(kThreads), 0, s, a);
-    if (mask && a.fast) hipLaunchKernelGGL((k_draft_exact<BF, true>), emitting, dim3(kThreads), 0, s, a);
-    else if (a.fast) hipLaunchKernelGGL((k_draft_exact<BF, false>), emitting, dim3(kThreads), 0, s, a);
+    auto stats = [&](auto masked, auto fast) {
+        constexpr bool MASK = decltype(masked)::value, FAST = decltype(fast)::value;
+        hipLaunchKernelGGL((k_draft_stats<BF, MASK, FAST>), rows, dim3(kThreads), 0, s, a);
+        if constexpr (FAST) hipLaunchKernelGGL((k_draft_exact<BF, MASK>), emitting, dim3(kThreads), 0, s, a);
+    };
+    auto by_mask = [&](auto fast) {
+        if (mask) stats(std::true_type(), fast);
+        else stats(std::false_type(), fast);
+    };
+    if constexpr (BF) {
+        if (a.fast) by_mask(std::true_type());
+        else by_mask(std::false_type());
+    } else {
+        by_mask(std::false_type());
+    }
     auto draw = [&](auto th, auto parts) {
         constexpr int TH = decltype(th)::value, PARTS = decltype(parts)::value;
         hipLaunchKernelGGL((k_draft_draw<BF, TH, PARTS>), dim3((uint32_t)(a.d.seqs * blocks((int64_t)a.S * PARTS, TH / 64))),
                            dim3(TH), 0, s, a);
     };
     // few rows: more waves a slice, for its latency; many: fewer (each starts with the
-    // sequence's own data), in smaller blocks. 8 of 512 threads against 4 of 256: one
-    // sequence 8.9 and 12.2 us, 64 (f32) 32 and 30, 256 (bf16) 112 and 94.
-    if ((int64_t)a.d.seqs * a.S < 4096) draw(std::integral_constant<int, 512>(), std::integral_constant<int, 8>());
-    else draw(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
+    // sequence's own data), in smaller blocks. 4 of 512 threads against 2 of 256: one
+    // sequence 9.3 and 11.4 us, 64 (f32) 33 and 30, 256 (bf16) 112 and 97.
+    if ((int64_t)a.d.seqs * a.S < 4096) draw(std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
+    else draw(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
     return hipGetLastError();
 }
 
@@ -1194,6 +1312,12 @@ extern "C" int ultima_hsamp_verify_draft(const ultima_hsamp_draft* d, void* hip_
     return e == hipSuccess ? ULTIMA_HSAMP_OK : ULTIMA_HSAMP_ERR_HIP;
 }
 
+extern "C" int64_t ultima_hsamp_verify_sets_work_bytes(int32_t seqs, int32_t set_cap) {
+    if (seqs < 1 || set_cap < 1 || set_cap > ULTIMA_HSAMP_MAX_VOCAB) return -1;
+    const int64_t tiles = ((int64_t)set_cap + hsamp::kSetTile - 1) / hsamp::kSetTile;
+    return tiles == 1 ? 0 : seqs * (tiles * 8 + 4);
+}
+
 extern "C" int ultima_hsamp_verify_sets(const ultima_hsamp_draft_sets* d, void* hip_stream) {
     using namespace hsamp;
     if (d == nullptr || d->seqs < 1 || d->max_draft < 0 || d->max_draft > ULTIMA_HSAMP_MAX_DRAFT)
@@ -1210,10 +1334,22 @@ extern "C" int ultima_hsamp_verify_sets(const ultima_hsamp_draft_sets* d, void* 
         return ULTIMA_HSAMP_ERR_INVALID;
     if (d->target_start == nullptr && (int64_t)d->seqs * (d->max_draft + 1) > d->rows) return ULTIMA_HSAMP_ERR_INVALID;
     if (d->draft_start == nullptr && (int64_t)d->seqs * d->max_draft > d->draft_rows) return ULTIMA_HSAMP_ERR_INVALID;
-    // sets of one tile of 4096, or of tiles of 8192
-    if (d->set_cap <= 512 * kEach)
-        hipLaunchKernelGGL(k_verify_sets<512>, dim3(d->seqs), dim3(512), 0, static_cast<hipStream_t>(hip_stream), *d);
-    else
-        hipLaunchKernelGGL(k_verify_sets<1024>, dim3(d->seqs), dim3(1024), 0, static_cast<hipStream_t>(hip_stream), *d);
+    if (d->seqs > 1 << 21) return ULTIMA_HSAMP_ERR_UNSUPPORTED;        // (a launch's threads in 32 bits)
+    SetsArgs a;
+    a.d = *d;
+    a.T = (d->set_cap + kSetTile - 1) / kSetTile;
+    a.sums = static_cast<double*>(d->work);
+    a.emits = reinterpret_cast<int32_t*>(a.sums + (int64_t)d->seqs * a.T);
+    hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    if (a.T == 1) {
+        a.blocks = 1;
+        hipLaunchKernelGGL(k_verify_sets<kSetsWhole>, dim3(d->seqs), dim3(kSetThreads), 0, s, a);
+    } else {
+        if (d->work == nullptr || reinterpret_cast<uintptr_t>(d->work) % 16 != 0) return ULTIMA_HSAMP_ERR_INVALID;
+        // a tile a block up to the 1024 blocks that the card holds at once
+        a.blocks = std::clamp(1024 / d->seqs, 1, a.T);
+        hipLaunchKernelGGL(k_verify_sets<kSetsTiles>, dim3(d->seqs * a.blocks), dim3(kSetThreads), 0, s, a);
+        hipLaunchKernelGGL(k_verify_sets<kSetsPick>, dim3(d->seqs), dim3(kSetThreads), 0, s, a);
+    }
     return hipGetLastError() == hipSuccess ? ULTIMA_HSAMP_OK : ULTIMA_HSAMP_ERR_HIP;
 }

@@ -190,6 +190,7 @@ class DraftSets(ctypes.Structure):
         ("draft_start", ctypes.c_void_p),
         ("u_accept", ctypes.c_void_p),
         ("u_draw", ctypes.c_void_p),
+        ("work", ctypes.c_void_p),
         ("out_tokens", ctypes.c_void_p),
         ("out_count", ctypes.c_void_p),
         ("accept_prob", ctypes.c_void_p),
@@ -289,6 +290,8 @@ def lib() -> ctypes.CDLL:
         L.ultima_hsamp_verify_draft_work_bytes.argtypes = [i32, i32, i32]
         L.ultima_hsamp_verify_draft.restype = ctypes.c_int
         L.ultima_hsamp_verify_draft.argtypes = [ctypes.POINTER(Draft), vp]
+        L.ultima_hsamp_verify_sets_work_bytes.restype = i64
+        L.ultima_hsamp_verify_sets_work_bytes.argtypes = [i32, i32]
         L.ultima_hsamp_verify_sets.restype = ctypes.c_int
         L.ultima_hsamp_verify_sets.argtypes = [ctypes.POINTER(DraftSets), vp]
         L.ultima_hsamp_linear.restype = ctypes.c_int
@@ -564,6 +567,16 @@ def _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_
     return out
 
 
+def _work(work, need, dev, what):
+    """The caller's scratch, looked over, or scratch of the current stream."""
+    import torch
+    if work is None:
+        return torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    if work.device != dev or not work.is_contiguous() or work.numel() * work.element_size() < need:
+        _refuse(f"{what}: work must be {need} contiguous bytes on {dev}")
+    return work
+
+
 def verify_draft(logits, draft, u_accept, u_draw, max_draft: int, draft_logits=None, temperature=None,
                  draft_temperature=None, mask=None, draft_mask=None, n_draft=None, target_start=None,
                  draft_start=None, accept: bool = True, work=None, outputs=None, stream=None):
@@ -613,11 +626,7 @@ def verify_draft(logits, draft, u_accept, u_draw, max_draft: int, draft_logits=N
             a.draft_mask, a.draft_mask_stride = at, stride
     a.temperature = _vector(temperature, B, f32, dev, what, "temperature")
     a.draft_temperature = _vector(draft_temperature, B, f32, dev, what, "draft_temperature")
-    need = lib().ultima_hsamp_verify_draft_work_bytes(B, a.max_draft, V)
-    if work is None:
-        work = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-    elif work.device != dev or not work.is_contiguous() or work.numel() * work.element_size() < need:
-        _refuse(f"verify_draft: work must be {need} contiguous bytes on {dev}")
+    work = _work(work, lib().ultima_hsamp_verify_draft_work_bytes(B, a.max_draft, V), dev, what)
     a.work = work.data_ptr()
     _launch(lib().ultima_hsamp_verify_draft, a, dev, what)
     return out
@@ -625,12 +634,12 @@ def verify_draft(logits, draft, u_accept, u_draw, max_draft: int, draft_logits=N
 
 def verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_draft: int, draft_idx=None,
                 draft_prob=None, draft_count=None, n_draft=None, target_start=None, draft_start=None,
-                accept: bool = True, outputs=None, stream=None):
+                accept: bool = True, work=None, outputs=None, stream=None):
     """ultima_hsamp_verify_sets on torch tensors of one device: drafted tokens
     against the kept sets that run() leaves for the target's rows (kept_idx int32
     [R, cap], kept_prob f32 [R, cap], kept_count int32 [R]) and, unless the drafts
     are certain, for the drafter's. The other arguments and the result as in
-    verify_draft."""
+    verify_draft; work: ultima_hsamp_verify_sets_work_bytes() bytes."""
     import torch
     what = "verify_sets"
     dev = kept_idx.device
@@ -639,8 +648,10 @@ def verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_dr
     there = _elsewhere(dev, stream)
     if there is not None:
         with there:
+            if work is not None and stream is not None:
+                work.record_stream(stream)
             return verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_draft, draft_idx, draft_prob,
-                               draft_count, n_draft, target_start, draft_start, accept, outputs)
+                               draft_count, n_draft, target_start, draft_start, accept, work, outputs)
 
     def sets(idx, prob, count, rows, names):
         if prob is None or count is None or idx.dtype != torch.int32 or prob.dtype != torch.float32 or \
@@ -663,6 +674,10 @@ def verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_dr
             a.draft_idx, a.draft_prob, a.draft_count = at
     elif draft_prob is not None or draft_count is not None:
         _refuse("verify_sets: draft_prob and draft_count go with draft_idx")
+    need = lib().ultima_hsamp_verify_sets_work_bytes(a.seqs, a.set_cap)
+    if need > 0 or work is not None:
+        work = _work(work, need, dev, what)
+        a.work = work.data_ptr()
     _launch(lib().ultima_hsamp_verify_sets, a, dev, what)
     return out
 
