@@ -40,6 +40,7 @@ constexpr float kNegInf = -__builtin_inff();
 constexpr float kFltMax = 3.402823466e38f;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
@@ -59,9 +60,16 @@ __device__ const double kPow[32] = {
     0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
     0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
 
+// (in LDS without (k & 31) << 15 in the upper half: adding k << 15 there then adds
+// k >> 5 to the exponent)
 __device__ __forceinline__ void load_table(double* t) {
-    if (threadIdx.x < 32) t[threadIdx.x] = kPow[threadIdx.x];
+    const int k = threadIdx.x;
+    if (k < 32) t[k] = __hiloint2double(__double2hiint(kPow[k]) - (k << 15), __double2loint(kPow[k]));
     __syncthreads();
+}
+__device__ __forceinline__ double power(const double* table, int k) {
+    const double b = table[k & 31];
+    return __hiloint2double(__double2hiint(b) + (k << 15), __double2loint(b));
 }
 
 constexpr double kPerE = 46.166241308446828384;          // 32 / ln 2
@@ -78,9 +86,8 @@ __device__ __forceinline__ double exp32(double d, double c, const double* table)
     double p = __builtin_fma(kPoly[3], f, kPoly[2]);
     p = __builtin_fma(p, f, kPoly[1]);
     p = __builtin_fma(p, f, kPoly[0]);
-    const double b = table[k & 31];
-    const double v = __builtin_fma(b * f, p, b);
-    return __hiloint2double(__double2hiint(v) + ((k & ~31) << 15), __double2loint(v));
+    const double b = power(table, k);
+    return __builtin_fma(b * f, p, b);
 }
 
 // N of them side by side, whose chains of operations overlap.
@@ -90,7 +97,7 @@ __device__ __forceinline__ void exp32n(const double (&d)[N], double c, const dou
 #pragma unroll
     for (int n = 0; n < N; ++n) u[n] = __builtin_fma(d[n], c, kRound);
 #pragma unroll
-    for (int n = 0; n < N; ++n) b[n] = table[__double2loint(u[n]) & 31];
+    for (int n = 0; n < N; ++n) b[n] = power(table, __double2loint(u[n]));
 #pragma unroll
     for (int n = 0; n < N; ++n) f[n] = kRound - u[n];
 #pragma unroll
@@ -105,9 +112,6 @@ __device__ __forceinline__ void exp32n(const double (&d)[N], double c, const dou
     for (int n = 0; n < N; ++n) f[n] = b[n] * f[n];
 #pragma unroll
     for (int n = 0; n < N; ++n) v[n] = __builtin_fma(f[n], p[n], b[n]);
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-        v[n] = __hiloint2double(__double2hiint(v[n]) + ((__double2loint(u[n]) & ~31) << 15), __double2loint(v[n]));
 }
 
 struct SliceStat {
@@ -224,6 +228,17 @@ struct Scale {
         for (int n = 0; n < N; ++n) d[n] = (double)__builtin_amdgcn_fmed3f(x[n], lo, kFltMax) - md;
         exp32n(d, c, table, v);
     }
+    // exactly 0 for what is not allowed and what lies below lo
+    __device__ __forceinline__ void of4(const float (&x)[4], const double* table, double (&v)[4]) const {
+        some(x, table, v);
+        const bool all = (x[0] > lo) & (x[1] > lo) & (x[2] > lo) & (x[3] > lo);
+        if (__ballot(!all) == 0) return;         // (a compare a value instead of three instructions)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            asm volatile("" : "+v"(v[n]));       // (else it is done without the branch)
+            v[n] = x[n] > lo ? v[n] : 0.0;
+        }
+    }
     __device__ __forceinline__ double of(float x, const double* table) const {
         if (!fast) return weight_of(clean(x), m, c, table);
         return x > lo ? some(x, table) : 0.0;
@@ -276,6 +291,16 @@ struct Row {
     }
     __device__ __forceinline__ uint32_t bits(int e0) const {
         return mask != nullptr && e0 < V ? mask[e0 >> 5] >> (e0 & 31) : 0xFFFFFFFFu;
+    }
+    // a chunk's ids that the bits leave out as -inf
+    __device__ __forceinline__ static u32x4 masked(u32x4 w, uint32_t bits) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+            if ((bits >> k & 1u) == 0) {
+                if (BF) w[k / 2] = k & 1 ? (w[k / 2] & 0xFFFFu) | 0xFF800000u : (w[k / 2] & 0xFFFF0000u) | 0xFF80u;
+                else w[k % 4] = 0xFF800000u;
+            }
+        return w;
     }
     // id k of a chunk: its logit, -inf where it is masked
     __device__ __forceinline__ static float raw(const u32x4& w, uint32_t bits, int k) {
@@ -406,7 +431,7 @@ __device__ __forceinline__ bool decide(const DraftArgs& a, const Seq& q, int b, 
 //
 // FAST: exponentials in float (twice the rate of those in double, which bound the
 // pass: 2304 + 2048 bf16 rows of 151936 525 us against 230). A slice's sum is then off
-// by at most 3e-6 of it: per term 3 |z| 2^-24 from the exponent z = (x - m) / T and 2^-23
+// by at most 3e-6 of it: per term 2 |z| 2^-24 from the exponent z = (x - m) / T and 2^-23
 // from exp2, where the terms' mean |z| is at most ln V < 17 (the entropy's bound);
 // 9 2^-24 from the float additions. Enough to decide most drafts (kUnsure below), not
 // to draw a token.
@@ -418,33 +443,57 @@ __device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, i
         u32x4 x[kStep];
         uint32_t bits[MASK ? kStep : 1];
     };
-    auto load = [&](Step& h, int n) {
+    auto load = [&](Step& h, int n) {          // a step wholly within the row
         const int e0 = n * (R::SLICE / kSteps) + lane * R::VEC;
-        if ((n + 1) * (R::SLICE / kSteps) <= r.V) {
 #pragma unroll
-            for (int j = 0; j < kStep; ++j) {
-                if (BF) h.x[j] = *reinterpret_cast<const u32x4_a2*>(static_cast<const uint16_t*>(r.row) + e0 + j * 64 * R::VEC);
-                else h.x[j] = *reinterpret_cast<const u32x4_a4*>(static_cast<const float*>(r.row) + e0 + j * 64 * R::VEC);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < kStep; ++j) h.x[j] = r.chunk(e0 + j * 64 * R::VEC);
+        for (int j = 0; j < kStep; ++j) {
+            if (BF) h.x[j] = *reinterpret_cast<const u32x4_a2*>(static_cast<const uint16_t*>(r.row) + e0 + j * 64 * R::VEC);
+            else h.x[j] = *reinterpret_cast<const u32x4_a4*>(static_cast<const float*>(r.row) + e0 + j * 64 * R::VEC);
         }
         if (MASK)
 #pragma unroll
-            for (int j = 0; j < kStep; ++j) h.bits[MASK ? j : 0] = r.bits(e0 + j * 64 * R::VEC);
+            for (int j = 0; j < kStep; ++j) h.bits[MASK ? j : 0] = r.mask != nullptr ? r.mask[(e0 + j * 64 * R::VEC) >> 5] : 0xFFFFFFFFu;
+        if (MASK)
+#pragma unroll
+            for (int j = 0; j < kStep; ++j) h.bits[MASK ? j : 0] >>= (e0 + j * 64 * R::VEC) & 31;
     };
     float m = kNegInf;       // of the slice so far
     double sum = 0.0;        // the lane's, at m
     int at = INT32_MAX;
     auto add = [&](Step& h, int n) {
         auto value = [&](int j, int k) { return R::raw(h.x[j], MASK ? h.bits[MASK ? j : 0] : 0xFFFFFFFFu, k); };
-        float top = kNegInf;
+        // the maximum by the bits as whole numbers, right where it comes out as a finite
+        // float >= 0: half an instruction a value
+        float top = -1.0f;
+        if (!MASK) {
+            int t = INT32_MIN;
+            if (BF) {
+                s16x2 v = __builtin_bit_cast(s16x2, 0x80008000u);
 #pragma unroll
-        for (int j = 0; j < kStep; ++j)
+                for (int j = 0; j < kStep; ++j)
 #pragma unroll
-            for (int k = 0; k < R::VEC; ++k) top = fmaxf(top, value(j, k));
-        top = fminf(wave_max(top), kFltMax);
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t two = h.x[j][k];       // (a cast of the element itself takes the first)
+                        v = __builtin_elementwise_max(v, __builtin_bit_cast(s16x2, two));
+                    }
+                t = max((int)v[0], (int)v[1]) << 16;
+            } else {
+#pragma unroll
+                for (int j = 0; j < kStep; ++j)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) t = max(t, (int)h.x[j][k]);
+            }
+            t = (int)(wave_max_u32((uint32_t)t ^ 0x80000000u) ^ 0x80000000u);
+            if (t >= 0 && t < 0x7F800000) top = __int_as_float(t);
+        }
+        if (top < 0.0f) {
+            top = kNegInf;
+#pragma unroll
+            for (int j = 0; j < kStep; ++j)
+#pragma unroll
+                for (int k = 0; k < R::VEC; ++k) top = fmaxf(top, value(j, k));
+            top = fminf(wave_max(top), kFltMax);
+        }
         // (the values are unpacked again below: kept, they take twice the registers)
 #pragma unroll
         for (int j = 0; j < kStep; ++j) asm volatile("" : "+v"(h.x[j]));
@@ -468,11 +517,13 @@ __device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, i
         const double per2 = c * 0.03125;             // log2 e / T
         const float flo = (float)((double)m - 160.0 / per2);
         const double flow = ((double)m - (double)flo) * per2;
-        if (FAST && flo > -3e38f && flow > 150.0 && flow < 170.0) {
-            // float exponentials, the factor in two floats; logits clamped to flo, whose
-            // weight is 0 (not for the temperatures that Scale leaves out either); the
-            // lane's four at a time in float, then in double
-            const float ch = (float)per2, cl = (float)(per2 - (double)ch);
+        const float ch = (float)per2, mch = (float)((double)m * per2);
+        if (FAST && flo > -3e38f && flow > 150.0 && flow < 170.0 && fabsf(mch) < 4096.0f) {
+            // float exponentials of x ch - mch; what the rounding of mch moves all of them
+            // by (below 2^-12) is taken out of their sum to the first order. Logits clamped
+            // to flo, whose weight is 0 (not for the temperatures that Scale leaves out
+            // either); the lane's four at a time in float, then in double
+            const double moved = 1.0 - ((double)m * (double)ch - (double)mch) * 0.693147180559945309;
             float part = 0.0f;
 #pragma unroll
             for (int j = 0; j < kStep; ++j)
@@ -481,12 +532,12 @@ __device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, i
                     float v[4];
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
-                        const float d = __builtin_amdgcn_fmed3f(value(j, k + n), flo, kFltMax) - m;
-                        v[n] = __builtin_amdgcn_exp2f(__builtin_fmaf(d, ch, d * cl));
+                        const float x = __builtin_amdgcn_fmed3f(value(j, k + n), flo, kFltMax);
+                        v[n] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, ch, -mch));
                     }
                     part += (v[0] + v[1]) + (v[2] + v[3]);
                 }
-            sum += (double)part;
+            sum += (double)part * moved;
             return;
         }
         const Scale e(m, c);
@@ -512,15 +563,7 @@ __device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, i
             }
         }
     };
-    Step h0, h1;
-    if (s0 < s1) load(h0, kSteps * s0);
-    for (int s = s0; s < s1; ++s) {
-        for (int n = kSteps * s; n < kSteps * (s + 1); n += 2) {
-            load(h1, n + 1);
-            add(h0, n);
-            load(h0, min(n + 2, kSteps * s1 - 2));
-            add(h1, n + 1);
-        }
+    auto done = [&](int s) {
         const double z = wave_sum(sum);
         if (lane == 0)
             put_stat(to + s,
@@ -528,7 +571,34 @@ __device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, i
         m = kNegInf;
         sum = 0.0;
         at = INT32_MAX;
+    };
+    // whole slices, their loads without a branch: else the compiler's wait for a step
+    // is one for all loads, the next step's with them
+    const int whole = min(s1, r.V / R::SLICE);
+    Step h0, h1;
+    if (s0 < whole) load(h0, kSteps * s0);
+    for (int s = s0; s < whole; ++s) {
+        for (int n = kSteps * s; n < kSteps * (s + 1); n += 2) {
+            load(h1, n + 1);
+            add(h0, n);
+            load(h0, min(n + 2, kSteps * whole - 2));
+            add(h1, n + 1);
+        }
+        done(s);
     }
+    if (max(s0, whole) >= s1) return;
+    // the row's last ids
+#pragma nounroll
+    for (int n = kSteps * (s1 - 1); n < kSteps * s1; ++n) {
+        const int e0 = n * (R::SLICE / kSteps) + lane * R::VEC;
+#pragma unroll
+        for (int j = 0; j < kStep; ++j) {
+            h0.x[j] = r.chunk(e0 + j * 64 * R::VEC);
+            if (MASK) h0.bits[MASK ? j : 0] = r.bits(e0 + j * 64 * R::VEC);
+        }
+        add(h0, n);
+    }
+    done(s1 - 1);
 }
 
 // Bound by the bytes of the rows that are read and, as much, by the exponentials beside
@@ -636,27 +706,32 @@ struct Weights {
             for (int k = 0; k < R::VEC; ++k) w[k] = of(c, e0, k, table);
             return;
         }
+        // (masks and the drafted id by branches that the whole block takes)
+        u32x4 cx = c.x, cy = c.y;
+        if (p.mask != nullptr) cx = R::masked(cx, c.bx);
+        if (two && q.mask != nullptr) cy = R::masked(cy, c.by);
 #pragma unroll
         for (int k0 = 0; k0 < R::VEC; k0 += 4) {
             float x[4];
             double v[4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) x[n] = R::raw(c.x, c.bx, k0 + n);
-            ep.some(x, table, v);
-#pragma unroll
-            for (int n = 0; n < 4; ++n) v[n] = x[n] > ep.lo ? v[n] : 0.0;
+            for (int n = 0; n < 4; ++n) x[n] = R::raw(cx, 0xFFFFFFFFu, k0 + n);
+            ep.of4(x, table, v);
             if (two) {
                 float y[4];
                 double q[4];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) y[n] = R::raw(c.y, c.by, k0 + n);
-                eq.some(y, table, q);
+                for (int n = 0; n < 4; ++n) y[n] = R::raw(cy, 0xFFFFFFFFu, k0 + n);
+                eq.of4(y, table, q);
 #pragma unroll
-                for (int n = 0; n < 4; ++n) v[n] = fmax(__builtin_fma(-share, y[n] > eq.lo ? q[n] : 0.0, v[n]), 0.0);
+                for (int n = 0; n < 4; ++n) v[n] = fmax(__builtin_fma(-share, q[n], v[n]), 0.0);
             }
 #pragma unroll
-            for (int n = 0; n < 4; ++n) w[k0 + n] = e0 + k0 + n == point ? 0.0 : v[n];
+            for (int n = 0; n < 4; ++n) w[k0 + n] = v[n];
         }
+        if (point >= 0)
+#pragma unroll
+            for (int k = 0; k < R::VEC; ++k) w[k] = e0 + k == point ? 0.0 : w[k];
     }
     __device__ __forceinline__ double of(const Chunk& c, int e0, int k, const double* table) const {
         double w = ep.of(R::raw(c.x, c.bx, k), table);
