@@ -429,8 +429,8 @@ __device__ __forceinline__ bool decide(const DraftArgs& a, const Seq& q, int b, 
 // One wave: slices s0 .. s1 - 1 of a row, each slice's statistics to to[s]. A step at
 // a time, the next one's loads in flight.
 //
-// FAST: exponentials in float (twice the rate of those in double, which bound the
-// pass: 2304 + 2048 bf16 rows of 151936 525 us against 230). A slice's sum is then off
+// FAST: exponentials in float (a third of the instructions of those in double, which
+// bound the pass: 256 sequences of 8 drafts 175 us against 303). A slice's sum is then off
 // by at most 3e-6 of it: per term 2 |z| 2^-24 from the exponent z = (x - m) / T and 2^-23
 // from exp2, where the terms' mean |z| is at most ln V < 17 (the entropy's bound);
 // 9 2^-24 from the float additions. Enough to decide most drafts (kUnsure below), not
@@ -602,11 +602,10 @@ __device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, i
 }
 
 // Bound by the bytes of the rows that are read and, as much, by the exponentials beside
-// them: 64 sequences of 4 drafts over 151936 f32 logits 74 us, 283 MB at 3.8 TB/s (350 MB
-// are there, the drafts up to the rejected ones need 224); 256 of 8 in bf16 207 us, 758 MB
-// (1.3 GB there, 690 needed). One sequence of 4: 12 us, its start, one slice a wave and the
-// decisions one after the other. Four waves a SIMD: their registers; with more (5, 6, 8)
-// the large call takes 233, 284, 525 us, spills.
+// them: 64 sequences of 4 drafts over 151936 f32 logits 69 us, 301 MB at 4.4 TB/s (350 MB
+// are there, the drafts up to the rejected ones need 224); 256 of 8 in bf16 175 us, 806 MB
+// at 4.6 TB/s (1.3 GB there, 690 needed). One sequence of 4: 11 us, its start, one slice a
+// wave and the decisions one after the other. Four waves a SIMD: their registers.
 template <bool BF, bool MASK, bool FAST>
 __global__ __launch_bounds__(kThreads, 4) void k_draft_stats(DraftArgs a) {
     using R = Row<BF>;
@@ -653,7 +652,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_draft_stats(DraftArgs a) {
 }
 
 // FAST calls: the emitting rows' slices in double. (Greedy rows need none.) Bound by the
-// exponentials: 256 sequences, 155 MB, 59 us.
+// exponentials: 256 sequences, 155 MB, 54 us.
 template <bool BF, bool MASK>
 __global__ __launch_bounds__(kThreads, 4) void k_draft_exact(DraftArgs a) {
     __shared__ double table[32];
@@ -766,7 +765,7 @@ __device__ __forceinline__ int first_reaching(F value, int n, double base, doubl
 
 // TH threads a block, a wave per part of a slice (PARTS of them). Few sequences: bound by
 // what waits for each other (statistics, part, count, parts' sums, the part again): one
-// 9 us. Many: two exponentials an id: 256 over 151936 92 us.
+// 9 us. Many: two exponentials an id: 256 over 151936 79 us.
 template <bool BF, int TH, int PARTS>
 __global__ __launch_bounds__(TH) void k_draft_draw(DraftArgs a) {
     using R = Row<BF>;
@@ -1267,9 +1266,9 @@ __global__ __launch_bounds__(kSetThreads) void k_verify_sets(SetsArgs a) {
 
 // Float exponentials first, and the emitting rows (one or two of the 2 max_draft + 1)
 // again in double: for bf16 rows, whose doubles take longer than their bytes, where
-// that is more than a launch. 256 sequences of 8 drafts over 151936 ids: 207 + 60 us
-// against 357; of 4 drafts in f32 66 + 19 against 74; 37 of 7 over 50257 in bf16
-// (26 MB) 20 + 9 against 26.
+// that is more than a launch. 256 sequences of 8 drafts over 151936 ids: 175 + 54 us
+// against 303; of 4 drafts in f32 66 + 18 against 69; 37 of 7 over 50257 in bf16
+// (26 MB) 18 + 9 against 23.
 constexpr int64_t kFastBytes = (int64_t)128 << 20;
 
 struct Layout {
@@ -1327,7 +1326,7 @@ hipError_t launch_draft(const DraftArgs& a, hipStream_t s) {
     };
     // few rows: more waves a slice, for its latency; many: fewer (each starts with the
     // sequence's own data), in smaller blocks. 4 of 512 threads against 2 of 256: one
-    // sequence 9.3 and 11.4 us, 64 (f32) 33 and 30, 256 (bf16) 112 and 97.
+    // sequence 9.0 and 11.4 us, 64 (f32) 31 and 28, 256 (bf16) 97 and 79.
     if ((int64_t)a.d.seqs * a.S < 4096) draw(std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
     else draw(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
     return hipGetLastError();
