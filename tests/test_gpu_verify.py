@@ -141,6 +141,35 @@ def test_draft_large_calls(hs, drafter):
     run_draft(hs, 13, B, 50 if drafter else 90, 40001, "bf16", drafter=drafter, n=n, t=t, td=td, pad=3, offset=1, big=True)
 
 
+@pytest.mark.parametrize("dtype,B,K,V,big", [("bf16", 40, 50, 40001, True), ("bf16", 20, 5, 9001, False), ("f32", 20, 5, 9001, False)])
+def test_draft_shifted_logits(hs, dtype, B, K, V, big):
+    """Rows all below zero, rows with one slice above it, rows so far from zero that the
+    product with 1 / T no longer fits the float exponentials, rows of zeroes of both
+    signs."""
+    n = [1 + i % 5 for i in range(B)]
+    t = np.resize([1.0, 0.7, 0.0, 0.004, 2.0], B)
+
+    def edit(x, y, d, u, v):
+        for rows in (x, y):
+            for r in range(rows.shape[0]):
+                kind = r % 7
+                if kind == 0:
+                    rows[r] = -np.abs(rows[r]) - 0.5
+                elif kind == 1:
+                    rows[r] -= 60.0
+                elif kind == 2:
+                    rows[r] = -np.abs(rows[r]) - 0.5
+                    rows[r, V // 2] = 3.0
+                elif kind == 3:
+                    rows[r] += 20000.0
+                elif kind == 4:
+                    rows[r] = np.where(rows[r] > 0, 0.0, -0.0)
+                elif kind == 5:
+                    rows[r] -= 20000.0
+
+    run_draft(hs, 77, B, K, V, dtype, n=n, t=t, td=t, edit=edit, big=big)
+
+
 def test_draft_large_calls_with_masks(hs):
     B, K, V = 24, 3, 40003
     rng = np.random.default_rng(14)
