@@ -102,6 +102,14 @@ def test_linear_sizes(hs, M, K, N, dtype, out):
     one(hs, M + K + N, None, M, K, N, dtype, ACTS[(M + K + N) % 6], out)
 
 
+@pytest.mark.parametrize("dtype,out", [("bf16", "f32"), ("f16", "same")])
+@pytest.mark.parametrize("M,K,N,G", [(200, 520, 4100, None), (256, 72, 3900, None), (129, 1000, 5400, None), (64, 8, 16380, None),
+                                     (60, 264, 4000, 4), (256, 2048, 4096, None)])
+def test_linear_of_a_block_per_cu(hs, M, K, N, G, dtype, out):
+    """Sizes whose 64 x 64 tiles are about one for each of the 256 CUs."""
+    one(hs, M + K, G, M, K, N, dtype, ACTS[(M + K) % 6], out)
+
+
 @pytest.mark.parametrize("M,K,N", [(1, 4096, 96), (7, 130, 50), (64, 513, 257), (130, 520, 300), (300, 1024, 520)])
 @pytest.mark.parametrize("pad,offset", [(1, 0), (0, 1), (3, 5), (8, 0), (8, 8), (4, 4)])
 def test_linear_strides_and_alignment(hs, M, K, N, pad, offset):

@@ -191,7 +191,7 @@ __device__ __forceinline__ void store_tiles(const Args& a, int g, int m0, int n0
 // step for each wave, whose sums meet in LDS at the end.
 //
 // Few rows: W's stream bounds it (one row of 4096 x 4096 8.3 us, 4.0 TB/s with the
-// launch and the ramp in it; four groups of 64 rows 37 us, 134 MB at 3.6 TB/s): hence
+// launch and the ramp in it; four groups of 64 rows 29 us, 134 MB at 4.6 TB/s): hence
 // narrow tiles, whose waves share K instead of columns, and many loads in the air.
 // Many: per stage the loads to LDS and the LDS reads beside the products: hence the
 // widest tile that the accumulators allow, whose operands are read least often
@@ -418,16 +418,18 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(Args a, int t
 // round of one block per CU (one[0]) and of two (one[1]) costs, in us at
 // K = 4096. Measured, N = 4096 and 16384 (bf16), rows 1 to 4096:
 //   16 x 16 rows 1: 7.8, 25 us; 32 x 32 rows 32: 14.5, 26; 64 x 16 rows 64: 15, 56;
-//   64 x 32 rows 64: 17.5, 37, rows 256: 31, 120; 64 x 64 rows 256: 34, 75, rows 512:
-//   39, 133; 128 x 128 rows 256: 41, 56, rows 1024: 52, 168; 160 x 128 rows 512:
-//   63, 83, rows 2048: 76, 284; 256 x 256 rows 1024: 101, 123, rows 4096 (f16): -, 462.
+//   64 x 32 rows 64: 17.5, 37, rows 256: 31, 120; 64 x 64 by 8 waves rows 256: 34, 75,
+//   rows 512: 39, 133; by 16, with twice the bytes in the air and one block to a CU,
+//   rows 64: -, 32, rows 256: 24, -; 128 x 128 rows 256: 41, 56, rows 1024: 52, 168;
+//   160 x 128 rows 512: 63, 83, rows 2048: 76, 284; 256 x 256 rows 1024: 101, 123, rows
+//   4096 (f16): -, 462.
 struct Form {
     int bm, bn, blocks;
     float one[2];
 };
 constexpr Form kForms[] = {
-    {16, 16, 2, {8, 12}},   {32, 32, 2, {13, 25}},   {64, 16, 1, {14.5f, 0}}, {64, 32, 1, {15.5f, 0}},
-    {64, 64, 2, {32, 39}},  {128, 128, 1, {44, 0}},  {160, 128, 2, {62, 84}}, {256, 256, 1, {112, 0}},
+    {16, 16, 2, {8, 12}}, {32, 32, 2, {13, 25}}, {64, 16, 1, {14.5f, 0}}, {64, 32, 1, {15.5f, 0}}, {64, 64, 2, {32, 39}},
+    {64, 64, 1, {24, 0}}, {128, 128, 1, {44, 0}}, {160, 128, 2, {62, 84}}, {256, 256, 1, {112, 0}},
 };
 
 // Blocks of one group.
@@ -476,7 +478,8 @@ hipError_t launch_linear(const Args& a, hipStream_t s) {
             case 1: return launch_tile<BF, true, 1, 1, 8, 2, 2, 2>(a, s);
             case 2:
             case 3: return launch_tile<BF, true, 1, 2, 4, 4, 1, 2>(a, s);
-            case 4: return launch_tile<BF, true, 2, 2, 2, 2, 2, 2>(a, s);
+            case 4:
+            case 5: return launch_tile<BF, true, 2, 2, 2, 2, 2, 2>(a, s);
             default: return launch_tile<BF, true, 2, 4, 1, 4, 2, 2>(a, s);
         }
     switch (f) {
@@ -485,8 +488,9 @@ hipError_t launch_linear(const Args& a, hipStream_t s) {
         case 2: return launch_tile<BF, false, 1, 1, 8, 4, 1, 4>(a, s);
         case 3: return launch_tile<BF, false, 1, 2, 4, 4, 1, 4>(a, s);
         case 4: return launch_tile<BF, false, 2, 2, 2, 2, 2, 4>(a, s);
-        case 5: return launch_tile<BF, false, 2, 4, 1, 4, 2, 4>(a, s);
-        case 6: return launch_tile<BF, false, 2, 4, 1, 5, 2, 2>(a, s);
+        case 5: return launch_tile<BF, false, 2, 2, 4, 2, 2, 4>(a, s);
+        case 6: return launch_tile<BF, false, 2, 4, 1, 4, 2, 4>(a, s);
+        case 7: return launch_tile<BF, false, 2, 4, 1, 5, 2, 2>(a, s);
         default: return launch_tile<BF, false, 2, 4, 1, 8, 4, 2>(a, s);
     }
 }
@@ -524,7 +528,7 @@ extern "C" int ultima_hsamp_linear(const ultima_hsamp_linear_args* a, void* hip_
         return ULTIMA_HSAMP_ERR_INVALID;
     // 32-bit rows and columns; a launch counts its threads in 32 bits
     if (a->groups > 65535 || std::max({a->rows, a->in_dim, a->out_dim}) > 1 << 30 ||
-        std::max(blocks_of(kForms[choose(*a)], *a), blocks_of(kForms[5], *a)) > 1 << 22)
+        std::max(blocks_of(kForms[choose(*a)], *a), blocks_of(kForms[6], *a)) > 1 << 22)
         return ULTIMA_HSAMP_ERR_UNSUPPORTED;
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
     const hipError_t e = a->dtype == ULTIMA_HSAMP_BF16 ? launch_linear<true>(*a, s) : launch_linear<false>(*a, s);
