@@ -499,12 +499,12 @@ __device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, i
         for (int j = 0; j < kStep; ++j) asm volatile("" : "+v"(h.x[j]));
         if (c == 0.0) {
             if (!(top > m)) return;      // (the lowest id: the earlier step's)
-            int here = INT32_MAX;
+            int here = INT32_MAX;        // (above top: +inf alone; a NaN is not at least top)
 #pragma unroll
             for (int j = 0; j < kStep; ++j)
 #pragma unroll
                 for (int k = 0; k < R::VEC; ++k)
-                    if (fminf(value(j, k), kFltMax) == top) here = min(here, n * (R::SLICE / kSteps) + (j * 64 + lane) * R::VEC + k);
+                    if (value(j, k) >= top) here = min(here, n * (R::SLICE / kSteps) + (j * 64 + lane) * R::VEC + k);
             at = wave_min(here);
             m = top;
             return;
