@@ -34,3 +34,28 @@ def test_greedy_rows_never_take_a_nan(hs, dtype, side, at):
     want = C.check(C.call(hs, c, t, td), c, ACCEPT_TOL, t, td)
     if side != "drafter":
         assert all(w[-1] == at + 700 for w in want)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("extra", [0, 900])      # with the rows behind the last sequence: a large call
+def test_nan_of_every_kind_has_no_weight(hs, dtype, masked, extra):
+    """Quiet and signalling NaN of both signs among the logits of both sides."""
+    import torch
+    dt = getattr(torch, dtype)
+    B, K, V = 6, 4, 40001
+    c = C.made_up(6, B, 200 if extra else K, V, dt, lens=[K] * B, extra=extra)
+    rows, D = B * (K + 1), B * K
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for t, n in ((c["x"], rows), (c["y"], D)):
+        for r in range(n):
+            for k, nan in enumerate(C.NANS[dt]):
+                if r % 6 in (k, 4):              # one kind, all of them, none
+                    C.bits(t)[r, torch.randint(0, V, (9,), generator=g, device="cuda")] = nan
+    mask = dmask = None
+    if masked:
+        rng = np.random.default_rng(2)
+        mask, dmask = (rng.integers(-2**31, 2**31, (n + extra, -(-V // 32)), dtype=np.int64).astype(np.int32) for n in (rows, D))
+    # float sums' quotients (bf16, large): 45 2^-24 each, see the kernel
+    tol = ACCEPT_TOL + (2 * 45 * 2.0 ** -24 if extra and dtype == "bfloat16" else 0.0)
+    C.check(C.call(hs, c, mask=mask, dmask=dmask), c, tol, mask=mask, dmask=dmask)

@@ -196,8 +196,19 @@ __device__ __forceinline__ double inv_temperature(const float* t, int b) {
     return v > 0.0f ? fmax(1.0 / (double)v, 1e-300) * kPerE : 0.0;
 }
 
-// NaN as -inf, +inf as the largest finite float.
-__device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, kNegInf), kFltMax); }
+// x between lo and the largest float, a quiet NaN as lo. A signalling one comes out as
+// NaN: the instruction takes the minimum of the three in their order where one is NaN, and
+// a minimum with a signalling NaN is NaN, without one the other value (hence x last, and
+// a constant that the compiler does not know, which it would put there).
+__device__ __forceinline__ float clamp(float x, float lo) {
+    float most = kFltMax;
+    asm("" : "+s"(most));
+    return __builtin_amdgcn_fmed3f(lo, most, x);
+}
+
+// NaN as -inf, +inf as the largest finite float. (By comparisons: the compiler's maximum
+// of three takes a signalling NaN for the other two.)
+__device__ __forceinline__ float clean(float x) { return x > kNegInf ? (x < kFltMax ? x : kFltMax) : kNegInf; }
 
 // exp((x - m) / T) exactly 0 for what is not allowed, and below 2^-1000.
 __device__ __forceinline__ double weight_of(float x, float m, double c, const double* table) {
@@ -217,15 +228,15 @@ struct Scale {
         const double low = (md - (double)lo) * c;
         fast = lo > -3e38f && low > 31900.0 && low < 32100.0;
     }
-    // (2^-1000 for what is not allowed)
+    // (2^-1000 for what is not allowed, a signalling NaN's NaN)
     __device__ __forceinline__ double some(float x, const double* table) const {
-        return exp32((double)__builtin_amdgcn_fmed3f(x, lo, kFltMax) - md, c, table);
+        return exp32((double)clamp(x, lo) - md, c, table);
     }
     template <int N>
     __device__ __forceinline__ void some(const float (&x)[N], const double* table, double (&v)[N]) const {
         double d[N];
 #pragma unroll
-        for (int n = 0; n < N; ++n) d[n] = (double)__builtin_amdgcn_fmed3f(x[n], lo, kFltMax) - md;
+        for (int n = 0; n < N; ++n) d[n] = (double)clamp(x[n], lo) - md;
         exp32n(d, c, table, v);
     }
     // exactly 0 for what is not allowed and what lies below lo
@@ -463,11 +474,16 @@ __device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, i
     auto add = [&](Step& h, int n) {
         auto value = [&](int j, int k) { return R::raw(h.x[j], MASK ? h.bits[MASK ? j : 0] : 0xFFFFFFFFu, k); };
         // the maximum by the bits as whole numbers, right where it comes out as a finite
-        // float >= 0: half an instruction a value
+        // float >= 0 (a NaN of positive sign lies above): half an instruction a value
         float top = -1.0f;
-        if (!MASK) {
+        {
             int t = INT32_MIN;
-            if (BF) {
+            if (MASK) {
+#pragma unroll
+                for (int j = 0; j < kStep; ++j)
+#pragma unroll
+                    for (int k = 0; k < R::VEC; ++k) t = max(t, __float_as_int(value(j, k)));
+            } else if (BF) {
                 s16x2 v = __builtin_bit_cast(s16x2, 0x80008000u);
 #pragma unroll
                 for (int j = 0; j < kStep; ++j)
@@ -491,7 +507,10 @@ __device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, i
 #pragma unroll
             for (int j = 0; j < kStep; ++j)
 #pragma unroll
-                for (int k = 0; k < R::VEC; ++k) top = fmaxf(top, value(j, k));
+                for (int k = 0; k < R::VEC; ++k) {
+                    const float x = value(j, k);
+                    top = x > top ? x : top;     // (a NaN is not above)
+                }
             top = fminf(wave_max(top), kFltMax);
         }
         // (the values are unpacked again below: kept, they take twice the registers)
@@ -532,15 +551,18 @@ __device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, i
                     float v[4];
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
-                        const float x = __builtin_amdgcn_fmed3f(value(j, k + n), flo, kFltMax);
+                        const float x = clamp(value(j, k + n), flo);
                         v[n] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, ch, -mch));
                     }
                     part += (v[0] + v[1]) + (v[2] + v[3]);
                 }
-            sum += (double)part * moved;
-            return;
+            if (__ballot(part != part) == 0) {      // (a signalling NaN: by the loop below)
+                sum += (double)part * moved;
+                return;
+            }
         }
         const Scale e(m, c);
+        const double before = sum;
         if (e.fast) {
             // (what is not allowed adds 2^-1000 here)
 #pragma unroll
@@ -555,12 +577,13 @@ __device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, i
                     sum += (v[0] + v[1]) + (v[2] + v[3]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-        } else {
+            if (__ballot(sum != sum) == 0) return;
+        }
+        sum = before;
 #pragma nounroll
-            for (int j = 0; j < kStep * R::VEC; ++j) {
-                const int id = n * (R::SLICE / kSteps) + j * 64 + lane;
-                if (id < r.V) sum += weight_of(r.at(id), m, c, table);
-            }
+        for (int j = 0; j < kStep * R::VEC; ++j) {
+            const int id = n * (R::SLICE / kSteps) + j * 64 + lane;
+            if (id < r.V) sum += weight_of(r.at(id), m, c, table);
         }
     };
     auto done = [&](int s) {
