@@ -244,3 +244,30 @@ def test_draft_heads_to_verified_tokens(hs, sampler, wl):
         want, _, near = R.verify(lambda i: R.chances(xv[b * 3 + i], tv), lambda i: R.chances(yv[b * 2 + i], tv),
                                  d[2 * b:2 * b + 2], u[2 * b:2 * b + 2], v[b])
         assert near > R.NEAR and list(tokens[b][:count[b]]) == want
+
+
+def exact_act(y, act, c):
+    return c * np.tanh(y / c)
+
+
+def one_column(hs, values, act, c=0.0):
+    """The activation of each value: rows of one element by a weight of one."""
+    import torch
+    x = values.to(torch.bfloat16).reshape(-1, 1)
+    got = hs.linear(x, torch.ones((1, 1), dtype=torch.bfloat16, device="cuda"), act=act, act_param=c, out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    return x[:, 0].double().cpu().numpy(), got[:, 0].double().cpu().numpy()
+
+
+@pytest.mark.parametrize("c", [1e-45, 1e-42, 2.0**-128, 2.0**-126, 1e-30, 0.5, 1e30, 2.0**126, 2.0**127, 3.402823466e38])
+def test_linear_caps_of_any_size(hs, c):
+    """c tanh(y / c) for caps from the smallest float to the largest; the quotient, the
+    function and the product round a few times each, and subnormal results by half of
+    2^-149 (c below 2^-126: c's own steps)."""
+    import torch
+    c = float(np.float32(c))
+    m = torch.logspace(-37, 38, 151, device="cuda")
+    y, got = one_column(hs, torch.cat([torch.zeros(2, device="cuda"), -torch.zeros(1, device="cuda"), m, -m]), "softcap", c)
+    with np.errstate(over="ignore"):
+        want = exact_act(y, "softcap", c)
+    assert np.all(np.abs(got - want) <= 16 * 2.0**-24 * np.abs(want) + 2.0**-149)

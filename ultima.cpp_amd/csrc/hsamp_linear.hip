@@ -46,9 +46,10 @@ __device__ __forceinline__ float sigmoid(float t) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t * -1.44269504f));
 }
 
-// tanh: to 1/2 its Taylor series (the next term is 10^-7 of the value there),
-// from there 1 - 2 / (1 + exp(2 |t|)).
-__device__ __forceinline__ float tanh_of(float t) {
+// c tanh(t), t = y / c: up to 1/2 by tanh's Taylor series (the next term is 10^-7 of the
+// value there) as y (1 + t^2 ...), right also where t is subnormal or 0; from there by
+// tanh(t) = 1 - 2 / (1 + exp(2 |t|)).
+__device__ __forceinline__ float cap_of(float y, float t, float c) {
     const float z = t * t, u = fabsf(t);
     float p = 21844.0f / 6081075.0f;
     p = __builtin_fmaf(p, z, -1382.0f / 155925.0f);
@@ -56,9 +57,9 @@ __device__ __forceinline__ float tanh_of(float t) {
     p = __builtin_fmaf(p, z, -17.0f / 315.0f);
     p = __builtin_fmaf(p, z, 2.0f / 15.0f);
     p = __builtin_fmaf(p, z, -1.0f / 3.0f);
-    const float low = __builtin_fmaf(t * z, p, t);
+    const float low = __builtin_fmaf(y * z, p, y);
     const float high = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * 2.88539008f)), 1.0f);
-    return u <= 0.5f ? low : __builtin_copysignf(high, t);       // (NaN: high's NaN)
+    return u <= 0.5f ? low : c * __builtin_copysignf(high, t);       // (NaN: high's NaN)
 }
 
 using Args = ultima_hsamp_linear_args;
@@ -113,9 +114,11 @@ __device__ __forceinline__ void finish(const Args& a, int g, int m, int n, float
                 y[e] = y[e] * sigmoid(1.59576912160573071f * (y[e] + 0.044715f * y[e] * y[e] * y[e]));
             break;
         case ULTIMA_HSAMP_ACT_SOFTCAP: {
-            const float inv = 1.0f / a.act_param;
+            // (both scaled where 1 / c would be subnormal or infinite)
+            const float c = a.act_param, scale = c < 0x1p-64f ? 0x1p64f : c > 0x1p64f ? 0x1p-64f : 1.0f;
+            const float inv = 1.0f / (c * scale);
 #pragma unroll
-            for (int e = 0; e < E; ++e) y[e] = a.act_param * tanh_of(y[e] * inv);
+            for (int e = 0; e < E; ++e) y[e] = cap_of(y[e], y[e] * scale * inv, c);
             break;
         }
     }
