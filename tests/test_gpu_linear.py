@@ -247,6 +247,13 @@ def test_draft_heads_to_verified_tokens(hs, sampler, wl):
 
 
 def exact_act(y, act, c):
+    """Without cancellation: relative to the value itself."""
+    if act == "gelu":
+        return 0.5 * y * np.vectorize(math.erfc)(-y / math.sqrt(2))
+    if act == "gelu_tanh":
+        return y / (1 + np.exp(-2 * math.sqrt(2 / math.pi) * (y + 0.044715 * y**3)))
+    if act == "silu":
+        return y / (1 + np.exp(-y))
     return c * np.tanh(y / c)
 
 
@@ -271,3 +278,15 @@ def test_linear_caps_of_any_size(hs, c):
     with np.errstate(over="ignore"):
         want = exact_act(y, "softcap", c)
     assert np.all(np.abs(got - want) <= 16 * 2.0**-24 * np.abs(want) + 2.0**-149)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_linear_tails_of_the_activations(hs, act):
+    """Each activation relative to its own value, far into the negative tail. The argument
+    a of exp (erfc: its square) has at most eight roundings of its own, so that the value
+    moves by 8 |a| 2^-24; twenty steps more for the functions and the products."""
+    import torch
+    y, got = one_column(hs, torch.linspace(-9.0, 9.0, 721, device="cuda"), act)
+    want = exact_act(y, act, 0.0)
+    a = {"silu": np.abs(y), "gelu": y * y, "gelu_tanh": np.abs(1.6 * y + 0.0715 * y**3)}[act]
+    assert np.all(np.abs(got - want) <= (8 * a + 20) * 2.0**-24 * np.abs(want) + 1e-37)
