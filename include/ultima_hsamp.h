@@ -402,7 +402,8 @@ int ultima_hsamp_lm_head(const ultima_hsamp_head* head, void* hip_stream);
  * arrays: count 0, every token -1.
  * accept_prob[i] = min(1, p_i(d_i) / q_i(d_i)) (q_i(d_i) = 0: 1 if p_i(d_i) > 0,
  * else 0) up to the first rejected draft, -1 for the drafts after it; rows of no
- * sequence are left as they were. (In bfloat16 calls of more than 128 MB of logits
+ * sequence, and of sequences whose n_draft or rows are out of range, are left as
+ * they were. (In bfloat16 calls of more than 128 MB of logits
  * and four drafts or more it may be off by 1e-5 of its value; else it is the
  * rounded double.)
  * Row layout: target rows of sequence b start at target_start[b], its drafted
@@ -457,7 +458,7 @@ int ultima_hsamp_verify_draft(const ultima_hsamp_draft* d, void* hip_stream);
  * id), so the emitted tokens are samples of what the sampler itself draws from.
  * Probabilities that are NaN or below 0 count as 0. A count below 0 or above its
  * capacity (a set that was cut off) makes its sequence invalid: count 0, every
- * token -1; an empty target set emits no token. */
+ * token and acceptance probability -1; an empty target set emits no token. */
 typedef struct ultima_hsamp_draft_sets {
     int32_t seqs;               /* sequences >= 1 */
     int32_t max_draft;          /* 0 .. ULTIMA_HSAMP_MAX_DRAFT */

@@ -723,3 +723,37 @@ def test_draft_sequences_that_share_rows(hs):
         w, _, near = R.verify(lambda i: R.chances(x[i]), lambda i: R.chances(y[2 * b + i]), d[2 * b:2 * b + 2],
                               u[2 * b:2 * b + 2], v[b])
         assert near > R.NEAR and list(tokens[b][:count[b]]) == w
+
+
+@pytest.mark.parametrize("cap", [16, 5000])
+def test_sets_that_were_cut_off_leave_no_acceptance(hs, cap):
+    """A set above its capacity or a count below 0 on either side: -1 for all of the
+    sequence's drafts, the others' as ever, rows of no sequence as they were."""
+    torch, dev = _torch()
+    rng = np.random.default_rng(72)
+    B, K, V = 5, 3, 6000
+    n = np.array([3, 2, 3, 3, 1], np.int32)
+    ts = np.concatenate([[0], np.cumsum(n + 1)[:-1]]).astype(np.int32)
+    ds = np.concatenate([[0], np.cumsum(n)[:-1]]).astype(np.int32)
+    D = int(n.sum())
+    P, Q = make_sets(rng, D + B, cap, V, [cap] * (D + B)), make_sets(rng, D, cap, V, [cap - 3] * D)
+    P[2][ts[0] + 3] = cap + 1          # sequence 0, its last row
+    Q[2][ds[1]] = cap + 7              # sequence 1, the drafter's
+    P[2][ts[3] + 1] = -1               # sequence 3
+    d = np.array([Q[0][r, 0] for r in range(D)], np.int32)
+    u, v = rng.random(D), rng.random(B)
+    to = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(dev)  # noqa: E731
+    more = lambda a, fill: to(np.concatenate([a, np.full((2, *a.shape[1:]), fill, a.dtype)]))  # noqa: E731
+    out = {"accept": torch.full((D + 2,), 9.0, device=dev)}
+    hs.verify_sets(*[to(a) for a in P], more(d, 0), more(u, 0), to(v), K, draft_idx=more(Q[0], 0), draft_prob=more(Q[1], 0),
+                   draft_count=more(Q[2], 0), n_draft=to(n), target_start=to(ts), draft_start=to(ds), outputs=out)
+    torch.cuda.synchronize()
+    accept, count = out["accept"].cpu().numpy(), out["count"].cpu().numpy()
+    for b in (0, 1, 3):
+        assert count[b] == 0 and (accept[ds[b]:ds[b] + n[b]] == -1.0).all()
+    for b in (2, 4):
+        toks, shares, near = R.verify(lambda i: R.dense(*(a[ts[b] + i] for a in P), V), lambda i: R.dense(*(a[ds[b] + i] for a in Q), V),
+                                      d[ds[b]:ds[b] + n[b]], u[ds[b]:ds[b] + n[b]], v[b])
+        assert near > R.NEAR and count[b] == len(toks)
+        np.testing.assert_allclose(accept[ds[b]:ds[b] + n[b]], shares + [-1.0] * (n[b] - len(shares)), rtol=ACCEPT_TOL, atol=1e-37)
+    assert (accept[D:] == 9.0).all()

@@ -1091,6 +1091,8 @@ __global__ __launch_bounds__(kSetThreads) void k_verify_sets(SetsArgs a) {
         if (__syncthreads_or(bad)) {
             if (!writes) return;
             for (int i = tid; i <= K; i += TH) out[i] = -1;
+            if (q.ok && d.accept_prob != nullptr)      // (else its rows are not known)
+                for (int i = tid; i < q.n; i += TH) d.accept_prob[q.d0 + i] = -1.0f;
             if (tid == 0) d.out_count[b] = 0;
             if (PART == kSetsTiles && tid == 0) a.emits[b] = -1;
             return;

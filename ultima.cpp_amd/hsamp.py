@@ -587,7 +587,9 @@ def verify_draft(logits, draft, u_accept, u_draw, max_draft: int, draft_logits=N
     greedy); mask, draft_mask int32 words per row; n_draft, target_start,
     draft_start int32 [B] for sequences of different lengths. Returns a dict:
     tokens int32 [B, max_draft + 1], count int32 [B] and, unless accept is False,
-    accept f32 [D] (their acceptance probabilities). work: a uint8 tensor of
+    accept f32 [D] (their acceptance probabilities; drafted rows of no sequence, and
+    of sequences whose n_draft or rows are out of range, are not written: what they
+    hold is then no probability). work: a uint8 tensor of
     ultima_hsamp_verify_draft_work_bytes() bytes of this call alone (allocated
     otherwise); outputs: a dict of tensors to write to."""
     import torch
