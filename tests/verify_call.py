@@ -52,7 +52,8 @@ def check(out, c, tol, t=None, td=None, drafter=True, mask=None, dmask=None):
     """Tokens and counts equal, acceptance probabilities within `tol` of their value."""
     torch.cuda.synchronize()
     B, K = len(c["lens"]), c["K"]
-    x, y = c["x"].float().cpu().numpy(), c["y"].float().cpu().numpy()
+    rows, drafted = int(c["ts"][-1] + c["lens"][-1]) + 1, int(c["ds"][-1] + c["lens"][-1])
+    x, y = c["x"][:rows].float().cpu().numpy(), c["y"][:drafted].float().cpu().numpy()
     T = np.ones(B, np.float32) if t is None else np.asarray(t, np.float32)
     TD = np.ones(B, np.float32) if td is None else np.asarray(td, np.float32)
     tokens, count, accept = (out[k].cpu().numpy() for k in ("tokens", "count", "accept"))

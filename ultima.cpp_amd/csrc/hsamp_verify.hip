@@ -1398,7 +1398,10 @@ extern "C" int ultima_hsamp_verify_draft(const ultima_hsamp_draft* d, void* hip_
     // a wave per slice of a row, numbered in 32 bits by their threads
     // (up to a block's waves more per row)
     if (std::max(jobs, (int64_t)d->seqs * kMaxParts) * (a.S + 8) > ((int64_t)1 << 32) / 64) return ULTIMA_HSAMP_ERR_UNSUPPORTED;
-    a.fast = d->dtype == ULTIMA_HSAMP_BF16 && d->max_draft >= 4 && jobs * d->vocab * (int64_t)es > kFastBytes;
+    // the rows and drafts that there are: with lengths of their own no more than the arrays hold
+    const int64_t held = d->n_draft == nullptr ? jobs : std::min(jobs, (int64_t)d->logits_rows + (drafter ? d->draft_rows : 0));
+    const bool drafts = d->max_draft >= 4 && (d->n_draft == nullptr || d->draft_rows / 4 >= d->seqs);
+    a.fast = d->dtype == ULTIMA_HSAMP_BF16 && drafts && held * d->vocab * (int64_t)es > kFastBytes;
     unsigned char* w = static_cast<unsigned char*>(d->work);
     a.stats = reinterpret_cast<SliceStat*>(w + l.stats);
     a.sums = reinterpret_cast<RowSum*>(w + l.sums);
