@@ -403,7 +403,7 @@ int ultima_hsamp_lm_head(const ultima_hsamp_head* head, void* hip_stream);
  * accept_prob[i] = min(1, p_i(d_i) / q_i(d_i)) (q_i(d_i) = 0: 1 if p_i(d_i) > 0,
  * else 0) up to the first rejected draft, -1 for the drafts after it; rows of no
  * sequence, and of sequences whose n_draft or rows are out of range, are left as
- * they were. (In bfloat16 calls whose arrays hold more than 128 MB of logits and four
+ * they were. (In bfloat16 calls whose arrays hold more than 1 GB of logits and four
  * drafts or more for each sequence it may be off by 1e-5 of its value; else it is the
  * rounded double.)
  * Row layout: target rows of sequence b start at target_start[b], its drafted

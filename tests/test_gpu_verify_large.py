@@ -1,5 +1,6 @@
 """verify_draft's large bfloat16 calls, whose rows are summed by float exponentials first:
-more than 128 MB of logits that the arrays hold, four drafts or more for each sequence. Here most of those rows belong to no sequence (and are NaN), so that the rule in 64 bits
+more than 1 GB of logits that the arrays hold, four drafts or more for each sequence.
+Here most of those rows belong to no sequence (and are NaN), so that the rule in 64 bits
 on the host is quick.
 
 Tokens and counts are equal. A row's sum is off by at most 45 2^-24 of it: two roundings
@@ -16,7 +17,7 @@ pytestmark = pytest.mark.gpu
 
 ACCEPT_TOL = 2.0 ** -24 + 1e-12
 ACCEPT_TOL_LARGE = ACCEPT_TOL + 2 * 45 * 2.0 ** -24
-LARGE = 128 << 20
+LARGE = 1 << 30
 V, K_MAX = 40001, 1000
 
 
@@ -35,6 +36,15 @@ def test_few_drafts_of_many(hs):
     B = 40
     c = C.made_up(13, B, K_MAX, V, torch.bfloat16, lens=[i % 6 for i in range(B)])
     assert B * (2 * K_MAX + 1) * V * 2 > LARGE > (c["x"].shape[0] + c["y"].shape[0]) * V * 2
+    C.check(C.call(hs, c), c, ACCEPT_TOL)
+
+
+def test_a_quarter_of_a_gigabyte_is_not_large(hs):
+    """Where doubles alone are the quicker ones, too: as exact as any small call."""
+    import torch
+    B = 20
+    c = C.made_up(14, B, K_MAX, V, torch.bfloat16, lens=[4 + i % 3 for i in range(B)], extra=1600)
+    assert LARGE > (c["x"].shape[0] + c["y"].shape[0]) * V * 2 > LARGE / 4 and c["d"].size >= 4 * B
     C.check(C.call(hs, c), c, ACCEPT_TOL)
 
 

@@ -1291,10 +1291,12 @@ __global__ __launch_bounds__(kSetThreads) void k_verify_sets(SetsArgs a) {
 
 // Float exponentials first, and the emitting rows (one or two of the 2 max_draft + 1)
 // again in double: for bf16 rows, whose doubles take longer than their bytes, where
-// that is more than a launch. 256 sequences of 8 drafts over 151936 ids: 175 + 54 us
-// against 303; of 4 drafts in f32 66 + 18 against 69; 37 of 7 over 50257 in bf16
-// (26 MB) 18 + 9 against 23.
-constexpr int64_t kFastBytes = (int64_t)128 << 20;
+// many more rows are read than emit. 256 sequences of 8 drafts over 151936 ids (1.3 GB):
+// the call 303 us against 353. Time against that of doubles alone, over 151936, 50257 and
+// 32000 ids: 128 MB of 4 drafts 1.09, 1.12, 1.12, of 8 1.04, 1.09, 1.05; 512 MB of 4 0.90,
+// 1.00, 0.97, of 8 1.03, 1.12, 1.09; 1 GB of 4 0.84, 1.01, 0.95, of 8 0.89, 0.90, 0.92;
+// 2 GB of 4 0.87, 0.95, 0.96, of 8 0.76, 0.95, 0.91; of 2 drafts 1 GB 0.95, 1.02, 1.02.
+constexpr int64_t kFastBytes = (int64_t)1 << 30;
 
 struct Layout {
     int S;
