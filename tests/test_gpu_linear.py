@@ -290,3 +290,19 @@ def test_linear_tails_of_the_activations(hs, act):
     want = exact_act(y, act, 0.0)
     a = {"silu": np.abs(y), "gelu": y * y, "gelu_tanh": np.abs(1.6 * y + 0.0715 * y**3)}[act]
     assert np.all(np.abs(got - want) <= (8 * a + 20) * 2.0**-24 * np.abs(want) + 1e-37)
+
+
+def test_streams_of_another_device_are_refused(hs):
+    import types
+
+    import torch
+    other = types.SimpleNamespace(device=torch.device("cuda", torch.cuda.current_device() + 1))
+    x, w, _, _ = tensors(1, None, 2, 64, 64, "bf16", False, False)
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32, device="cuda")  # noqa: E731
+    f64 = lambda n: torch.zeros(n, dtype=torch.float64, device="cuda")  # noqa: E731
+    p = torch.zeros((2, 8), device="cuda")
+    for call in (lambda: hs.linear(x, w, stream=other), lambda: hs.verify_draft(p, i32(1), f64(1), f64(1), 1, stream=other),
+                 lambda: hs.verify_sets(i32(2, 8), p, i32(2), i32(1), f64(1), f64(1), 1, stream=other)):
+        with pytest.raises(hs.HsampError) as e:
+            call()
+        assert e.value.status == hs.ERR_INVALID

@@ -505,11 +505,13 @@ def _refuse(what: str):
     raise HsampError(ERR_INVALID, what)
 
 
-def _elsewhere(dev, stream):
+def _elsewhere(dev, stream, what):
     """The context that makes `stream` (None: the device's current one) and its device
     current, or None where they are: the call, and what it allocates, then go there."""
     import torch
     if stream is not None:
+        if stream.device != dev:
+            _refuse(f"{what}: the stream must be one of {dev}")
         return torch.cuda.stream(stream)
     return None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
@@ -597,7 +599,7 @@ def verify_draft(logits, draft, u_accept, u_draw, max_draft: int, draft_logits=N
     dev = logits.device
     if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in (f32, torch.bfloat16):
         _refuse("verify_draft: logits must be a float32 or bfloat16 matrix on the GPU")
-    there = _elsewhere(dev, stream)
+    there = _elsewhere(dev, stream, what)
     if there is not None:
         with there:
             if work is not None and stream is not None:
@@ -647,7 +649,7 @@ def verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_dr
     dev = kept_idx.device
     if not kept_idx.is_cuda or kept_idx.dim() != 2:
         _refuse("verify_sets: kept_idx must be a matrix on the GPU")
-    there = _elsewhere(dev, stream)
+    there = _elsewhere(dev, stream, what)
     if there is not None:
         with there:
             if work is not None and stream is not None:
@@ -709,7 +711,7 @@ def linear(x, weight, bias=None, act: str = "none", act_param: float = 0.0, resi
         _refuse("linear: x and weight must be bfloat16 or float16 matrices (or batches of them) on the GPU")
     if act not in ACTS:
         _refuse(f"linear: act must be one of {', '.join(ACTS)}")
-    there = _elsewhere(dev, stream)
+    there = _elsewhere(dev, stream, "linear")
     if there is not None:
         with there:
             return linear(x, weight, bias, act, act_param, residual, out, out_dtype)
