@@ -306,3 +306,47 @@ def test_streams_of_another_device_are_refused(hs):
         with pytest.raises(hs.HsampError) as e:
             call()
         assert e.value.status == hs.ERR_INVALID
+
+
+def test_tensors_of_calls_on_another_stream_are_kept(hs):
+    """What a call on another stream reads and writes is dropped while that stream waits;
+    memory handed out meanwhile and overwritten is not theirs."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(3)
+    V, B, K = 20011, 3, 2
+
+    def normal(*shape):
+        return torch.randn(shape, generator=g, device="cuda")
+
+    x, w = normal(64, 512).to(torch.bfloat16), normal(700, 512).to(torch.bfloat16)
+    b, r = normal(700).to(torch.bfloat16), normal(64, 700).to(torch.bfloat16)
+    p, q = normal(B * (K + 1), V), normal(B * K, V)
+    u, v = torch.rand(B * K, generator=g, device="cuda", dtype=torch.float64), torch.rand(B, generator=g, device="cuda", dtype=torch.float64)
+    d, t = q.argmax(1).to(torch.int32), torch.full((B,), 0.8, device="cuda")
+    n = torch.full((B,), K, dtype=torch.int32, device="cuda")
+    idx = torch.arange(64, dtype=torch.int32, device="cuda").expand(B * (K + 1), 64).contiguous()
+    prob, count = torch.softmax(normal(B * (K + 1), 64), 1), torch.full((B * (K + 1),), 64, dtype=torch.int32, device="cuda")
+    few = d % 64
+    calls = [
+        (hs.linear, (x, w), dict(bias=b, residual=r)),
+        (hs.verify_draft, (p, d, u, v, K), dict(draft_logits=q, temperature=t, draft_temperature=t, n_draft=n)),
+        (hs.verify_sets, (idx, prob, count, few, u, v, K), dict(draft_idx=idx[:B * K].contiguous(), draft_prob=prob[:B * K].contiguous(),
+                                                              draft_count=count[:B * K].contiguous(), n_draft=n)),
+    ]
+    s = torch.cuda.Stream()
+    copy = lambda a: a.clone() if torch.is_tensor(a) else a  # noqa: E731
+    for fn, args, kw in calls:
+        want = fn(*args, **kw)
+        mine, named = [copy(a) for a in args], {k: copy(a) for k, a in kw.items()}
+        sizes = [(a.shape, a.dtype) for a in [*mine, *named.values()] if torch.is_tensor(a)]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(100_000_000)
+        got = fn(*mine, **named, stream=s)
+        mine.clear()
+        named.clear()
+        later = [torch.full(shape, 3, dtype=dtype, device="cuda") for shape, dtype in sizes]
+        torch.cuda.synchronize()
+        del later
+        for a, e in zip(got.values() if isinstance(got, dict) else [got], want.values() if isinstance(want, dict) else [want]):
+            assert torch.equal(a, e)

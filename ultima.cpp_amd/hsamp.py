@@ -516,6 +516,14 @@ def _elsewhere(dev, stream, what):
     return None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
+def _used_on(stream, *tensors):
+    """Their memory is not handed out again before `stream` is done with what it has."""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
 def _launch(fn, a, dev, what):
     import torch
     status = fn(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev.index))
@@ -593,7 +601,9 @@ def verify_draft(logits, draft, u_accept, u_draw, max_draft: int, draft_logits=N
     of sequences whose n_draft or rows are out of range, are not written: what they
     hold is then no probability). work: a uint8 tensor of
     ultima_hsamp_verify_draft_work_bytes() bytes of this call alone (allocated
-    otherwise); outputs: a dict of tensors to write to."""
+    otherwise); outputs: a dict of tensors to write to; stream: a stream of their
+    device to run on instead of the current one (it has to wait for what makes the
+    tensors; their memory is kept until it is done with this call)."""
     import torch
     what, f32 = "verify_draft", torch.float32
     dev = logits.device
@@ -602,10 +612,11 @@ def verify_draft(logits, draft, u_accept, u_draw, max_draft: int, draft_logits=N
     there = _elsewhere(dev, stream, what)
     if there is not None:
         with there:
-            if work is not None and stream is not None:
-                work.record_stream(stream)       # the caller's scratch lives until this stream is done with it
-            return verify_draft(logits, draft, u_accept, u_draw, max_draft, draft_logits, temperature, draft_temperature,
-                                mask, draft_mask, n_draft, target_start, draft_start, accept, work, outputs)
+            out = verify_draft(logits, draft, u_accept, u_draw, max_draft, draft_logits, temperature, draft_temperature,
+                               mask, draft_mask, n_draft, target_start, draft_start, accept, work, outputs)
+        _used_on(stream, logits, draft, u_accept, u_draw, draft_logits, temperature, draft_temperature, mask, draft_mask,
+                 n_draft, target_start, draft_start, work, *out.values())
+        return out
     rows, V = logits.shape
     a = Draft()
     out = _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_start, draft_start, accept,
@@ -652,10 +663,11 @@ def verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_dr
     there = _elsewhere(dev, stream, what)
     if there is not None:
         with there:
-            if work is not None and stream is not None:
-                work.record_stream(stream)
-            return verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_draft, draft_idx, draft_prob,
-                               draft_count, n_draft, target_start, draft_start, accept, work, outputs)
+            out = verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_draft, draft_idx, draft_prob,
+                              draft_count, n_draft, target_start, draft_start, accept, work, outputs)
+        _used_on(stream, kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, draft_idx, draft_prob, draft_count,
+                 n_draft, target_start, draft_start, work, *out.values())
+        return out
 
     def sets(idx, prob, count, rows, names):
         if prob is None or count is None or idx.dtype != torch.int32 or prob.dtype != torch.float32 or \
@@ -704,7 +716,8 @@ def linear(x, weight, bias=None, act: str = "none", act_param: float = 0.0, resi
     + residual, x [M, K] and weight [N, K], or with a leading dimension of groups
     on all of them (expanded dimensions are fine); bfloat16 or float16, the output
     in that type or in float32 (out_dtype; out: the tensor to write, which may be
-    the residual). act: one of ACTS; act_param: the cap of "softcap"."""
+    the residual). act: one of ACTS; act_param: the cap of "softcap"; stream: as in
+    verify_draft."""
     import torch
     dev, dt = x.device, x.dtype
     if not x.is_cuda or dt not in (torch.bfloat16, torch.float16) or x.dim() not in (2, 3) or weight.dim() != x.dim():
@@ -714,7 +727,9 @@ def linear(x, weight, bias=None, act: str = "none", act_param: float = 0.0, resi
     there = _elsewhere(dev, stream, "linear")
     if there is not None:
         with there:
-            return linear(x, weight, bias, act, act_param, residual, out, out_dtype)
+            out = linear(x, weight, bias, act, act_param, residual, out, out_dtype)
+        _used_on(stream, x, weight, bias, residual, out)
+        return out
     lead = x.shape[:-2]
     M, K = x.shape[-2:]
     N = weight.shape[-2]
