@@ -552,11 +552,13 @@ def _seq_args(a, what, dev, draft, u_accept, u_draw, max_draft, n_draft, target_
     """The fields of Draft and DraftSets that say which rows are whose."""
     import torch
     i32, f64 = torch.int32, torch.float64
-    a.u_draw = _vector(u_draw, None, f64, dev, what, "u_draw")
+    if u_draw is None:
+        _refuse(f"{what}: u_draw is missing")
+    a.u_draw, at = _vector(u_draw, None, f64, dev, what, "u_draw"), _vector(draft, None, i32, dev, what, "draft")
     B, K, D = u_draw.shape[0], int(max_draft), 0 if draft is None else draft.shape[0]
     if B < 1 or not 0 <= K <= MAX_DRAFT or (u_accept is None) != (draft is None):
         _refuse(f"{what}: at least one sequence, max_draft 0 .. {MAX_DRAFT}, draft and u_accept together")
-    at, u = _vector(draft, D, i32, dev, what, "draft"), _vector(u_accept, D, f64, dev, what, "u_accept")
+    u = _vector(u_accept, D, f64, dev, what, "u_accept")
     a.seqs, a.max_draft, a.draft_rows = B, K, D
     if D:
         a.draft, a.u_accept = at, u
