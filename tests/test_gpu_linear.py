@@ -350,3 +350,48 @@ def test_tensors_of_calls_on_another_stream_are_kept(hs):
         del later
         for a, e in zip(got.values() if isinstance(got, dict) else [got], want.values() if isinstance(want, dict) else [want]):
             assert torch.equal(a, e)
+
+
+def test_draft_heads_side_by_side_to_verified_sets(hs, sampler, wl):
+    """Several slots, four heads each, written side by side so that the drafter's rows stand
+    slot by slot as the verification takes them: each slot's tokens are the rule's on its
+    own sets, whatever the other slots hold."""
+    import torch
+
+    import verify_reference as R
+    B, K, H, V, cap = 5, 4, 256, 1003, 32
+    g = torch.Generator(device="cuda").manual_seed(19)
+    rng = np.random.default_rng(19)
+
+    def normal(*shape, scale=1.0):
+        return (torch.randn(shape, generator=g, device="cuda") * scale).to(torch.bfloat16)
+
+    hidden, w, bias, lm = normal(B, H), normal(K, H, H, scale=H**-0.5), normal(K, H, scale=0.1), normal(V, H, scale=0.2)
+    heads = torch.empty((B, K, H), dtype=hidden.dtype, device="cuda")
+    hs.linear(hidden.expand(K, -1, -1), w, bias, act="silu", residual=hidden.expand(K, -1, -1), out=heads.transpose(0, 1))
+    drafter = hs.linear(heads.view(-1, H), lm, out_dtype=torch.float32)
+    h64 = hidden.double().cpu().numpy()
+    y = np.einsum("bh,koh->bko", h64, w.double().cpu().numpy()) + bias.double().cpu().numpy()
+    want_heads = torch.from_numpy(y / (1 + np.exp(-y)) + h64[:, None]).cuda()
+    # half a step of bf16; sums of 257 terms whose magnitudes add up to less than 25 by 257 2^-23
+    # of that, stretched by 1.13 at most: 9e-4
+    assert torch.all((heads.double() - want_heads).abs() <= 2.0**-8 * want_heads.abs() + 1e-3)
+    to = lambda a: torch.from_numpy(a).cuda()  # noqa: E731
+    knobs = wl.identity_params(temperature=0.9, top_k=20)
+    drafted = sampler.run(drafter, [knobs] * (B * K), to(rng.random(B * K)), want_sets=True, set_cap=cap)
+    # the target's hidden states near the heads', so that drafts are accepted now and then
+    state = torch.cat([heads + 0.2 * normal(B, K, H), normal(B, 1, H)], 1)
+    logits = hs.linear(state.view(-1, H), lm, out_dtype=torch.float32)
+    target = sampler.run(logits, [knobs] * (B * (K + 1)), to(rng.random(B * (K + 1))), want_sets=True, set_cap=cap)
+    u, v = rng.random(B * K), rng.random(B)
+    out = hs.verify_sets(target["kept_idx"], target["kept_prob"], target["kept_count"], drafted["token"], to(u), to(v), K,
+                         draft_idx=drafted["kept_idx"], draft_prob=drafted["kept_prob"], draft_count=drafted["kept_count"])
+    torch.cuda.synchronize()
+    P, Q = ([r[k].cpu().numpy() for k in ("kept_idx", "kept_prob", "kept_count")] for r in (target, drafted))
+    d, tokens, count = drafted["token"].cpu().numpy(), out["tokens"].cpu().numpy(), out["count"].cpu().numpy()
+    for b in range(B):
+        sl = slice(b * K, b * K + K)
+        want, _, near = R.verify(lambda i: R.dense(*(a[b * (K + 1) + i] for a in P), V),
+                                 lambda i: R.dense(*(a[b * K + i] for a in Q), V), d[sl], u[sl], v[b])
+        assert near > R.NEAR and count[b] == len(want) and list(tokens[b][:len(want)]) == want
+    assert any(c > 1 for c in count)
