@@ -408,7 +408,9 @@ int ultima_hsamp_lm_head(const ultima_hsamp_head* head, void* hip_stream);
  * rounded double.)
  * Row layout: target rows of sequence b start at target_start[b], its drafted
  * rows at draft_start[b] (device int32 [seqs]), so that sequences with fewer
- * drafts take fewer rows; NULL: b * (max_draft + 1) and b * max_draft.
+ * drafts take fewer rows; NULL: b * (max_draft + 1) and b * max_draft. Sequences
+ * may share target rows; a drafted row of two sequences keeps one of their two
+ * acceptance probabilities. No output overlaps an input or another output.
  *
  * On logits: p = softmax(x / T) over the allowed ids, x the logits as they are
  * (no penalties, no top-k: for those, the kept sets below). T <= 0 or NaN: all
@@ -450,7 +452,10 @@ typedef struct ultima_hsamp_draft {
 int64_t ultima_hsamp_verify_draft_work_bytes(int32_t seqs, int32_t max_draft, int32_t vocab);
 
 /* All pointers are device memory of the current device, hip_stream one of its
- * streams; asynchronous, allocates nothing (graph-capturable). */
+ * streams; asynchronous, allocates nothing (graph-capturable).
+ * ULTIMA_HSAMP_ERR_UNSUPPORTED: more waves than a launch numbers, 2^26 of one for
+ * each 8 KB of the rows there could be (64 sequences of 128 drafts over 151936 ids
+ * in float take 1.4 million). */
 int ultima_hsamp_verify_draft(const ultima_hsamp_draft* d, void* hip_stream);
 
 /* On kept sets: p and q are the sets ultima_hsamp_run() leaves (kept_idx,
@@ -488,7 +493,8 @@ typedef struct ultima_hsamp_draft_sets {
  * (-1 for invalid sizes). */
 int64_t ultima_hsamp_verify_sets_work_bytes(int32_t seqs, int32_t set_cap);
 
-/* Asynchronous on hip_stream, allocates nothing (graph-capturable). */
+/* Asynchronous on hip_stream, allocates nothing (graph-capturable); up to 2^21
+ * sequences. */
 int ultima_hsamp_verify_sets(const ultima_hsamp_draft_sets* d, void* hip_stream);
 
 /* ---- The product with its epilogue ---------------------------------------------
@@ -497,7 +503,9 @@ int ultima_hsamp_verify_sets(const ultima_hsamp_draft_sets* d, void* hip_stream)
  * head's residual block (x + silu(W x + b) on the final hidden states), several
  * heads in one call (groups), the vocabulary product over all positions of
  * drafted blocks (with a logit soft cap). 16-bit inputs, sums in float, bias,
- * activation and residual in float, rounded once to the output's type. */
+ * activation and residual in float, rounded once to the output's type. The same
+ * call gives the same bits every time; where a row's sum begins goes by the tile
+ * it is in, so its last bits may differ with rows, columns and groups. */
 #define ULTIMA_HSAMP_F16 9           /* IEEE half (ultima_hsamp_linear) */
 #define ULTIMA_HSAMP_ACT_NONE 0
 #define ULTIMA_HSAMP_ACT_RELU 1

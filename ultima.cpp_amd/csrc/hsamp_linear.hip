@@ -39,8 +39,9 @@ __device__ __forceinline__ uint16_t from_f32(float f) {   // to nearest, ties to
 }
 
 // 1 / (1 + exp(-t)) by the hardware's exp2 and reciprocal (one step of 2^-23
-// each); the exponent's rounding moves exp(-t) by |t| 2^-24, at most 2^-17 of a
-// value below 2^-126. exp(-t) past the largest float is infinite, the result 0.
+// each); the roundings of the exponent and of log2 e move exp(-t) by 1.3 |t| 2^-24 of
+// it (5e-6 at 64), at most 2^-17 where the value is below 2^-126. exp(-t) past the
+// largest float is infinite, the result 0.
 // (With expf and a division the epilogue of 256 x 256 tiles took 90 of 554 us.)
 __device__ __forceinline__ float sigmoid(float t) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t * -1.44269504f));
@@ -201,10 +202,12 @@ __device__ __forceinline__ void store_tiles(const Args& a, int g, int m0, int n0
 // narrow tiles, whose waves share K instead of columns, and many loads in the air.
 // Many: per stage the loads to LDS and the LDS reads beside the products: hence the
 // widest tile that the accumulators allow, whose operands are read least often
-// (4096 rows of 4096 x 16384 462 us, 1190 TFLOP/s, where 8192 cubed reaches 1215 in
-// the library; with bias, tanh and residual 519). 320 rows of 4096 x 151936: 440 us
-// (with the soft cap in float 458), 905 TFLOP/s: 190 MB are written, and two and a
-// half tiles of rows need 160 of 128.
+// (4096 rows of 4096 x 16384 462 us, 1190 TFLOP/s, where 8192 cubed reaches 1215 to
+// 1415 in the library, by card and clock; with bias, tanh and residual 533). Of its 1350
+// MB from memory x is most: an XCD's 32 tiles in the air are all 16 of the rows by 2 of
+// the columns, so each reads x four times (8 x 4 x 34 MB), the weight and the residual
+// (134 MB each) come once. 320 rows of 4096 x 151936: 440 us (with the soft cap in float
+// 463), 905 TFLOP/s: 194 MB are written, and two and a half tiles of rows need 160 of 128.
 // ANY: rows at any element's address, a last piece of less than eight columns
 // (loads to LDS take neither): one stage in registers, two in LDS.
 template <bool BF, bool ANY, int WM, int WN, int WK, int TM, int TN, int ST>
@@ -429,6 +432,10 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(Args a, int t
 //   rows 64: -, 32, rows 256: 24, -; 128 x 128 rows 256: 41, 56, rows 1024: 52, 168;
 //   160 x 128 rows 512: 63, 83, rows 2048: 76, 284; 256 x 256 rows 1024: 101, 123, rows
 //   4096 (f16): -, 462.
+// Rows at any alignment take the nearest of three tiles by the same costs, which are not
+// theirs. K = 4097, the tile it takes and the best of the three: N = 4096, rows 64 22, 22;
+// 256 47, 36; 512 58, 56; 1024 68, 66; 2048 99, 95. N = 16384, rows 64 47, 36; 128 58,
+// 57; 256 68, 66; 1024 191, 187.
 struct Form {
     int bm, bn, blocks;
     float one[2];

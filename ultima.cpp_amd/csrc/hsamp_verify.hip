@@ -403,7 +403,7 @@ __global__ __launch_bounds__(kThreads) void k_draft_start(DraftArgs a) {
 
 // Draft i of sequence b, all slices of its rows known: one wave. False, and nothing
 // written: its u is within `margin` (of the larger side) of the border.
-constexpr double kUnsure = 1e-5;             // both rows' sums are off by at most 3e-6
+constexpr double kUnsure = 1e-5;             // each row's sum is off by at most 2.7e-6
 template <bool BF>
 __device__ __forceinline__ bool decide(const DraftArgs& a, const Seq& q, int b, int i, double margin, const double* table) {
     const int lane = threadIdx.x & 63;
@@ -441,10 +441,10 @@ __device__ __forceinline__ bool decide(const DraftArgs& a, const Seq& q, int b, 
 // a time, the next one's loads in flight.
 //
 // FAST: exponentials in float (a third of the instructions of those in double, which
-// bound the pass: 256 sequences of 8 drafts 175 us against 303). A slice's sum is then off
-// by at most 3e-6 of it: per term 2 |z| 2^-24 from the exponent z = (x - m) / T and 2^-23
-// from exp2, where the terms' mean |z| is at most ln V < 17 (the entropy's bound);
-// 9 2^-24 from the float additions. Enough to decide most drafts (kUnsure below), not
+// bound the pass). A slice's sum is then off by at most 45 2^-24 = 2.7e-6 of it: per term
+// 2 |z| 2^-24 from the exponent z = (x - m) / T (the factor's rounding and the product's)
+// and 2^-23 from exp2, where the terms' mean |z| is at most ln V < 17 (the entropy's
+// bound); 9 2^-24 from the float additions. Enough to decide most drafts (kUnsure below), not
 // to draw a token.
 template <bool BF, bool MASK, bool FAST>
 __device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, int s1, const double* table, SliceStat* to) {
@@ -625,10 +625,13 @@ __device__ __forceinline__ void row_slices(const Row<BF>& r, double c, int s0, i
 }
 
 // Bound by the bytes of the rows that are read and, as much, by the exponentials beside
-// them: 64 sequences of 4 drafts over 151936 f32 logits 69 us, 301 MB at 4.4 TB/s (350 MB
-// are there, the drafts up to the rejected ones need 224); 256 of 8 in bf16 175 us, 806 MB
-// at 4.6 TB/s (1.3 GB there, 690 needed). One sequence of 4: 11 us, its start, one slice a
-// wave and the decisions one after the other. Four waves a SIMD: their registers.
+// them: 64 sequences of 4 drafts over 151936 f32 logits 69 us, 311 MB at 4.5 TB/s (350 MB
+// are there, the drafts up to the rejected ones need 267); 256 of 8 in bf16 179 us, 811 MB
+// at 4.5 TB/s (1.3 GB there, 726 needed). 16 of 15 without a drafter 32 us, 87 MB (160
+// there with their masks, 26 needed): positions in the air before a rejection is known.
+// One sequence of 4: 11 us for 6 MB, the reads that wait for each other: a slice, and in
+// the block that completes a position its count, the slices' sums, the drafted id, the
+// logits at it. Four waves a SIMD: their registers.
 template <bool BF, bool MASK, bool FAST>
 __global__ __launch_bounds__(kThreads, 4) void k_draft_stats(DraftArgs a) {
     using R = Row<BF>;
@@ -675,7 +678,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_draft_stats(DraftArgs a) {
 }
 
 // FAST calls: the emitting rows' slices in double. (Greedy rows need none.) Bound by the
-// exponentials: 256 sequences, 155 MB, 54 us.
+// exponentials: 256 sequences, 148 MB, 52 us.
 template <bool BF, bool MASK>
 __global__ __launch_bounds__(kThreads, 4) void k_draft_exact(DraftArgs a) {
     __shared__ double table[32];
@@ -788,7 +791,7 @@ __device__ __forceinline__ int first_reaching(F value, int n, double base, doubl
 
 // TH threads a block, a wave per part of a slice (PARTS of them). Few sequences: bound by
 // what waits for each other (statistics, part, count, parts' sums, the part again): one
-// 9 us. Many: two exponentials an id: 256 over 151936 79 us.
+// 9 us. Many: two exponentials an id: 256 over 151936 76 us.
 template <bool BF, int TH, int PARTS>
 __global__ __launch_bounds__(TH) void k_draft_draw(DraftArgs a) {
     using R = Row<BF>;
@@ -1055,7 +1058,7 @@ enum SetsPart { kSetsWhole, kSetsTiles, kSetsPick };
 // each entry of the target's looks for its own. What bounds it are the chains of reads
 // that wait for each other (rows, counts, three or four steps of a search, a tile): 8 us
 // for one sequence of sets up to 64, 11 for 64 of up to 1024. Larger sets would follow
-// one block's tiles one after the other: 32 of up to 32768 ids 62 us, as here 24 + 16.
+// one block's tiles one after the other: 32 of up to 32768 ids 62 us, as here 21 + 15.
 //   kSetsWhole: sets of one tile, one block per sequence
 //   kSetsTiles: the tiles' sums, tiles shared out to a sequence's blocks (each finds
 //               the emitting position by itself)
