@@ -544,6 +544,183 @@ typedef struct ultima_hsamp_linear_args {
  * (graph-capturable). */
 int ultima_hsamp_linear(const ultima_hsamp_linear_args* a, void* hip_stream);
 
+/* ---- The product in 8-bit integers ----------------------------------------------
+ * out = act(s_m s_n sum_k(x_mk w_nk) + bias) + residual: ultima_hsamp_linear on
+ * 8-bit rows and weights with a scale for each row (token) and each output column
+ * (channel). Half the weight's bytes, twice the rate of the matrix cores; the sums
+ * are exact, rounded to float before the scales. */
+#define ULTIMA_HSAMP_MAX_I8_DIM 131071   /* in_dim: sums of products of up to 2^14 stay below 2^31 */
+typedef struct ultima_hsamp_linear_i8_args {
+    int32_t rows;               /* M >= 1 */
+    int32_t in_dim;             /* K, 1 .. ULTIMA_HSAMP_MAX_I8_DIM */
+    int32_t out_dim;            /* N >= 1 */
+    int32_t groups;             /* products in the call, >= 1 (65535 at most) */
+    int32_t dtype;              /* of bias and residual: ULTIMA_HSAMP_BF16 or ULTIMA_HSAMP_F16 */
+    int32_t out_dtype;          /* dtype, or ULTIMA_HSAMP_F32 */
+    int32_t act;                /* ULTIMA_HSAMP_ACT_* */
+    float act_param;            /* ULTIMA_HSAMP_ACT_SOFTCAP: the cap; else ignored */
+    const int8_t* x;            /* [M, K], rows x_stride elements apart */
+    int64_t x_stride;           /* >= K */
+    int64_t x_group;            /* elements between groups (0: one x for all) */
+    const float* x_scale;       /* [M] */
+    int64_t x_scale_group;
+    const int8_t* weight;       /* [N, K], rows weight_stride elements apart */
+    int64_t weight_stride;      /* >= K */
+    int64_t weight_group;
+    const float* weight_scale;  /* [N] */
+    int64_t weight_scale_group;
+    const void* bias;           /* [N] or NULL; from here as in ultima_hsamp_linear_args */
+    int64_t bias_group;
+    const void* residual;       /* [M, N] or NULL; may be out itself (same type, strides and group) */
+    int64_t residual_stride;    /* >= N */
+    int64_t residual_group;
+    void* out;                  /* [M, N]; no overlap with the inputs but the one above */
+    int64_t out_stride;         /* >= N */
+    int64_t out_group;
+} ultima_hsamp_linear_i8_args;
+
+/* As ultima_hsamp_linear: device memory of the current device aligned to its
+ * elements, asynchronous on hip_stream, allocates nothing (graph-capturable). */
+int ultima_hsamp_linear_i8(const ultima_hsamp_linear_i8_args* a, void* hip_stream);
+
+/* Rows (of tokens; of a weight: its channels) in 8 bits: scale_m = max_k |x_mk| / 127,
+ * q_mk the whole number nearest to 127 x_mk / max_k |x_mk| (halves to even, by the
+ * exact quotient), -127 .. 127. A row of zeros has scale 0; a row that holds an
+ * infinity or a NaN scale NaN and q 0, so that its products are NaN. */
+typedef struct ultima_hsamp_quantize_args {
+    int32_t rows;               /* 1 .. 2^24 - 1 */
+    int32_t in_dim;             /* 1 .. 2^30 */
+    int32_t dtype;              /* ULTIMA_HSAMP_F32, _BF16 or _F16 */
+    const void* x;              /* [rows, in_dim], rows x_stride elements apart */
+    int64_t x_stride;           /* >= in_dim */
+    int8_t* q;                  /* [rows, in_dim] out, rows q_stride apart */
+    int64_t q_stride;           /* >= in_dim */
+    float* scale;               /* [rows] out */
+} ultima_hsamp_quantize_args;
+
+/* Asynchronous on hip_stream, allocates nothing (graph-capturable). */
+int ultima_hsamp_quantize_rows(const ultima_hsamp_quantize_args* a, void* hip_stream);
+
+/* ---- Cross entropy over the vocabulary, without its logits -----------------------
+ * For each row m and its token t: z = x W^T (with a soft cap c: c tanh(z / c)),
+ *   lse_m = log sum_v exp(z_mv),   loss_m = lse_m - z_mt
+ * (minus the log-probability of the token), the product made piece by piece and
+ * never stored: the log-probabilities of given tokens (a sampled one, a whole
+ * prompt's) and the loss that trains a head. A target outside [0, vocab) is ignored:
+ * loss 0 (lse stands). 16-bit inputs, float sums and statistics. A row with a logit
+ * that is NaN or +inf has NaN for both; -inf logits have probability 0. */
+typedef struct ultima_hsamp_cross_entropy_args {
+    int32_t rows;               /* M >= 1 */
+    int32_t in_dim;             /* K >= 1 */
+    int32_t vocab;              /* V, 1 .. ULTIMA_HSAMP_MAX_VOCAB */
+    int32_t dtype;              /* of x and weight: ULTIMA_HSAMP_BF16 or ULTIMA_HSAMP_F16 */
+    float softcap;              /* 0: none; c > 0 */
+    const void* x;              /* [M, K], rows x_stride elements apart */
+    int64_t x_stride;           /* >= K */
+    const void* weight;         /* [V, K], rows weight_stride elements apart */
+    int64_t weight_stride;      /* >= K */
+    const int32_t* target;      /* [M] */
+    float* loss;                /* [M] out */
+    float* lse;                 /* [M] out */
+    void* work;                 /* ultima_hsamp_cross_entropy_work_bytes() bytes, 16-byte aligned, of this call
+                                   alone until it completes; needs no initial contents */
+} ultima_hsamp_cross_entropy_args;
+
+/* Bytes of workspace ultima_hsamp_cross_entropy needs (-1 for invalid sizes). */
+int64_t ultima_hsamp_cross_entropy_work_bytes(int32_t rows, int32_t vocab);
+
+/* All pointers are device memory of the current device, aligned to their elements;
+ * hip_stream one of its streams; asynchronous, allocates nothing (graph-capturable). */
+int ultima_hsamp_cross_entropy(const ultima_hsamp_cross_entropy_args* a, void* hip_stream);
+
+/* Its gradients. grad_m is the loss's gradient with respect to loss_m (ignored rows:
+ * not looked at, taken as 0); lse as ultima_hsamp_cross_entropy left it.
+ *   dz_mv = grad_m (exp(z_mv - lse_m) - [v = t_m]) (with a soft cap: times 1 - (z_mv / c)^2)
+ *   d_x = dz W,   d_weight = dz^T x  (accumulate: added to what d_weight holds)
+ * The logits are made again, a piece of the vocabulary at a time; dz is rounded to
+ * x's type before the two products (half precision: grad / max |grad| stands in for
+ * grad there, and dz / grad is scaled by 2^15, so that no probability above 2^-39
+ * is lost), whose sums are float. Rows whose lse is NaN have NaN gradients. */
+typedef struct ultima_hsamp_cross_entropy_grad_args {
+    int32_t rows;               /* as in ultima_hsamp_cross_entropy_args, to target */
+    int32_t in_dim;
+    int32_t vocab;
+    int32_t dtype;
+    float softcap;
+    int32_t accumulate;         /* nonzero: d_weight += */
+    const void* x;
+    int64_t x_stride;
+    const void* weight;
+    int64_t weight_stride;
+    const int32_t* target;
+    const float* lse;           /* [M] */
+    const float* grad;          /* [M] */
+    void* d_x;                  /* [M, K] out, or NULL: not needed */
+    int64_t d_x_stride;         /* >= K */
+    void* d_weight;             /* [V, K] out, or NULL: not needed */
+    int64_t d_weight_stride;    /* >= K */
+    int32_t d_x_dtype;          /* dtype, or ULTIMA_HSAMP_F32 */
+    int32_t d_weight_dtype;     /* dtype, or ULTIMA_HSAMP_F32 */
+    void* work;                 /* ultima_hsamp_cross_entropy_grad_work_bytes() bytes, as above */
+} ultima_hsamp_cross_entropy_grad_args;
+
+/* Bytes of workspace ultima_hsamp_cross_entropy_grad needs (-1 for invalid sizes): a
+ * piece of dz and float sums of d_x, 0.1 to 0.5 GB at large sizes whatever the vocabulary. */
+int64_t ultima_hsamp_cross_entropy_grad_work_bytes(int32_t rows, int32_t in_dim, int32_t vocab);
+
+/* As ultima_hsamp_cross_entropy; the same call gives the same bits every time. */
+int ultima_hsamp_cross_entropy_grad(const ultima_hsamp_cross_entropy_grad_args* a, void* hip_stream);
+
+/* ---- Embedding -----------------------------------------------------------------
+ * out_i = scale * table[id_i]: the sampled tokens' rows of the (tied) vocabulary
+ * matrix, the next step's input. An id outside [0, vocab) (an ended slot's -1) gives
+ * a row of zeros. */
+typedef struct ultima_hsamp_embed_args {
+    int32_t tokens;             /* N >= 1 */
+    int32_t width;              /* H >= 1 */
+    int32_t vocab;              /* 1 .. ULTIMA_HSAMP_MAX_VOCAB */
+    int32_t dtype;              /* of the table: ULTIMA_HSAMP_F32, _BF16 or _F16 */
+    int32_t out_dtype;          /* dtype, or ULTIMA_HSAMP_F32 */
+    float scale;
+    const void* table;          /* [vocab, H], rows table_stride elements apart */
+    int64_t table_stride;       /* >= H */
+    const int32_t* ids;         /* [N] */
+    void* out;                  /* [N, H] out, rows out_stride elements apart */
+    int64_t out_stride;         /* >= H */
+} ultima_hsamp_embed_args;
+
+/* Device memory of the current device aligned to its elements, asynchronous on
+ * hip_stream, allocates nothing (graph-capturable). */
+int ultima_hsamp_embed(const ultima_hsamp_embed_args* a, void* hip_stream);
+
+/* The gradient of that: out_v = scale * (the sum of d_out_i over the i with id_i = v),
+ * every row of the table (zeros where no token is; accumulate: added to what out
+ * holds, rows without tokens left alone). Tokens are sorted, sums are float in an
+ * order that goes by the tokens alone (no atomics): the same call gives the same
+ * bits every time. */
+typedef struct ultima_hsamp_embed_grad_args {
+    int32_t tokens;             /* N >= 1 */
+    int32_t width;              /* H >= 1 */
+    int32_t vocab;              /* 1 .. ULTIMA_HSAMP_MAX_VOCAB */
+    int32_t dtype;              /* of d_out: ULTIMA_HSAMP_F32, _BF16 or _F16 */
+    int32_t out_dtype;          /* dtype, or ULTIMA_HSAMP_F32 */
+    int32_t accumulate;         /* nonzero: out += */
+    float scale;
+    const void* d_out;          /* [N, H], rows d_out_stride elements apart */
+    int64_t d_out_stride;       /* >= H */
+    const int32_t* ids;         /* [N] */
+    void* out;                  /* [vocab, H] out, rows out_stride elements apart */
+    int64_t out_stride;         /* >= H */
+    void* work;                 /* ultima_hsamp_embed_grad_work_bytes() bytes, 16-byte aligned, of this call
+                                   alone until it completes; needs no initial contents */
+} ultima_hsamp_embed_grad_args;
+
+/* Bytes of workspace ultima_hsamp_embed_grad needs (-1 for invalid sizes). */
+int64_t ultima_hsamp_embed_grad_work_bytes(int32_t tokens, int32_t width, int32_t vocab);
+
+/* As ultima_hsamp_embed. */
+int ultima_hsamp_embed_grad(const ultima_hsamp_embed_grad_args* a, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,188 @@
+"""embed and embed_grad against the host.
+
+embed: one product in float and one rounding: equal bits. embed_grad: a sum of n rows
+in float, n - 1 additions of half a step (2^-24) of at most the sum of magnitudes S;
+with the scale, the old value and the result's rounding: (n + 2) 2^-24 |scale| S and
+half a step of the type."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+DTYPES = [("bfloat16", "bfloat16"), ("bfloat16", "float32"), ("float16", "float16"), ("float16", "float32"), ("float32", "float32")]
+
+
+def padded(g, rows, width, dtype, pad, offset=0):
+    """Rows `pad` elements apart, `offset` elements into NaN."""
+    import torch
+    dt = getattr(torch, dtype)
+    buf = torch.full((offset + rows * (width + pad),), float("nan"), dtype=dt, device="cuda")
+    t = buf[offset:].view(rows, width + pad)[:, :width]
+    t.copy_(torch.randn((rows, width), generator=g, device="cuda"))
+    return t
+
+
+@pytest.mark.parametrize("dtype,out", DTYPES)
+@pytest.mark.parametrize("N,H,V", [(1, 1, 1), (1, 4096, 1000), (7, 5, 3), (64, 1002, 777), (300, 2049, 50), (1000, 64, 5000)])
+@pytest.mark.parametrize("pad,offset", [(0, 0), (3, 1)])
+def test_embed(hs, N, H, V, dtype, out, pad, offset):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(N + H)
+    w = padded(g, V, H, dtype, pad, offset)
+    ids = torch.randint(0, V, (N,), generator=g, device="cuda", dtype=torch.int32)
+    ids[N // 2:N // 2 + 2] = -1
+    if N > 20:
+        ids[3], ids[4], ids[5], ids[6] = V, 2**31 - 1, -2**31, V - 1
+    odt = getattr(torch, out)
+    full = torch.full((N, H + 3), 77.0, dtype=odt, device="cuda")
+    for scale in (1.0, 0.3, -64.0):
+        got = hs.embed(w, ids, scale=scale, out=full[:, :H])
+        torch.cuda.synchronize()
+        i = ids.long()
+        ok = (i >= 0) & (i < V)
+        want = torch.where(ok[:, None], w[torch.where(ok, i, 0)].float() * scale, 0.0).to(odt)
+        assert torch.equal(got, want) and torch.all(full[:, H:] == 77.0)
+    assert torch.equal(hs.embed(w, ids, scale=0.3, out_dtype=odt), hs.embed(w, ids, scale=0.3, out=full[:, :H]))
+
+
+def test_embed_values(hs):
+    """Infinities and NaN of a row stay in it; a row that no token names is not looked at."""
+    import torch
+    w = torch.randn((10, 40), device="cuda").to(torch.bfloat16)
+    w[3, 7], w[4, 1], w[9] = float("inf"), float("nan"), float("nan")
+    got = hs.embed(w, torch.tensor([3, 4, 5, -1, 10], dtype=torch.int32, device="cuda"), scale=2.0)
+    assert torch.isinf(got[0, 7]) and torch.isnan(got[1, 1]) and torch.isfinite(got[2:]).all() and not got[3:].any()
+    assert torch.isfinite(got[0]).sum() == 39
+
+
+def compare(got, d, ids, V, scale, old=None):
+    import torch
+    i = ids.long()
+    ok = (i >= 0) & (i < V)
+    rows, at = d.double()[ok], i[ok]
+    sums, mags = (torch.zeros((V, d.shape[1]), dtype=torch.float64, device="cuda").index_add_(0, at, r) for r in (rows, rows.abs()))
+    n = torch.bincount(at, minlength=V).double()[:, None]
+    want = sums * scale
+    tol = (n + 2) * 2.0**-24 * abs(scale) * mags
+    if old is not None:
+        want = want + old.double()
+        tol = tol + 2.0**-24 * old.double().abs()
+    tol = tol + torch.finfo(got.dtype).eps / 2 * (want.abs() + tol) + (2.0**-25 if got.dtype == torch.float16 else 1e-38)
+    off = ((got.double() - want).abs() / tol).nan_to_num(nan=9.0)
+    assert off.max() <= 1, f"{off.max().item()} times the bound at {np.unravel_index(off.argmax().item(), off.shape)}"
+    none = (n[:, 0] == 0)
+    assert torch.equal(got[none], old[none] if old is not None else torch.zeros_like(got[none]))
+
+
+def tokens(g, N, V, skew):
+    """Ids, some out of range; skew: most of them a few."""
+    import torch
+    ids = torch.randint(0, V, (N,), generator=g, device="cuda", dtype=torch.int32)
+    if skew == "one":
+        ids[:] = V // 2
+    elif skew == "few":
+        u = torch.rand(N, generator=g, device="cuda")
+        ids = torch.where(u < 0.5, V // 3, torch.where(u < 0.8, V - 1, ids)).to(torch.int32)
+    elif skew == "runs":
+        ids = (torch.arange(N, device="cuda") // 70 % V).to(torch.int32)
+    if N > 10 and skew != "one":
+        ids[1], ids[5], ids[7], ids[-1] = -1, V, -2**31, 2**31 - 1
+    return ids
+
+
+@pytest.mark.parametrize("skew", ["flat", "one", "few", "runs"])
+@pytest.mark.parametrize("N,H,V", [(1, 1, 1), (3, 5, 1000), (64, 512, 64), (65, 100, 7), (700, 1002, 5021), (1024, 8, 1025), (5000, 520, 300),
+                                   (9000, 64, 20000), (20000, 17, 2)])
+def test_embed_grad(hs, N, H, V, skew):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(N + V)
+    ids = tokens(g, N, V, skew)
+    for k, (dtype, out) in enumerate(DTYPES):
+        d = padded(g, N, H, dtype, 3 * (k % 2), k % 3)
+        full = torch.full((V, H + 3), 77.0, dtype=getattr(torch, out), device="cuda")
+        got = hs.embed_grad(d, ids, V, scale=0.7, out=full[:, :H])
+        torch.cuda.synchronize()
+        assert torch.all(full[:, H:] == 77.0)
+        compare(got, d, ids, V, np.float32(0.7).item())
+        again = hs.embed_grad(d, ids, V, scale=0.7, out_dtype=getattr(torch, out))
+        old = torch.randn((V, H), generator=g, device="cuda").to(getattr(torch, out))
+        more = hs.embed_grad(d, ids, V, scale=-2.0, out=old.clone(), accumulate=True)
+        torch.cuda.synchronize()
+        assert torch.equal(again, got)
+        compare(more, d, ids, V, -2.0, old)
+
+
+def test_embed_grad_many_tokens(hs):
+    """Chunks of more than 64 positions; a vocabulary of more ids than blocks of a thousand."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for N, H, V, skew in ((150_000, 16, 3000, "few"), (70_000, 9, 700_000, "flat"), (66_000, 24, 300_000, "one")):
+        ids = tokens(g, N, V, skew)
+        d = padded(g, N, H, "bfloat16", 0)
+        got = hs.embed_grad(d, ids, V, out_dtype=torch.float32)
+        torch.cuda.synchronize()
+        compare(got, d, ids, V, 1.0)
+
+
+def test_embed_grad_no_token_counts(hs):
+    import torch
+    ids = torch.full((100,), -1, dtype=torch.int32, device="cuda")
+    d = torch.full((100, 33), float("nan"), device="cuda")
+    got = hs.embed_grad(d, ids, 50)
+    assert not torch.any(got)
+
+
+def test_gradient_of_embed(hs):
+    """<embed(w), d> = <w, embed_grad(d)>, in whole numbers: both sides exact."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(4)
+    V, N, H = 500, 900, 72
+    whole = lambda *s: torch.randint(-4, 5, s, generator=g, device="cuda").float()  # noqa: E731
+    w, d, ids = whole(V, H), whole(N, H), tokens(g, N, V, "few")
+    y, dw = hs.embed(w, ids, scale=2.0), hs.embed_grad(d, ids, V, scale=2.0)
+    assert (y.double() * d.double()).sum() == (w.double() * dw.double()).sum()
+    # and by differences: one entry of the table moved by 1
+    for v, c in ((V // 3, 0), (V - 1, 71), (17, 5)):
+        w2 = w.clone()
+        w2[v, c] += 1
+        moved = ((hs.embed(w2, ids, scale=2.0) - y).double() * d.double()).sum()
+        assert moved == dw[v, c].double()
+
+
+def test_captured_with_other_work_between(hs):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(5)
+    V, N, H = 3000, 2000, 200
+    w, ids, d = padded(g, V, H, "bfloat16", 0), tokens(g, N, V, "few"), padded(g, N, H, "bfloat16", 0)
+    out, dw = hs.embed(w, ids), hs.embed_grad(d, ids, V)
+    work = torch.empty(hs.lib().ultima_hsamp_embed_grad_work_bytes(N, H, V), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        hs.embed(w, ids, out=out)
+        hs.embed_grad(d, ids, V, out=dw, work=work)
+    s = torch.cuda.Stream()
+    for skew in ("flat", "one", "runs", "few"):
+        ids.copy_(tokens(g, N, V, skew))
+        d.copy_(torch.randn(d.shape, generator=g, device="cuda"))
+        work.fill_(255)
+        want = hs.embed(w, ids), hs.embed_grad(d, ids, V)
+        torch.cuda.synchronize()
+        other = hs.embed(w, ids, stream=s), hs.embed_grad(d, ids, V, stream=s)
+        out.fill_(1), dw.fill_(1)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(dw, want[1]) and torch.equal(other[0], want[0]) and torch.equal(other[1], want[1])
+
+
+def test_past_32_bit_offsets(hs):
+    """A table of more than 2^32 elements: its last rows, read and written."""
+    import torch
+    V, H = 1_100_000, 4096
+    w = torch.zeros((V, H), dtype=torch.bfloat16, device="cuda")
+    w[-3:] = torch.randn((3, H), device="cuda").to(torch.bfloat16)
+    ids = torch.tensor([V - 1, 0, V - 3, V], dtype=torch.int32, device="cuda")
+    got = hs.embed(w, ids)
+    assert torch.equal(got[0], w[-1]) and torch.equal(got[2], w[-3]) and not got[1].any() and not got[3].any()
+    dw = hs.embed_grad(got, ids, V, out=w)
+    torch.cuda.synchronize()
+    assert torch.equal(dw[-1], got[0]) and torch.equal(dw[-3], got[2]) and not dw[-2].any() and not dw[:1000].any()

@@ -1,0 +1,375 @@
+"""cross_entropy and cross_entropy_grad against 64 bits.
+
+Inputs. "whole": rows of small whole numbers and weights in eighths, whose products'
+sums are exact in float (up to 2^20 steps of 1/8), so that what is left is the softmax's
+own error. "normal": the sums are off by K 2^-23 of the sum of magnitudes S.
+
+Forward. E: the largest error of a row's logits; a soft cap adds 2^-20 of |z|. An
+exponential exp(t) is off by (2 |t| + 4) 2^-24 of itself, and so is each time a partial
+sum is moved to a larger maximum (t then being the difference; the mean of (2 |t| + 4)
+e^t over what counts is below 5): at most tiles / 64 + 20 times. With J = V / 1024 + 120
+of these and of additions, the sum is off by r = 2^-24 (5 J + 2 sum p |t|) of itself.
+lse: E + r + 2^-24 |lse|. loss: that and the target's own error, 2^-23 |loss|.
+
+Gradients. dz = g (p - [t]) z': p is off by p (E + 2^-24 (2 |z - lse| + 4)), z' by 2^-20; then a
+rounding of half a step of the type, h |dz| (half precision: and 2^-25 2^-15 max |g|).
+d_x = dz W: these through |W|, and a float sum of V terms, (V + 40) 2^-23 of their
+magnitudes; then the result's type. d_weight the same with M terms."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def inputs(seed, M, K, V, dtype="bfloat16", kind="whole", pad=0, offset=0, sure=0.5, ignored=0.2):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    dt = getattr(torch, dtype)
+
+    def rows(n, values):
+        """`pad` elements apart, `offset` elements into NaN."""
+        buf = torch.full((offset + n * (K + pad),), float("nan"), dtype=dt, device="cuda")
+        t = buf[offset:].view(n, K + pad)[:, :K]
+        t.copy_(values)
+        return t
+
+    t = torch.randint(0, V, (M,), generator=g, device="cuda", dtype=torch.int32)
+    if kind == "whole":
+        w = rows(V, torch.randint(-3, 4, (V, K), generator=g, device="cuda") / 8 * (torch.rand((V, K), generator=g, device="cuda") < min(1, 64 / K)))
+        x = torch.randint(-2, 3, (M, K), generator=g, device="cuda").float()
+    else:
+        w = rows(V, torch.randn((V, K), generator=g, device="cuda") * 2 * K**-0.5)
+        x = torch.randn((M, K), generator=g, device="cuda")
+    point = (torch.rand((M, 1), generator=g, device="cuda") < sure) * (8.0 if kind == "whole" else 2.5)
+    x = rows(M, x + point * w[t.long()].float())
+    if ignored and M > 3:
+        t = torch.where(torch.rand(M, generator=g, device="cuda") < ignored, -1, t).to(torch.int32)
+        t[0], t[1] = V, 2**31 - 1
+    grad = torch.rand(M, generator=g, device="cuda") * 2 - 0.5
+    return x, w, t, grad
+
+
+def reference(x, w, t, cap, kind):
+    """64-bit logits, their bound, lse, loss."""
+    import torch
+    x, w = x.double(), w.double()
+    y = x @ w.t().contiguous()
+    E = torch.zeros_like(y) if kind == "whole" else x.shape[1] * 2.0**-23 * (x.abs() @ w.abs().t().contiguous())
+    z = y
+    if cap:
+        z = cap * torch.tanh(y / cap)
+        E = E + 2.0**-20 * z.abs()
+    lse = torch.logsumexp(z, 1)
+    ok = (t >= 0) & (t < w.shape[0])
+    at = torch.where(ok, t, 0).long()
+    loss = torch.where(ok, -torch.log_softmax(z, 1).gather(1, at[:, None])[:, 0], 0.0)
+    return z, E, lse, loss, ok, at
+
+
+def worst(off, what):
+    off = off.nan_to_num(nan=9.0)
+    assert off.max() <= 1, f"{what}: {off.max().item()} times the bound at {np.unravel_index(off.argmax().item(), off.shape)}"
+
+
+def check_forward(out, x, w, t, cap, kind):
+    z, E, lse, loss, ok, at = reference(x, w, t, cap, kind)
+    V = w.shape[0]
+    far = (torch_exp(z - lse[:, None]) * (z - z.amax(1, keepdim=True)).abs()).sum(1)
+    r = 2.0**-24 * (5 * (V / 1024 + 120) + 2 * far)
+    tol = E.amax(1) + r + 2.0**-24 * lse.abs()
+    worst((out["lse"].double() - lse).abs() / tol, "lse")
+    tol = tol + E.gather(1, at[:, None])[:, 0] + 2.0**-23 * loss.abs()
+    worst(torch_where(ok, (out["loss"].double() - loss).abs() / tol, out["loss"].double().abs() * 1e30), "loss")
+
+
+def torch_exp(a):
+    import torch
+    return torch.exp(a)
+
+
+def torch_where(c, a, b):
+    import torch
+    return torch.where(c, a, b)
+
+
+def check_grads(out, x, w, t, lse, grad, cap, kind, old=None):
+    import torch
+    z, E, _, _, ok, at = reference(x, w, t, cap, kind)
+    x, w, lse = x.double(), w.double(), lse.double()
+    dt = torch.float16 if out["kind"] == "float16" else torch.bfloat16
+    h = torch.finfo(dt).eps / 2
+    g = torch.where(ok, grad, 0.0).double()[:, None]
+    p = torch.exp(z - lse[:, None])
+    d = p.clone()
+    d[torch.arange(len(t)), at] -= ok.double()
+    slope = 1 - (z / cap)**2 if cap else torch.ones_like(z)
+    dz = g * d * slope
+    off = g.abs() * (p * (E + 2.0**-24 * (2 * (z - lse[:, None]).abs() + 4)) + 2.0**-23 * d.abs() + (2.0**-19 * d.abs() if cap else 0))
+    off = off + h * (dz.abs() + off) + (2.0**-40 * g.abs().max() if dt == torch.float16 else 1e-38)
+    for name, a, b, n in (("d_x", (dz, off), w, w.shape[0]), ("d_weight", (dz.t().contiguous(), off.t().contiguous()), x, x.shape[0])):
+        if name not in out:
+            continue
+        want = a[0] @ b
+        tol = a[1] @ b.abs() + (n + 40) * 2.0**-23 * (a[0].abs() @ b.abs())
+        if name == "d_weight" and old is not None:
+            want = want + old.double()
+            tol = tol + 2.0**-24 * (want.abs() + old.double().abs())
+        tol = tol + torch.finfo(out[name].dtype).eps / 2 * (want.abs() + tol) + (2.0**-24 if out[name].dtype == torch.float16 else 1e-37)
+        worst((out[name].double() - want).abs() / tol, name)
+
+
+def one(hs, seed, M, K, V, dtype="bfloat16", cap=0.0, kind="whole", pad=0, offset=0, out_f32=True, grads=True, **kw):
+    import torch
+    x, w, t, grad = inputs(seed, M, K, V, dtype, kind, pad, offset, **kw)
+    out = hs.cross_entropy(x, w, t, softcap=cap)
+    torch.cuda.synchronize()
+    check_forward(out, x, w, t, cap, kind)
+    if not grads:
+        return
+    odt = torch.float32 if out_f32 else x.dtype
+    dx, dw = (torch.full((n, K + 3), 77.0, dtype=odt, device="cuda") for n in (M, V))
+    got = hs.cross_entropy_grad(x, w, t, out["lse"], grad, softcap=cap, outputs={"d_x": dx[:, :K], "d_weight": dw[:, :K]})
+    torch.cuda.synchronize()
+    assert torch.all(dx[:, K:] == 77.0) and torch.all(dw[:, K:] == 77.0)
+    check_grads({**got, "kind": dtype}, x, w, t, out["lse"], grad, cap, kind)
+
+
+SIZES = [
+    (1, 1, 1), (1, 8, 2), (1, 64, 1000), (2, 33, 17), (3, 512, 151), (16, 128, 3001), (17, 40, 513), (32, 72, 2000), (33, 96, 700), (50, 256, 1111),
+    (64, 64, 4097), (65, 100, 300), (130, 264, 1500), (200, 128, 6000), (257, 65, 2500), (300, 320, 999), (513, 72, 5000),
+]
+
+
+@pytest.mark.parametrize("dtype,cap", [("bfloat16", 0.0), ("float16", 0.0), ("bfloat16", 5.0), ("float16", 20.0)])
+@pytest.mark.parametrize("M,K,V", SIZES)
+def test_sizes(hs, M, K, V, dtype, cap):
+    one(hs, M + K + V, M, K, V, dtype, cap, out_f32=(M + V) % 2 == 0)
+
+
+@pytest.mark.parametrize("M,K,V", [(1, 4096, 5000), (40, 1000, 3000), (300, 2048, 4000)])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_normal_values(hs, M, K, V, dtype):
+    one(hs, M, M, K, V, dtype, 30.0 if M == 40 else 0.0, kind="normal", out_f32=False)
+
+
+@pytest.mark.parametrize("M,K,V", [(1, 64, 500), (20, 130, 600), (70, 513, 257), (300, 72, 1000)])
+@pytest.mark.parametrize("pad,offset", [(1, 0), (0, 1), (3, 5), (8, 0), (8, 8), (4, 4)])
+def test_strides_and_alignment(hs, M, K, V, pad, offset):
+    one(hs, M + K, M, K, V, "bfloat16", 0.0, pad=pad, offset=offset)
+
+
+@pytest.mark.parametrize("M,K,V", [(5, 64, 151936), (300, 32, 100_003), (2049, 16, 70_000)])
+def test_pieces_of_the_vocabulary(hs, M, K, V):
+    """Vocabularies of many tiles; several pieces with many rows."""
+    one(hs, M, M, K, V, "bfloat16", 0.0)
+    if M == 2049:
+        one(hs, M + 1, M, K, V, "float16", 0.0, out_f32=False)
+
+
+def test_many_rows(hs):
+    one(hs, 3, 9000, 72, 17_000, "bfloat16", 0.0)
+
+
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_sure_and_hopeless_tokens(hs, M):
+    """Losses near 0 keep their value; targets far below the rest too."""
+    import torch
+    x, w, t, _ = inputs(7, M, 64, 900, ignored=0.0, sure=0.0)
+    x.zero_()
+    x[:, 0], x[:, 1] = 1.0, 0.0
+    w.zero_()
+    w[:, 0] = -torch.arange(900, device="cuda") % 16
+    w[0, 0] = 14.0
+    t.zero_()
+    out = hs.cross_entropy(x, w, t)
+    torch.cuda.synchronize()
+    z = (x.double() @ w.double().t().contiguous())
+    want = torch.log1p(torch.exp(z[:, 1:] - z[:, :1]).sum(1))
+    # float sums of 1 + 4e-5 or so: half a step of 1, 2^-24, at every addition to it
+    assert torch.all((out["loss"].double() - want).abs() <= 64 * 2.0**-24 + 2.0**-20 * want)
+    t.fill_(1)
+    out = hs.cross_entropy(x, w, t)
+    torch.cuda.synchronize()
+    check_forward(out, x, w, t, 0.0, "whole")
+
+
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_infinite_and_nan_logits_stay_in_their_row(hs, M):
+    import torch
+    x, w, t, grad = inputs(8, M, 64, 700, ignored=0.0)
+    w[:, 5] = 0.0
+    w[3, 5] = 1.0
+    want = hs.cross_entropy(x, w, t)
+    wg = hs.cross_entropy_grad(x, w, t, want["lse"], grad)
+    x2, t2 = x.clone(), t.clone()
+    x2[M // 2, 6] = float("nan")
+    got = hs.cross_entropy(x2, w, t2)
+    gg = hs.cross_entropy_grad(x2, w, t2, got["lse"], grad)
+    torch.cuda.synchronize()
+    other = torch.arange(M, device="cuda") != M // 2
+    for a, b in ((got["loss"], want["loss"]), (got["lse"], want["lse"]), (gg["d_x"], wg["d_x"])):
+        assert torch.all(torch.isnan(a[M // 2])) and torch.equal(a[other], b[other])
+    # the same row ignored: its gradient is 0 and it reaches nobody
+    t2[M // 2] = -1
+    gg = hs.cross_entropy_grad(x2, w, t2, got["lse"], grad)
+    torch.cuda.synchronize()
+    assert not gg["d_x"][M // 2].any() and torch.equal(gg["d_x"][other], wg["d_x"][other])
+    # logits of -inf have probability 0, of +inf make the row NaN
+    x3, w3 = x.clone(), w.clone()
+    x3[:, 5], w3[:, 5] = 1.0, 0.0
+    w3[3, 5] = float("-inf")
+    t3 = torch.full_like(t, 4)
+    out = hs.cross_entropy(x3, w3, t3)
+    w4, t4 = w3.clone(), torch.full_like(t, 3)
+    keep = [v for v in range(700) if v != 3]
+    w4[3] = w4[4]                                                      # (never looked at below)
+    z = (x3.double() @ w4.double().t().contiguous())[:, keep]
+    torch.cuda.synchronize()
+    assert torch.all((out["lse"].double() - torch.logsumexp(z, 1)).abs() < 1e-4)
+    assert torch.all(torch.isinf(hs.cross_entropy(x3, w3, t4)["loss"]))
+    w3[3, 5] = float("inf")
+    out = hs.cross_entropy(x3, w3, t3)
+    torch.cuda.synchronize()
+    assert torch.all(torch.isnan(out["loss"])) and torch.all(torch.isnan(out["lse"]))
+
+
+def test_all_rows_ignored(hs):
+    import torch
+    for dtype in ("bfloat16", "float16"):
+        x, w, t, grad = inputs(9, 70, 72, 500, dtype)
+        t.fill_(-1)
+        grad.fill_(float("nan"))
+        out = hs.cross_entropy(x, w, t)
+        got = hs.cross_entropy_grad(x, w, t, out["lse"], grad)
+        torch.cuda.synchronize()
+        assert not out["loss"].any() and torch.isfinite(out["lse"]).all() and not got["d_x"].any() and not got["d_weight"].any()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("scale", [1e-6, 1.0, 65536.0])
+def test_scaled_gradients(hs, dtype, scale):
+    """Gradients of any size, rows of very different ones; results in float."""
+    import torch
+    x, w, t, grad = inputs(10, 150, 72, 800, dtype)
+    grad = grad * scale
+    grad[::3] *= 1e-3
+    lse = hs.cross_entropy(x, w, t)["lse"]
+    dx, dw = torch.empty((150, 72), device="cuda"), torch.empty((800, 72), device="cuda")
+    got = hs.cross_entropy_grad(x, w, t, lse, grad, outputs={"d_x": dx, "d_weight": dw})
+    torch.cuda.synchronize()
+    check_grads({**got, "kind": dtype}, x, w, t, lse, grad, 0.0, "whole")
+
+
+@pytest.mark.parametrize("dtype,out", [("bfloat16", "bfloat16"), ("bfloat16", "float32"), ("float16", "float16"), ("float16", "float32")])
+def test_one_gradient_alone_and_accumulated(hs, dtype, out):
+    import torch
+    x, w, t, grad = inputs(11, 90, 104, 1300, dtype)
+    lse = hs.cross_entropy(x, w, t)["lse"]
+    both = hs.cross_entropy_grad(x, w, t, lse, grad)
+    assert torch.equal(hs.cross_entropy_grad(x, w, t, lse, grad, need_weight=False)["d_x"], both["d_x"])
+    alone = hs.cross_entropy_grad(x, w, t, lse, grad, need_x=False)
+    assert set(alone) == {"d_weight"} and torch.equal(alone["d_weight"], both["d_weight"])
+    old = torch.randn((1300, 104), device="cuda").to(getattr(torch, out))
+    got = hs.cross_entropy_grad(x, w, t, lse, grad, accumulate=True, outputs={"d_weight": old.clone()})
+    torch.cuda.synchronize()
+    check_grads({"d_weight": got["d_weight"], "kind": dtype}, x, w, t, lse, grad, 0.0, "whole", old)
+
+
+def test_gradient_by_differences(hs):
+    """Central differences of the kernel's own losses, h = 1/16. The third derivative of a
+    row's loss along an entry of x is the third cumulant of that column of W, at most
+    0.1 range^3 <= 0.1 (range: 0.75), along an entry of W at most 0.1 |x|^3: so off by
+    h^2 / 6 of these; the losses' own error 3e-5 / h; the gradients' bfloat16 steps."""
+    import torch
+    M, K, V, h = 40, 32, 300, 1 / 16
+    x, w, t, grad = inputs(12, M, K, V, sure=0.3)
+    base = hs.cross_entropy(x, w, t)
+    dx, dw = torch.empty((M, K), device="cuda"), torch.empty((V, K), device="cuda")
+    hs.cross_entropy_grad(x, w, t, base["lse"], grad, outputs={"d_x": dx, "d_weight": dw})
+
+    def loss(x, w):
+        return hs.cross_entropy(x, w, t)["loss"].double() * grad.double()
+
+    def moved(a, at, by):
+        a = a.clone()
+        a[at] += by
+        assert a[at].float().mean() != 0 or by != 0
+        return a
+
+    h2 = 2.0**-7 * dx.abs().max().item()
+    for k in (0, 7, 31):
+        at = (slice(None), k)
+        x64 = x.double()
+        up, down = moved(x, at, h), moved(x, at, -h)
+        step = (up.double() - down.double())[:, k]
+        diff = (loss(up, w) - loss(down, w)) / step
+        exact_step = (up.double()[:, k] - x64[:, k] == h) & (x64[:, k] - down.double()[:, k] == h)
+        worst(((diff - dx[:, k].double()).abs() / (grad.double().abs() * (h * h / 60 + 1e-3) + h2))[exact_step], "d_x")
+        assert exact_step.sum() > 20
+    scale = x.double().abs().max().item()
+    h3 = 2.0**-7 * (grad.double().abs() @ x.double().abs()).max().item()
+    picked = int(t[(t >= 0) & (t < V)][5])
+    for v, k in ((picked, 3), (17, 9), (299, 31)):
+        diff = (loss(x, moved(w, (v, k), h)).sum() - loss(x, moved(w, (v, k), -h)).sum()) / (2 * h)
+        assert (diff - dw[v, k].double()).abs() <= M * 1.5 * (h * h / 60 * scale**3 + 1e-3) + h3
+
+
+@pytest.mark.parametrize("M,dtype", [(1, "bfloat16"), (70, "float16"), (600, "bfloat16")])
+def test_the_same_every_time_captured_or_not(hs, M, dtype):
+    import torch
+    K, V = 136, 3000
+    x, w, t, grad = state = inputs(13, M, K, V, dtype)
+    L = hs.lib()
+    work = torch.empty(L.ultima_hsamp_cross_entropy_work_bytes(M, V), dtype=torch.uint8, device="cuda")
+    gwork = torch.empty(L.ultima_hsamp_cross_entropy_grad_work_bytes(M, K, V), dtype=torch.uint8, device="cuda")
+    out = hs.cross_entropy(x, w, t, work=work)
+    got = hs.cross_entropy_grad(x, w, t, out["lse"], grad, work=gwork)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        hs.cross_entropy(x, w, t, work=work, outputs=out)
+        hs.cross_entropy_grad(x, w, t, out["lse"], grad, work=gwork, outputs=got)
+    s = torch.cuda.Stream()
+    for seed in range(20, 24):
+        for a, b in zip(state, inputs(seed, M, K, V, dtype)):
+            a.copy_(b)
+        work.fill_(255)
+        gwork.fill_(255)
+        want = hs.cross_entropy(x, w, t)
+        wg = hs.cross_entropy_grad(x, w, t, want["lse"], grad)
+        torch.cuda.synchronize()
+        other = hs.cross_entropy(x, w, t, stream=s)
+        og = hs.cross_entropy_grad(x, w, t, other["lse"], grad, stream=s)
+        for a in (*out.values(), *got.values()):
+            a.fill_(1)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b, c in zip((*out.values(), *got.values()), (*want.values(), *wg.values()), (*other.values(), *og.values())):
+            assert torch.equal(a, b) and torch.equal(c, b)
+
+
+def test_past_32_bit_offsets(hs):
+    """A weight of more than 2^32 bytes; what is past them counts, and gets its gradient."""
+    import torch
+    K, V = 16384, 140_000
+    w = torch.zeros((V, K), dtype=torch.bfloat16, device="cuda")
+    w[-64:] = torch.randn((64, K), device="cuda").to(torch.bfloat16) * (2 * K**-0.5)
+    for M in (1, 300):
+        x = torch.randn((M, K), device="cuda").to(torch.bfloat16)
+        t = torch.full((M,), V - 3, dtype=torch.int32, device="cuda")
+        out = hs.cross_entropy(x, w, t)
+        grad = torch.ones(M, device="cuda")
+        got = hs.cross_entropy_grad(x, w, t, out["lse"], grad)
+        torch.cuda.synchronize()
+        z = torch.cat([x.double() @ w[-64:].double().t().contiguous(), torch.zeros((M, 1), device="cuda", dtype=torch.float64)], 1)
+        count = torch.zeros(65, dtype=torch.float64, device="cuda")
+        count[64] = np.log(V - 64)
+        lse = torch.logsumexp(z + count, 1)
+        bound = K * 2.0**-23 * (x.double().abs() @ w[-64:].double().abs().t().contiguous()).amax(1) + 1e-4
+        assert torch.all((out["lse"].double() - lse).abs() <= bound) and torch.all((out["loss"].double() - (lse - z[:, 61])).abs() <= 2 * bound)
+        d = torch.exp(z[:, :64] - lse[:, None])
+        d[:, 61] -= 1
+        off = d.abs() * 2.0**-8 + (d.abs() + 1) * bound[:, None]
+        for a, want, tol in ((got["d_x"], d @ w[-64:].double(), off @ w[-64:].double().abs()),
+                             (got["d_weight"][-64:], d.t().contiguous() @ x.double(), off.t().contiguous() @ x.double().abs())):
+            worst((a.double() - want).abs() / (tol + 2.0**-8 * want.abs() + 1e-6), "past 32 bits")

@@ -70,6 +70,9 @@ def build_all() -> None:
         "hsamp_callers.o": CSRC / "hsamp_callers.hip",
         "hsamp_verify.o": CSRC / "hsamp_verify.hip",
         "hsamp_linear.o": CSRC / "hsamp_linear.hip",
+        "hsamp_linear_i8.o": CSRC / "hsamp_linear_i8.hip",
+        "hsamp_loss.o": CSRC / "hsamp_loss.hip",
+        "hsamp_embed.o": CSRC / "hsamp_embed.hip",
     }
     with ThreadPoolExecutor(max_workers=4) as ex:
         futs = [ex.submit(_run, [HIPCC, *HIP_FLAGS, "-x", "hip", "-c", str(src), "-o", str(BUILD / o)])

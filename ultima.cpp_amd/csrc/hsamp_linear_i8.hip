@@ -1,0 +1,170 @@
+// The product in 8-bit integers (ultima_hsamp_linear_i8): out = act(s_m s_n sum(x w) +
+// bias) + residual, and the rows laid out for it (ultima_hsamp_quantize_rows).
+//
+// v_mfma_i32_16x16x64 takes 64 bytes a row in the cycles that the 16-bit form takes 32
+// elements: the tiles, loads and forms are those of the 16-bit product, byte for byte.
+// Sums are exact (in_dim up to 131071: 131071 x 128^2 < 2^31) and rounded once, to
+// float, before the two scales.
+#include "hsamp_product.h"
+
+namespace hsamp {
+namespace {
+
+template <bool BF>
+struct LinearI8 {
+    static constexpr bool kByRows = false;
+    using Args = ultima_hsamp_linear_i8_args;
+    using Element = int8_t;
+    using Sum = i32x4;
+    struct Columns {
+        u32x4 bias;
+        float scale[8];
+    };
+    struct Row {
+        u32x4 residual;
+        float scale;
+    };
+    static __device__ __forceinline__ Sum mfma(u32x4 w, u32x4 x, Sum c) {
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, x), c, 0, 0, 0);
+    }
+    template <int E>
+    static __device__ __forceinline__ Columns columns(const Args& a, int g, int n) {
+        Columns c = {};
+        const float* s = a.weight_scale + g * a.weight_scale_group + n;
+        const int left = a.out_dim - n;
+        if (E == 8) c.bias = bias8(a, g, n);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (e < left) c.scale[e] = s[e];
+        return c;
+    }
+    template <int E>
+    static __device__ __forceinline__ Row row(const Args& a, int g, int m, int n) {
+        return {E == 8 ? residual8(a, g, m, n) : u32x4{}, m < a.rows ? a.x_scale[g * a.x_scale_group + m] : 0.0f};
+    }
+    template <int E>
+    static __device__ __forceinline__ void finish(const Args& a, int g, int m, int n, const int32_t (&sum)[E], const Columns& c, const Row& r) {
+        float y[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = (float)sum[e] * r.scale * c.scale[e];
+        hsamp::finish<BF, E>(a, g, m, n, y, c.bias, r.residual);
+    }
+    template <int TN, int TM, int WM, int WN>
+    static __device__ __forceinline__ void tiles(const Args& a, int g, int m0, int n0, int wave, const Sum (&acc)[TN][TM], int32_t* lds) {
+        store_tiles<LinearI8, TN, TM>(a, g, m0 + wave % WM * 16 * TM, n0 + wave / WM % WN * 16 * TN, acc,
+                                      lds + wave * 16 * (16 * TN + 4));
+    }
+};
+
+// A row's largest magnitude, then its values in steps of a 127th of it. Bound by the
+// row's read and write; a block keeps up to 8192 values in registers between the two.
+// Magnitudes are compared as whole numbers (infinities and NaN above all others).
+template <class T>
+__global__ __launch_bounds__(256) void k_quantize_rows(ultima_hsamp_quantize_args a) {
+    constexpr int KEEP = 4;                       // pieces of eight values a thread keeps
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    __shared__ uint32_t tops[4];
+    const int tid = threadIdx.x, K = a.in_dim;
+    const int64_t m = blockIdx.x;
+    const T* x = static_cast<const T*>(a.x) + m * a.x_stride;
+    int8_t* q = a.q + m * a.q_stride;
+    const bool wide = reinterpret_cast<uintptr_t>(x) % (8 * sizeof(T)) == 0;
+    const bool wide_q = reinterpret_cast<uintptr_t>(q) % 8 == 0;
+    auto get = [&](int k, float (&v)[8]) {
+        if (wide && k + 8 <= K) {
+            typedef T T8 __attribute__((ext_vector_type(8)));
+            const T8 t = *reinterpret_cast<const T8*>(x + k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (float)t[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = k + e < K ? (float)x[k + e] : 0.0f;
+        }
+    };
+    uint32_t top = 0;
+    float kept[KEEP][8];
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) {
+        get((j * 256 + tid) * 8, kept[j]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(kept[j][e]) & 0x7FFFFFFFu);
+    }
+    for (int k = (KEEP * 256 + tid) * 8; k < K; k += 2048) {
+        float v[8];
+        get(k, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+    if (tid % 64 == 0) tops[tid / 64] = top;
+    __syncthreads();
+    top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+    const bool finite = top < 0x7F800000u;
+    const float amax = __uint_as_float(top);
+    if (tid == 0) a.scale[m] = finite ? amax / 127.0f : __uint_as_float(0x7FC00000u);
+    // (rows so small that their step's reciprocal passes the largest float: both sides larger)
+    const float up = amax < 0x1p-100f ? 0x1p80f : 1.0f;
+    const float r = finite && top != 0 ? 127.0f / (amax * up) : 0.0f;
+    auto put = [&](int k, const float (&v)[8]) {
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float t = finite ? v[e] * up * r : 0.0f;      // off by less than 2^-15
+            float n = __builtin_rintf(t);
+            // beside a half the exact quotient decides (in double its halves are exact, and
+            // other quotients of two floats are farther than a rounding from them)
+            if (fabsf(fabsf(t - n) - 0.5f) < 0x1p-14f) n = (float)__builtin_rint((double)v[e] * 127.0 / (double)amax);
+            w[e / 4] |= ((uint32_t)(int)n & 255u) << (8 * (e & 3));
+        }
+        if (wide_q && k + 8 <= K) {
+            *reinterpret_cast<u32x2*>(q + k) = u32x2{w[0], w[1]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (k + e < K) q[k + e] = (int8_t)(w[e / 4] >> (8 * (e & 3)));
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j)
+        if ((j * 256 + tid) * 8 < K) put((j * 256 + tid) * 8, kept[j]);
+    for (int k = (KEEP * 256 + tid) * 8; k < K; k += 2048) {
+        float v[8];
+        get(k, v);
+        put(k, v);
+    }
+}
+
+}  // namespace
+}  // namespace hsamp
+
+extern "C" int ultima_hsamp_linear_i8(const ultima_hsamp_linear_i8_args* a, void* hip_stream) {
+    using namespace hsamp;
+    if (a == nullptr || a->x_scale == nullptr || a->weight_scale == nullptr) return ULTIMA_HSAMP_ERR_INVALID;
+    if ((reinterpret_cast<uintptr_t>(a->x_scale) | reinterpret_cast<uintptr_t>(a->weight_scale)) % 4 != 0) return ULTIMA_HSAMP_ERR_INVALID;
+    if (a->out == a->x_scale || a->out == a->weight_scale) return ULTIMA_HSAMP_ERR_INVALID;
+    const int status = check_product(*a, 1);
+    if (status != ULTIMA_HSAMP_OK) return status;
+    if (a->in_dim > ULTIMA_HSAMP_MAX_I8_DIM) return ULTIMA_HSAMP_ERR_UNSUPPORTED;
+    hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    const hipError_t e = a->dtype == ULTIMA_HSAMP_BF16 ? launch_product<LinearI8<true>>(*a, s) : launch_product<LinearI8<false>>(*a, s);
+    return e == hipSuccess ? ULTIMA_HSAMP_OK : ULTIMA_HSAMP_ERR_HIP;
+}
+
+extern "C" int ultima_hsamp_quantize_rows(const ultima_hsamp_quantize_args* a, void* hip_stream) {
+    using namespace hsamp;
+    if (a == nullptr || a->x == nullptr || a->q == nullptr || a->scale == nullptr) return ULTIMA_HSAMP_ERR_INVALID;
+    if (a->dtype != ULTIMA_HSAMP_BF16 && a->dtype != ULTIMA_HSAMP_F16 && a->dtype != ULTIMA_HSAMP_F32) return ULTIMA_HSAMP_ERR_INVALID;
+    if (a->rows < 1 || a->in_dim < 1 || a->x_stride < a->in_dim || a->q_stride < a->in_dim) return ULTIMA_HSAMP_ERR_INVALID;
+    if (reinterpret_cast<uintptr_t>(a->x) % (a->dtype == ULTIMA_HSAMP_F32 ? 4 : 2) != 0 || reinterpret_cast<uintptr_t>(a->scale) % 4 != 0)
+        return ULTIMA_HSAMP_ERR_INVALID;
+    if (static_cast<const void*>(a->q) == a->x || static_cast<const void*>(a->scale) == a->x) return ULTIMA_HSAMP_ERR_INVALID;
+    // a launch counts its threads in 32 bits; columns in steps past the end
+    if (a->rows > (1 << 24) - 1 || a->in_dim > 1 << 30) return ULTIMA_HSAMP_ERR_UNSUPPORTED;
+    hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    const dim3 grid(a->rows), block(256);
+    if (a->dtype == ULTIMA_HSAMP_F32) hipLaunchKernelGGL(k_quantize_rows<float>, grid, block, 0, s, *a);
+    else if (a->dtype == ULTIMA_HSAMP_F16) hipLaunchKernelGGL(k_quantize_rows<_Float16>, grid, block, 0, s, *a);
+    else hipLaunchKernelGGL(k_quantize_rows<__bf16>, grid, block, 0, s, *a);
+    return hipGetLastError() == hipSuccess ? ULTIMA_HSAMP_OK : ULTIMA_HSAMP_ERR_HIP;
+}

@@ -1,0 +1,654 @@
+// Cross entropy over the vocabulary without its logits (ultima_hsamp_cross_entropy) and
+// its gradients (ultima_hsamp_cross_entropy_grad).
+//
+// Forward: the tiles of x W^T leave one maximum and one sum of exponentials per row
+// and tile of the vocabulary, and the target's logit; a second launch joins them.
+// Gradients, a piece of the vocabulary at a time: the logits again, whose tiles store
+// dz = grad (exp(z - lse) - [v = t]) in 16 bits (the piece stays in the caches),
+// then d_x += dz W and d_weight = dz^T x.
+#include "hsamp_product.h"
+
+namespace hsamp {
+namespace {
+
+constexpr float kLog2e = 1.44269504f;
+
+// exp(t) by the hardware's exp2: off by the rounding of t log2 e, 1.5 |t| 2^-24, and a
+// step or two of 2^-24.
+__device__ __forceinline__ float exp_of(float t) { return __builtin_amdgcn_exp2f(t * kLog2e); }
+
+// What all of the kernels here know of a call. x, weight and out_dim: of a piece.
+struct LossArgs {
+    int32_t rows, in_dim, out_dim, groups;
+    const void* x;
+    int64_t x_stride, x_group;
+    const void* weight;
+    int64_t weight_stride, weight_group;
+    const int32_t* target;
+    int32_t first, vocab;           // the piece's first id; ids there are
+    float cap, cap_scale, cap_inv;  // cap 0: none
+    // forward
+    float2* partial;                // [tiles of the vocabulary][rows] maximum, sum
+    float* at_target;               // [rows]
+    // gradients
+    const float* lse;
+    const float* grad;
+    const float* top_grad;          // half precision: max |grad|
+    uint16_t* dz;                   // [rows, dz_stride]
+    int64_t dz_stride;
+};
+
+__device__ __forceinline__ float capped(const LossArgs& a, float y) {
+    return a.cap > 0.0f ? cap_of(y, y * a.cap_scale * a.cap_inv, a.cap) : y;
+}
+
+// The maximum and the sum of exponentials relative to it, of two.
+__device__ __forceinline__ void join(float& top, float& sum, float top2, float sum2) {
+    const float t = fmaxf(top, top2), ref = t == -__builtin_inff() ? 0.0f : t;
+    sum = sum * exp_of(top - ref) + sum2 * exp_of(top2 - ref);
+    top = t;
+}
+
+template <bool BF>
+struct LossRows {
+    static constexpr bool kByRows = true;
+    using Args = LossArgs;
+    using Element = uint16_t;
+    using Sum = f32x4;
+    static __device__ __forceinline__ Sum mfma(u32x4 w, u32x4 x, Sum c) { return hsamp::mfma<BF>(w, x, c); }
+
+    // Eight lanes to a row of a small tile.
+    template <int BM, int BN, class Get>
+    static __device__ __forceinline__ void rows(const Args& a, int m0, int n0, Get get) {
+        const int row = threadIdx.x >> 3, l = threadIdx.x & 7, m = m0 + row;
+        if (row >= BM || m >= a.rows) return;
+        const int t = a.target[m] - n0;
+        float z[BN / 8], top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < BN / 8; ++k) {
+            const int n = l + 8 * k;
+            z[k] = n0 + n < a.out_dim ? capped(a, get(row, n)) : -__builtin_inff();
+            if (n == t && n0 + n < a.out_dim) a.at_target[m] = z[k];
+            top = fmaxf(top, z[k]);
+        }
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        const float ref = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+        for (int k = 0; k < BN / 8; ++k) sum += exp_of(z[k] - ref);
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) sum += __shfl_xor(sum, d);
+        if (l == 0) a.partial[(int64_t)(n0 / BN) * a.rows + m] = float2{top, sum};
+    }
+
+    // A wave's 16 TM rows: a lane's sums are 4 TN columns of TM of them.
+    template <int TN, int TM, int WM, int WN>
+    static __device__ __forceinline__ void tiles(const Args& a, int, int m0, int n0, int wave, const Sum (&acc)[TN][TM], float* lds) {
+        constexpr int BM = 16 * WM * TM, BN = 16 * WN * TN;
+        const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+        const int wm = wave % WM * 16 * TM, wn = wave / WM, n = n0 + wn * 16 * TN + 4 * q;
+        float2* parts = reinterpret_cast<float2*>(lds);       // [WN][BM]
+#pragma unroll
+        for (int u = 0; u < TM; ++u) {
+            const int row = wm + 16 * u + i, m = m0 + row;
+            float z[4 * TN], top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+            for (int s = 0; s < TN; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float y = capped(a, acc[s][u][e]);
+                    z[4 * s + e] = n + 16 * s + e < a.out_dim ? y : -__builtin_inff();
+                    top = fmaxf(top, z[4 * s + e]);
+                }
+            const int t = m < a.rows ? a.target[m] - n : -1;
+            if (t >= 0 && t < 16 * TN && (t & 12) == 0 && n + t < a.out_dim) {
+#pragma unroll
+                for (int s = 0; s < TN; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (t == 16 * s + e) a.at_target[m] = z[4 * s + e];
+            }
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float ref = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+            for (int k = 0; k < 4 * TN; ++k) sum += exp_of(z[k] - ref);
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (q == 0) parts[wn * BM + row] = float2{top, sum};
+        }
+        __syncthreads();
+        for (int row = threadIdx.x; row < BM; row += 64 * WM * WN) {
+            if (m0 + row >= a.rows) continue;
+            float2 p = parts[row];
+#pragma unroll
+            for (int k = 1; k < WN; ++k) join(p.x, p.y, parts[k * BM + row].x, parts[k * BM + row].y);
+            a.partial[(int64_t)(n0 / BN) * a.rows + m0 + row] = p;
+        }
+    }
+};
+
+// 2^log_rows rows a block of 1024 threads, the rest of them over the tiles.
+__global__ __launch_bounds__(1024) void k_loss_join(const float2* partial, const float* at_target, const int32_t* target, int rows,
+                                                    int vocab, int tiles, int log_rows, float* loss, float* lse) {
+    __shared__ float2 sm[1024];
+    const int r = threadIdx.x & ((1 << log_rows) - 1), m = (blockIdx.x << log_rows) + r;
+    float top = -__builtin_inff(), sum = 0.0f;
+    if (m < rows)
+        for (int t = threadIdx.x >> log_rows; t < tiles; t += 1024 >> log_rows) {
+            const float2 p = partial[(int64_t)t * rows + m];
+            join(top, sum, p.x, p.y);
+        }
+    sm[threadIdx.x] = float2{top, sum};
+    __syncthreads();
+    for (int d = 512; d >= 1 << log_rows; d >>= 1) {
+        if ((int)threadIdx.x < d) {
+            const float2 p = sm[threadIdx.x + d];
+            join(top, sum, p.x, p.y);
+            sm[threadIdx.x] = float2{top, sum};
+        }
+        __syncthreads();
+    }
+    if ((int)threadIdx.x >= 1 << log_rows || m >= rows) return;
+    // (in double, and the target's logit before the logarithm: a sure token's loss is the logarithm alone)
+    const double rest = log((double)sum);
+    const int t = target[m];
+    lse[m] = (float)((double)top + rest);
+    loss[m] = t >= 0 && t < vocab ? (float)(((double)top - (double)at_target[m]) + rest) : 0.0f;
+}
+
+// ---- Gradients ---------------------------------------------------------------------
+
+// dz of a piece. Half precision holds 2^-24 of its largest values: rows' gradients are
+// taken relative to the largest one and everything times 2^15.
+template <bool BF>
+struct LossGrad {
+    static constexpr bool kByRows = false;
+    using Args = LossArgs;
+    using Element = uint16_t;
+    using Sum = f32x4;
+    struct Columns {};
+    struct Row {
+        float lse, grad;
+        int target;         // within the piece
+        bool used;
+    };
+    static __device__ __forceinline__ Sum mfma(u32x4 w, u32x4 x, Sum c) { return hsamp::mfma<BF>(w, x, c); }
+    template <int E>
+    static __device__ __forceinline__ Columns columns(const Args&, int, int) { return {}; }
+    template <int E>
+    static __device__ __forceinline__ Row row(const Args& a, int, int m, int) {
+        if (m >= a.rows) return {0.0f, 0.0f, -1, false};
+        const int t = a.target[m];
+        float g = a.grad[m];
+        if (!BF) {
+            const float top = *a.top_grad;
+            g = top > 0.0f ? g / top * 0x1p15f : g;
+        }
+        return {a.lse[m], g, t - a.first, t >= 0 && t < a.vocab};
+    }
+    template <int E>
+    static __device__ __forceinline__ void finish(const Args& a, int, int m, int n, float (&y)[E], Columns, Row r) {
+        if (m >= a.rows) return;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float z = capped(a, y[e]);
+            float d = exp_of(z - r.lse);
+            if (n + e == r.target) d -= 1.0f;
+            if (a.cap > 0.0f) {
+                const float t = z * a.cap_scale * a.cap_inv;
+                d *= (1.0f - t) * (1.0f + t);
+            }
+            // (columns past the piece, up to the tile's end, are read with it)
+            y[e] = r.used && n + e < a.out_dim ? d * r.grad : 0.0f;
+        }
+        uint16_t* p = a.dz + m * a.dz_stride + n;
+        if (E == 8) {
+            u32x4 v = {};
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) v[e] = (uint32_t)from_f32<BF>(y[2 * e]) | (uint32_t)from_f32<BF>(y[(2 * e + 1) % E]) << 16;
+            *reinterpret_cast<u32x4*>(p) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) p[e] = from_f32<BF>(y[e]);
+        }
+    }
+    template <int TN, int TM, int WM, int WN>
+    static __device__ __forceinline__ void tiles(const Args& a, int g, int m0, int n0, int wave, const Sum (&acc)[TN][TM], float* lds) {
+        store_tiles<LossGrad, TN, TM>(a, g, m0 + wave % WM * 16 * TM, n0 + wave / WM % WN * 16 * TN, acc,
+                                      lds + wave * 16 * (16 * TN + 4));
+    }
+};
+
+// max |grad| of the rows that count, for half precision.
+__global__ __launch_bounds__(1024) void k_top_grad(const float* grad, const int32_t* target, int rows, int vocab, float* top) {
+    __shared__ float sm[16];
+    float t = 0.0f;
+    for (int m = threadIdx.x; m < rows; m += 1024)
+        if (target[m] >= 0 && target[m] < vocab) t = fmaxf(t, fabsf(grad[m]));
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) t = fmaxf(t, __shfl_xor(t, d));
+    if (threadIdx.x % 64 == 0) sm[threadIdx.x / 64] = t;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) t = fmaxf(t, sm[w]);
+        *top = t;
+    }
+}
+
+// Rows laid out for the products: eight columns a piece, the last one filled up with zeros.
+__global__ __launch_bounds__(256) void k_lay_out(const uint16_t* from, int64_t stride, int64_t rows, int columns, uint16_t* to, int pieces) {
+    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t r = k / pieces;
+    const int c = (int)(k % pieces) * 8;
+    if (r >= rows) return;
+    u32x4 v = {};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (c + e < columns) v[e / 2] |= (uint32_t)from[r * stride + c + e] << (16 * (e & 1));
+    *reinterpret_cast<u32x4*>(to + k * 8) = v;
+}
+
+// out[m, n] (+)= scale * sum_k A(m, k) B(k, n): B's rows are k; A's rows are m (A_T
+// false) or k (true). Rows and addresses of A and B in steps of 16 bytes.
+struct GradArgs {
+    int32_t rows, out_dim, k;       // M, N (a multiple of 8 in memory), K
+    int32_t k_split;                // of one block of z, a multiple of 64
+    const uint16_t* a;
+    int64_t a_stride;
+    int32_t a_columns;              // that may be read
+    const uint16_t* b;
+    int64_t b_stride;
+    int32_t b_columns;
+    void* out;
+    int64_t out_stride, out_split;
+    int32_t out_f32, add;
+    const float* top_grad;          // half precision, where the sums are to be in grad's scale again
+};
+
+template <bool BF>
+struct GradStore {
+    using Args = GradArgs;
+    using Row = u32x4;
+    template <int E>
+    static __device__ __forceinline__ float columns(const Args& a, int, int) {
+        if (BF || a.top_grad == nullptr) return 1.0f;
+        const float top = *a.top_grad;
+        return top > 0.0f ? top * 0x1p-15f : 1.0f;
+    }
+    template <int E>
+    static __device__ __forceinline__ Row row(const Args& a, int, int m, int n) {
+        if (!a.add || a.out_f32 || m >= a.rows || n + 8 > a.out_dim) return u32x4{};
+        return load16(static_cast<const uint16_t*>(a.out) + m * a.out_stride + n);
+    }
+    template <int E>
+    static __device__ __forceinline__ void finish(const Args& a, int z, int m, int n, float (&y)[E], float scale, Row old) {
+        typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
+        const int left = a.out_dim - n;
+        if (m >= a.rows || left <= 0) return;
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] *= scale;
+        const int64_t at = z * a.out_split + m * a.out_stride + n;
+        if (a.out_f32) {
+            float* p = static_cast<float*>(a.out) + at;
+            if (left >= E) {
+#pragma unroll
+                for (int e = 0; e < E; e += 4) {
+                    f32x4 v = {y[e], y[e + 1], y[e + 2], y[e + 3]};
+                    if (a.add) v += *reinterpret_cast<const f32x4_a4*>(p + e);
+                    *reinterpret_cast<f32x4_a4*>(p + e) = v;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (e < left) p[e] = a.add ? p[e] + y[e] : y[e];
+            }
+            return;
+        }
+        uint16_t* p = static_cast<uint16_t*>(a.out) + at;
+        if (left >= E) {
+            u32x4 v = {};
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) {
+                if (a.add) {
+                    y[2 * e] += to_f32<BF>((uint16_t)old[e]);
+                    y[2 * e + 1] += to_f32<BF>((uint16_t)(old[e] >> 16));
+                }
+                v[e] = (uint32_t)from_f32<BF>(y[2 * e]) | (uint32_t)from_f32<BF>(y[2 * e + 1]) << 16;
+            }
+            *reinterpret_cast<u32x4_a2*>(p) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e < left) p[e] = from_f32<BF>(a.add ? to_f32<BF>(p[e]) + y[e] : y[e]);
+        }
+    }
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Four rows of sixteen columns, read by sixteen lanes (lane i: row i / 4, columns
+// 4 (i % 4) ..) and turned: lane i gets column i's four values.
+__device__ __forceinline__ uint64_t read_turned(const uint16_t* p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    return __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)(const_cast<uint16_t*>(p))));
+#else
+    return 0;
+#endif
+}
+
+// 256 x 256 tiles by eight waves of 128 x 64, stages of 64 k, two in LDS. Operands whose
+// rows are k stand in LDS as they do in memory, [64][256], and are turned on the way to
+// the registers; the sixteen-column blocks of row k stand at block ^ (k % 4 + 4 (k / 8 % 2)),
+// so that the eight rows of 32 bytes that a read takes at a time lie in different banks.
+template <bool BF, bool A_T>
+__global__ __launch_bounds__(512) void k_grad_tile(GradArgs a, int tiles_m, int tiles_n) {
+#ifdef __HIP_DEVICE_COMPILE__
+    constexpr int WM = 2, TM = 8, TN = 4, BM = 256, BN = 256, BK = 64, SB = (BM + BN) * BK;
+    constexpr uint32_t kOutside = 0x80000000u;
+    typedef __attribute__((address_space(3))) void* lds_ptr;
+    __shared__ __attribute__((aligned(16))) uint16_t sm[2 * SB];
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int total = tiles_m * tiles_n, per = total / 8, more = total % 8;
+    const int xcd = blockIdx.x % 8, tile = xcd * per + min(xcd, more) + blockIdx.x / 8;
+    const int m0 = tile % tiles_m * BM, n0 = tile / tiles_m * BN;
+    const int k0 = blockIdx.z * a.k_split, K = min(a.k_split, a.k - k0);
+    const uint16_t* A = a.a + (A_T ? (int64_t)k0 * a.a_stride + m0 : (int64_t)m0 * a.a_stride + k0);
+    const uint16_t* B = a.b + (int64_t)k0 * a.b_stride + n0;
+    // loads: A (32 of 1 KB), then B; four of each for a wave
+    uint32_t va[4], vb[4];
+    int ka[4], kb[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int c = wave + 8 * j, k = 2 * c + (lane >> 5), turn = ((k & 3) | (k >> 1 & 4)) << 1;
+        const int col = ((lane & 31) ^ turn) * 8;
+        kb[j] = k;
+        vb[j] = n0 + col < a.b_columns ? (uint32_t)(k * (int)a.b_stride + col) * 2u : kOutside;
+        if (A_T) {
+            ka[j] = k;
+            va[j] = m0 + col < a.a_columns ? (uint32_t)(k * (int)a.a_stride + col) * 2u : kOutside;
+        } else {
+            const int r = c * 8 + (lane >> 3), p = ((lane & 7) ^ (r >> 1 & 7)) * 8;
+            ka[j] = p;
+            va[j] = m0 + r < a.rows ? (uint32_t)(r * (int)a.a_stride + p) * 2u : kOutside;
+        }
+    }
+    const int T = (K + BK - 1) / BK;
+    auto issue = [&](int t) {
+        const int left = K - t * BK;       // (below 0 past the last stage: zeros)
+        const int64_t s = t < T ? t : 0;
+        const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(A + s * (A_T ? BK * a.a_stride : BK)), 0, 0x7FFFFFFF, 0x00027000);
+        const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(B + s * BK * a.b_stride), 0, 0x7FFFFFFF, 0x00027000);
+        uint16_t* to = sm + (t & 1) * SB;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr)(to + (wave + 8 * j) * 512), 16, ka[j] < left ? va[j] : kOutside, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr)(to + BM * BK + (wave + 8 * j) * 512), 16, kb[j] < left ? vb[j] : kOutside, 0, 0, 0);
+    };
+    auto wait = [&](auto loads) {
+        constexpr int A = decltype(loads)::value;
+        __builtin_amdgcn_s_waitcnt((A & 15) | (A >> 4) << 14 | 7 << 4);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    struct Operands {
+        u32x4 b[TN], a[TM];
+    };
+    const int wm = wave % WM * 16 * TM, wn = wave / WM * 16 * TN;
+    const int turned = (8 * q + (i >> 2)) * 256 + (i & 3) * 4, turn = (i >> 2) | (q & 1) << 2;
+    auto turned_at = [&](const uint16_t* from, int block) {
+        const uint16_t* p = from + turned + ((block ^ turn) << 4);
+        const uint64_t lo = read_turned(p), hi = read_turned(p + 4 * 256);
+        return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+    };
+    auto read = [&](Operands& o, int t, int step) {
+        const uint16_t* fa = sm + (t & 1) * SB;
+        const uint16_t* fb = fa + BM * BK + step * 32 * 256;
+#pragma unroll
+        for (int s = 0; s < TN; ++s) o.b[s] = turned_at(fb, wn / 16 + s);
+#pragma unroll
+        for (int u = 0; u < TM; ++u) {
+            if (A_T) o.a[u] = turned_at(fa + step * 32 * 256, wm / 16 + u);
+            else o.a[u] = *reinterpret_cast<const u32x4*>(fa + (wm + 16 * u + i) * 64 + ((step * 4 + q) ^ (i >> 1)) * 8);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    f32x4 acc[TN][TM] = {};
+    auto multiply = [&](const Operands& o) {
+#pragma unroll
+        for (int s = 0; s < TN; ++s)
+#pragma unroll
+            for (int u = 0; u < TM; ++u) acc[s][u] = mfma<BF>(o.b[s], o.a[u], acc[s][u]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    using std::integral_constant;
+    Operands oa, ob;
+    issue(0);
+    issue(1);
+    wait(integral_constant<int, 8>());
+    read(oa, 0, 0);
+    for (int t = 0; t < T; ++t) {
+        read(ob, t, 1);
+        multiply(oa);
+        wait(integral_constant<int, 0>());       // (all of stage t is read, stage t + 1 is there)
+        issue(t + 2);
+        read(oa, t + 1, 0);
+        multiply(ob);
+    }
+    wait(integral_constant<int, 0>());
+    store_tiles<GradStore<BF>, TN, TM>(a, blockIdx.z, m0 + wm, n0 + wn, acc, reinterpret_cast<float*>(sm) + wave * 16 * (16 * TN + 4));
+#endif
+}
+
+// d_x from its float sums over the parts of the vocabulary.
+template <bool BF>
+__global__ __launch_bounds__(256) void k_grad_join(const float* parts, int n, int64_t part, int64_t stride, int rows, int columns,
+                                                   const float* top_grad, void* out, int64_t out_stride, int out_f32) {
+    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t m = k / stride;
+    const int c = (int)(k % stride);
+    if (m >= rows || c >= columns) return;
+    float sum = parts[k];
+    for (int p = 1; p < n; ++p) sum += parts[p * part + k];
+    if (!BF) {
+        const float top = *top_grad;
+        sum *= top > 0.0f ? top * 0x1p-15f : 1.0f;
+    }
+    if (out_f32) static_cast<float*>(out)[m * out_stride + c] = sum;
+    else static_cast<uint16_t*>(out)[m * out_stride + c] = from_f32<BF>(sum);
+}
+
+int64_t up(int64_t n, int64_t step) { return (n + step - 1) / step * step; }
+
+// How a gradient call cuts the vocabulary. A piece's dz and its part of the weight are
+// up to 128 and 256 MB (2^26, 2^27 elements), so that they stay in the caches; pieces are
+// as long as each other. d_x's tiles are made by as many parts of the piece as fill the
+// CUs, at least 512 ids each.
+struct Pieces {
+    int64_t width, columns;         // ids of a piece; in_dim in steps of eight
+    int count, splits, split;       // pieces; parts of a piece for d_x, ids of one
+};
+Pieces pieces_of(int64_t rows, int64_t in_dim, int64_t vocab) {
+    Pieces p;
+    p.columns = up(in_dim, 8);
+    const int64_t most = std::max<int64_t>(256, std::min({(int64_t)1 << 20, ((int64_t)1 << 26) / rows, ((int64_t)1 << 27) / p.columns}) / 256 * 256);
+    p.count = (int)((vocab + most - 1) / most);
+    p.width = up((vocab + p.count - 1) / p.count, 256);
+    p.count = (int)((vocab + p.width - 1) / p.width);
+    const int64_t tiles = ((rows + 255) / 256) * ((in_dim + 255) / 256);
+    const int64_t splits = std::max<int64_t>(1, std::min(256 / tiles, p.width / 512));
+    p.split = (int)up((p.width + splits - 1) / splits, 64);
+    p.splits = (int)((p.width + p.split - 1) / p.split);
+    return p;
+}
+struct GradWork {
+    int64_t dz, parts, x, weight, bytes;      // where they begin; 16 bytes for the largest gradient first
+};
+GradWork grad_work(const Pieces& p, int64_t rows) {
+    GradWork w;
+    w.dz = 256;
+    w.parts = up(w.dz + rows * p.width * 2, 256);
+    w.x = up(w.parts + p.splits * rows * p.columns * 4, 256);
+    w.weight = up(w.x + rows * p.columns * 2, 256);
+    w.bytes = up(w.weight + p.width * p.columns * 2, 256);
+    return w;
+}
+
+LossArgs loss_args(int rows, int in_dim, int vocab, const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                   const int32_t* target, float cap) {
+    LossArgs l = {};
+    l.rows = rows, l.in_dim = in_dim, l.out_dim = vocab, l.groups = 1;
+    l.x = x, l.x_stride = x_stride, l.weight = weight, l.weight_stride = weight_stride;
+    l.target = target, l.vocab = vocab, l.cap = cap;
+    // (both scaled where 1 / c would be subnormal or infinite)
+    l.cap_scale = cap < 0x1p-64f ? 0x1p64f : cap > 0x1p64f ? 0x1p-64f : 1.0f;
+    l.cap_inv = cap > 0.0f ? 1.0f / (cap * l.cap_scale) : 0.0f;
+    return l;
+}
+
+// What both calls ask of their sizes and operands.
+template <class Args>
+int check_loss(const Args& a) {
+    if (a.x == nullptr || a.weight == nullptr || a.target == nullptr || a.lse == nullptr || a.work == nullptr) return ULTIMA_HSAMP_ERR_INVALID;
+    if (a.rows < 1 || a.in_dim < 1 || a.vocab < 1 || a.vocab > ULTIMA_HSAMP_MAX_VOCAB) return ULTIMA_HSAMP_ERR_INVALID;
+    if (a.dtype != ULTIMA_HSAMP_BF16 && a.dtype != ULTIMA_HSAMP_F16) return ULTIMA_HSAMP_ERR_INVALID;
+    if (!(a.softcap >= 0.0f && a.softcap <= 3.402823466e38f)) return ULTIMA_HSAMP_ERR_INVALID;
+    if (a.x_stride < a.in_dim || a.weight_stride < a.in_dim) return ULTIMA_HSAMP_ERR_INVALID;
+    if ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.weight)) % 2 != 0 ||
+        (reinterpret_cast<uintptr_t>(a.target) | reinterpret_cast<uintptr_t>(a.lse)) % 4 != 0 || reinterpret_cast<uintptr_t>(a.work) % 16 != 0)
+        return ULTIMA_HSAMP_ERR_INVALID;
+    return ULTIMA_HSAMP_OK;
+}
+bool too_large(int rows, int in_dim, int vocab) {
+    LossArgs l = loss_args(rows, in_dim, vocab, nullptr, 0, nullptr, 0, nullptr, 0.0f);
+    // 32-bit rows and columns; a launch counts its threads in 32 bits
+    return rows > 1 << 22 || in_dim > 1 << 20 || (int64_t)rows * in_dim > (int64_t)1 << 31 || std::max(blocks_of(kForms[choose(l)], l), blocks_of(kForms[6], l)) > 1 << 22;
+}
+
+template <bool BF>
+hipError_t launch_grads(const ultima_hsamp_cross_entropy_grad_args& a, hipStream_t s) {
+    const Pieces p = pieces_of(a.rows, a.in_dim, a.vocab);
+    const GradWork at = grad_work(p, a.rows);
+    char* work = static_cast<char*>(a.work);
+    float* top = reinterpret_cast<float*>(work);
+    uint16_t* dz = reinterpret_cast<uint16_t*>(work + at.dz);
+    float* parts = reinterpret_cast<float*>(work + at.parts);
+    if (!BF) hipLaunchKernelGGL(k_top_grad, dim3(1), dim3(1024), 0, s, a.grad, a.target, a.rows, a.vocab, top);
+    // operands at other addresses than whole 16 bytes are laid out first
+    const auto odd = [&](const void* q, int64_t stride) {
+        return a.in_dim % 8 != 0 || reinterpret_cast<uintptr_t>(q) % 16 != 0 || stride % 8 != 0 || stride > 1 << 20;
+    };
+    const auto lay_out = [&](const uint16_t* from, int64_t stride, int64_t rows, uint16_t* to) {
+        const int pieces = (int)(p.columns / 8);
+        hipLaunchKernelGGL(k_lay_out, dim3((uint32_t)((rows * pieces + 255) / 256)), dim3(256), 0, s, from, stride, rows, a.in_dim, to, pieces);
+    };
+    const uint16_t* x = static_cast<const uint16_t*>(a.x);
+    int64_t x_stride = a.x_stride;
+    if (odd(a.x, a.x_stride)) {
+        uint16_t* to = reinterpret_cast<uint16_t*>(work + at.x);
+        lay_out(x, x_stride, a.rows, to);
+        x = to, x_stride = p.columns;
+    }
+    const bool odd_weight = odd(a.weight, a.weight_stride);
+    const int es = a.d_weight_dtype == ULTIMA_HSAMP_F32 ? 4 : 2;
+    for (int k = 0; k < p.count; ++k) {
+        const int64_t first = k * p.width;
+        const int width = (int)std::min(p.width, a.vocab - first);
+        const uint16_t* w = static_cast<const uint16_t*>(a.weight) + first * a.weight_stride;
+        int64_t w_stride = a.weight_stride;
+        if (odd_weight) {
+            uint16_t* to = reinterpret_cast<uint16_t*>(work + at.weight);
+            lay_out(w, w_stride, width, to);
+            w = to, w_stride = p.columns;
+        }
+        LossArgs l = loss_args(a.rows, (int)p.columns, width, x, x_stride, w, w_stride, a.target, a.softcap);
+        l.vocab = a.vocab, l.first = (int)first;
+        l.lse = a.lse, l.grad = a.grad, l.top_grad = top, l.dz = dz, l.dz_stride = p.width;
+        hipError_t e = launch_product<LossGrad<BF>>(l, s);
+        if (e != hipSuccess) return e;
+        if (a.d_x != nullptr) {
+            GradArgs g = {};
+            g.rows = a.rows, g.out_dim = (int)p.columns, g.k = width, g.k_split = p.split;
+            g.a = dz, g.a_stride = p.width, g.a_columns = width;
+            g.b = w, g.b_stride = w_stride, g.b_columns = (int)p.columns;
+            g.out = parts, g.out_stride = p.columns, g.out_split = a.rows * p.columns, g.out_f32 = 1, g.add = k > 0;
+            const int tm = (a.rows + 255) / 256, tn = (int)((p.columns + 255) / 256);
+            hipLaunchKernelGGL((k_grad_tile<BF, false>), dim3(tm * tn, 1, p.splits), dim3(512), 0, s, g, tm, tn);
+        }
+        if (a.d_weight != nullptr) {
+            GradArgs g = {};
+            g.rows = width, g.out_dim = a.in_dim, g.k = a.rows, g.k_split = (int)up(a.rows, 64);
+            g.a = dz, g.a_stride = p.width, g.a_columns = (int)up(width, 8);
+            g.b = x, g.b_stride = x_stride, g.b_columns = (int)p.columns;
+            g.out = static_cast<char*>(a.d_weight) + first * a.d_weight_stride * es, g.out_stride = a.d_weight_stride;
+            g.out_f32 = es == 4, g.add = a.accumulate != 0, g.top_grad = BF ? nullptr : top;
+            const int tm = (width + 255) / 256, tn = (a.in_dim + 255) / 256;
+            hipLaunchKernelGGL((k_grad_tile<BF, true>), dim3(tm * tn), dim3(512), 0, s, g, tm, tn);
+        }
+    }
+    if (a.d_x != nullptr)
+        hipLaunchKernelGGL(k_grad_join<BF>, dim3((uint32_t)((a.rows * p.columns + 255) / 256)), dim3(256), 0, s, (const float*)parts, p.splits,
+                           a.rows * p.columns, p.columns, a.rows, a.in_dim, (const float*)top, a.d_x, a.d_x_stride,
+                           (int)(a.d_x_dtype == ULTIMA_HSAMP_F32));
+    return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace hsamp
+
+extern "C" int64_t ultima_hsamp_cross_entropy_work_bytes(int32_t rows, int32_t vocab) {
+    using namespace hsamp;
+    if (rows < 1 || vocab < 1 || vocab > ULTIMA_HSAMP_MAX_VOCAB) return -1;
+    return up((int64_t)rows * 4, 16) + (int64_t)rows * ((vocab + 15) / 16) * 8;
+}
+
+extern "C" int ultima_hsamp_cross_entropy(const ultima_hsamp_cross_entropy_args* a, void* hip_stream) {
+    using namespace hsamp;
+    if (a == nullptr || a->loss == nullptr || reinterpret_cast<uintptr_t>(a->loss) % 4 != 0 || a->loss == a->lse) return ULTIMA_HSAMP_ERR_INVALID;
+    const int status = check_loss(*a);
+    if (status != ULTIMA_HSAMP_OK) return status;
+    if (too_large(a->rows, a->in_dim, a->vocab)) return ULTIMA_HSAMP_ERR_UNSUPPORTED;
+    hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    LossArgs l = loss_args(a->rows, a->in_dim, a->vocab, a->x, a->x_stride, a->weight, a->weight_stride, a->target, a->softcap);
+    l.at_target = static_cast<float*>(a->work);
+    l.partial = reinterpret_cast<float2*>(static_cast<char*>(a->work) + up((int64_t)a->rows * 4, 16));
+    hipError_t e = a->dtype == ULTIMA_HSAMP_BF16 ? launch_product<LossRows<true>>(l, s) : launch_product<LossRows<false>>(l, s);
+    if (e == hipSuccess) {
+        const int bn = columns_of<LossRows<true>>(l), tiles = (a->vocab + bn - 1) / bn, log_rows = a->rows >= 16 ? 4 : 0;
+        hipLaunchKernelGGL(k_loss_join, dim3((a->rows + (1 << log_rows) - 1) >> log_rows), dim3(1024), 0, s, (const float2*)l.partial,
+                           (const float*)l.at_target, a->target, a->rows, a->vocab, tiles, log_rows, a->loss, a->lse);
+        e = hipGetLastError();
+    }
+    return e == hipSuccess ? ULTIMA_HSAMP_OK : ULTIMA_HSAMP_ERR_HIP;
+}
+
+extern "C" int64_t ultima_hsamp_cross_entropy_grad_work_bytes(int32_t rows, int32_t in_dim, int32_t vocab) {
+    using namespace hsamp;
+    if (rows < 1 || in_dim < 1 || vocab < 1 || vocab > ULTIMA_HSAMP_MAX_VOCAB) return -1;
+    return grad_work(pieces_of(rows, in_dim, vocab), rows).bytes;
+}
+
+extern "C" int ultima_hsamp_cross_entropy_grad(const ultima_hsamp_cross_entropy_grad_args* a, void* hip_stream) {
+    using namespace hsamp;
+    if (a == nullptr || a->grad == nullptr || reinterpret_cast<uintptr_t>(a->grad) % 4 != 0 || (a->d_x == nullptr && a->d_weight == nullptr))
+        return ULTIMA_HSAMP_ERR_INVALID;
+    const int status = check_loss(*a);
+    if (status != ULTIMA_HSAMP_OK) return status;
+    const auto bad = [&](const void* out, int64_t stride, int dtype) {
+        if (out == nullptr) return false;
+        return out == a->x || out == a->weight || out == a->work || out == static_cast<const void*>(a->lse) || out == static_cast<const void*>(a->grad) ||
+               out == static_cast<const void*>(a->target) || stride < a->in_dim || (dtype != a->dtype && dtype != ULTIMA_HSAMP_F32) ||
+               reinterpret_cast<uintptr_t>(out) % (dtype == ULTIMA_HSAMP_F32 ? 4 : 2) != 0;
+    };
+    if (bad(a->d_x, a->d_x_stride, a->d_x_dtype) || bad(a->d_weight, a->d_weight_stride, a->d_weight_dtype)) return ULTIMA_HSAMP_ERR_INVALID;
+    if (a->d_x != nullptr && a->d_x == a->d_weight) return ULTIMA_HSAMP_ERR_INVALID;
+    if (too_large(a->rows, a->in_dim, a->vocab)) return ULTIMA_HSAMP_ERR_UNSUPPORTED;
+    hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    const hipError_t e = a->dtype == ULTIMA_HSAMP_BF16 ? launch_grads<true>(*a, s) : launch_grads<false>(*a, s);
+    return e == hipSuccess ? ULTIMA_HSAMP_OK : ULTIMA_HSAMP_ERR_HIP;
+}

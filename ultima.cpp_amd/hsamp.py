@@ -225,6 +225,133 @@ class LinearArgs(ctypes.Structure):
     ]
 
 
+class LinearI8Args(ctypes.Structure):
+    """ultima_hsamp_linear_i8_args (include/ultima_hsamp.h)."""
+    _fields_ = [
+        ("rows", ctypes.c_int32),
+        ("in_dim", ctypes.c_int32),
+        ("out_dim", ctypes.c_int32),
+        ("groups", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("act", ctypes.c_int32),
+        ("act_param", ctypes.c_float),
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("x_group", ctypes.c_int64),
+        ("x_scale", ctypes.c_void_p),
+        ("x_scale_group", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("weight_stride", ctypes.c_int64),
+        ("weight_group", ctypes.c_int64),
+        ("weight_scale", ctypes.c_void_p),
+        ("weight_scale_group", ctypes.c_int64),
+        ("bias", ctypes.c_void_p),
+        ("bias_group", ctypes.c_int64),
+        ("residual", ctypes.c_void_p),
+        ("residual_stride", ctypes.c_int64),
+        ("residual_group", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_stride", ctypes.c_int64),
+        ("out_group", ctypes.c_int64),
+    ]
+
+
+class QuantizeArgs(ctypes.Structure):
+    """ultima_hsamp_quantize_args (include/ultima_hsamp.h)."""
+    _fields_ = [
+        ("rows", ctypes.c_int32),
+        ("in_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64),
+        ("scale", ctypes.c_void_p),
+    ]
+
+
+class CrossEntropyArgs(ctypes.Structure):
+    """ultima_hsamp_cross_entropy_args (include/ultima_hsamp.h)."""
+    _fields_ = [
+        ("rows", ctypes.c_int32),
+        ("in_dim", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("softcap", ctypes.c_float),
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("weight_stride", ctypes.c_int64),
+        ("target", ctypes.c_void_p),
+        ("loss", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("work", ctypes.c_void_p),
+    ]
+
+
+class CrossEntropyGradArgs(ctypes.Structure):
+    """ultima_hsamp_cross_entropy_grad_args (include/ultima_hsamp.h)."""
+    _fields_ = [
+        ("rows", ctypes.c_int32),
+        ("in_dim", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("softcap", ctypes.c_float),
+        ("accumulate", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("weight_stride", ctypes.c_int64),
+        ("target", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("d_x", ctypes.c_void_p),
+        ("d_x_stride", ctypes.c_int64),
+        ("d_weight", ctypes.c_void_p),
+        ("d_weight_stride", ctypes.c_int64),
+        ("d_x_dtype", ctypes.c_int32),
+        ("d_weight_dtype", ctypes.c_int32),
+        ("work", ctypes.c_void_p),
+    ]
+
+
+class EmbedArgs(ctypes.Structure):
+    """ultima_hsamp_embed_args (include/ultima_hsamp.h)."""
+    _fields_ = [
+        ("tokens", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("ids", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("out_stride", ctypes.c_int64),
+    ]
+
+
+class EmbedGradArgs(ctypes.Structure):
+    """ultima_hsamp_embed_grad_args (include/ultima_hsamp.h)."""
+    _fields_ = [
+        ("tokens", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("accumulate", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("d_out", ctypes.c_void_p),
+        ("d_out_stride", ctypes.c_int64),
+        ("ids", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("out_stride", ctypes.c_int64),
+        ("work", ctypes.c_void_p),
+    ]
+
+
 def declared_symbols(header: Path = HEADER) -> list[str]:
     """Function names declared in a header (default include/ultima_hsamp.h)."""
     import re
@@ -296,6 +423,14 @@ def lib() -> ctypes.CDLL:
         L.ultima_hsamp_verify_sets.argtypes = [ctypes.POINTER(DraftSets), vp]
         L.ultima_hsamp_linear.restype = ctypes.c_int
         L.ultima_hsamp_linear.argtypes = [ctypes.POINTER(LinearArgs), vp]
+        for name, args in (("linear_i8", LinearI8Args), ("quantize_rows", QuantizeArgs), ("cross_entropy", CrossEntropyArgs),
+                           ("cross_entropy_grad", CrossEntropyGradArgs), ("embed", EmbedArgs),
+                           ("embed_grad", EmbedGradArgs)):
+            fn = getattr(L, f"ultima_hsamp_{name}")
+            fn.restype, fn.argtypes = ctypes.c_int, [ctypes.POINTER(args), vp]
+        for name, sizes in (("cross_entropy", 2), ("cross_entropy_grad", 3), ("embed_grad", 3)):
+            fn = getattr(L, f"ultima_hsamp_{name}_work_bytes")
+            fn.restype, fn.argtypes = i64, [i32] * sizes
         _lib = L
     return _lib
 
@@ -703,13 +838,23 @@ def verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_dr
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "softcap": 5}
 
 
-def _matrix(t, lead, rows, columns, dtype, dev, name):
+def _matrix(t, lead, rows, columns, dtype, dev, name, what="linear"):
     """The address, row stride and group stride of a [*lead, rows, columns] operand."""
     shape, stride = t.shape, t.stride()
     if shape[:-2] != lead or len(shape) < 2 or shape[-2] != rows or shape[-1] != columns or t.dtype != dtype or \
             t.device != dev or (columns > 1 and stride[-1] != 1):
-        _refuse(f"linear: {name} must be {dtype} {(*lead, rows, columns)} on {dev}, contiguous in its last dimension")
+        _refuse(f"{what}: {name} must be {dtype} {(*lead, rows, columns)} on {dev}, contiguous in its last dimension")
     return t.data_ptr(), stride[-2] if rows > 1 else max(columns, stride[-2]), stride[0] if lead else 0
+
+
+def _epilogue(a, bias, residual, lead, M, N, dt, dev, what):
+    """The bias and residual of LinearArgs and LinearI8Args."""
+    if bias is not None:
+        if bias.shape != (*lead, N) or bias.dtype != dt or bias.device != dev or (N > 1 and bias.stride(-1) != 1):
+            _refuse(f"{what}: bias must be {dt} {(*lead, N)} on {dev}, contiguous in its last dimension")
+        a.bias, a.bias_group = bias.data_ptr(), bias.stride(0) if lead else 0
+    if residual is not None:
+        a.residual, a.residual_stride, a.residual_group = _matrix(residual, lead, M, N, dt, dev, "residual", what)
 
 
 def linear(x, weight, bias=None, act: str = "none", act_param: float = 0.0, residual=None, out=None, out_dtype=None,
@@ -744,14 +889,264 @@ def linear(x, weight, bias=None, act: str = "none", act_param: float = 0.0, resi
     a = LinearArgs(M, K, N, lead[0] if lead else 1, kind, F32 if odt == torch.float32 else kind, ACTS[act], act_param)
     a.x, a.x_stride, a.x_group = _matrix(x, lead, M, K, dt, dev, "x")
     a.weight, a.weight_stride, a.weight_group = _matrix(weight, lead, N, K, dt, dev, "weight")
-    if bias is not None:
-        if bias.shape != (*lead, N) or bias.dtype != dt or bias.device != dev or (N > 1 and bias.stride(-1) != 1):
-            _refuse(f"linear: bias must be {dt} {(*lead, N)} on {dev}, contiguous in its last dimension")
-        a.bias, a.bias_group = bias.data_ptr(), bias.stride(0) if lead else 0
-    if residual is not None:
-        a.residual, a.residual_stride, a.residual_group = _matrix(residual, lead, M, N, dt, dev, "residual")
+    _epilogue(a, bias, residual, lead, M, N, dt, dev, "linear")
     a.out, a.out_stride, a.out_group = _matrix(out, lead, M, N, odt, dev, "out")
     _launch(lib().ultima_hsamp_linear, a, dev, "linear")
+    return out
+
+
+def quantize_rows(x, q=None, scale=None, stream=None):
+    """ultima_hsamp_quantize_rows on torch tensors of one device: x [M, K] float32,
+    bfloat16 or float16 in 8 bits, a scale for each row (for tokens before linear_i8;
+    for a weight, once, its channels). Returns (q int8 [M, K], scale f32 [M]); the
+    outputs may be passed in. stream: as in verify_draft."""
+    import torch
+    what, dev = "quantize_rows", x.device
+    kinds = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+    if not x.is_cuda or x.dim() != 2 or x.dtype not in kinds:
+        _refuse(f"{what}: x must be a float32, bfloat16 or float16 matrix on the GPU")
+    there = _elsewhere(dev, stream, what)
+    if there is not None:
+        with there:
+            out = quantize_rows(x, q, scale)
+        _used_on(stream, x, *out)
+        return out
+    M, K = x.shape
+    if q is None:
+        q = torch.empty((M, K), dtype=torch.int8, device=dev)
+    if scale is None:
+        scale = torch.empty(M, dtype=torch.float32, device=dev)
+    a = QuantizeArgs(M, K, kinds[x.dtype])
+    a.x, a.x_stride, _ = _matrix(x, (), M, K, x.dtype, dev, "x", what)
+    a.q, a.q_stride, _ = _matrix(q, (), M, K, torch.int8, dev, "q", what)
+    a.scale = _vector(scale, M, torch.float32, dev, what, "scale")
+    _launch(lib().ultima_hsamp_quantize_rows, a, dev, what)
+    return q, scale
+
+
+def linear_i8(x, x_scale, weight, weight_scale, bias=None, act: str = "none", act_param: float = 0.0, residual=None,
+              out=None, out_dtype=None, dtype=None, stream=None):
+    """ultima_hsamp_linear_i8 on torch tensors of one device: act(x_scale weight_scale
+    (x weight^T) + bias) + residual, x int8 [M, K] with x_scale f32 [M] and weight int8
+    [N, K] with weight_scale f32 [N] (quantize_rows), or with a leading dimension of
+    groups on all of them; bias and residual in dtype (bfloat16, the default, or
+    float16), the output in that type or in float32. The other arguments as in
+    linear."""
+    import torch
+    what, dev = "linear_i8", x.device
+    if not x.is_cuda or x.dtype != torch.int8 or x.dim() not in (2, 3) or weight.dim() != x.dim():
+        _refuse(f"{what}: x and weight must be int8 matrices (or batches of them) on the GPU")
+    if act not in ACTS:
+        _refuse(f"{what}: act must be one of {', '.join(ACTS)}")
+    there = _elsewhere(dev, stream, what)
+    if there is not None:
+        with there:
+            out = linear_i8(x, x_scale, weight, weight_scale, bias, act, act_param, residual, out, out_dtype, dtype)
+        _used_on(stream, x, x_scale, weight, weight_scale, bias, residual, out)
+        return out
+    lead = x.shape[:-2]
+    M, K = x.shape[-2:]
+    N = weight.shape[-2]
+    if dtype is None:
+        given = [t.dtype for t in (bias, residual) if t is not None] + [d for d in (out_dtype, getattr(out, "dtype", None)) if d == torch.float16]
+        dtype = given[0] if given else torch.bfloat16
+    if dtype not in (torch.bfloat16, torch.float16):
+        _refuse(f"{what}: bias and residual are bfloat16 or float16")
+    if out is None:
+        out = torch.empty((*lead, M, N), dtype=out_dtype or dtype, device=dev)
+    odt = out.dtype
+    if odt not in (dtype, torch.float32) or out_dtype not in (None, odt):
+        _refuse(f"{what}: the output must be {dtype} or torch.float32")
+    kind = BF16 if dtype == torch.bfloat16 else F16
+    a = LinearI8Args(M, K, N, lead[0] if lead else 1, kind, F32 if odt == torch.float32 else kind, ACTS[act], act_param)
+    a.x, a.x_stride, a.x_group = _matrix(x, lead, M, K, torch.int8, dev, "x", what)
+    a.weight, a.weight_stride, a.weight_group = _matrix(weight, lead, N, K, torch.int8, dev, "weight", what)
+    for t, n, name in ((x_scale, M, "x_scale"), (weight_scale, N, "weight_scale")):
+        if t is None or t.shape != (*lead, n) or t.dtype != torch.float32 or t.device != dev or (n > 1 and t.stride(-1) != 1):
+            _refuse(f"{what}: {name} must be torch.float32 {(*lead, n)} on {dev}, contiguous in its last dimension")
+    a.x_scale, a.x_scale_group = x_scale.data_ptr(), x_scale.stride(0) if lead else 0
+    a.weight_scale, a.weight_scale_group = weight_scale.data_ptr(), weight_scale.stride(0) if lead else 0
+    _epilogue(a, bias, residual, lead, M, N, dtype, dev, what)
+    a.out, a.out_stride, a.out_group = _matrix(out, lead, M, N, odt, dev, "out", what)
+    _launch(lib().ultima_hsamp_linear_i8, a, dev, what)
+    return out
+
+
+def _loss_args(a, x, weight, target, softcap, what, dev):
+    """The fields of CrossEntropyArgs and CrossEntropyGradArgs that say what the logits are."""
+    import torch
+    M, K = x.shape
+    V = weight.shape[0]
+    a.rows, a.in_dim, a.vocab, a.dtype = M, K, V, BF16 if x.dtype == torch.bfloat16 else F16
+    a.softcap = softcap
+    a.x, a.x_stride, _ = _matrix(x, (), M, K, x.dtype, dev, "x", what)
+    a.weight, a.weight_stride, _ = _matrix(weight, (), V, K, x.dtype, dev, "weight", what)
+    if target is None:
+        _refuse(f"{what}: target is missing")
+    a.target = _vector(target, M, torch.int32, dev, what, "target")
+    return M, K, V
+
+
+def _loss_operands(x, weight, what):
+    import torch
+    if not x.is_cuda or x.dim() != 2 or weight.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16):
+        _refuse(f"{what}: x and weight must be bfloat16 or float16 matrices on the GPU")
+
+
+def cross_entropy(x, weight, target, softcap: float = 0.0, work=None, outputs=None, stream=None):
+    """ultima_hsamp_cross_entropy on torch tensors of one device: each row's cross
+    entropy (minus the log-probability of its target) over the logits x weight^T,
+    x [M, K] and weight [V, K] bfloat16 or float16, target int32 [M] (outside [0, V):
+    ignored, loss 0), softcap: logits c tanh(z / c). Returns a dict: loss f32 [M], lse
+    f32 [M] (which cross_entropy_grad takes). work: a uint8 tensor of
+    ultima_hsamp_cross_entropy_work_bytes() bytes of this call alone (allocated
+    otherwise); outputs: a dict of tensors to write to; stream: as in verify_draft."""
+    import torch
+    what, dev = "cross_entropy", x.device
+    _loss_operands(x, weight, what)
+    there = _elsewhere(dev, stream, what)
+    if there is not None:
+        with there:
+            out = cross_entropy(x, weight, target, softcap, work, outputs)
+        _used_on(stream, x, weight, target, work, *out.values())
+        return out
+    a = CrossEntropyArgs()
+    M, K, V = _loss_args(a, x, weight, target, softcap, what, dev)
+    out = {} if outputs is None else outputs
+    for name in ("loss", "lse"):
+        if out.get(name) is None:
+            out[name] = torch.empty(M, dtype=torch.float32, device=dev)
+        setattr(a, name, _vector(out[name], M, torch.float32, dev, what, name))
+    work = _work(work, lib().ultima_hsamp_cross_entropy_work_bytes(M, V), dev, what)
+    a.work = work.data_ptr()
+    _launch(lib().ultima_hsamp_cross_entropy, a, dev, what)
+    return out
+
+
+def cross_entropy_grad(x, weight, target, lse, grad, softcap: float = 0.0, need_x: bool = True, need_weight: bool = True,
+                       accumulate: bool = False, work=None, outputs=None, stream=None):
+    """ultima_hsamp_cross_entropy_grad on torch tensors of one device: the gradients
+    of cross_entropy's losses, weighted by grad f32 [M] (ignored rows' is not looked
+    at), with the lse that it returned. Returns a dict: d_x [M, K] and d_weight
+    [V, K], each in x's type unless outputs brings a tensor (of that type or float32)
+    to write to; need_x, need_weight: leave one out; accumulate: add to
+    outputs["d_weight"]. The other arguments as in cross_entropy."""
+    import torch
+    what, dev = "cross_entropy_grad", x.device
+    _loss_operands(x, weight, what)
+    there = _elsewhere(dev, stream, what)
+    if there is not None:
+        with there:
+            out = cross_entropy_grad(x, weight, target, lse, grad, softcap, need_x, need_weight, accumulate, work, outputs)
+        _used_on(stream, x, weight, target, lse, grad, work, *out.values())
+        return out
+    a = CrossEntropyGradArgs()
+    M, K, V = _loss_args(a, x, weight, target, softcap, what, dev)
+    if lse is None or grad is None:
+        _refuse(f"{what}: lse and grad are missing")
+    a.lse, a.grad = (_vector(t, M, torch.float32, dev, what, name) for t, name in ((lse, "lse"), (grad, "grad")))
+    out = {} if outputs is None else outputs
+    if accumulate and (not need_weight or out.get("d_weight") is None):
+        _refuse(f"{what}: accumulate goes with outputs['d_weight']")
+    for name, rows, need in (("d_x", M, need_x), ("d_weight", V, need_weight)):
+        if not need:
+            continue
+        if out.get(name) is None:
+            out[name] = torch.empty((rows, K), dtype=x.dtype, device=dev)
+        t = out[name]
+        if t.dtype not in (x.dtype, torch.float32):
+            _refuse(f"{what}: {name} must be {x.dtype} or torch.float32")
+        at, stride, _ = _matrix(t, (), rows, K, t.dtype, dev, name, what)
+        setattr(a, name, at)
+        setattr(a, f"{name}_stride", stride)
+        setattr(a, f"{name}_dtype", F32 if t.dtype == torch.float32 else a.dtype)
+    a.accumulate = bool(accumulate)
+    work = _work(work, lib().ultima_hsamp_cross_entropy_grad_work_bytes(M, K, V), dev, what)
+    a.work = work.data_ptr()
+    _launch(lib().ultima_hsamp_cross_entropy_grad, a, dev, what)
+    return out
+
+
+def _embed_types(dt, out_dtype, what):
+    import torch
+    kinds = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+    if dt not in kinds or out_dtype not in (dt, torch.float32):
+        _refuse(f"{what}: rows are float32, bfloat16 or float16, the output in their type or in float32")
+    return kinds[dt], kinds[out_dtype]
+
+
+def embed(table, tokens, scale: float = 1.0, out=None, out_dtype=None, stream=None):
+    """ultima_hsamp_embed on torch tensors of one device: scale * table[tokens], table
+    [V, H] float32, bfloat16 or float16, tokens int32 [N] (outside [0, V), an ended
+    slot's -1: a row of zeros), the output [N, H] in the table's type or in float32
+    (out_dtype; out: the tensor to write). stream: as in verify_draft."""
+    import torch
+    what, dev = "embed", table.device
+    if not table.is_cuda or table.dim() != 2:
+        _refuse(f"{what}: table must be a matrix on the GPU")
+    there = _elsewhere(dev, stream, what)
+    if there is not None:
+        with there:
+            out = embed(table, tokens, scale, out, out_dtype)
+        _used_on(stream, table, tokens, out)
+        return out
+    a = EmbedArgs()
+    V, H = table.shape
+    if tokens is None:
+        _refuse(f"{what}: tokens are missing")
+    a.ids = _vector(tokens, None, torch.int32, dev, what, "tokens")
+    n = tokens.shape[0]
+    odt = out.dtype if out is not None else out_dtype or table.dtype
+    if out_dtype not in (None, odt):
+        _refuse(f"{what}: out must be {out_dtype}")
+    a.dtype, a.out_dtype = _embed_types(table.dtype, odt, what)
+    if out is None:
+        out = torch.empty((n, H), dtype=odt, device=dev)
+    a.tokens, a.width, a.vocab, a.scale = n, H, V, scale
+    a.table, a.table_stride, _ = _matrix(table, (), V, H, table.dtype, dev, "table", what)
+    a.out, a.out_stride, _ = _matrix(out, (), n, H, odt, dev, "out", what)
+    _launch(lib().ultima_hsamp_embed, a, dev, what)
+    return out
+
+
+def embed_grad(d_out, tokens, vocab: int, scale: float = 1.0, out=None, out_dtype=None, accumulate: bool = False,
+               work=None, stream=None):
+    """ultima_hsamp_embed_grad on torch tensors of one device: the gradient of embed
+    with respect to its table, from d_out [N, H] float32, bfloat16 or float16 and
+    tokens int32 [N]: [vocab, H] in d_out's type or in float32 (out_dtype; out: the
+    tensor to write, accumulate: to add to). work: a uint8 tensor of
+    ultima_hsamp_embed_grad_work_bytes() bytes of this call alone (allocated
+    otherwise); stream: as in verify_draft."""
+    import torch
+    what, dev = "embed_grad", d_out.device
+    if not d_out.is_cuda or d_out.dim() != 2:
+        _refuse(f"{what}: d_out must be a matrix on the GPU")
+    there = _elsewhere(dev, stream, what)
+    if there is not None:
+        with there:
+            out = embed_grad(d_out, tokens, vocab, scale, out, out_dtype, accumulate, work)
+        _used_on(stream, d_out, tokens, work, out)
+        return out
+    a = EmbedGradArgs()
+    n, H = d_out.shape
+    if tokens is None:
+        _refuse(f"{what}: tokens are missing")
+    a.ids = _vector(tokens, n, torch.int32, dev, what, "tokens")
+    odt = out.dtype if out is not None else out_dtype or d_out.dtype
+    if out_dtype not in (None, odt) or (accumulate and out is None):
+        _refuse(f"{what}: out must be {out_dtype}; accumulate goes with out")
+    a.dtype, a.out_dtype = _embed_types(d_out.dtype, odt, what)
+    need = lib().ultima_hsamp_embed_grad_work_bytes(n, H, vocab)
+    if need < 0:
+        _refuse(f"{what}: at least one token, one column and one row, 2^24 rows at most")
+    if out is None:
+        out = torch.empty((vocab, H), dtype=odt, device=dev)
+    a.tokens, a.width, a.vocab, a.scale, a.accumulate = n, H, vocab, scale, bool(accumulate)
+    a.d_out, a.d_out_stride, _ = _matrix(d_out, (), n, H, d_out.dtype, dev, "d_out", what)
+    a.out, a.out_stride, _ = _matrix(out, (), vocab, H, odt, dev, "out", what)
+    work = _work(work, need, dev, what)
+    a.work = work.data_ptr()
+    _launch(lib().ultima_hsamp_embed_grad, a, dev, what)
     return out
 
 
