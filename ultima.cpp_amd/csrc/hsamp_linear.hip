@@ -6,30 +6,36 @@ namespace hsamp {
 namespace {
 
 template <bool BF>
-struct Linear {
+struct Linear : RowsOfK<ultima_hsamp_linear_args, uint16_t> {
     static constexpr bool kByRows = false;
     using Args = ultima_hsamp_linear_args;
-    using Element = uint16_t;
     using Sum = f32x4;
-    using Columns = u32x4;      // eight columns' bias
-    using Row = u32x4;          // eight values of the residual
+    using Columns = u32x4;      // a piece of the bias
+    using Row = u32x4;          // a piece of the residual
     static __device__ __forceinline__ Sum mfma(u32x4 w, u32x4 x, Sum c) { return hsamp::mfma<BF>(w, x, c); }
+    template <bool ACC>
+    static __device__ __forceinline__ void mfma_in_place(Sum& c, u32x4 w, u32x4 x) { hsamp::mfma_in_place<BF, ACC>(c, w, x); }
     template <int E>
     static __device__ __forceinline__ Columns columns(const Args& a, int g, int n) {
-        return E == 8 ? bias8(a, g, n) : u32x4{};
+        return bias_piece<E>(a, g, n);
     }
     template <int E>
     static __device__ __forceinline__ Row row(const Args& a, int g, int m, int n) {
-        return E == 8 ? residual8(a, g, m, n) : u32x4{};
+        return residual_piece<E>(a, g, m, n);
     }
-    template <int E>
+    template <int E, int ACT = kAnyAct, bool WHOLE = false>
     static __device__ __forceinline__ void finish(const Args& a, int g, int m, int n, float (&y)[E], Columns c, Row r) {
-        hsamp::finish<BF, E>(a, g, m, n, y, c, r);
+        hsamp::finish<BF, E, ACT, WHOLE>(a, g, m, n, y, c, r);
     }
-    template <int TN, int TM, int WM, int WN>
+    template <int TN, int TM, int WM, int WN, int PU>
     static __device__ __forceinline__ void tiles(const Args& a, int g, int m0, int n0, int wave, const Sum (&acc)[TN][TM], float* lds) {
-        store_tiles<Linear, TN, TM>(a, g, m0 + wave % WM * 16 * TM, n0 + wave / WM % WN * 16 * TN, acc,
-                                    lds + wave * 16 * (16 * TN + 4));
+        by_act(a.act, [&](auto act) {
+            store_tiles<Linear, decltype(act)::value, TN, TM, PU>(a, g, m0 + wave % WM * 16 * TM, n0 + wave / WM % WN * 16 * TN, acc, lds + wave * 256 * PU * TN);
+        });
+    }
+    template <int TN, int TM>
+    static __device__ __forceinline__ void wide(const Args& a, int g, int m0, int n0, const Sum (&acc)[TN][TM], uint16_t* lds) {
+        by_act(a.act, [&](auto act) { store_sixteens<Linear, decltype(act)::value>(a, g, m0, n0, acc, lds); });
     }
 };
 

@@ -11,10 +11,9 @@ namespace hsamp {
 namespace {
 
 template <bool BF>
-struct LinearI8 {
+struct LinearI8 : RowsOfK<ultima_hsamp_linear_i8_args, int8_t> {
     static constexpr bool kByRows = false;
     using Args = ultima_hsamp_linear_i8_args;
-    using Element = int8_t;
     using Sum = i32x4;
     struct Columns {
         u32x4 bias;
@@ -27,12 +26,19 @@ struct LinearI8 {
     static __device__ __forceinline__ Sum mfma(u32x4 w, u32x4 x, Sum c) {
         return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, x), c, 0, 0, 0);
     }
+    template <bool ACC>
+    static __device__ __forceinline__ void mfma_in_place(Sum& c, u32x4 w, u32x4 x) {
+#ifdef __HIP_DEVICE_COMPILE__
+        if constexpr (ACC) asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(w), "v"(x));
+        else asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+v"(c) : "v"(w), "v"(x));
+#endif
+    }
     template <int E>
     static __device__ __forceinline__ Columns columns(const Args& a, int g, int n) {
         Columns c = {};
         const float* s = a.weight_scale + g * a.weight_scale_group + n;
         const int left = a.out_dim - n;
-        if (E == 8) c.bias = bias8(a, g, n);
+        c.bias = bias_piece<E>(a, g, n);
 #pragma unroll
         for (int e = 0; e < E; ++e)
             if (e < left) c.scale[e] = s[e];
@@ -40,19 +46,24 @@ struct LinearI8 {
     }
     template <int E>
     static __device__ __forceinline__ Row row(const Args& a, int g, int m, int n) {
-        return {E == 8 ? residual8(a, g, m, n) : u32x4{}, m < a.rows ? a.x_scale[g * a.x_scale_group + m] : 0.0f};
+        return {residual_piece<E>(a, g, m, n), m < a.rows ? a.x_scale[g * a.x_scale_group + m] : 0.0f};
     }
-    template <int E>
+    template <int E, int ACT = kAnyAct, bool WHOLE = false>
     static __device__ __forceinline__ void finish(const Args& a, int g, int m, int n, const int32_t (&sum)[E], const Columns& c, const Row& r) {
         float y[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) y[e] = (float)sum[e] * r.scale * c.scale[e];
-        hsamp::finish<BF, E>(a, g, m, n, y, c.bias, r.residual);
+        hsamp::finish<BF, E, ACT, WHOLE>(a, g, m, n, y, c.bias, r.residual);
     }
-    template <int TN, int TM, int WM, int WN>
+    template <int TN, int TM, int WM, int WN, int PU>
     static __device__ __forceinline__ void tiles(const Args& a, int g, int m0, int n0, int wave, const Sum (&acc)[TN][TM], int32_t* lds) {
-        store_tiles<LinearI8, TN, TM>(a, g, m0 + wave % WM * 16 * TM, n0 + wave / WM % WN * 16 * TN, acc,
-                                      lds + wave * 16 * (16 * TN + 4));
+        by_act(a.act, [&](auto act) {
+            store_tiles<LinearI8, decltype(act)::value, TN, TM, PU>(a, g, m0 + wave % WM * 16 * TM, n0 + wave / WM % WN * 16 * TN, acc, lds + wave * 256 * PU * TN);
+        });
+    }
+    template <int TN, int TM>
+    static __device__ __forceinline__ void wide(const Args& a, int g, int m0, int n0, const Sum (&acc)[TN][TM], uint16_t* lds) {
+        by_act(a.act, [&](auto act) { store_sixteens<LinearI8, decltype(act)::value>(a, g, m0, n0, acc, lds); });
     }
 };
 

@@ -38,8 +38,11 @@ struct LossArgs {
     int64_t dz_stride;
 };
 
+// The logit of a sum; ACT: ULTIMA_HSAMP_ACT_NONE, _SOFTCAP, or as the arguments say.
+template <int ACT = kAnyAct>
 __device__ __forceinline__ float capped(const LossArgs& a, float y) {
-    return a.cap > 0.0f ? cap_of(y, y * a.cap_scale * a.cap_inv, a.cap) : y;
+    const bool cap = ACT == kAnyAct ? a.cap > 0.0f : ACT == ULTIMA_HSAMP_ACT_SOFTCAP;
+    return cap ? cap_of(y, y * a.cap_scale * a.cap_inv, a.cap) : y;
 }
 
 // The maximum and the sum of exponentials relative to it, of two.
@@ -50,12 +53,14 @@ __device__ __forceinline__ void join(float& top, float& sum, float top2, float s
 }
 
 template <bool BF>
-struct LossRows {
+struct LossRows : RowsOfK<LossArgs, uint16_t> {
+    static constexpr int kWideLds = 8192;
     static constexpr bool kByRows = true;
     using Args = LossArgs;
-    using Element = uint16_t;
     using Sum = f32x4;
     static __device__ __forceinline__ Sum mfma(u32x4 w, u32x4 x, Sum c) { return hsamp::mfma<BF>(w, x, c); }
+    template <bool ACC>
+    static __device__ __forceinline__ void mfma_in_place(Sum& c, u32x4 w, u32x4 x) { hsamp::mfma_in_place<BF, ACC>(c, w, x); }
 
     // Eight lanes to a row of a small tile.
     template <int BM, int BN, class Get>
@@ -82,49 +87,85 @@ struct LossRows {
     }
 
     // A wave's 16 TM rows: a lane's sums are 4 TN columns of TM of them.
-    template <int TN, int TM, int WM, int WN>
+    template <int TN, int TM, int WM, int WN, int PU>
     static __device__ __forceinline__ void tiles(const Args& a, int, int m0, int n0, int wave, const Sum (&acc)[TN][TM], float* lds) {
-        constexpr int BM = 16 * WM * TM, BN = 16 * WN * TN;
-        const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
-        const int wm = wave % WM * 16 * TM, wn = wave / WM, n = n0 + wn * 16 * TN + 4 * q;
-        float2* parts = reinterpret_cast<float2*>(lds);       // [WN][BM]
+        if (a.cap > 0.0f) statistics<ULTIMA_HSAMP_ACT_SOFTCAP, TN, TM, WM, WN>(a, m0, n0, wave, acc, lds);
+        else statistics<ULTIMA_HSAMP_ACT_NONE, TN, TM, WM, WN>(a, m0, n0, wave, acc, lds);
+    }
+    template <int TN, int TM>
+    static __device__ __forceinline__ void wide(const Args& a, int, int m0, int n0, const Sum (&acc)[TN][TM], uint16_t* lds) {
+        if (a.cap > 0.0f) wide_statistics<ULTIMA_HSAMP_ACT_SOFTCAP>(a, m0, n0, acc, lds);
+        else wide_statistics<ULTIMA_HSAMP_ACT_NONE>(a, m0, n0, acc, lds);
+    }
+    // Of a wave's 16 TM rows by 16 TN columns: a lane's sums are 4 TN columns of a row of each
+    // sixteen. parts: [columns' waves][BM] in LDS.
+    template <int ACT, int TN, class Z>
+    static __device__ __forceinline__ float2 row_statistics(const Args& a, int m, int n, Z z_of) {
+        float z[4 * TN], top = -__builtin_inff(), sum = 0.0f;
 #pragma unroll
-        for (int u = 0; u < TM; ++u) {
-            const int row = wm + 16 * u + i, m = m0 + row;
-            float z[4 * TN], top = -__builtin_inff(), sum = 0.0f;
+        for (int s = 0; s < TN; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float y = capped<ACT>(a, z_of(s, e));
+                z[4 * s + e] = n + 16 * s + e < a.out_dim ? y : -__builtin_inff();
+                top = fmaxf(top, z[4 * s + e]);
+            }
+        const int t = m < a.rows ? a.target[m] - n : -1;
+        if (t >= 0 && t < 16 * TN && (t & 12) == 0 && n + t < a.out_dim) {
 #pragma unroll
             for (int s = 0; s < TN; ++s)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float y = capped(a, acc[s][u][e]);
-                    z[4 * s + e] = n + 16 * s + e < a.out_dim ? y : -__builtin_inff();
-                    top = fmaxf(top, z[4 * s + e]);
-                }
-            const int t = m < a.rows ? a.target[m] - n : -1;
-            if (t >= 0 && t < 16 * TN && (t & 12) == 0 && n + t < a.out_dim) {
-#pragma unroll
-                for (int s = 0; s < TN; ++s)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (t == 16 * s + e) a.at_target[m] = z[4 * s + e];
-            }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float ref = top == -__builtin_inff() ? 0.0f : top;
-#pragma unroll
-            for (int k = 0; k < 4 * TN; ++k) sum += exp_of(z[k] - ref);
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (q == 0) parts[wn * BM + row] = float2{top, sum};
+                for (int e = 0; e < 4; ++e)
+                    if (t == 16 * s + e) a.at_target[m] = z[4 * s + e];
         }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float ref = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+        for (int k = 0; k < 4 * TN; ++k) sum += exp_of(z[k] - ref);
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        return {top, sum};
+    }
+    template <int BM, int WN, int THREADS>
+    static __device__ __forceinline__ void join_columns(const Args& a, int m0, int tile, const float2* parts) {
         __syncthreads();
-        for (int row = threadIdx.x; row < BM; row += 64 * WM * WN) {
+        for (int row = threadIdx.x; row < BM; row += THREADS) {
             if (m0 + row >= a.rows) continue;
             float2 p = parts[row];
 #pragma unroll
             for (int k = 1; k < WN; ++k) join(p.x, p.y, parts[k * BM + row].x, parts[k * BM + row].y);
-            a.partial[(int64_t)(n0 / BN) * a.rows + m0 + row] = p;
+            a.partial[(int64_t)tile * a.rows + m0 + row] = p;
         }
+    }
+    template <int ACT, int TN, int TM, int WM, int WN>
+    static __device__ __forceinline__ void statistics(const Args& a, int m0, int n0, int wave, const Sum (&acc)[TN][TM], float* lds) {
+        constexpr int BM = 16 * WM * TM, BN = 16 * WN * TN;
+        const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+        const int wm = wave % WM * 16 * TM, wn = wave / WM;
+        float2* parts = reinterpret_cast<float2*>(lds);
+#pragma unroll
+        for (int u = 0; u < TM; ++u) {
+            const int row = wm + 16 * u + i;
+            const float2 p = row_statistics<ACT, TN>(a, m0 + row, n0 + wn * 16 * TN + 4 * q, [&](int s, int e) { return acc[s][u][e]; });
+            if (q == 0) parts[wn * BM + row] = p;
+        }
+        join_columns<BM, WN, 64 * WM * WN>(a, m0, n0 / BN, parts);
+    }
+    // Of two by 16 / TN waves, sixteen rows at a time.
+    template <int ACT, int TN, int TM>
+    static __device__ __forceinline__ void wide_statistics(const Args& a, int m0, int n0, const Sum (&acc)[TN][TM], uint16_t* lds) {
+        constexpr int BM = 32 * TM, BN = 256, WN = 16 / TN;
+        const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+        float2* parts = reinterpret_cast<float2*>(lds);
+#pragma unroll 1
+        for (int u = 0; u < TM; ++u) {
+            Sum t[TN];
+            pick(t, acc, u);
+            const float2 p = row_statistics<ACT, TN>(a, m0 + 16 * u + i, n0 + 4 * q, [&](int s, int e) { return t[s][e]; });
+            if (q == 0) parts[n0 / (16 * TN) % WN * BM + m0 % BM + 16 * u + i] = p;
+        }
+        join_columns<BM, WN, 128 * WN>(a, m0 / BM * BM, n0 / BN, parts);
     }
 };
 
@@ -162,10 +203,10 @@ __global__ __launch_bounds__(1024) void k_loss_join(const float2* partial, const
 // dz of a piece. Half precision holds 2^-24 of its largest values: rows' gradients are
 // taken relative to the largest one and everything times 2^15.
 template <bool BF>
-struct LossGrad {
+struct LossGrad : RowsOfK<LossArgs, uint16_t> {
+    static __device__ __forceinline__ int end(const LossArgs& a) { return (a.out_dim + 7) & ~7; }
     static constexpr bool kByRows = false;
     using Args = LossArgs;
-    using Element = uint16_t;
     using Sum = f32x4;
     struct Columns {};
     struct Row {
@@ -174,6 +215,8 @@ struct LossGrad {
         bool used;
     };
     static __device__ __forceinline__ Sum mfma(u32x4 w, u32x4 x, Sum c) { return hsamp::mfma<BF>(w, x, c); }
+    template <bool ACC>
+    static __device__ __forceinline__ void mfma_in_place(Sum& c, u32x4 w, u32x4 x) { hsamp::mfma_in_place<BF, ACC>(c, w, x); }
     template <int E>
     static __device__ __forceinline__ Columns columns(const Args&, int, int) { return {}; }
     template <int E>
@@ -187,36 +230,41 @@ struct LossGrad {
         }
         return {a.lse[m], g, t - a.first, t >= 0 && t < a.vocab};
     }
-    template <int E>
+    template <int E, int ACT = kAnyAct, bool WHOLE = false>
     static __device__ __forceinline__ void finish(const Args& a, int, int m, int n, float (&y)[E], Columns, Row r) {
         if (m >= a.rows) return;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float z = capped(a, y[e]);
+            const float z = capped<ACT>(a, y[e]);
             float d = exp_of(z - r.lse);
             if (n + e == r.target) d -= 1.0f;
-            if (a.cap > 0.0f) {
+            if (ACT == kAnyAct ? a.cap > 0.0f : ACT == ULTIMA_HSAMP_ACT_SOFTCAP) {
                 const float t = z * a.cap_scale * a.cap_inv;
                 d *= (1.0f - t) * (1.0f + t);
             }
-            // (columns past the piece, up to the tile's end, are read with it)
+            // (columns past the piece, up to the next eight, are read with it)
             y[e] = r.used && n + e < a.out_dim ? d * r.grad : 0.0f;
         }
         uint16_t* p = a.dz + m * a.dz_stride + n;
-        if (E == 8) {
-            u32x4 v = {};
-#pragma unroll
-            for (int e = 0; e < E / 2; ++e) v[e] = (uint32_t)from_f32<BF>(y[2 * e]) | (uint32_t)from_f32<BF>(y[(2 * e + 1) % E]) << 16;
-            *reinterpret_cast<u32x4*>(p) = v;
+        if constexpr (E == 8) {
+            store_piece<BF>(p, y);
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e) p[e] = from_f32<BF>(y[e]);
         }
     }
-    template <int TN, int TM, int WM, int WN>
+    template <int TN, int TM, int WM, int WN, int PU>
     static __device__ __forceinline__ void tiles(const Args& a, int g, int m0, int n0, int wave, const Sum (&acc)[TN][TM], float* lds) {
-        store_tiles<LossGrad, TN, TM>(a, g, m0 + wave % WM * 16 * TM, n0 + wave / WM % WN * 16 * TN, acc,
-                                      lds + wave * 16 * (16 * TN + 4));
+        m0 += wave % WM * 16 * TM;
+        n0 += wave / WM * 16 * TN;
+        lds += wave * 256 * PU * TN;
+        if (a.cap > 0.0f) store_tiles<LossGrad, ULTIMA_HSAMP_ACT_SOFTCAP, TN, TM, PU>(a, g, m0, n0, acc, lds);
+        else store_tiles<LossGrad, ULTIMA_HSAMP_ACT_NONE, TN, TM, PU>(a, g, m0, n0, acc, lds);
+    }
+    template <int TN, int TM>
+    static __device__ __forceinline__ void wide(const Args& a, int g, int m0, int n0, const Sum (&acc)[TN][TM], uint16_t* lds) {
+        if (a.cap > 0.0f) store_sixteens<LossGrad, ULTIMA_HSAMP_ACT_SOFTCAP>(a, g, m0, n0, acc, lds);
+        else store_sixteens<LossGrad, ULTIMA_HSAMP_ACT_NONE>(a, g, m0, n0, acc, lds);
     }
 };
 
@@ -249,201 +297,94 @@ __global__ __launch_bounds__(256) void k_lay_out(const uint16_t* from, int64_t s
     *reinterpret_cast<u32x4*>(to + k * 8) = v;
 }
 
-// out[m, n] (+)= scale * sum_k A(m, k) B(k, n): B's rows are k; A's rows are m (A_T
-// false) or k (true). Rows and addresses of A and B in steps of 16 bytes.
+// out[m, n] (+)= scale * sum_k x(m, k) w(k, n): w's rows are k; x's rows are m, or k
+// (TURN_X). Rows and addresses of both in steps of 16 bytes.
 struct GradArgs {
-    int32_t rows, out_dim, k;       // M, N (a multiple of 8 in memory), K
-    int32_t k_split;                // of one block of z, a multiple of 64
-    const uint16_t* a;
-    int64_t a_stride;
-    int32_t a_columns;              // that may be read
-    const uint16_t* b;
-    int64_t b_stride;
-    int32_t b_columns;
+    int32_t rows, out_dim, groups;  // M, N; parts of k
+    int32_t k, k_split;             // K; of one part, a multiple of 64
+    const uint16_t* x;
+    int64_t x_stride;
+    const uint16_t* weight;
+    int64_t weight_stride;
+    int32_t x_columns, weight_columns;      // that may be read where rows are k
     void* out;
     int64_t out_stride, out_split;
     int32_t out_f32, add;
     const float* top_grad;          // half precision, where the sums are to be in grad's scale again
 };
 
-template <bool BF>
-struct GradStore {
+template <bool BF, bool TURN_X>
+struct GradSums {
+    using Element = uint16_t;
+    using Sum = f32x4;
+    static constexpr bool kTurnX = TURN_X, kTurnW = true;
+    static constexpr int kWideLds = 32768, kWideWaves = 8;
+    static __device__ __forceinline__ Sum mfma(u32x4 w, u32x4 x, Sum c) { return hsamp::mfma<BF>(w, x, c); }
+    static __device__ __forceinline__ int end(const GradArgs& a) { return a.out_dim; }
     using Args = GradArgs;
-    using Row = u32x4;
+    template <bool ACC>
+    static __device__ __forceinline__ void mfma_in_place(Sum& c, u32x4 w, u32x4 x) { hsamp::mfma_in_place<BF, ACC>(c, w, x); }
+    static __device__ __forceinline__ int depth(const Args& a, int z) { return max(0, min(a.k_split, a.k - z * a.k_split)); }
+    static __device__ __forceinline__ const uint16_t* x_at(const Args& a, int z, int m) {
+        const int64_t k = z * a.k_split;
+        return a.x + (TURN_X ? k * a.x_stride + m : m * a.x_stride + k);
+    }
+    static __device__ __forceinline__ const uint16_t* w_at(const Args& a, int z, int n) { return a.weight + (int64_t)z * a.k_split * a.weight_stride + n; }
+    static __device__ __forceinline__ int x_columns(const Args& a) { return a.x_columns; }
+    static __device__ __forceinline__ int w_columns(const Args& a) { return a.weight_columns; }
     template <int E>
     static __device__ __forceinline__ float columns(const Args& a, int, int) {
         if (BF || a.top_grad == nullptr) return 1.0f;
         const float top = *a.top_grad;
         return top > 0.0f ? top * 0x1p-15f : 1.0f;
     }
+    // what is added to: eight floats, or eight of 16 bits
+    struct Row {
+        u32x4 lo, hi;
+    };
     template <int E>
-    static __device__ __forceinline__ Row row(const Args& a, int, int m, int n) {
-        if (!a.add || a.out_f32 || m >= a.rows || n + 8 > a.out_dim) return u32x4{};
-        return load16(static_cast<const uint16_t*>(a.out) + m * a.out_stride + n);
-    }
-    template <int E>
-    static __device__ __forceinline__ void finish(const Args& a, int z, int m, int n, float (&y)[E], float scale, Row old) {
-        typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
-        const int left = a.out_dim - n;
-        if (m >= a.rows || left <= 0) return;
-#pragma unroll
-        for (int e = 0; e < E; ++e) y[e] *= scale;
+    static __device__ __forceinline__ Row row(const Args& a, int z, int m, int n) {
+        Row r = {};
+        if (E == 1 || !a.add || m >= a.rows || n + 8 > a.out_dim) return r;
         const int64_t at = z * a.out_split + m * a.out_stride + n;
         if (a.out_f32) {
-            float* p = static_cast<float*>(a.out) + at;
-            if (left >= E) {
-#pragma unroll
-                for (int e = 0; e < E; e += 4) {
-                    f32x4 v = {y[e], y[e + 1], y[e + 2], y[e + 3]};
-                    if (a.add) v += *reinterpret_cast<const f32x4_a4*>(p + e);
-                    *reinterpret_cast<f32x4_a4*>(p + e) = v;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (e < left) p[e] = a.add ? p[e] + y[e] : y[e];
-            }
-            return;
-        }
-        uint16_t* p = static_cast<uint16_t*>(a.out) + at;
-        if (left >= E) {
-            u32x4 v = {};
-#pragma unroll
-            for (int e = 0; e < E / 2; ++e) {
-                if (a.add) {
-                    y[2 * e] += to_f32<BF>((uint16_t)old[e]);
-                    y[2 * e + 1] += to_f32<BF>((uint16_t)(old[e] >> 16));
-                }
-                v[e] = (uint32_t)from_f32<BF>(y[2 * e]) | (uint32_t)from_f32<BF>(y[2 * e + 1]) << 16;
-            }
-            *reinterpret_cast<u32x4_a2*>(p) = v;
+            const f32x4_a4* p = reinterpret_cast<const f32x4_a4*>(static_cast<const float*>(a.out) + at);
+            r.lo = __builtin_bit_cast(u32x4, (f32x4)p[0]);
+            r.hi = __builtin_bit_cast(u32x4, (f32x4)p[1]);
         } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (e < left) p[e] = from_f32<BF>(a.add ? to_f32<BF>(p[e]) + y[e] : y[e]);
+            r.lo = load16(static_cast<const uint16_t*>(a.out) + at);
         }
+        return r;
+    }
+    template <int E, int ACT = kAnyAct, bool WHOLE = false>
+    static __device__ __forceinline__ void finish(const Args& a, int z, int m, int n, float (&y)[E], float scale, const Row& old) {
+        static_assert(E == 1 || WHOLE);
+        const int64_t at = z * a.out_split + m * a.out_stride + n;
+        float* f = static_cast<float*>(a.out) + at;
+        uint16_t* h = static_cast<uint16_t*>(a.out) + at;
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] *= scale;
+        if constexpr (E == 1) {
+            if (a.add) y[0] += a.out_f32 ? *f : to_f32<BF>(*h);
+            if (a.out_f32) *f = y[0];
+            else *h = from_f32<BF>(y[0]);
+        } else if (a.out_f32) {
+            f32x4 lo = {y[0], y[1], y[2], y[3]}, hi = {y[4], y[5], y[6], y[7]};
+            if (a.add) lo += __builtin_bit_cast(f32x4, old.lo), hi += __builtin_bit_cast(f32x4, old.hi);
+            reinterpret_cast<f32x4_a4*>(f)[0] = lo;
+            reinterpret_cast<f32x4_a4*>(f)[1] = hi;
+        } else {
+            if (a.add)
+#pragma unroll
+                for (int e = 0; e < E; ++e) y[e] += to_f32<BF>((uint16_t)(old.lo[e / 2] >> (16 * (e & 1))));
+            store_piece<BF>(h, y);
+        }
+    }
+    template <int TN, int TM>
+    static __device__ __forceinline__ void wide(const Args& a, int z, int m0, int n0, const Sum (&acc)[TN][TM], uint16_t* lds) {
+        store_sixteens<GradSums, ULTIMA_HSAMP_ACT_NONE>(a, z, m0, n0, acc, lds);
     }
 };
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-// Four rows of sixteen columns, read by sixteen lanes (lane i: row i / 4, columns
-// 4 (i % 4) ..) and turned: lane i gets column i's four values.
-__device__ __forceinline__ uint64_t read_turned(const uint16_t* p) {
-#ifdef __HIP_DEVICE_COMPILE__
-    return __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (__attribute__((address_space(3))) s16x4*)(const_cast<uint16_t*>(p))));
-#else
-    return 0;
-#endif
-}
-
-// 256 x 256 tiles by eight waves of 128 x 64, stages of 64 k, two in LDS. Operands whose
-// rows are k stand in LDS as they do in memory, [64][256], and are turned on the way to
-// the registers; the sixteen-column blocks of row k stand at block ^ (k % 4 + 4 (k / 8 % 2)),
-// so that the eight rows of 32 bytes that a read takes at a time lie in different banks.
-template <bool BF, bool A_T>
-__global__ __launch_bounds__(512) void k_grad_tile(GradArgs a, int tiles_m, int tiles_n) {
-#ifdef __HIP_DEVICE_COMPILE__
-    constexpr int WM = 2, TM = 8, TN = 4, BM = 256, BN = 256, BK = 64, SB = (BM + BN) * BK;
-    constexpr uint32_t kOutside = 0x80000000u;
-    typedef __attribute__((address_space(3))) void* lds_ptr;
-    __shared__ __attribute__((aligned(16))) uint16_t sm[2 * SB];
-    const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, q = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int total = tiles_m * tiles_n, per = total / 8, more = total % 8;
-    const int xcd = blockIdx.x % 8, tile = xcd * per + min(xcd, more) + blockIdx.x / 8;
-    const int m0 = tile % tiles_m * BM, n0 = tile / tiles_m * BN;
-    const int k0 = blockIdx.z * a.k_split, K = min(a.k_split, a.k - k0);
-    const uint16_t* A = a.a + (A_T ? (int64_t)k0 * a.a_stride + m0 : (int64_t)m0 * a.a_stride + k0);
-    const uint16_t* B = a.b + (int64_t)k0 * a.b_stride + n0;
-    // loads: A (32 of 1 KB), then B; four of each for a wave
-    uint32_t va[4], vb[4];
-    int ka[4], kb[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int c = wave + 8 * j, k = 2 * c + (lane >> 5), turn = ((k & 3) | (k >> 1 & 4)) << 1;
-        const int col = ((lane & 31) ^ turn) * 8;
-        kb[j] = k;
-        vb[j] = n0 + col < a.b_columns ? (uint32_t)(k * (int)a.b_stride + col) * 2u : kOutside;
-        if (A_T) {
-            ka[j] = k;
-            va[j] = m0 + col < a.a_columns ? (uint32_t)(k * (int)a.a_stride + col) * 2u : kOutside;
-        } else {
-            const int r = c * 8 + (lane >> 3), p = ((lane & 7) ^ (r >> 1 & 7)) * 8;
-            ka[j] = p;
-            va[j] = m0 + r < a.rows ? (uint32_t)(r * (int)a.a_stride + p) * 2u : kOutside;
-        }
-    }
-    const int T = (K + BK - 1) / BK;
-    auto issue = [&](int t) {
-        const int left = K - t * BK;       // (below 0 past the last stage: zeros)
-        const int64_t s = t < T ? t : 0;
-        const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(A + s * (A_T ? BK * a.a_stride : BK)), 0, 0x7FFFFFFF, 0x00027000);
-        const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(B + s * BK * a.b_stride), 0, 0x7FFFFFFF, 0x00027000);
-        uint16_t* to = sm + (t & 1) * SB;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr)(to + (wave + 8 * j) * 512), 16, ka[j] < left ? va[j] : kOutside, 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr)(to + BM * BK + (wave + 8 * j) * 512), 16, kb[j] < left ? vb[j] : kOutside, 0, 0, 0);
-    };
-    auto wait = [&](auto loads) {
-        constexpr int A = decltype(loads)::value;
-        __builtin_amdgcn_s_waitcnt((A & 15) | (A >> 4) << 14 | 7 << 4);
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    };
-    struct Operands {
-        u32x4 b[TN], a[TM];
-    };
-    const int wm = wave % WM * 16 * TM, wn = wave / WM * 16 * TN;
-    const int turned = (8 * q + (i >> 2)) * 256 + (i & 3) * 4, turn = (i >> 2) | (q & 1) << 2;
-    auto turned_at = [&](const uint16_t* from, int block) {
-        const uint16_t* p = from + turned + ((block ^ turn) << 4);
-        const uint64_t lo = read_turned(p), hi = read_turned(p + 4 * 256);
-        return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
-    };
-    auto read = [&](Operands& o, int t, int step) {
-        const uint16_t* fa = sm + (t & 1) * SB;
-        const uint16_t* fb = fa + BM * BK + step * 32 * 256;
-#pragma unroll
-        for (int s = 0; s < TN; ++s) o.b[s] = turned_at(fb, wn / 16 + s);
-#pragma unroll
-        for (int u = 0; u < TM; ++u) {
-            if (A_T) o.a[u] = turned_at(fa + step * 32 * 256, wm / 16 + u);
-            else o.a[u] = *reinterpret_cast<const u32x4*>(fa + (wm + 16 * u + i) * 64 + ((step * 4 + q) ^ (i >> 1)) * 8);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    f32x4 acc[TN][TM] = {};
-    auto multiply = [&](const Operands& o) {
-#pragma unroll
-        for (int s = 0; s < TN; ++s)
-#pragma unroll
-            for (int u = 0; u < TM; ++u) acc[s][u] = mfma<BF>(o.b[s], o.a[u], acc[s][u]);
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    using std::integral_constant;
-    Operands oa, ob;
-    issue(0);
-    issue(1);
-    wait(integral_constant<int, 8>());
-    read(oa, 0, 0);
-    for (int t = 0; t < T; ++t) {
-        read(ob, t, 1);
-        multiply(oa);
-        wait(integral_constant<int, 0>());       // (all of stage t is read, stage t + 1 is there)
-        issue(t + 2);
-        read(oa, t + 1, 0);
-        multiply(ob);
-    }
-    wait(integral_constant<int, 0>());
-    store_tiles<GradStore<BF>, TN, TM>(a, blockIdx.z, m0 + wm, n0 + wn, acc, reinterpret_cast<float*>(sm) + wave * 16 * (16 * TN + 4));
-#endif
-}
 
 // d_x from its float sums over the parts of the vocabulary.
 template <bool BF>
@@ -573,22 +514,22 @@ hipError_t launch_grads(const ultima_hsamp_cross_entropy_grad_args& a, hipStream
         if (e != hipSuccess) return e;
         if (a.d_x != nullptr) {
             GradArgs g = {};
-            g.rows = a.rows, g.out_dim = (int)p.columns, g.k = width, g.k_split = p.split;
-            g.a = dz, g.a_stride = p.width, g.a_columns = width;
-            g.b = w, g.b_stride = w_stride, g.b_columns = (int)p.columns;
+            g.rows = a.rows, g.out_dim = (int)p.columns, g.groups = p.splits, g.k = width, g.k_split = p.split;
+            g.x = dz, g.x_stride = p.width;
+            g.weight = w, g.weight_stride = w_stride, g.weight_columns = (int)p.columns;
             g.out = parts, g.out_stride = p.columns, g.out_split = a.rows * p.columns, g.out_f32 = 1, g.add = k > 0;
-            const int tm = (a.rows + 255) / 256, tn = (int)((p.columns + 255) / 256);
-            hipLaunchKernelGGL((k_grad_tile<BF, false>), dim3(tm * tn, 1, p.splits), dim3(512), 0, s, g, tm, tn);
+            e = launch_wide<GradSums<BF, false>>(g, s);
+            if (e != hipSuccess) return e;
         }
         if (a.d_weight != nullptr) {
             GradArgs g = {};
-            g.rows = width, g.out_dim = a.in_dim, g.k = a.rows, g.k_split = (int)up(a.rows, 64);
-            g.a = dz, g.a_stride = p.width, g.a_columns = (int)up(width, 8);
-            g.b = x, g.b_stride = x_stride, g.b_columns = (int)p.columns;
+            g.rows = width, g.out_dim = a.in_dim, g.groups = 1, g.k = a.rows, g.k_split = (int)up(a.rows, 64);
+            g.x = dz, g.x_stride = p.width, g.x_columns = (int)up(width, 8);
+            g.weight = x, g.weight_stride = x_stride, g.weight_columns = (int)p.columns;
             g.out = static_cast<char*>(a.d_weight) + first * a.d_weight_stride * es, g.out_stride = a.d_weight_stride;
             g.out_f32 = es == 4, g.add = a.accumulate != 0, g.top_grad = BF ? nullptr : top;
-            const int tm = (width + 255) / 256, tn = (a.in_dim + 255) / 256;
-            hipLaunchKernelGGL((k_grad_tile<BF, true>), dim3(tm * tn), dim3(512), 0, s, g, tm, tn);
+            e = launch_wide<GradSums<BF, true>>(g, s);
+            if (e != hipSuccess) return e;
         }
     }
     if (a.d_x != nullptr)

@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
+#include <utility>
 
 #include "ultima_hsamp.h"
 
@@ -23,8 +24,11 @@ typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_a1 __attribute__((aligned(1)));      // 16 bytes on any element's boundary
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr uint32_t kOutside = 0x80000000u;      // a buffer offset past every buffer: reads as zeros
 
 template <bool BF>
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
@@ -34,6 +38,24 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 
 __device__ __forceinline__ u32x4 load16(const int8_t* p) { return *reinterpret_cast<const u32x4_a1*>(p); }
 __device__ __forceinline__ u32x4 load16(const uint16_t* p) { return *reinterpret_cast<const u32x4_a2*>(p); }
+
+// f(0), f(1) ..: loops whose counter is a constant.
+template <int... I, class F>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) {
+    (f(std::integral_constant<int, I>()), ...);
+}
+
+// The sum written over, in an accumulation register or (ACC false) an ordinary one
+// (k_linear_wide).
+template <bool BF, bool ACC>
+__device__ __forceinline__ void mfma_in_place(f32x4& c, u32x4 a, u32x4 b) {
+#ifdef __HIP_DEVICE_COMPILE__
+    if constexpr (ACC && BF) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    else if constexpr (ACC) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    else if constexpr (BF) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+    else asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+#endif
+}
 
 template <bool BF>
 __device__ __forceinline__ float to_f32(uint16_t h) {
@@ -70,41 +92,41 @@ __device__ __forceinline__ float cap_of(float y, float t, float c) {
     return u <= 0.5f ? low : c * __builtin_copysignf(high, t);       // (NaN: high's NaN)
 }
 
-// The eight values of row m's columns n .. n + 7, where all of them are there.
-template <class Args>
-__device__ __forceinline__ u32x4 eight(const Args& a, const void* base, int64_t at, int m, int n) {
-    if (base == nullptr || m >= a.rows || n + 8 > a.out_dim) return u32x4{0, 0, 0, 0};
-    return *reinterpret_cast<const u32x4_a2*>(static_cast<const uint16_t*>(base) + at);
+// The eight values of row m's columns n .. n + 7, where all of them are there (E = 1: none).
+template <int E, class Args>
+__device__ __forceinline__ u32x4 piece(const Args& a, const void* base, int64_t at, int m, int n) {
+    if (E == 1 || base == nullptr || m >= a.rows || n + 8 > a.out_dim) return u32x4{0, 0, 0, 0};
+    return load16(static_cast<const uint16_t*>(base) + at);
 }
-template <class Args>
-__device__ __forceinline__ u32x4 residual8(const Args& a, int g, int m, int n) {
-    return eight(a, a.residual, g * a.residual_group + m * a.residual_stride + n, m, n);
+template <int E, class Args>
+__device__ __forceinline__ u32x4 residual_piece(const Args& a, int g, int m, int n) {
+    return piece<E>(a, a.residual, g * a.residual_group + m * a.residual_stride + n, m, n);
 }
-template <class Args>
-__device__ __forceinline__ u32x4 bias8(const Args& a, int g, int n) {
-    return eight(a, a.bias, g * a.bias_group + n, 0, n);
+template <int E, class Args>
+__device__ __forceinline__ u32x4 bias_piece(const Args& a, int g, int n) {
+    return piece<E>(a, a.bias, g * a.bias_group + n, 0, n);
 }
 
-// E outputs (columns n .. n + E - 1 of row m, those there are) from their finished
-// sums; bias, residual: eight()'s values.
-template <bool BF, int E, class Args>
-__device__ __forceinline__ void finish(const Args& a, int g, int m, int n, float (&y)[E], u32x4 bias, u32x4 residual) {
-    typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
-    const int left = a.out_dim - n;
-    if (m >= a.rows || left <= 0) return;
-    auto add = [&](const void* base, int64_t at, u32x4 v) {
-        const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-        if (E == 8 && left >= 8) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) y[e] += to_f32<BF>((uint16_t)(v[e / 2 % 4] >> (16 * (e & 1))));
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (e < left) y[e] += to_f32<BF>(p[e]);
-        }
-    };
-    if (a.bias != nullptr) add(a.bias, g * a.bias_group + n, bias);
-    switch (a.act) {
+template <bool BF>
+__device__ __forceinline__ uint32_t pair(float lo, float hi) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    if (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), f16x2));
+}
+
+template <bool BF>
+__device__ __forceinline__ void store_piece(uint16_t* p, const float (&y)[8]) {
+    *reinterpret_cast<u32x4_a2*>(p) = u32x4{pair<BF>(y[0], y[1]), pair<BF>(y[2], y[3]), pair<BF>(y[4], y[5]), pair<BF>(y[6], y[7])};
+}
+
+constexpr int kAnyAct = -1;      // an activation that the arguments name
+
+template <int ACT, int E, class Args>
+__device__ __forceinline__ void activate(const Args& a, float (&y)[E]) {
+    switch (ACT == kAnyAct ? a.act : ACT) {
+        case ULTIMA_HSAMP_ACT_NONE: break;
         case ULTIMA_HSAMP_ACT_RELU:
 #pragma unroll
             for (int e = 0; e < E; ++e) y[e] = y[e] < 0.0f ? 0.0f : y[e];       // (NaN stays)
@@ -134,11 +156,32 @@ __device__ __forceinline__ void finish(const Args& a, int g, int m, int n, float
             break;
         }
     }
+}
+
+// E outputs (columns n .. n + E - 1 of row m, those there are) from their finished
+// sums; bias, residual: piece()'s values. WHOLE: all of them are there.
+template <bool BF, int E, int ACT = kAnyAct, bool WHOLE = false, class Args>
+__device__ __forceinline__ void finish(const Args& a, int g, int m, int n, float (&y)[E], u32x4 bias, u32x4 residual) {
+    const int left = a.out_dim - n;
+    if (!WHOLE && (m >= a.rows || left <= 0)) return;
+    auto add = [&](const void* base, int64_t at, u32x4 v) {
+        const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+        if (E == 8 && (WHOLE || left >= 8)) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] += to_f32<BF>((uint16_t)(v[e / 2 % 4] >> (16 * (e & 1))));
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e < left) y[e] += to_f32<BF>(p[e]);
+        }
+    };
+    if (a.bias != nullptr) add(a.bias, g * a.bias_group + n, bias);
+    activate<ACT>(a, y);
     if (a.residual != nullptr) add(a.residual, g * a.residual_group + m * a.residual_stride + n, residual);
     const int64_t at = g * a.out_group + m * a.out_stride + n;
     if (a.out_dtype == ULTIMA_HSAMP_F32) {
         float* p = static_cast<float*>(a.out) + at;
-        if (E == 8 && left >= 8) {
+        if (E == 8 && (WHOLE || left >= 8)) {
 #pragma unroll
             for (int e = 0; e < E; e += 4)
                 *reinterpret_cast<f32x4_a4*>(p + e) = f32x4{y[e], y[(e + 1) % E], y[(e + 2) % E], y[(e + 3) % E]};
@@ -150,55 +193,158 @@ __device__ __forceinline__ void finish(const Args& a, int g, int m, int n, float
         return;
     }
     uint16_t* p = static_cast<uint16_t*>(a.out) + at;
-    if (E == 8 && left >= 8) {
-        u32x4 v = {};
-#pragma unroll
-        for (int e = 0; e < E / 2; ++e) v[e] = (uint32_t)from_f32<BF>(y[2 * e]) | (uint32_t)from_f32<BF>(y[(2 * e + 1) % E]) << 16;
-        *reinterpret_cast<u32x4_a2*>(p) = v;
-    } else {
+    if constexpr (E == 8) {
+        if (WHOLE || left >= 8) return store_piece<BF>(p, y);
+    }
+    {
 #pragma unroll
         for (int e = 0; e < E; ++e)
             if (e < left) p[e] = from_f32<BF>(y[e]);
     }
 }
 
-// A wave's 16 TM rows by 16 TN columns of sums, out through its own 16 rows of
-// 16 TN + 4 floats of LDS, so that every lane finishes eight neighbouring
-// columns.
-template <class Op, int TN, int TM, class Sum, class Scalar>
-__device__ __forceinline__ void store_tiles(const typename Op::Args& a, int g, int m0, int n0, const Sum (&acc)[TN][TM], Scalar* lds) {
-    constexpr int LS = 16 * TN + 4, PR = 2 * TN;       // pieces of eight columns per row
-    constexpr int NP = TN < 2 ? 1 : TN / 2;            // pieces of one lane per 16 rows
-    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
-    const int c = lane % PR * 8, row = lane / PR;
-    const bool on = row < 16;
-    const auto columns = Op::template columns<8>(a, g, n0 + c);
-    typename Op::Row rows[NP];
-#pragma unroll
-    for (int p = 0; p < NP; ++p) rows[p] = Op::template row<8>(a, g, m0 + row + 64 / PR * p, n0 + c);
-#pragma unroll
-    for (int u = 0; u < TM; ++u) {
-        typename Op::Row next[NP] = {};
-        if (u + 1 < TM)
-#pragma unroll
-            for (int p = 0; p < NP; ++p) next[p] = Op::template row<8>(a, g, m0 + 16 * (u + 1) + row + 64 / PR * p, n0 + c);
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int s = 0; s < TN; ++s) *reinterpret_cast<Sum*>(&lds[i * LS + 16 * s + 4 * q]) = acc[s][u];
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int p = 0; p < NP; ++p) {
-            const int r = row + 64 / PR * p;
-            if (!on) continue;
-            const Sum lo = *reinterpret_cast<const Sum*>(&lds[r * LS + c]);
-            const Sum hi = *reinterpret_cast<const Sum*>(&lds[r * LS + c + 4]);
-            Scalar y[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            Op::template finish<8>(a, g, m0 + 16 * u + r, n0 + c, y, columns, rows[p]);
-        }
-#pragma unroll
-        for (int p = 0; p < NP; ++p) rows[p] = next[p];
+// Eight columns of a row from LDS: at once, or, where fewer are there, one by one.
+template <class Op, int ACT, class Sum, class Scalar, class Columns>
+__device__ __forceinline__ void finish_eight(const typename Op::Args& a, int g, int m, int n, const Scalar* lo, const Scalar* hi, const Columns& columns,
+                                             const typename Op::Row& row) {
+    if (m >= a.rows || n >= Op::end(a)) return;
+    if (n + 8 <= Op::end(a)) {
+        const Sum l = *reinterpret_cast<const Sum*>(lo), h = *reinterpret_cast<const Sum*>(hi);
+        Scalar y[8] = {l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
+        Op::template finish<8, ACT, true>(a, g, m, n, y, columns, row);
+        return;
+    }
+#pragma unroll 1
+    for (int e = 0; n + e < Op::end(a); ++e) {
+        Scalar y[1] = {e < 4 ? lo[e] : hi[e - 4]};
+        Op::template finish<1, ACT, false>(a, g, m, n + e, y, Op::template columns<1>(a, g, n + e), Op::template row<1>(a, g, m, n + e));
     }
 }
+
+// A wave's 16 TM rows by 16 TN columns of sums, out through its own 16 PU rows of LDS, so
+// that every lane finishes eight neighbouring columns. What is done with a row's sums
+// comes four rows at a time (their residuals in the air meanwhile), not unrolled over all
+// of them: code that runs once comes from beyond the instruction cache (256 x 256 tiles
+// with every activation in every unrolled copy: 12.4 us a tile of 126).
+// Row r's piece p of four floats stands at p ^ r % (4 TN): a store's 16 rows lie in
+// different banks.
+template <class Op, int ACT, int TN, int TM, int PU, class Sum, class Scalar>
+__device__ __forceinline__ void store_tiles(const typename Op::Args& a, int g, int m0, int n0, const Sum (&acc)[TN][TM], Scalar* lds) {
+    constexpr int PC = 4 * TN, PR = 2 * TN, RS = 64 / PR;      // pieces of four and of eight columns per row; rows of a step
+    constexpr int AHEAD = 4;
+    static_assert(PU % 4 == 0 || TM <= PU);
+    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+    const int c = lane % PR, row = lane / PR, n = n0 + 8 * c;
+    const auto columns = Op::template columns<8>(a, g, n);
+    typename Op::Row rows[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) rows[k] = Op::template row<8>(a, g, m0 + row + RS * k, n);
+#pragma unroll
+    for (int p = 0; p < TM; p += PU) {
+        constexpr int U = PU;
+        const int last = 16 * (TM - p < U ? TM - p : U);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (p + u < TM)
+#pragma unroll
+                for (int s = 0; s < TN; ++s)
+                    *reinterpret_cast<Sum*>(&lds[((16 * u + i) * PC + ((4 * s + q) ^ (i & (PC - 1)))) * 4]) = acc[s][p + u < TM ? p + u : 0];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int r0 = 0; r0 < last; r0 += RS * AHEAD) {
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const int r = r0 + RS * k + row, m = m0 + 16 * p + r;
+                if (r0 + RS * k >= last) break;
+                const typename Op::Row now = rows[k];
+                rows[k] = Op::template row<8>(a, g, m + RS * AHEAD, n);
+                finish_eight<Op, ACT, Sum>(a, g, m, n, &lds[(r * PC + ((2 * c) ^ (r & (PC - 1)))) * 4], &lds[(r * PC + ((2 * c + 1) ^ (r & (PC - 1)))) * 4],
+                                           columns, now);
+            }
+        }
+    }
+}
+
+// t[s] = acc[s][u] for a u that is no constant. (Without the statement behind them the
+// branches become one, with the sums in memory for it to choose from.)
+template <int TN, int TM, class Sum>
+__device__ __forceinline__ void pick(Sum (&t)[TN], const Sum (&acc)[TN][TM], int u) {
+#pragma unroll
+    for (int v = 0; v < TM; ++v)
+        if (u == v) {
+#pragma unroll
+            for (int s = 0; s < TN; ++s) {
+                Sum c = acc[s][v];
+#ifdef __HIP_DEVICE_COMPILE__
+                asm volatile("; %1" : "+v"(c) : "n"(v));
+#endif
+                t[s] = c;
+            }
+        }
+}
+
+// The same of a wave that has room for sixteen rows (16 TN x 64 bytes): one copy of the code.
+template <class Op, int ACT, int TN, int TM, class Sum>
+__device__ __forceinline__ void store_sixteens(const typename Op::Args& a, int g, int m0, int n0, const Sum (&acc)[TN][TM], uint16_t* area) {
+    using Scalar = std::remove_cvref_t<decltype(Sum{}[0])>;
+    constexpr int PC = 4 * TN, PR = 2 * TN, RS = 64 / PR, STEPS = 16 / RS;
+    Scalar* lds = reinterpret_cast<Scalar*>(area) + threadIdx.x / 64 * (256 * TN);
+    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+    const int c = lane % PR, row = lane / PR, n = n0 + 8 * c;
+    const auto columns = Op::template columns<8>(a, g, n);
+    typename Op::Row next[STEPS];
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) next[k] = Op::template row<8>(a, g, m0 + row + RS * k, n);
+#pragma unroll 1
+    for (int u = 0; u < TM; ++u) {
+        Sum t[TN];
+        pick(t, acc, u);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int s = 0; s < TN; ++s) *reinterpret_cast<Sum*>(&lds[(i * PC + ((4 * s + q) ^ i)) * 4]) = t[s];
+        __builtin_amdgcn_wave_barrier();
+        typename Op::Row now[STEPS];
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+            now[k] = next[k];
+            next[k] = Op::template row<8>(a, g, m0 + 16 * (u + 1) + RS * k + row, n);
+        }
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+            const int r = RS * k + row;
+            finish_eight<Op, ACT, Sum>(a, g, m0 + 16 * u + r, n, &lds[(r * PC + ((2 * c) ^ r)) * 4], &lds[(r * PC + ((2 * c + 1) ^ r)) * 4], columns, now[k]);
+        }
+    }
+}
+
+// The wave's part of a tile, by its activation: store(ACT).
+template <class Store>
+__device__ __forceinline__ void by_act(int act, Store store) {
+    switch (act) {
+        case ULTIMA_HSAMP_ACT_NONE: return store(std::integral_constant<int, ULTIMA_HSAMP_ACT_NONE>());
+        case ULTIMA_HSAMP_ACT_RELU: return store(std::integral_constant<int, ULTIMA_HSAMP_ACT_RELU>());
+        case ULTIMA_HSAMP_ACT_SILU: return store(std::integral_constant<int, ULTIMA_HSAMP_ACT_SILU>());
+        case ULTIMA_HSAMP_ACT_GELU: return store(std::integral_constant<int, ULTIMA_HSAMP_ACT_GELU>());
+        case ULTIMA_HSAMP_ACT_GELU_TANH: return store(std::integral_constant<int, ULTIMA_HSAMP_ACT_GELU_TANH>());
+        default: return store(std::integral_constant<int, ULTIMA_HSAMP_ACT_SOFTCAP>());
+    }
+}
+
+// What an Op has of its operands where both lie as rows of k.
+template <class Arguments, class E>
+struct RowsOfK {
+    using Args = Arguments;
+    using Element = E;
+    static constexpr bool kTurnX = false, kTurnW = false;
+    static constexpr int kWideLds = 32768, kWideWaves = 8;
+    static __device__ __forceinline__ int depth(const Args& a, int) { return a.in_dim; }
+    static __device__ __forceinline__ const E* x_at(const Args& a, int g, int m) { return static_cast<const E*>(a.x) + g * a.x_group + m * a.x_stride; }
+    static __device__ __forceinline__ const E* w_at(const Args& a, int g, int n) { return static_cast<const E*>(a.weight) + g * a.weight_group + n * a.weight_stride; }
+    static __device__ __forceinline__ int x_columns(const Args&) { return 0; }
+    static __device__ __forceinline__ int w_columns(const Args&) { return 0; }
+    static __device__ __forceinline__ int end(const Args& a) { return a.out_dim; }      // of the columns that are finished
+};
 
 // 16 WM TM rows of x by 16 WN TN rows of W by WM x WN x WK waves (WK of
 // them sharing each tile's columns): global memory to LDS without registers, ST
@@ -234,10 +380,10 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(typename Op::
     constexpr int CX = BM / 8, CR = (BM + BN) / 8;       // loads (8 rows of 128 bytes) of x, of all rows
     constexpr int CT = CR * NS;                          // per stage
     constexpr int NL = (CT + NW - 1) / NW;                     // of one wave, at most
-    constexpr uint32_t kOutside = 0x80000000u;           // a buffer offset past every buffer: reads as zeros
     typedef __attribute__((address_space(3))) void* lds_ptr;
     constexpr int SB = (BM + BN) * 64 * NS;              // half words per stage: by 128 bytes x's rows, then W's
-    constexpr int EB = WK == 1 ? NW * 16 * (16 * TN + 4) : NW * 256 * TM * TN;   // floats of the waves' sums in LDS
+    constexpr int PU = std::min(TM, ST * SB / 2 / (NW * 256 * TN));                // a wave's rows of 16 in LDS at a time
+    constexpr int EB = NW * 256 * TN * (WK == 1 ? PU : TM);                        // the waves' sums in LDS
     static_assert((ST & (ST - 1)) == 0 && (!ANY || ST == 2) && ST * SB * 2 >= EB * 4 && ST * SB * 2 <= 160 * 1024);
     __shared__ __attribute__((aligned(16))) uint16_t sm[ST * SB];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, q = lane >> 4;
@@ -273,20 +419,21 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(typename Op::
     // Each XCD starts at another eighth of the columns: rows a power of two apart
     // lie in the same memory channels, and blocks in step would all read one.
     const int t0 = (int)((int64_t)xcd * T / 8);
-    auto issue = [&](int s) {
+    auto issue_one = [&](int s, int j) {
         const int t = s + t0 < T ? s + t0 : s + t0 - T;
         const int left = s < T ? K - t * BK : 0;
         uint16_t* to = sm + (s & (ST - 1)) * SB;
+        const int c = wave + NW * j;
+        const uint32_t v = col[j] < left ? vo[j] : kOutside;
+        if (j == NL - 1 && CT % NW != 0 && !full) {
+        } else if ((NS == 1 && NW * j + NW - 1 < CX) || c % CR < CX)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(to + c * 512), 16, v, t * BK * ES, 0, 0);
+        else
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(to + c * 512), 16, v, t * BK * ES, 0, 0);
+    };
+    auto issue = [&](int s) {
 #pragma unroll
-        for (int j = 0; j < NL; ++j) {
-            const int c = wave + NW * j;
-            const uint32_t v = col[j] < left ? vo[j] : kOutside;
-            if (j == NL - 1 && CT % NW != 0 && !full) {
-            } else if ((NS == 1 && NW * j + NW - 1 < CX) || c % CR < CX)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(to + c * 512), 16, v, t * BK * ES, 0, 0);
-            else
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(to + c * 512), 16, v, t * BK * ES, 0, 0);
-        }
+        for (int j = 0; j < NL; ++j) issue_one(s, j);
     };
     u32x4 held[ANY ? NL : 1];
     auto fetch = [&](int s) {
@@ -376,7 +523,36 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(typename Op::
         for (int t = 0; t < ST; ++t) issue(t);
         wait(integral_constant<int, ST - 1>());
         // (a stage past the last reads as zeros)
-        if (WK == 1) {
+        if constexpr (WK == 1 && TM * TN >= 32) {
+            // reads and loads stand between the products, so that the matrix pipe need not wait for their issue
+            auto half = [&](const Operands& now, Operands& next, int t, int step, auto load, int tl) {
+                constexpr int G = 8, P = TN * TM / G, R = (TN + TM + G - 1) / G, L = (NL + G - 1) / G;   // groups; products, reads, loads of one
+                const uint16_t* from = sm + (t & (ST - 1)) * SB + ((step * 4 + q) ^ (i >> 1)) * 8;
+#pragma unroll
+                for (int k = 0; k < G; ++k) {
+#pragma unroll
+                    for (int r = k * R; r < (k + 1) * R; ++r) {
+                        if (r < TN) next.w[r % TN] = *reinterpret_cast<const u32x4*>(from + (BM + wn + 16 * (r % TN) + i) * 64);
+                        else if (r < TN + TM) next.x[(r - TN) % TM] = *reinterpret_cast<const u32x4*>(from + (wm + 16 * ((r - TN) % TM) + i) * 64);
+                    }
+                    if constexpr (decltype(load)::value) {
+#pragma unroll
+                        for (int j = k * L; j < (k + 1) * L; ++j)
+                            if (j < NL) issue_one(tl, j);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int e = k * P; e < (k + 1) * P; ++e) acc[e / TM][e % TM] = Op::mfma(now.w[e / TM], now.x[e % TM], acc[e / TM][e % TM]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            read(oa, 0, 0);
+            for (int t = 0; t < T; ++t) {
+                half(oa, ob, t, 1, std::false_type(), 0);
+                wait(integral_constant<int, ST - 2>());
+                half(ob, oa, t + 1, 0, std::true_type(), t + ST);
+            }
+        } else if (WK == 1) {
             read(oa, 0, 0);
             for (int t = 0; t < T; ++t) {
                 read(ob, t, 1);
@@ -403,7 +579,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(typename Op::
     }
     Scalar* sums = reinterpret_cast<Scalar*>(sm);
     if constexpr (WK == 1) {
-        Op::template tiles<TN, TM, WM, WN>(a, g, m0, n0, wave, acc, sums);
+        Op::template tiles<TN, TM, WM, WN, PU>(a, g, m0, n0, wave, acc, sums);
         return;
     }
     // rows of 4 TN pieces of four floats, row r's piece p at p ^ r % (4 TN): the 16
@@ -447,6 +623,176 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(typename Op::
         Op::template rows<BM, BN>(a, m0, n0, [&](int m, int n) {
             return sums[place(n / (16 * TN) * WM + m / (16 * TM), m % (16 * TM), n % (16 * TN) / 4) + n % 4];
         });
+    }
+#endif
+}
+
+// 256 x 256 tiles by four waves of 128 x 128, one to a SIMD, for calls of many rows: a
+// block to a CU goes from tile to tile, the next one's first two stages in the air under
+// the last one's epilogue. An operand's rows are rows of the tile (128 bytes of k a stage,
+// as above), or k (kTurnX, kTurnW: 64 rows of 256 columns a stage, which the reads turn).
+// Against eight waves of 128 x 64 a wave reads two thirds of the LDS bytes for a product,
+// which the power that the clocks go by shows more than the LDS does.
+//
+// The sums fill all 256 accumulation registers. They are named in assembly, tied to
+// themselves, since the compiler otherwise moves them about between the products; it knows
+// nothing of their latency then, hence the waits before and after the loop (drained()).
+__device__ __forceinline__ void drained() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Four rows of sixteen columns, read by sixteen lanes (lane i: row i / 4, columns
+// 4 (i % 4) ..) and turned: lane i gets column i's four values.
+__device__ __forceinline__ uint64_t read_turned(const uint16_t* p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    return __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)(const_cast<uint16_t*>(p))));
+#else
+    return 0;
+#endif
+}
+
+template <class Op, int WN>
+__global__ __launch_bounds__(128 * WN, WN / 2) void k_linear_wide(typename Op::Args a, int tiles_m, int tiles_n) {
+#ifdef __HIP_DEVICE_COMPILE__
+    using Element = typename Op::Element;
+    using Sum = typename Op::Sum;
+    constexpr int ES = sizeof(Element), PE = 16 / ES, BK = 8 * PE;      // elements of 16 bytes; of a stage
+    constexpr int NW = 2 * WN, TM = 8, TN = 16 / WN, TO = TN + TM;      // waves; sixteens a wave has of rows, of columns
+    constexpr int NL = 32 / NW;                                         // its loads of an operand's stage
+    constexpr int HALF = 256 * 64;                                      // half words of an operand's stage
+    static_assert(!(Op::kTurnX || Op::kTurnW) || ES == 2);
+    typedef __attribute__((address_space(3))) void* lds_ptr;
+    __shared__ __attribute__((aligned(16))) uint16_t sm[4 * HALF + Op::kWideLds / 2];      // two stages, what the epilogue takes
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = blockIdx.z, K = Op::depth(a, g);
+    const int total = tiles_m * tiles_n, per = total / 8, more = total % 8;
+    const int xcd = blockIdx.x % 8, from = xcd * per + min(xcd, more), here = per + (xcd < more);
+    const int S = (K + BK - 1) / BK, s0 = (int)((int64_t)xcd * S / 8);
+    const int wm = wave % 2 * 128, wn = wave / 2 * (16 * TN);
+
+    struct Place {
+        int m0, n0;
+        const Element* x;
+        const Element* w;
+        uint32_t vx[NL], vw[NL];      // byte offsets of this wave's loads
+    };
+    // the first k of a lane's part of its first load (NW a multiple of eight: of every load, where rows are the tile's)
+    static_assert(NW == 8);
+    const int in_row = ((lane & 7) ^ ((wave * 8 + (lane >> 3)) >> 1 & 7)) * PE, of_rows = wave * 2 + (lane >> 5);
+    auto place = [&](Place& p, int tile) {
+        p.m0 = tile % tiles_m * 256, p.n0 = tile / tiles_m * 256;
+        p.x = Op::x_at(a, g, p.m0), p.w = Op::w_at(a, g, p.n0);
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+            const int c = wave + NW * j;
+            const int r = c * 8 + (lane >> 3), k = c * 2 + (lane >> 5), col = ((lane & 31) ^ (((k & 3) | (k >> 1 & 4)) << 1)) * 8;
+            if (Op::kTurnX) p.vx[j] = p.m0 + col < Op::x_columns(a) ? (uint32_t)(k * (int)a.x_stride + col) * ES : kOutside;
+            else p.vx[j] = p.m0 + r < a.rows ? (uint32_t)(r * (int)a.x_stride + in_row) * ES : kOutside;
+            if (Op::kTurnW) p.vw[j] = p.n0 + col < Op::w_columns(a) ? (uint32_t)(k * (int)a.weight_stride + col) * ES : kOutside;
+            else p.vw[j] = p.n0 + r < a.out_dim ? (uint32_t)(r * (int)a.weight_stride + in_row) * ES : kOutside;
+        }
+    };
+    // a stage's loads (past the last one: zeros), load(to, l): its l-th, of each operand in turn
+    auto issue = [&](const Place& p, int s, auto with) {
+        const int t = s + s0 < S ? s + s0 : s + s0 - S, left = s < S ? K - t * BK : 0;
+        const auto rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<Element*>(p.x + (int64_t)t * BK * (Op::kTurnX ? a.x_stride : 1)), 0, 0x7FFFFFFF, 0x00027000);
+        const auto rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<Element*>(p.w + (int64_t)t * BK * (Op::kTurnW ? a.weight_stride : 1)), 0, 0x7FFFFFFF, 0x00027000);
+        with(sm + (s & 1) * 2 * HALF, [&](uint16_t* to, int l) {
+            const int j = l / 2;
+            if (l % 2 == 0)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(to + (wave + NW * j) * 512), 16,
+                                                         (Op::kTurnX ? of_rows + 2 * NW * j : in_row) < left ? p.vx[j] : kOutside, 0, 0, 0);
+            else
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(to + HALF + (wave + NW * j) * 512), 16,
+                                                         (Op::kTurnW ? of_rows + 2 * NW * j : in_row) < left ? p.vw[j] : kOutside, 0, 0, 0);
+        });
+    };
+    auto all = [](uint16_t* to, auto load) {
+#pragma unroll
+        for (int l = 0; l < 2 * NL; ++l) load(to, l);
+    };
+    auto wait = [&]() {      // all of this wave's loads are in LDS, its reads done, everybody's
+        __builtin_amdgcn_s_waitcnt(7 << 4);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    // sixteen b of an operand at a step of 32 k (64 bytes)
+    const int turned = (8 * q + (i >> 2)) * 256 + (i & 3) * 4, turn = (i >> 2) | (q & 1) << 2;
+    auto sixteen = [&](auto turn_it, const uint16_t* area, int first, int b, int step) {
+        if constexpr (decltype(turn_it)::value) {
+            const uint16_t* p = area + step * 32 * 256 + turned + ((first / 16 + b ^ turn) << 4);
+            const uint64_t lo = read_turned(p), hi = read_turned(p + 4 * 256);
+            return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+        } else {
+            return *reinterpret_cast<const u32x4*>(area + (first + 16 * b + i) * 64 + ((step * 4 + q) ^ (i >> 1)) * 8);
+        }
+    };
+    // operand o of a step: the sixteens of w, then of x
+    auto operand = [&](const uint16_t* area, int step, auto which) {
+        constexpr int o = decltype(which)::value;
+        if constexpr (o < TN) return sixteen(std::bool_constant<Op::kTurnW>(), area + HALF, wn, o, step);
+        else return sixteen(std::bool_constant<Op::kTurnX>(), area, wm, o - TN, step);
+    };
+
+    Place p;
+    int k = blockIdx.x / 8;
+    if (k >= here) return;
+    place(p, from + k);
+    issue(p, 0, all);
+    issue(p, 1, all);
+    for (;;) {
+        Sum acc[TN][TM];
+#pragma unroll
+        for (int s = 0; s < TN; ++s)
+#pragma unroll
+            for (int u = 0; u < TM; ++u) acc[s][u] = Sum{};
+        wait();
+        u32x4 oa[TO], ob[TO];
+        each_of(std::make_integer_sequence<int, TO>(), [&](auto r) { oa[r.value] = operand(sm, 0, r); });
+        // reads and loads stand between the products, four at a time (what they read and write
+        // lies apart: the compiler waits for the loads before it turns a read otherwise)
+        auto half = [&](const u32x4 (&now)[TO], u32x4 (&next)[TO], const uint16_t* __restrict area, uint16_t* __restrict to, int step, auto load) {
+            each_of(std::make_integer_sequence<int, TN * TM / 4>(), [&](auto r) {
+                constexpr int G = TN * TM / 4, R = (TO + G - 1) / G, k = decltype(r)::value;
+                each_of(std::make_integer_sequence<int, R>(), [&](auto f) {
+                    constexpr int o = k * R + decltype(f)::value;
+                    if constexpr (o < TO) next[o] = operand(area, step, std::integral_constant<int, o>());
+                });
+                if constexpr (k < 2 * NL) load(to, k);
+                __builtin_amdgcn_sched_barrier(0);
+                each_of(std::make_integer_sequence<int, 4>(), [&](auto f) {
+                    constexpr int e = 4 * k + decltype(f)::value, s = e / TM, u = e % TM;
+                    if constexpr (WN == 4) acc[s][u] = Op::mfma(now[s], now[TN + u], acc[s][u]);
+                    else Op::template mfma_in_place<(s < TN - 1)>(acc[s][u], now[s], now[TN + u]);
+                });
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+        if (WN == 2) drained();       // (the zeros are written)
+        for (int s = 0; s < S; ++s) {
+            half(oa, ob, sm + (s & 1) * 2 * HALF, nullptr, 1, [](uint16_t*, int) {});
+            wait();
+            // (past the last stage: what is there, unused)
+            issue(p, s + 2, [&](uint16_t* to, auto load) { half(ob, oa, sm + (s + 1 & 1) * 2 * HALF, to, 0, load); });
+        }
+        if (WN == 2) drained();
+        wait();
+        const int m0 = p.m0, n0 = p.n0;
+        k += gridDim.x / 8;
+        if (k < here) {
+            place(p, from + k);
+            issue(p, 0, all);
+            issue(p, 1, all);
+        }
+        Op::template wide<TN, TM>(a, g, m0 + wm, n0 + wn, acc, sm + 4 * HALF);
+        if (k >= here) return;
     }
 #endif
 }
@@ -508,6 +854,13 @@ hipError_t launch_tile(const typename Op::Args& a, hipStream_t s) {
     return hipGetLastError();
 }
 
+template <class Op>
+hipError_t launch_wide(const typename Op::Args& a, hipStream_t s) {
+    const int tm = (a.rows + 255) / 256, tn = (a.out_dim + 255) / 256;
+    hipLaunchKernelGGL((k_linear_wide<Op, Op::kWideWaves / 2>), dim3(std::min(256, (tm * tn + 7) / 8 * 8), 1, a.groups), dim3(64 * Op::kWideWaves), 0, s, a, tm, tn);
+    return hipGetLastError();
+}
+
 // 16-byte loads of whole pieces, 32-bit offsets within a tile
 template <class Op>
 bool whole_pieces(const typename Op::Args& a) {
@@ -546,7 +899,7 @@ hipError_t launch_product(const typename Op::Args& a, hipStream_t s) {
         case 5: return launch_tile<Op, false, 2, 2, 4, 2, 2, 4>(a, s);
         case 6: return launch_tile<Op, false, 2, 4, 1, 4, 2, 4>(a, s);
         case 7: return launch_tile<Op, false, 2, 4, 1, 5, 2, 2>(a, s);
-        default: return launch_tile<Op, false, 2, 4, 1, 8, 4, 2>(a, s);
+        default: return launch_wide<Op>(a, s);
     }
 }
 
