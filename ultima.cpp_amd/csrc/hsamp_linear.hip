@@ -8,13 +8,12 @@ namespace {
 template <bool BF>
 struct Linear : RowsOfK<ultima_hsamp_linear_args, uint16_t> {
     static constexpr bool kByRows = false;
+    static constexpr int kBand = 0;      // (tiles on the XCDs that they were on: the same bits)
     using Args = ultima_hsamp_linear_args;
     using Sum = f32x4;
     using Columns = u32x4;      // a piece of the bias
     using Row = u32x4;          // a piece of the residual
     static __device__ __forceinline__ Sum mfma(u32x4 w, u32x4 x, Sum c) { return hsamp::mfma<BF>(w, x, c); }
-    template <bool ACC>
-    static __device__ __forceinline__ void mfma_in_place(Sum& c, u32x4 w, u32x4 x) { hsamp::mfma_in_place<BF, ACC>(c, w, x); }
     template <int E>
     static __device__ __forceinline__ Columns columns(const Args& a, int g, int n) {
         return bias_piece<E>(a, g, n);

@@ -26,13 +26,6 @@ struct LinearI8 : RowsOfK<ultima_hsamp_linear_i8_args, int8_t> {
     static __device__ __forceinline__ Sum mfma(u32x4 w, u32x4 x, Sum c) {
         return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, x), c, 0, 0, 0);
     }
-    template <bool ACC>
-    static __device__ __forceinline__ void mfma_in_place(Sum& c, u32x4 w, u32x4 x) {
-#ifdef __HIP_DEVICE_COMPILE__
-        if constexpr (ACC) asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(w), "v"(x));
-        else asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+v"(c) : "v"(w), "v"(x));
-#endif
-    }
     template <int E>
     static __device__ __forceinline__ Columns columns(const Args& a, int g, int n) {
         Columns c = {};

@@ -59,8 +59,6 @@ struct LossRows : RowsOfK<LossArgs, uint16_t> {
     using Args = LossArgs;
     using Sum = f32x4;
     static __device__ __forceinline__ Sum mfma(u32x4 w, u32x4 x, Sum c) { return hsamp::mfma<BF>(w, x, c); }
-    template <bool ACC>
-    static __device__ __forceinline__ void mfma_in_place(Sum& c, u32x4 w, u32x4 x) { hsamp::mfma_in_place<BF, ACC>(c, w, x); }
 
     // Eight lanes to a row of a small tile.
     template <int BM, int BN, class Get>
@@ -215,8 +213,6 @@ struct LossGrad : RowsOfK<LossArgs, uint16_t> {
         bool used;
     };
     static __device__ __forceinline__ Sum mfma(u32x4 w, u32x4 x, Sum c) { return hsamp::mfma<BF>(w, x, c); }
-    template <bool ACC>
-    static __device__ __forceinline__ void mfma_in_place(Sum& c, u32x4 w, u32x4 x) { hsamp::mfma_in_place<BF, ACC>(c, w, x); }
     template <int E>
     static __device__ __forceinline__ Columns columns(const Args&, int, int) { return {}; }
     template <int E>
@@ -318,12 +314,10 @@ struct GradSums {
     using Element = uint16_t;
     using Sum = f32x4;
     static constexpr bool kTurnX = TURN_X, kTurnW = true;
-    static constexpr int kWideLds = 32768, kWideWaves = 8;
+    static constexpr int kWideLds = 32768, kBand = 8;
     static __device__ __forceinline__ Sum mfma(u32x4 w, u32x4 x, Sum c) { return hsamp::mfma<BF>(w, x, c); }
     static __device__ __forceinline__ int end(const GradArgs& a) { return a.out_dim; }
     using Args = GradArgs;
-    template <bool ACC>
-    static __device__ __forceinline__ void mfma_in_place(Sum& c, u32x4 w, u32x4 x) { hsamp::mfma_in_place<BF, ACC>(c, w, x); }
     static __device__ __forceinline__ int depth(const Args& a, int z) { return max(0, min(a.k_split, a.k - z * a.k_split)); }
     static __device__ __forceinline__ const uint16_t* x_at(const Args& a, int z, int m) {
         const int64_t k = z * a.k_split;

@@ -45,18 +45,6 @@ __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) {
     (f(std::integral_constant<int, I>()), ...);
 }
 
-// The sum written over, in an accumulation register or (ACC false) an ordinary one
-// (k_linear_wide).
-template <bool BF, bool ACC>
-__device__ __forceinline__ void mfma_in_place(f32x4& c, u32x4 a, u32x4 b) {
-#ifdef __HIP_DEVICE_COMPILE__
-    if constexpr (ACC && BF) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-    else if constexpr (ACC) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-    else if constexpr (BF) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
-    else asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
-#endif
-}
-
 template <bool BF>
 __device__ __forceinline__ float to_f32(uint16_t h) {
     return BF ? __uint_as_float((uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
@@ -337,7 +325,7 @@ struct RowsOfK {
     using Args = Arguments;
     using Element = E;
     static constexpr bool kTurnX = false, kTurnW = false;
-    static constexpr int kWideLds = 32768, kWideWaves = 8;
+    static constexpr int kWideLds = 32768, kBand = 8;
     static __device__ __forceinline__ int depth(const Args& a, int) { return a.in_dim; }
     static __device__ __forceinline__ const E* x_at(const Args& a, int g, int m) { return static_cast<const E*>(a.x) + g * a.x_group + m * a.x_stride; }
     static __device__ __forceinline__ const E* w_at(const Args& a, int g, int n) { return static_cast<const E*>(a.weight) + g * a.weight_group + n * a.weight_stride; }
@@ -627,22 +615,20 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(typename Op::
 #endif
 }
 
-// 256 x 256 tiles by four waves of 128 x 128, one to a SIMD, for calls of many rows: a
-// block to a CU goes from tile to tile, the next one's first two stages in the air under
-// the last one's epilogue. An operand's rows are rows of the tile (128 bytes of k a stage,
-// as above), or k (kTurnX, kTurnW: 64 rows of 256 columns a stage, which the reads turn).
-// Against eight waves of 128 x 64 a wave reads two thirds of the LDS bytes for a product,
-// which the power that the clocks go by shows more than the LDS does.
+// 256 x 256 tiles by eight waves of 128 x 64, for calls of many rows: a block to a CU goes
+// from tile to tile, the next one's first two stages in the air under the last one's
+// epilogue. An operand's rows are rows of the tile (128 bytes of k a stage, as above), or k
+// (kTurnX, kTurnW: 64 rows of 256 columns a stage, which the reads turn).
 //
-// The sums fill all 256 accumulation registers. They are named in assembly, tied to
-// themselves, since the compiler otherwise moves them about between the products; it knows
-// nothing of their latency then, hence the waits before and after the loop (drained()).
-__device__ __forceinline__ void drained() {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-}
-
+// Bound by the matrix pipe and by the power that it takes: a stage takes 2500 cycles where
+// the products alone take 2048, and the clock falls to 1.5 - 1.7 GHz (a library product runs
+// 2400 at 1.7: 8192 cubed 1518 TFLOP/s). 4096 rows of 151936 x 4096 with the softmax's
+// statistics 1360 TFLOP/s; 8-bit 4096 x 4096 x 16384 2330 TOP/s (a library's 2130).
+// Measured and not kept: four waves of 128 x 128 (two thirds of the LDS reads; 3070 cycles a
+// stage: nobody issues products while the only wave of a SIMD issues loads; rows of k alike),
+// stores straight from the registers (32 bytes of a row each: 2 to 9 in a hundred slower),
+// loads in one go after the wait (466 against 445 us), the products of a half stage in one
+// run behind its reads (460 against 445).
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // Four rows of sixteen columns, read by sixteen lanes (lane i: row i / 4, columns
@@ -656,13 +642,13 @@ __device__ __forceinline__ uint64_t read_turned(const uint16_t* p) {
 #endif
 }
 
-template <class Op, int WN>
-__global__ __launch_bounds__(128 * WN, WN / 2) void k_linear_wide(typename Op::Args a, int tiles_m, int tiles_n) {
+template <class Op>
+__global__ __launch_bounds__(512) void k_linear_wide(typename Op::Args a, int tiles_m, int tiles_n) {
 #ifdef __HIP_DEVICE_COMPILE__
     using Element = typename Op::Element;
     using Sum = typename Op::Sum;
     constexpr int ES = sizeof(Element), PE = 16 / ES, BK = 8 * PE;      // elements of 16 bytes; of a stage
-    constexpr int NW = 2 * WN, TM = 8, TN = 16 / WN, TO = TN + TM;      // waves; sixteens a wave has of rows, of columns
+    constexpr int NW = 8, TM = 8, TN = 4, TO = TN + TM;                 // waves; sixteens a wave has of rows, of columns
     constexpr int NL = 32 / NW;                                         // its loads of an operand's stage
     constexpr int HALF = 256 * 64;                                      // half words of an operand's stage
     static_assert(!(Op::kTurnX || Op::kTurnW) || ES == 2);
@@ -683,10 +669,14 @@ __global__ __launch_bounds__(128 * WN, WN / 2) void k_linear_wide(typename Op::A
         uint32_t vx[NL], vw[NL];      // byte offsets of this wave's loads
     };
     // the first k of a lane's part of its first load (NW a multiple of eight: of every load, where rows are the tile's)
-    static_assert(NW == 8);
     const int in_row = ((lane & 7) ^ ((wave * 8 + (lane >> 3)) >> 1 & 7)) * PE, of_rows = wave * 2 + (lane >> 5);
     auto place = [&](Place& p, int tile) {
-        p.m0 = tile % tiles_m * 256, p.n0 = tile / tiles_m * 256;
+        // Bands of kBand rows of tiles, column after column: what an XCD has in the air is eight
+        // by four of them, which read 12 operands' stages where 16 by two read 18 (4096 rows of
+        // 4096 x 16384 453 -> 416 us, 8-bit 261 -> 236). 0: all rows.
+        const int rows = Op::kBand > 0 ? Op::kBand : tiles_m, band = tile / (rows * tiles_n), first = band * rows;
+        const int high = min(rows, tiles_m - first), in = tile - first * tiles_n;
+        p.m0 = (first + in % high) * 256, p.n0 = in / high * 256;
         p.x = Op::x_at(a, g, p.m0), p.w = Op::w_at(a, g, p.n0);
 #pragma unroll
         for (int j = 0; j < NL; ++j) {
@@ -769,20 +759,17 @@ __global__ __launch_bounds__(128 * WN, WN / 2) void k_linear_wide(typename Op::A
                 __builtin_amdgcn_sched_barrier(0);
                 each_of(std::make_integer_sequence<int, 4>(), [&](auto f) {
                     constexpr int e = 4 * k + decltype(f)::value, s = e / TM, u = e % TM;
-                    if constexpr (WN == 4) acc[s][u] = Op::mfma(now[s], now[TN + u], acc[s][u]);
-                    else Op::template mfma_in_place<(s < TN - 1)>(acc[s][u], now[s], now[TN + u]);
+                    acc[s][u] = Op::mfma(now[s], now[TN + u], acc[s][u]);
                 });
                 __builtin_amdgcn_sched_barrier(0);
             });
         };
-        if (WN == 2) drained();       // (the zeros are written)
         for (int s = 0; s < S; ++s) {
             half(oa, ob, sm + (s & 1) * 2 * HALF, nullptr, 1, [](uint16_t*, int) {});
             wait();
             // (past the last stage: what is there, unused)
             issue(p, s + 2, [&](uint16_t* to, auto load) { half(ob, oa, sm + (s + 1 & 1) * 2 * HALF, to, 0, load); });
         }
-        if (WN == 2) drained();
         wait();
         const int m0 = p.m0, n0 = p.n0;
         k += gridDim.x / 8;
@@ -857,7 +844,7 @@ hipError_t launch_tile(const typename Op::Args& a, hipStream_t s) {
 template <class Op>
 hipError_t launch_wide(const typename Op::Args& a, hipStream_t s) {
     const int tm = (a.rows + 255) / 256, tn = (a.out_dim + 255) / 256;
-    hipLaunchKernelGGL((k_linear_wide<Op, Op::kWideWaves / 2>), dim3(std::min(256, (tm * tn + 7) / 8 * 8), 1, a.groups), dim3(64 * Op::kWideWaves), 0, s, a, tm, tn);
+    hipLaunchKernelGGL((k_linear_wide<Op>), dim3(std::min(256, (tm * tn + 7) / 8 * 8), 1, a.groups), dim3(512), 0, s, a, tm, tn);
     return hipGetLastError();
 }
 
