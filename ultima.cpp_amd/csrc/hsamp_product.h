@@ -511,10 +511,10 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(typename Op::
         for (int t = 0; t < ST; ++t) issue(t);
         wait(integral_constant<int, ST - 1>());
         // (a stage past the last reads as zeros)
-        if constexpr (WK == 1 && TM * TN >= 32) {
+        if constexpr (WK == 1) {
             // reads and loads stand between the products, so that the matrix pipe need not wait for their issue
             auto half = [&](const Operands& now, Operands& next, int t, int step, auto load, int tl) {
-                constexpr int G = 8, P = TN * TM / G, R = (TN + TM + G - 1) / G, L = (NL + G - 1) / G;   // groups; products, reads, loads of one
+                constexpr int P = 2, G = TN * TM / P, R = (TN + TM + G - 1) / G, L = (NL + G - 1) / G;   // groups; products, reads, loads of one
                 const uint16_t* from = sm + (t & (ST - 1)) * SB + ((step * 4 + q) ^ (i >> 1)) * 8;
 #pragma unroll
                 for (int k = 0; k < G; ++k) {
@@ -539,16 +539,6 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(typename Op::
                 half(oa, ob, t, 1, std::false_type(), 0);
                 wait(integral_constant<int, ST - 2>());
                 half(ob, oa, t + 1, 0, std::true_type(), t + ST);
-            }
-        } else if (WK == 1) {
-            read(oa, 0, 0);
-            for (int t = 0; t < T; ++t) {
-                read(ob, t, 1);
-                multiply(oa);
-                wait(integral_constant<int, ST - 2>());
-                issue(t + ST);
-                read(oa, t + 1, 0);
-                multiply(ob);
             }
         } else {
             read(oa, 0, wk);
