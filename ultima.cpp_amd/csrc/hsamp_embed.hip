@@ -17,17 +17,20 @@ struct Eight {
 
 // Eight values at any element's address; those past the row's end are not there.
 template <class T>
-__device__ __forceinline__ void load(const T* p, int left, float (&v)[N]) {
+__device__ __forceinline__ typename Eight<T>::type raw(const T* p, int left) {
     typedef typename Eight<T>::type V;
     struct __attribute__((packed, aligned(sizeof(T)))) Any { V v; };
-    if (left >= N) {
-        const V t = reinterpret_cast<const Any*>(p)->v;
+    if (left >= N) return reinterpret_cast<const Any*>(p)->v;
+    V t;
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = (float)t[e];
-    } else {
+    for (int e = 0; e < N; ++e) t[e] = e < left ? p[e] : (T)0.0f;
+    return t;
+}
+template <class T>
+__device__ __forceinline__ void load(const T* p, int left, float (&v)[N]) {
+    const auto t = raw(p, left);
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = e < left ? (float)p[e] : 0.0f;
-    }
+    for (int e = 0; e < N; ++e) v[e] = (float)t[e];
 }
 template <class T>
 __device__ __forceinline__ void store(T* p, int left, const float (&v)[N]) {
@@ -63,14 +66,14 @@ __global__ __launch_bounds__(256) void k_embed(ultima_hsamp_embed_args a, int sl
 }
 
 // ---- The gradient -------------------------------------------------------------------
-// Positions sorted by id, each id's in order, then each id's rows added up: no atomics
-// on sums, so that their order is the tokens' alone.
+// Positions sorted by id, each id's in an order that goes by the tokens alone, then each
+// id's rows added up in it, without atomics.
 //
 // The sort in one launch: a block owns a range of ids and looks at all of the tokens
 // twice. What lies below its range is where its positions begin, so that no block waits
 // for another; each of its waves counts and later places a run of consecutive tokens,
-// wave after wave, 64 after 64, lane after lane. Its reads are the tokens (4 bytes each)
-// once for each block, out of the caches.
+// wave after wave, 256 after 256, of these every fourth together. Its reads are the tokens
+// (4 bytes each) once for each block, out of the caches, 2048 of a wave in the air.
 struct Sorted {
     int32_t* start;      // [vocab + 1] where an id's positions begin
     int32_t* order;      // [tokens] the positions
@@ -80,20 +83,49 @@ constexpr int kWaves = 16, kRange = 1024;      // waves of a block; ids of one, 
 int ranges_of(int vocab) { return std::max((vocab + kRange - 1) / kRange, std::min(256, (vocab + 63) / 64)); }
 
 __global__ __launch_bounds__(64 * kWaves) void k_sort_ids(const int32_t* ids, int tokens, int vocab, int range, Sorted out) {
+    constexpr int U = 8;
+    struct Four { int v[4]; };              // (at any token)
     __shared__ int at[kWaves * kRange];     // a wave's tokens of an id, then where its next one goes
     __shared__ int below[kWaves], sums[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int lo = blockIdx.x * range, hi = min(vocab, lo + range);
+    const int64_t per = ((int64_t)tokens + 256 * kWaves - 1) / (256 * kWaves) * 256;   // of one wave
+    const int first = (int)min((int64_t)tokens, wave * per), last = (int)min((int64_t)tokens, (wave + 1) * per);
+    auto each = [&](auto use) {      // use(k, id): every token k of the wave, 64 at a time; -1 where there is none
+        for (int k = first; k < last; k += 256 * U) {
+            int id[U][4];
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const int at = k + 256 * j + 4 * lane;
+                if (at + 4 <= last) {
+                    const Four v = *reinterpret_cast<const Four*>(ids + at);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) id[j][e] = v.v[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) id[j][e] = -1;
+                    if (at < last) {
+#pragma unroll
+                        for (int e = 0; e < 3; ++e)
+                            if (at + e < last) id[j][e] = ids[at + e];
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                if (k + 256 * j >= last) break;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) use(k + 256 * j + 4 * lane + e, id[j][e]);
+            }
+        }
+    };
     for (int k = tid; k < kWaves * kRange; k += 64 * kWaves) at[k] = 0;
     __syncthreads();
-    const int64_t per = ((int64_t)tokens + 64 * kWaves - 1) / (64 * kWaves) * 64;      // of one wave
-    const int first = (int)min((int64_t)tokens, wave * per), last = (int)min((int64_t)tokens, (wave + 1) * per);
     int lower = 0;
-    for (int k = first; k < last; k += 64) {
-        const int id = k + lane < last ? ids[k + lane] : -1;
+    each([&](int, int id) {
         lower += id >= 0 && id < lo;
         if (id >= lo && id < hi) atomicAdd(&at[wave * kRange + id - lo], 1);
-    }
+    });
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) lower += __shfl_xor(lower, d);
     if (lane == 0) below[wave] = lower;
@@ -124,79 +156,38 @@ __global__ __launch_bounds__(64 * kWaves) void k_sort_ids(const int32_t* ids, in
         from += c;
     }
     __syncthreads();
-    for (int k = first; k < last; k += 64) {
-        const int id = k + lane < last ? ids[k + lane] : -1;
-        uint64_t todo = __ballot(id >= lo && id < hi);
+    each([&](int k, int id) {
+        const bool mine = id >= lo && id < hi;
+        uint64_t todo = __ballot(mine);
+        if (todo == 0) return;
+        int* next = &at[wave * kRange + (mine ? id - lo : 0)];
+        const int begin = *next;
+        int rank = 0, more = 0;      // of this lane's id: lanes before it, lanes in all
         while (todo != 0) {          // once for each id there is among the 64
-            const int leader = __builtin_ctzll(todo), which = __builtin_amdgcn_readlane(id, leader);
+            const int which = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
             const uint64_t same = __ballot(id == which);
-            int next = 0;
-            if (lane == leader) next = atomicAdd(&at[wave * kRange + which - lo], __popcll(same));
-            next = __builtin_amdgcn_readlane(next, leader);
-            if (id == which) out.order[next + __popcll(same & ((1ull << lane) - 1))] = k + lane;
+            if (id == which) rank = __popcll(same & ((1ull << lane) - 1)), more = __popcll(same);
             todo &= ~same;
         }
-    }
+        if (mine) out.order[begin + rank] = k;
+        if (mine && rank == more - 1) *next = begin + more;
+    });
 }
 
-// Chunks of `chunk` sorted positions that hold a single id are added up first, a block
-// per chunk and 2048 columns, so that a frequent id's rows are read by many blocks.
-int chunk_of(int tokens) { return std::max(64, (tokens + 1023) / 1024); }
+// The sums. The sorted positions are cut into chunks, a block per chunk and 2048 columns,
+// so that a frequent id's rows are read by many blocks: an id whose positions lie in one
+// chunk is finished there; the sums of one that crosses a border are left in float, at
+// most two to a chunk (of the id that came in, of the one that goes on), for the launch
+// after it.
+// A chunk has 32 positions, or 8 where that few blocks would leave most CUs idle.
+constexpr int kChunk = 32, kEmpty = 16;      // positions of a chunk, at most; ids of a block of the others
+int chunk_of(int tokens) { return tokens <= 8192 ? 8 : kChunk; }
 
-template <class T>
-__global__ __launch_bounds__(256) void k_embed_chunks(ultima_hsamp_embed_grad_args a, Sorted s, float* partial, int chunk, int slices) {
-    const int c = (blockIdx.x % slices * 256 + threadIdx.x) * N, left = a.width - c;
-    const int64_t at = blockIdx.x / slices, first = at * chunk;
-    if (first + chunk > s.start[a.vocab]) return;
-    if (a.ids[s.order[first]] != a.ids[s.order[first + chunk - 1]] || left <= 0) return;
-    float sum[N] = {};
-    for (int64_t k = first; k < first + chunk; ++k) {
-        float v[N];
-        load(static_cast<const T*>(a.d_out) + s.order[k] * a.d_out_stride + c, left, v);
-#pragma unroll
-        for (int e = 0; e < N; ++e) sum[e] += v[e];
-    }
-    const int64_t padded = (a.width + N - 1) / N * N;
-    store(partial + at * padded + c, N, sum);
-}
+__device__ __forceinline__ int64_t padded(int width) { return (width + N - 1) / N * N; }
 
-// A wave per id and 512 columns: the rows before its first whole chunk, the chunks, the
-// rows behind them.
-template <class T, class O>
-__global__ __launch_bounds__(256) void k_embed_rows(ultima_hsamp_embed_grad_args a, Sorted s, const float* partial, int chunk, int slices) {
-    const int64_t item = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    const int64_t id = item / slices;
-    const int c = (int)(item % slices * 64 + threadIdx.x % 64) * N, left = a.width - c;
-    if (id >= a.vocab || left <= 0) return;
-    const int first = s.start[id], last = s.start[id + 1];
+template <class O>
+__device__ __forceinline__ void finish(const ultima_hsamp_embed_grad_args& a, int64_t id, int c, int left, float (&sum)[N]) {
     O* out = static_cast<O*>(a.out) + id * a.out_stride + c;
-    float sum[N] = {};
-    if (first == last) {
-        if (!a.accumulate) store(out, left, sum);
-        return;
-    }
-    auto add = [&](int from, int to) {
-        for (int k = from; k < to; ++k) {
-            float v[N];
-            load(static_cast<const T*>(a.d_out) + s.order[k] * a.d_out_stride + c, left, v);
-#pragma unroll
-            for (int e = 0; e < N; ++e) sum[e] += v[e];
-        }
-    };
-    const int whole = (first + chunk - 1) / chunk, end = last / chunk;
-    if (whole < end) {
-        const int64_t padded = (a.width + N - 1) / N * N;
-        add(first, whole * chunk);
-        for (int64_t k = whole; k < end; ++k) {
-            float v[N];
-            load(partial + k * padded + c, N, v);
-#pragma unroll
-            for (int e = 0; e < N; ++e) sum[e] += v[e];
-        }
-        add(end * chunk, last);
-    } else {
-        add(first, last);
-    }
 #pragma unroll
     for (int e = 0; e < N; ++e) sum[e] *= a.scale;
     if (a.accumulate) {
@@ -208,6 +199,92 @@ __global__ __launch_bounds__(256) void k_embed_rows(ultima_hsamp_embed_grad_args
     store(out, left, sum);
 }
 
+template <class T, class O>
+__global__ __launch_bounds__(256) void k_embed_sums(ultima_hsamp_embed_grad_args a, Sorted s, float* partial, int chunk, int slices) {
+    constexpr int U = 8;
+    const int c = (blockIdx.x % slices * 256 + threadIdx.x) * N, left = a.width - c;
+    const int at = blockIdx.x / slices, first = at * chunk, total = s.start[a.vocab], last = min(first + chunk, total);
+    __shared__ int position[kChunk + U], ids[kChunk + 2];      // of the chunk; with the ones before and behind it
+    if (threadIdx.x < kChunk + U) {
+        const int k = first + threadIdx.x;
+        position[threadIdx.x] = k < last ? s.order[k] : 0;
+    }
+    if ((int)threadIdx.x < chunk + 2) {
+        const int k = first + (int)threadIdx.x - 1;
+        ids[threadIdx.x] = k >= 0 && k < total ? a.ids[s.order[k]] : -1;
+    }
+    __syncthreads();
+    if (first >= last || left <= 0) return;
+    float sum[N] = {};
+    for (int k0 = 0; k0 < last - first; k0 += U) {
+        typename Eight<T>::type v[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j] = raw(static_cast<const T*>(a.d_out) + position[k0 + j] * a.d_out_stride + c, left);
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int k = k0 + j, id = ids[k + 1];
+            if (k >= last - first) break;
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum[e] += (float)v[j][e];
+            const bool ends = ids[k + 2] != id || first + k + 1 >= total, border = k + 1 == chunk;
+            if (!ends && !border) continue;
+            const bool came_in = ids[0] == id;
+            if (ends && !came_in) finish<O>(a, id, c, left, sum);
+            else store(partial + (2 * (int64_t)at + !came_in) * padded(a.width) + c, N, sum);
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum[e] = 0.0f;
+        }
+    }
+}
+
+// The ids that cross borders, by the chunk that they end in: the sum of the chunk that they
+// began in, then of the ones they go through, eight in the air at a time. The blocks behind
+// these write the rows of ids without tokens, a wave to a row, and hide them.
+template <class O>
+__global__ __launch_bounds__(256) void k_embed_join(ultima_hsamp_embed_grad_args a, Sorted s, const float* partial, int chunk, int joins, int slices) {
+    constexpr int U = 8;
+    if ((int)blockIdx.x >= joins) {
+        struct __attribute__((packed, aligned(sizeof(O)))) Sixteen { uint32_t v[4]; };
+        constexpr int E = 16 / sizeof(O);
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int64_t id0 = (int64_t)(blockIdx.x - joins) * kEmpty;
+        const int begins = lane <= kEmpty && id0 + lane <= a.vocab ? s.start[id0 + lane] : 0, ends = __shfl_down(begins, 1);
+        const uint64_t empty = __ballot(lane < kEmpty && id0 + lane < a.vocab && begins == ends);
+#pragma unroll
+        for (int k = 0; k < kEmpty / 4; ++k) {
+            if ((empty >> (4 * k + wave) & 1) == 0) continue;
+            O* row = static_cast<O*>(a.out) + (id0 + 4 * k + wave) * a.out_stride;
+            for (int c = lane * E; c < a.width; c += 64 * E) {
+                if (c + E <= a.width) {
+                    *reinterpret_cast<Sixteen*>(row + c) = Sixteen{};
+                } else {
+                    for (int e = c; e < a.width; ++e) row[e] = (O)0.0f;
+                }
+            }
+        }
+        return;
+    }
+    const int c = (blockIdx.x % slices * 256 + threadIdx.x) * N, left = a.width - c;
+    const int at = blockIdx.x / slices + 1, first = at * chunk;
+    if (first >= s.start[a.vocab]) return;
+    const int id = a.ids[s.order[first]], begin = s.start[id], end = s.start[id + 1];
+    if (begin >= first || end > first + chunk || left <= 0) return;
+    const int64_t row = padded(a.width);
+    float sum[N];
+    load(partial + (2 * (int64_t)(begin / chunk) + 1) * row + c, N, sum);
+    for (int k0 = begin / chunk + 1; k0 <= at; k0 += U) {
+        float v[U][N];
+#pragma unroll
+        for (int j = 0; j < U; ++j) load(partial + 2 * (int64_t)min(k0 + j, at) * row + c, N, v[j]);
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            if (k0 + j <= at)
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum[e] += v[j][e];
+    }
+    finish<O>(a, id, c, left, sum);
+}
+
 int64_t up16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 
 template <class T, class O>
@@ -215,13 +292,14 @@ hipError_t launch_grad(const ultima_hsamp_embed_grad_args& a, hipStream_t s) {
     char* work = static_cast<char*>(a.work);
     const Sorted sorted = {reinterpret_cast<int32_t*>(work), reinterpret_cast<int32_t*>(work + up16(4 * ((int64_t)a.vocab + 1)))};
     float* partial = reinterpret_cast<float*>(work + up16(4 * ((int64_t)a.vocab + 1)) + up16(4 * (int64_t)a.tokens));
-    const int blocks = ranges_of(a.vocab), range = (a.vocab + blocks - 1) / blocks, chunk = chunk_of(a.tokens);
+    const int blocks = ranges_of(a.vocab), range = (a.vocab + blocks - 1) / blocks;
     hipLaunchKernelGGL(k_sort_ids, dim3((a.vocab + range - 1) / range), dim3(64 * kWaves), 0, s, a.ids, a.tokens, a.vocab, range, sorted);
-    const int wide = (a.width + 2047) / 2048, slices = (a.width + 511) / 512;
-    if (a.tokens >= chunk)
-        hipLaunchKernelGGL(k_embed_chunks<T>, dim3(a.tokens / chunk * wide), dim3(256), 0, s, a, sorted, partial, chunk, wide);
-    hipLaunchKernelGGL((k_embed_rows<T, O>), dim3((uint32_t)(((int64_t)a.vocab * slices + 3) / 4)), dim3(256), 0, s, a, sorted,
-                       (const float*)partial, chunk, slices);
+    const int chunk = chunk_of(a.tokens), chunks = (a.tokens + chunk - 1) / chunk, slices = (a.width + 256 * N - 1) / (256 * N);
+    const int empty = a.accumulate ? 0 : (a.vocab + kEmpty - 1) / kEmpty;
+    const int joins = (chunks - 1) * slices;
+    hipLaunchKernelGGL((k_embed_sums<T, O>), dim3(chunks * slices), dim3(256), 0, s, a, sorted, partial, chunk, slices);
+    if (joins + empty > 0)
+        hipLaunchKernelGGL((k_embed_join<O>), dim3(joins + empty), dim3(256), 0, s, a, sorted, (const float*)partial, chunk, joins, slices);
     return hipGetLastError();
 }
 
@@ -270,8 +348,8 @@ extern "C" int ultima_hsamp_embed(const ultima_hsamp_embed_args* a, void* hip_st
 extern "C" int64_t ultima_hsamp_embed_grad_work_bytes(int32_t tokens, int32_t width, int32_t vocab) {
     using namespace hsamp;
     if (tokens < 1 || width < 1 || vocab < 1 || vocab > ULTIMA_HSAMP_MAX_VOCAB) return -1;
-    const int64_t padded = ((int64_t)width + N - 1) / N * N;
-    return up16(4 * ((int64_t)vocab + 1)) + up16(4 * (int64_t)tokens) + tokens / chunk_of(tokens) * padded * 4;
+    const int64_t row = ((int64_t)width + N - 1) / N * N;
+    return up16(4 * ((int64_t)vocab + 1)) + up16(4 * (int64_t)tokens) + ((int64_t)tokens + chunk_of(tokens) - 1) / chunk_of(tokens) * 2 * row * 4;
 }
 
 extern "C" int ultima_hsamp_embed_grad(const ultima_hsamp_embed_grad_args* a, void* hip_stream) {
