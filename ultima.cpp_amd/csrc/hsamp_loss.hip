@@ -54,7 +54,7 @@ __device__ __forceinline__ void join(float& top, float& sum, float top2, float s
 
 template <bool BF>
 struct LossRows : RowsOfK<LossArgs, uint16_t> {
-    static constexpr int kWideLds = 8192;
+    static constexpr int kWideLds = 2048;
     static constexpr bool kByRows = true;
     using Args = LossArgs;
     using Sum = f32x4;
@@ -173,10 +173,20 @@ __global__ __launch_bounds__(1024) void k_loss_join(const float2* partial, const
     __shared__ float2 sm[1024];
     const int r = threadIdx.x & ((1 << log_rows) - 1), m = (blockIdx.x << log_rows) + r;
     float top = -__builtin_inff(), sum = 0.0f;
+    const int step = 1024 >> log_rows;
     if (m < rows)
-        for (int t = threadIdx.x >> log_rows; t < tiles; t += 1024 >> log_rows) {
-            const float2 p = partial[(int64_t)t * rows + m];
-            join(top, sum, p.x, p.y);
+        for (int t = threadIdx.x >> log_rows; t < tiles; t += 8 * step) {      // eight in the air
+            float2 p[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) p[k] = t + k * step < tiles ? partial[(int64_t)(t + k * step) * rows + m] : float2{-__builtin_inff(), 0.0f};
+            float most = top;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) most = fmaxf(most, p[k].x);
+            const float ref = most == -__builtin_inff() ? 0.0f : most;
+            sum *= exp_of(top - ref);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum += p[k].y * exp_of(p[k].x - ref);
+            top = most;
         }
     sm[threadIdx.x] = float2{top, sum};
     __syncthreads();
@@ -286,10 +296,15 @@ __global__ __launch_bounds__(256) void k_lay_out(const uint16_t* from, int64_t s
     const int64_t r = k / pieces;
     const int c = (int)(k % pieces) * 8;
     if (r >= rows) return;
+    const uint16_t* p = from + r * stride + c;
     u32x4 v = {};
+    if (c + 8 <= columns) {
+        v = load16(p);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (c + e < columns) v[e / 2] |= (uint32_t)from[r * stride + c + e] << (16 * (e & 1));
+        for (int e = 0; e < 8; ++e)
+            if (c + e < columns) v[e / 2] |= (uint32_t)p[e] << (16 * (e & 1));
+    }
     *reinterpret_cast<u32x4*>(to + k * 8) = v;
 }
 
@@ -314,7 +329,7 @@ struct GradSums {
     using Element = uint16_t;
     using Sum = f32x4;
     static constexpr bool kTurnX = TURN_X, kTurnW = true;
-    static constexpr int kWideLds = 32768, kBand = 8;
+    static constexpr int kWideLds = 8192, kBand = 8;
     static __device__ __forceinline__ Sum mfma(u32x4 w, u32x4 x, Sum c) { return hsamp::mfma<BF>(w, x, c); }
     static __device__ __forceinline__ int end(const GradArgs& a) { return a.out_dim; }
     using Args = GradArgs;
@@ -380,46 +395,62 @@ struct GradSums {
     }
 };
 
-// d_x from its float sums over the parts of the vocabulary.
+// d_x from its float sums over the parts of the vocabulary, four columns a thread.
 template <bool BF>
 __global__ __launch_bounds__(256) void k_grad_join(const float* parts, int n, int64_t part, int64_t stride, int rows, int columns,
                                                    const float* top_grad, void* out, int64_t out_stride, int out_f32) {
-    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t k = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     const int64_t m = k / stride;
     const int c = (int)(k % stride);
-    if (m >= rows || c >= columns) return;
-    float sum = parts[k];
-    for (int p = 1; p < n; ++p) sum += parts[p * part + k];
+    if (m >= rows) return;
+    f32x4 sum = *reinterpret_cast<const f32x4*>(parts + k);
+#pragma unroll 8
+    for (int p = 1; p < n; ++p) sum += *reinterpret_cast<const f32x4*>(parts + p * part + k);
     if (!BF) {
         const float top = *top_grad;
         sum *= top > 0.0f ? top * 0x1p-15f : 1.0f;
     }
-    if (out_f32) static_cast<float*>(out)[m * out_stride + c] = sum;
-    else static_cast<uint16_t*>(out)[m * out_stride + c] = from_f32<BF>(sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (c + e >= columns) continue;
+        if (out_f32) static_cast<float*>(out)[m * out_stride + c + e] = sum[e];
+        else static_cast<uint16_t*>(out)[m * out_stride + c + e] = from_f32<BF>(sum[e]);
+    }
 }
 
 int64_t up(int64_t n, int64_t step) { return (n + step - 1) / step * step; }
 
 // How a gradient call cuts the vocabulary. A piece's dz and its part of the weight are
-// up to 128 and 256 MB (2^26, 2^27 elements), so that they stay in the caches; pieces are
-// as long as each other. d_x's tiles are made by as many parts of the piece as fill the
-// CUs, at least 512 ids each.
+// up to 128 and 256 MB (2^26, 2^27 elements), so that they stay in the caches. d_x's tiles
+// are made by as many parts of the piece as fill the CUs, at least 512 ids each.
+//
+// Tiles of 128 x 128, two blocks to a CU, where 256 x 256 ones would be mostly empty or too
+// few. Measured, us, 256 / 128, d_x alone: 1 row of 4096 176 / 148, 129 257 / 261, 301 of
+// 1000 139 / 138, 512 of 1000 170 / 185, 800 of 256 348 / 303, 2048 of 256 707 / 725;
+// d_weight alone: 301 rows of 4096 445 / 390, 512 548 / 514, 800 735 / 740, 2048
+// 1601 / 1745, 4096 of 1000 (200 tiles) 985 / 1110, 2048 of 256 (98 tiles) 674 / 606.
 struct Pieces {
     int64_t width, columns;         // ids of a piece; in_dim in steps of eight
-    int count, splits, split;       // pieces; parts of a piece for d_x, ids of one
+    int count, splits;              // pieces; parts of each for d_x
+    bool small_x;
 };
 Pieces pieces_of(int64_t rows, int64_t in_dim, int64_t vocab) {
+    const auto tiles = [&](int64_t side) { return ((rows + side - 1) / side) * ((in_dim + side - 1) / side); };
     Pieces p;
     p.columns = up(in_dim, 8);
     const int64_t most = std::max<int64_t>(256, std::min({(int64_t)1 << 20, ((int64_t)1 << 26) / rows, ((int64_t)1 << 27) / p.columns}) / 256 * 256);
+    // whole rounds of tiles over the 256 CUs (10 pieces of 60 tiles 3.75 rounds each; 9 of 64 and a rest 38 in all)
+    const int64_t round = (256 + (rows + 255) / 256 - 1) / ((rows + 255) / 256) * 256;
     p.count = (int)((vocab + most - 1) / most);
-    p.width = up((vocab + p.count - 1) / p.count, 256);
+    p.width = most >= round ? std::min(most / round * round, up(vocab, 256)) : up((vocab + p.count - 1) / p.count, 256);
     p.count = (int)((vocab + p.width - 1) / p.width);
-    const int64_t tiles = ((rows + 255) / 256) * ((in_dim + 255) / 256);
-    const int64_t splits = std::max<int64_t>(1, std::min(256 / tiles, p.width / 512));
-    p.split = (int)up((p.width + splits - 1) / splits, 64);
-    p.splits = (int)((p.width + p.split - 1) / p.split);
+    p.small_x = rows <= 256 || tiles(256) <= 4;
+    const int64_t splits = std::max<int64_t>(1, std::min(p.small_x ? 512 / tiles(128) : 256 / tiles(256), p.width / 512));
+    p.splits = (int)splits;
     return p;
+}
+bool small_weight(int64_t width, int64_t rows, int64_t in_dim) {
+    return rows <= 640 || ((width + 255) / 256) * ((in_dim + 255) / 256) < 128;
 }
 struct GradWork {
     int64_t dz, parts, x, weight, bytes;      // where they begin; 16 bytes for the largest gradient first
@@ -508,11 +539,11 @@ hipError_t launch_grads(const ultima_hsamp_cross_entropy_grad_args& a, hipStream
         if (e != hipSuccess) return e;
         if (a.d_x != nullptr) {
             GradArgs g = {};
-            g.rows = a.rows, g.out_dim = (int)p.columns, g.groups = p.splits, g.k = width, g.k_split = p.split;
+            g.rows = a.rows, g.out_dim = (int)p.columns, g.groups = p.splits, g.k = width, g.k_split = (int)up((width + p.splits - 1) / p.splits, 64);
             g.x = dz, g.x_stride = p.width;
             g.weight = w, g.weight_stride = w_stride, g.weight_columns = (int)p.columns;
             g.out = parts, g.out_stride = p.columns, g.out_split = a.rows * p.columns, g.out_f32 = 1, g.add = k > 0;
-            e = launch_wide<GradSums<BF, false>>(g, s);
+            e = p.small_x ? launch_wide<GradSums<BF, false>, 4, 2>(g, s) : launch_wide<GradSums<BF, false>>(g, s);
             if (e != hipSuccess) return e;
         }
         if (a.d_weight != nullptr) {
@@ -522,12 +553,12 @@ hipError_t launch_grads(const ultima_hsamp_cross_entropy_grad_args& a, hipStream
             g.weight = x, g.weight_stride = x_stride, g.weight_columns = (int)p.columns;
             g.out = static_cast<char*>(a.d_weight) + first * a.d_weight_stride * es, g.out_stride = a.d_weight_stride;
             g.out_f32 = es == 4, g.add = a.accumulate != 0, g.top_grad = BF ? nullptr : top;
-            e = launch_wide<GradSums<BF, true>>(g, s);
+            e = small_weight(width, a.rows, a.in_dim) ? launch_wide<GradSums<BF, true>, 4, 2>(g, s) : launch_wide<GradSums<BF, true>>(g, s);
             if (e != hipSuccess) return e;
         }
     }
     if (a.d_x != nullptr)
-        hipLaunchKernelGGL(k_grad_join<BF>, dim3((uint32_t)((a.rows * p.columns + 255) / 256)), dim3(256), 0, s, (const float*)parts, p.splits,
+        hipLaunchKernelGGL(k_grad_join<BF>, dim3((uint32_t)((a.rows * p.columns + 1023) / 1024)), dim3(256), 0, s, (const float*)parts, p.splits,
                            a.rows * p.columns, p.columns, a.rows, a.in_dim, (const float*)top, a.d_x, a.d_x_stride,
                            (int)(a.d_x_dtype == ULTIMA_HSAMP_F32));
     return hipGetLastError();

@@ -290,7 +290,7 @@ __device__ __forceinline__ void store_sixteens(const typename Op::Args& a, int g
         pick(t, acc, u);
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int s = 0; s < TN; ++s) *reinterpret_cast<Sum*>(&lds[(i * PC + ((4 * s + q) ^ i)) * 4]) = t[s];
+        for (int s = 0; s < TN; ++s) *reinterpret_cast<Sum*>(&lds[(i * PC + ((4 * s + q) ^ (i & (PC - 1)))) * 4]) = t[s];
         __builtin_amdgcn_wave_barrier();
         typename Op::Row now[STEPS];
 #pragma unroll
@@ -301,7 +301,7 @@ __device__ __forceinline__ void store_sixteens(const typename Op::Args& a, int g
 #pragma unroll
         for (int k = 0; k < STEPS; ++k) {
             const int r = RS * k + row;
-            finish_eight<Op, ACT, Sum>(a, g, m0 + 16 * u + r, n, &lds[(r * PC + ((2 * c) ^ r)) * 4], &lds[(r * PC + ((2 * c + 1) ^ r)) * 4], columns, now[k]);
+            finish_eight<Op, ACT, Sum>(a, g, m0 + 16 * u + r, n, &lds[(r * PC + ((2 * c) ^ (r & (PC - 1)))) * 4], &lds[(r * PC + ((2 * c + 1) ^ (r & (PC - 1)))) * 4], columns, now[k]);
         }
     }
 }
@@ -325,7 +325,7 @@ struct RowsOfK {
     using Args = Arguments;
     using Element = E;
     static constexpr bool kTurnX = false, kTurnW = false;
-    static constexpr int kWideLds = 32768, kBand = 8;
+    static constexpr int kWideLds = 8192, kBand = 8;      // bytes that the epilogue takes for each TN
     static __device__ __forceinline__ int depth(const Args& a, int) { return a.in_dim; }
     static __device__ __forceinline__ const E* x_at(const Args& a, int g, int m) { return static_cast<const E*>(a.x) + g * a.x_group + m * a.x_stride; }
     static __device__ __forceinline__ const E* w_at(const Args& a, int g, int n) { return static_cast<const E*>(a.weight) + g * a.weight_group + n * a.weight_stride; }
@@ -632,25 +632,26 @@ __device__ __forceinline__ uint64_t read_turned(const uint16_t* p) {
 #endif
 }
 
-template <class Op>
-__global__ __launch_bounds__(512) void k_linear_wide(typename Op::Args a, int tiles_m, int tiles_n) {
+template <class Op, int TM, int TN>
+__global__ __launch_bounds__(512, TM == 8 ? 2 : 4) void k_linear_wide(typename Op::Args a, int tiles_m, int tiles_n) {
 #ifdef __HIP_DEVICE_COMPILE__
     using Element = typename Op::Element;
     using Sum = typename Op::Sum;
     constexpr int ES = sizeof(Element), PE = 16 / ES, BK = 8 * PE;      // elements of 16 bytes; of a stage
-    constexpr int NW = 8, TM = 8, TN = 4, TO = TN + TM;                 // waves; sixteens a wave has of rows, of columns
-    constexpr int NL = 32 / NW;                                         // its loads of an operand's stage
-    constexpr int HALF = 256 * 64;                                      // half words of an operand's stage
-    static_assert(!(Op::kTurnX || Op::kTurnW) || ES == 2);
+    constexpr int NW = 8, B = 32 * TM, TO = TN + TM;                    // waves; the tile; sixteens a wave has of columns and rows
+    constexpr int NL = B / 64;                                          // a wave's loads of an operand's stage
+    constexpr int HALF = B * 64;                                        // half words of an operand's stage
+    constexpr int LR = B / 8, R = 64 / LR;                              // lanes to a row of k, rows of a load
+    static_assert((!(Op::kTurnX || Op::kTurnW) || ES == 2) && TM == 2 * TN && (TM == 8 || TM == 4));
     typedef __attribute__((address_space(3))) void* lds_ptr;
-    __shared__ __attribute__((aligned(16))) uint16_t sm[4 * HALF + Op::kWideLds / 2];      // two stages, what the epilogue takes
+    __shared__ __attribute__((aligned(16))) uint16_t sm[4 * HALF + Op::kWideLds * TN / 2];      // two stages, what the epilogue takes
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = blockIdx.z, K = Op::depth(a, g);
     const int total = tiles_m * tiles_n, per = total / 8, more = total % 8;
     const int xcd = blockIdx.x % 8, from = xcd * per + min(xcd, more), here = per + (xcd < more);
     const int S = (K + BK - 1) / BK, s0 = (int)((int64_t)xcd * S / 8);
-    const int wm = wave % 2 * 128, wn = wave / 2 * (16 * TN);
+    const int wm = wave % 2 * (16 * TM), wn = wave / 2 * (16 * TN);
 
     struct Place {
         int m0, n0;
@@ -659,19 +660,19 @@ __global__ __launch_bounds__(512) void k_linear_wide(typename Op::Args a, int ti
         uint32_t vx[NL], vw[NL];      // byte offsets of this wave's loads
     };
     // the first k of a lane's part of its first load (NW a multiple of eight: of every load, where rows are the tile's)
-    const int in_row = ((lane & 7) ^ ((wave * 8 + (lane >> 3)) >> 1 & 7)) * PE, of_rows = wave * 2 + (lane >> 5);
+    const int in_row = ((lane & 7) ^ ((wave * 8 + (lane >> 3)) >> 1 & 7)) * PE, of_rows = wave * R + lane / LR;
     auto place = [&](Place& p, int tile) {
         // Bands of kBand rows of tiles, column after column: what an XCD has in the air is eight
         // by four of them, which read 12 operands' stages where 16 by two read 18 (4096 rows of
         // 4096 x 16384 453 -> 416 us, 8-bit 261 -> 236). 0: all rows.
         const int rows = Op::kBand > 0 ? Op::kBand : tiles_m, band = tile / (rows * tiles_n), first = band * rows;
         const int high = min(rows, tiles_m - first), in = tile - first * tiles_n;
-        p.m0 = (first + in % high) * 256, p.n0 = in / high * 256;
+        p.m0 = (first + in % high) * B, p.n0 = in / high * B;
         p.x = Op::x_at(a, g, p.m0), p.w = Op::w_at(a, g, p.n0);
 #pragma unroll
         for (int j = 0; j < NL; ++j) {
             const int c = wave + NW * j;
-            const int r = c * 8 + (lane >> 3), k = c * 2 + (lane >> 5), col = ((lane & 31) ^ (((k & 3) | (k >> 1 & 4)) << 1)) * 8;
+            const int r = c * 8 + (lane >> 3), k = c * R + lane / LR, col = ((lane % LR) ^ (((k & 3) | (k >> 1 & 4)) << 1)) * 8;
             if (Op::kTurnX) p.vx[j] = p.m0 + col < Op::x_columns(a) ? (uint32_t)(k * (int)a.x_stride + col) * ES : kOutside;
             else p.vx[j] = p.m0 + r < a.rows ? (uint32_t)(r * (int)a.x_stride + in_row) * ES : kOutside;
             if (Op::kTurnW) p.vw[j] = p.n0 + col < Op::w_columns(a) ? (uint32_t)(k * (int)a.weight_stride + col) * ES : kOutside;
@@ -687,10 +688,10 @@ __global__ __launch_bounds__(512) void k_linear_wide(typename Op::Args a, int ti
             const int j = l / 2;
             if (l % 2 == 0)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(to + (wave + NW * j) * 512), 16,
-                                                         (Op::kTurnX ? of_rows + 2 * NW * j : in_row) < left ? p.vx[j] : kOutside, 0, 0, 0);
+                                                         (Op::kTurnX ? of_rows + R * NW * j : in_row) < left ? p.vx[j] : kOutside, 0, 0, 0);
             else
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(to + HALF + (wave + NW * j) * 512), 16,
-                                                         (Op::kTurnW ? of_rows + 2 * NW * j : in_row) < left ? p.vw[j] : kOutside, 0, 0, 0);
+                                                         (Op::kTurnW ? of_rows + R * NW * j : in_row) < left ? p.vw[j] : kOutside, 0, 0, 0);
         });
     };
     auto all = [](uint16_t* to, auto load) {
@@ -704,11 +705,11 @@ __global__ __launch_bounds__(512) void k_linear_wide(typename Op::Args a, int ti
         asm volatile("" ::: "memory");
     };
     // sixteen b of an operand at a step of 32 k (64 bytes)
-    const int turned = (8 * q + (i >> 2)) * 256 + (i & 3) * 4, turn = (i >> 2) | (q & 1) << 2;
+    const int turned = (8 * q + (i >> 2)) * B + (i & 3) * 4, turn = (i >> 2) | (q & 1) << 2;
     auto sixteen = [&](auto turn_it, const uint16_t* area, int first, int b, int step) {
         if constexpr (decltype(turn_it)::value) {
-            const uint16_t* p = area + step * 32 * 256 + turned + ((first / 16 + b ^ turn) << 4);
-            const uint64_t lo = read_turned(p), hi = read_turned(p + 4 * 256);
+            const uint16_t* p = area + step * 32 * B + turned + ((first / 16 + b ^ turn) << 4);
+            const uint64_t lo = read_turned(p), hi = read_turned(p + 4 * B);
             return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
         } else {
             return *reinterpret_cast<const u32x4*>(area + (first + 16 * b + i) * 64 + ((step * 4 + q) ^ (i >> 1)) * 8);
@@ -736,19 +737,20 @@ __global__ __launch_bounds__(512) void k_linear_wide(typename Op::Args a, int ti
         wait();
         u32x4 oa[TO], ob[TO];
         each_of(std::make_integer_sequence<int, TO>(), [&](auto r) { oa[r.value] = operand(sm, 0, r); });
-        // reads and loads stand between the products, four at a time (what they read and write
+        // reads and loads stand between the products, a few at a time (what they read and write
         // lies apart: the compiler waits for the loads before it turns a read otherwise)
         auto half = [&](const u32x4 (&now)[TO], u32x4 (&next)[TO], const uint16_t* __restrict area, uint16_t* __restrict to, int step, auto load) {
-            each_of(std::make_integer_sequence<int, TN * TM / 4>(), [&](auto r) {
-                constexpr int G = TN * TM / 4, R = (TO + G - 1) / G, k = decltype(r)::value;
-                each_of(std::make_integer_sequence<int, R>(), [&](auto f) {
-                    constexpr int o = k * R + decltype(f)::value;
+            constexpr int P = TM == 8 ? 4 : 2, G = TN * TM / P, RD = (TO + G - 1) / G;      // products of a group; groups; its reads
+            each_of(std::make_integer_sequence<int, G>(), [&](auto r) {
+                constexpr int k = decltype(r)::value;
+                each_of(std::make_integer_sequence<int, RD>(), [&](auto f) {
+                    constexpr int o = k * RD + decltype(f)::value;
                     if constexpr (o < TO) next[o] = operand(area, step, std::integral_constant<int, o>());
                 });
                 if constexpr (k < 2 * NL) load(to, k);
                 __builtin_amdgcn_sched_barrier(0);
-                each_of(std::make_integer_sequence<int, 4>(), [&](auto f) {
-                    constexpr int e = 4 * k + decltype(f)::value, s = e / TM, u = e % TM;
+                each_of(std::make_integer_sequence<int, P>(), [&](auto f) {
+                    constexpr int e = P * k + decltype(f)::value, s = e / TM, u = e % TM;
                     acc[s][u] = Op::mfma(now[s], now[TN + u], acc[s][u]);
                 });
                 __builtin_amdgcn_sched_barrier(0);
@@ -831,10 +833,11 @@ hipError_t launch_tile(const typename Op::Args& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <class Op>
+template <class Op, int TM = 8, int TN = 4>
 hipError_t launch_wide(const typename Op::Args& a, hipStream_t s) {
-    const int tm = (a.rows + 255) / 256, tn = (a.out_dim + 255) / 256;
-    hipLaunchKernelGGL((k_linear_wide<Op>), dim3(std::min(256, (tm * tn + 7) / 8 * 8), 1, a.groups), dim3(512), 0, s, a, tm, tn);
+    constexpr int B = 32 * TM, most = TM == 8 ? 256 : 512;      // as many blocks as the CUs hold
+    const int tm = (a.rows + B - 1) / B, tn = (a.out_dim + B - 1) / B;
+    hipLaunchKernelGGL((k_linear_wide<Op, TM, TN>), dim3(std::min(most, (tm * tn + 7) / 8 * 8), 1, a.groups), dim3(512), 0, s, a, tm, tn);
     return hipGetLastError();
 }
 
