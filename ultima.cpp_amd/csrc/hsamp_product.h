@@ -797,6 +797,11 @@ constexpr Form kForms[] = {
     {16, 16, 2, {8, 12}}, {32, 32, 2, {13, 25}}, {64, 16, 1, {14.5f, 0}}, {64, 32, 1, {15.5f, 0}}, {64, 64, 2, {32, 39}},
     {64, 64, 1, {24, 0}}, {128, 128, 1, {44, 0}}, {160, 128, 2, {62, 84}}, {256, 256, 1, {112, 0}},
 };
+// The same in 8 bits (K = 4096, half the bytes): 64 x 16 rows 64: 8.5 us; 64 x 32 rows 128:
+// 8.4; 64 x 64 rows 256: 24.7, rows 512: 26.9, by 16 waves rows 256: 11.0, rows 512: 20.9;
+// 128 x 128 rows 512: 18.8, 1024: 22.4; 160 x 128 rows 320 of 16384: 28.4, 2048: 41.8;
+// 256 x 256 rows 2048 of 8192: 61.6.
+constexpr float kBytes[][2] = {{6, 8}, {7, 13.5f}, {8.5f, 0}, {8.4f, 0}, {24.7f, 27}, {11, 0}, {21, 0}, {28, 42}, {60, 0}};
 
 // Blocks of one group.
 template <class Args>
@@ -808,6 +813,7 @@ int64_t blocks_of(const Form& f, const Args& a) {
 // width). More: the form whose rounds over the 256 CUs cost least.
 template <class Args>
 int choose(const Args& a) {
+    constexpr bool bytes = std::is_same_v<decltype(a.x), const int8_t*>;
     if (a.rows <= 32) return a.rows <= 16 ? 0 : 1;
     int best = 0;
     float least = 0;
@@ -815,8 +821,8 @@ int choose(const Args& a) {
         const Form& v = kForms[f];
         const int64_t blocks = blocks_of(v, a) * a.groups;
         const int64_t round = 256 * v.blocks, rest = blocks % round;
-        const float cost = (float)(blocks / round) * v.one[v.blocks - 1] +
-                           (rest == 0 ? 0.0f : rest <= 256 ? v.one[0] : v.one[v.blocks - 1]);
+        const float* one = bytes ? kBytes[f] : v.one;
+        const float cost = (float)(blocks / round) * one[v.blocks - 1] + (rest == 0 ? 0.0f : rest <= 256 ? one[0] : one[v.blocks - 1]);
         if (f == 2 || cost < least) {
             best = f;
             least = cost;

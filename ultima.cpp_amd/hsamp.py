@@ -648,7 +648,7 @@ def _elsewhere(dev, stream, what):
         if stream.device != dev:
             _refuse(f"{what}: the stream must be one of {dev}")
         return torch.cuda.stream(stream)
-    return None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return None if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 def _used_on(stream, *tensors):
@@ -840,9 +840,8 @@ ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "softcap": 5
 
 def _matrix(t, lead, rows, columns, dtype, dev, name, what="linear"):
     """The address, row stride and group stride of a [*lead, rows, columns] operand."""
-    shape, stride = t.shape, t.stride()
-    if shape[:-2] != lead or len(shape) < 2 or shape[-2] != rows or shape[-1] != columns or t.dtype != dtype or \
-            t.device != dev or (columns > 1 and stride[-1] != 1):
+    stride = t.stride()
+    if t.shape != (*lead, rows, columns) or t.dtype is not dtype or t.device != dev or (columns > 1 and stride[-1] != 1):
         _refuse(f"{what}: {name} must be {dtype} {(*lead, rows, columns)} on {dev}, contiguous in its last dimension")
     return t.data_ptr(), stride[-2] if rows > 1 else max(columns, stride[-2]), stride[0] if lead else 0
 
