@@ -1,0 +1,227 @@
+"""The operators around the vocabulary's matrix as a program runs them together: a
+training step on a matrix that is embedding and head at once, and a decode step whose
+logits are made in 8 bits."""
+import numpy as np
+import pytest
+
+from test_gpu_linear_i8 import compare as compare_i8
+from test_gpu_loss import check_forward
+
+pytestmark = pytest.mark.gpu
+
+
+def tied(seed, n=230, V=1003, H=72):
+    """Weights in eighths, so that 8 w is exact, and tokens, some of them ended."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = (torch.randint(-3, 4, (V, H), generator=g, device="cuda") / 8).to(torch.bfloat16)
+    tokens = torch.randint(0, V, (n,), generator=g, device="cuda", dtype=torch.int32)
+    tokens[torch.rand(n, generator=g, device="cuda") < 0.3] = 5           # a frequent one
+    tokens[::17] = -1
+    return w, tokens
+
+
+def step(hs, w, tokens, grad=None, stream=None, outputs=None, work=(None, None, None)):
+    """Next-token losses of scaled embeddings against the same matrix, and its gradient."""
+    import torch
+    V, H = w.shape
+    x = hs.embed(w, tokens[:-1].contiguous(), scale=8.0, stream=stream)
+    target = tokens[1:].contiguous()
+    out = hs.cross_entropy(x, w, target, work=work[0], stream=stream)
+    if grad is None:
+        grad = torch.full((len(target),), 1 / len(target), device="cuda")
+    dw = torch.empty((V, H), dtype=torch.float32, device="cuda") if outputs is None else outputs
+    got = hs.cross_entropy_grad(x, w, target, out["lse"], grad, outputs={"d_weight": dw}, work=work[1], stream=stream)
+    hs.embed_grad(got["d_x"].float(), tokens[:-1].contiguous(), V, scale=8.0, out=dw, accumulate=True, work=work[2], stream=stream)
+    return x, target, grad, out, dw
+
+
+def test_a_tied_training_step(hs):
+    import torch
+    w, tokens = tied(1)
+    x, target, grad, out, dw = step(hs, w, tokens)
+    torch.cuda.synchronize()
+    ok = tokens[:-1] >= 0
+    assert torch.equal(x[ok].float(), 8 * w[tokens[:-1][ok].long()].float()) and not x[~ok].any()
+    check_forward(out, x, w, target, 0.0, "whole")
+    # the gradient in 64 bits by autograd
+    w64 = w.double().cpu().requires_grad_()
+    t = tokens.long().cpu()
+    x64 = 8 * w64[t[:-1].clamp(min=0)] * (t[:-1, None] >= 0)
+    logp = torch.log_softmax(x64 @ w64.t(), 1)
+    used = t[1:] >= 0
+    loss = -(logp[torch.arange(len(t) - 1), t[1:].clamp(min=0)] * used * grad.double().cpu()).sum()
+    loss.backward()
+    # dz rounded to bfloat16, 2^-8 of itself; with the lse's and the exponential's errors below 2^-16 p
+    p = torch.exp(logp.detach())
+    d = p.clone()
+    d[torch.arange(len(t) - 1), t[1:].clamp(min=0)] -= used.double()
+    g = (grad.double().cpu() * used)[:, None]
+    off = 2.0**-8 * g * d.abs() + 2.0**-16 * g * p
+    W = w.double().cpu()
+    offx = off @ W.abs() + 2.0**-8 * ((g * d) @ W).abs() + 2.0**-8 * (off @ W.abs())        # d_x is bfloat16
+    tol = off.t() @ x64.detach().abs()
+    tol.index_add_(0, t[:-1].clamp(min=0), 8 * offx * (t[:-1, None] >= 0))
+    tol = tol + 2.0**-14 * (g * d).abs().t() @ x64.detach().abs() + 1e-9
+    err = (dw.double().cpu() - w64.grad).abs() / tol
+    assert err.max() <= 1, err.max()
+
+
+def test_the_step_captured_and_on_a_stream(hs):
+    import torch
+    w, tokens = tied(2)
+    dw = torch.empty(w.shape, dtype=torch.float32, device="cuda")
+    grad = torch.rand(len(tokens) - 1, device="cuda")
+    step(hs, w, tokens, grad, outputs=dw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x, _, _, out, _ = step(hs, w, tokens, grad, outputs=dw)
+    s = torch.cuda.Stream()
+    for seed in range(3, 7):
+        a, b = tied(seed)
+        w.copy_(a), tokens.copy_(b)
+        want = step(hs, w, tokens, grad)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            other = step(hs, w, tokens, grad)
+        dw.fill_(1)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got in ((out["loss"], out["lse"], dw), (other[3]["loss"], other[3]["lse"], other[4])):
+            for g, e in zip(got, (want[3]["loss"], want[3]["lse"], want[4])):
+                assert torch.equal(g, e)
+
+
+def test_decode_in_eight_bits(hs, sampler, wl, orc):
+    """Tokens -> embedding -> 8-bit logits -> sampler -> log-probabilities of what it took."""
+    import torch
+    B, V, H = 9, 2011, 128
+    g = torch.Generator(device="cuda").manual_seed(7)
+    w = (torch.randn((V, H), generator=g, device="cuda") * 0.3).to(torch.bfloat16)
+    wq, ws = hs.quantize_rows(w)
+    tokens = torch.randint(0, V, (B,), generator=g, device="cuda", dtype=torch.int32)
+    rng = np.random.default_rng(8)
+    knobs = wl.identity_params(temperature=0.8, top_k=40)
+    for _ in range(3):
+        x = hs.embed(w, tokens, scale=H**0.5)
+        q, s = hs.quantize_rows(x)
+        logits = hs.linear_i8(q, s, wq, ws, act="softcap", act_param=30.0, out_dtype=torch.float32)
+        u = rng.random(B)
+        tokens = sampler.run(logits, [knobs] * B, torch.from_numpy(u).cuda())["token"]
+        out = hs.cross_entropy(x, w, tokens, softcap=30.0)
+        torch.cuda.synchronize()
+        compare_i8(logits, q, s, wq, ws, None, "softcap", 30.0, None)
+        rows = logits.cpu().numpy()
+        assert list(tokens.cpu().numpy()) == [orc.sample_row(rows[b], knobs, u=float(u[b])).token for b in range(B)]
+        check_forward(out, x, w, tokens, 30.0, "normal")
+        # the 8-bit logits stand near the 16-bit ones: each factor is off by half a step of its row's
+        # largest value, so a product's sum by (|x| steps of w + |w| steps of x) / 2 and a little
+        z = x.double() @ w.double().t().contiguous()
+        off = (x.double().abs().sum(1)[:, None] * ws.double() + w.double().abs().sum(1) * s.double()[:, None]) / 2 + H * s.double()[:, None] * ws.double() / 4
+        assert torch.all((logits.double() - 30 * torch.tanh(z / 30)).abs() <= off + 1e-3)
+
+
+def calls(hs, seed):
+    """Every operator once, as (function, arguments, named arguments)."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*shape):
+        return torch.randn(shape, generator=g, device="cuda")
+
+    x, w, b = normal(64, 512).to(torch.bfloat16), normal(700, 512).to(torch.bfloat16), normal(700).to(torch.bfloat16)
+    q, s = hs.quantize_rows(x)
+    wq, ws = hs.quantize_rows(w)
+    t = torch.randint(-1, 700, (64,), generator=g, device="cuda", dtype=torch.int32)
+    lse = hs.cross_entropy(x, w, t)["lse"]
+    return [
+        (hs.quantize_rows, (x,), {}),
+        (hs.linear_i8, (q, s, wq, ws), dict(bias=b, residual=normal(64, 700).to(torch.bfloat16))),
+        (hs.cross_entropy, (x, w, t), dict(softcap=20.0)),
+        (hs.cross_entropy_grad, (x, w, t, lse, normal(64)), {}),
+        (hs.embed, (w, t), dict(scale=3.0)),
+        (hs.embed_grad, (x, t, 700), {}),
+    ]
+
+
+def tensors_of(r):
+    return list(r.values()) if isinstance(r, dict) else list(r) if isinstance(r, tuple) else [r]
+
+
+def test_streams_of_another_device_are_refused(hs):
+    import types
+
+    import torch
+    other = types.SimpleNamespace(device=torch.device("cuda", torch.cuda.current_device() + 1))
+    for fn, args, kw in calls(hs, 1):
+        with pytest.raises(hs.HsampError) as e:
+            fn(*args, **kw, stream=other)
+        assert e.value.status == hs.ERR_INVALID
+
+
+def test_tensors_of_calls_on_another_stream_are_kept(hs):
+    """What a call on another stream reads and writes is dropped while that stream waits;
+    memory handed out meanwhile and overwritten is not theirs."""
+    import torch
+    s = torch.cuda.Stream()
+    copy = lambda a: a.clone() if torch.is_tensor(a) else a  # noqa: E731
+    for fn, args, kw in calls(hs, 2):
+        want = fn(*args, **kw)
+        mine, named = [copy(a) for a in args], {k: copy(a) for k, a in kw.items()}
+        sizes = [(a.shape, a.dtype) for a in [*mine, *named.values()] if torch.is_tensor(a)]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(100_000_000)
+        got = fn(*mine, **named, stream=s)
+        mine.clear()
+        named.clear()
+        later = [torch.full(shape, 3, dtype=dtype, device="cuda") for shape, dtype in sizes]
+        torch.cuda.synchronize()
+        del later
+        for a, e in zip(tensors_of(got), tensors_of(want)):
+            assert torch.equal(a, e), fn.__name__
+
+
+def test_calls_on_two_streams_at_once(hs):
+    """Each call has its own workspace: two of them side by side, many times, are what they are alone."""
+    import torch
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    sets = [calls(hs, 3), calls(hs, 4)]
+    want = [[tensors_of(fn(*args, **kw)) for fn, args, kw in c] for c in sets]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = [[], []]
+        for k in range(len(sets[0])):
+            for i, s in enumerate(streams):
+                fn, args, kw = sets[i][k]
+                got[i].append(tensors_of(fn(*args, **kw, stream=s)))
+        torch.cuda.synchronize()
+        for g, e in zip(got, want):
+            for a, b in zip(g, e):
+                for p, r in zip(a, b):
+                    assert torch.equal(p, r)
+
+
+@pytest.mark.parametrize("bad", ["dtype", "shape", "missing", "device", "strides"])
+def test_the_bindings_refuse(hs, bad):
+    import torch
+    for fn, args, kw in calls(hs, 5):
+        args = list(args)
+        k = 1 if len(args) > 1 and torch.is_tensor(args[1]) else 0
+        t = args[k]
+        if bad == "dtype":
+            args[k] = t.double()
+        elif bad == "shape":
+            args[k] = t[..., None]
+        elif bad == "missing" and k:
+            args[k] = None if t.dim() == 1 else t[:0]
+        elif bad == "device":
+            args[k] = t.cpu()
+        elif bad == "strides":
+            args[k] = t.t() if t.dim() == 2 and t.shape[0] != t.shape[1] else t.repeat_interleave(2)[::2]
+        if args[k] is t:
+            continue
+        with pytest.raises(hs.HsampError) as e:
+            fn(*args, **kw)
+        assert e.value.status in (hs.ERR_INVALID, hs.ERR_UNSUPPORTED), fn.__name__
