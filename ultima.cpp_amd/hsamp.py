@@ -835,6 +835,12 @@ def verify_sets(kept_idx, kept_prob, kept_count, draft, u_accept, u_draw, max_dr
     return out
 
 
+def _kind(dtype):
+    """ULTIMA_HSAMP_* of a row's type, or None."""
+    import torch
+    return F32 if dtype is torch.float32 else BF16 if dtype is torch.bfloat16 else F16 if dtype is torch.float16 else None
+
+
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "softcap": 5}
 
 
@@ -901,8 +907,8 @@ def quantize_rows(x, q=None, scale=None, stream=None):
     outputs may be passed in. stream: as in verify_draft."""
     import torch
     what, dev = "quantize_rows", x.device
-    kinds = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
-    if not x.is_cuda or x.dim() != 2 or x.dtype not in kinds:
+    kind = _kind(x.dtype)
+    if not x.is_cuda or x.dim() != 2 or kind is None:
         _refuse(f"{what}: x must be a float32, bfloat16 or float16 matrix on the GPU")
     there = _elsewhere(dev, stream, what)
     if there is not None:
@@ -911,14 +917,18 @@ def quantize_rows(x, q=None, scale=None, stream=None):
         _used_on(stream, x, *out)
         return out
     M, K = x.shape
+    a = QuantizeArgs(M, K, kind)
+    a.x, a.x_stride, _ = _matrix(x, (), M, K, x.dtype, dev, "x", what)
     if q is None:
         q = torch.empty((M, K), dtype=torch.int8, device=dev)
+        a.q, a.q_stride = q.data_ptr(), K
+    else:
+        a.q, a.q_stride, _ = _matrix(q, (), M, K, torch.int8, dev, "q", what)
     if scale is None:
         scale = torch.empty(M, dtype=torch.float32, device=dev)
-    a = QuantizeArgs(M, K, kinds[x.dtype])
-    a.x, a.x_stride, _ = _matrix(x, (), M, K, x.dtype, dev, "x", what)
-    a.q, a.q_stride, _ = _matrix(q, (), M, K, torch.int8, dev, "q", what)
-    a.scale = _vector(scale, M, torch.float32, dev, what, "scale")
+        a.scale = scale.data_ptr()
+    else:
+        a.scale = _vector(scale, M, torch.float32, dev, what, "scale")
     _launch(lib().ultima_hsamp_quantize_rows, a, dev, what)
     return q, scale
 
@@ -951,9 +961,7 @@ def linear_i8(x, x_scale, weight, weight_scale, bias=None, act: str = "none", ac
         dtype = given[0] if given else torch.bfloat16
     if dtype not in (torch.bfloat16, torch.float16):
         _refuse(f"{what}: bias and residual are bfloat16 or float16")
-    if out is None:
-        out = torch.empty((*lead, M, N), dtype=out_dtype or dtype, device=dev)
-    odt = out.dtype
+    odt = out_dtype or dtype if out is None else out.dtype
     if odt not in (dtype, torch.float32) or out_dtype not in (None, odt):
         _refuse(f"{what}: the output must be {dtype} or torch.float32")
     kind = BF16 if dtype == torch.bfloat16 else F16
@@ -961,12 +969,16 @@ def linear_i8(x, x_scale, weight, weight_scale, bias=None, act: str = "none", ac
     a.x, a.x_stride, a.x_group = _matrix(x, lead, M, K, torch.int8, dev, "x", what)
     a.weight, a.weight_stride, a.weight_group = _matrix(weight, lead, N, K, torch.int8, dev, "weight", what)
     for t, n, name in ((x_scale, M, "x_scale"), (weight_scale, N, "weight_scale")):
-        if t is None or t.shape != (*lead, n) or t.dtype != torch.float32 or t.device != dev or (n > 1 and t.stride(-1) != 1):
+        if t is None or t.shape != (*lead, n) or t.dtype is not torch.float32 or t.device != dev or (n > 1 and t.stride(-1) != 1):
             _refuse(f"{what}: {name} must be torch.float32 {(*lead, n)} on {dev}, contiguous in its last dimension")
     a.x_scale, a.x_scale_group = x_scale.data_ptr(), x_scale.stride(0) if lead else 0
     a.weight_scale, a.weight_scale_group = weight_scale.data_ptr(), weight_scale.stride(0) if lead else 0
     _epilogue(a, bias, residual, lead, M, N, dtype, dev, what)
-    a.out, a.out_stride, a.out_group = _matrix(out, lead, M, N, odt, dev, "out", what)
+    if out is None:
+        out = torch.empty((*lead, M, N), dtype=odt, device=dev)
+        a.out, a.out_stride, a.out_group = out.data_ptr(), N, M * N
+    else:
+        a.out, a.out_stride, a.out_group = _matrix(out, lead, M, N, odt, dev, "out", what)
     _launch(lib().ultima_hsamp_linear_i8, a, dev, what)
     return out
 
@@ -1068,10 +1080,10 @@ def cross_entropy_grad(x, weight, target, lse, grad, softcap: float = 0.0, need_
 
 def _embed_types(dt, out_dtype, what):
     import torch
-    kinds = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
-    if dt not in kinds or out_dtype not in (dt, torch.float32):
+    kind = _kind(dt)
+    if kind is None or out_dtype not in (dt, torch.float32):
         _refuse(f"{what}: rows are float32, bfloat16 or float16, the output in their type or in float32")
-    return kinds[dt], kinds[out_dtype]
+    return kind, _kind(out_dtype)
 
 
 def embed(table, tokens, scale: float = 1.0, out=None, out_dtype=None, stream=None):
