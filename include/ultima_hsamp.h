@@ -586,7 +586,8 @@ int ultima_hsamp_linear_i8(const ultima_hsamp_linear_i8_args* a, void* hip_strea
 /* Rows (of tokens; of a weight: its channels) in 8 bits: scale_m = max_k |x_mk| / 127,
  * q_mk the whole number nearest to 127 x_mk / max_k |x_mk| (halves to even, by the
  * exact quotient), -127 .. 127. A row of zeros has scale 0; a row that holds an
- * infinity or a NaN scale NaN and q 0, so that its products are NaN. */
+ * infinity or a NaN scale NaN and q 0, so that its products are NaN. No output overlaps
+ * an input or the other one. */
 typedef struct ultima_hsamp_quantize_args {
     int32_t rows;               /* 1 .. 2^24 - 1 */
     int32_t in_dim;             /* 1 .. 2^30 */
@@ -608,7 +609,8 @@ int ultima_hsamp_quantize_rows(const ultima_hsamp_quantize_args* a, void* hip_st
  * never stored: the log-probabilities of given tokens (a sampled one, a whole
  * prompt's) and the loss that trains a head. A target outside [0, vocab) is ignored:
  * loss 0 (lse stands). 16-bit inputs, float sums and statistics. A row with a logit
- * that is NaN or +inf has NaN for both; -inf logits have probability 0. */
+ * that is NaN or +inf has NaN for both; -inf logits have probability 0. No output
+ * overlaps an input or another one. */
 typedef struct ultima_hsamp_cross_entropy_args {
     int32_t rows;               /* M >= 1 */
     int32_t in_dim;             /* K >= 1 */
@@ -633,14 +635,17 @@ int64_t ultima_hsamp_cross_entropy_work_bytes(int32_t rows, int32_t vocab);
  * hip_stream one of its streams; asynchronous, allocates nothing (graph-capturable). */
 int ultima_hsamp_cross_entropy(const ultima_hsamp_cross_entropy_args* a, void* hip_stream);
 
-/* Its gradients. grad_m is the loss's gradient with respect to loss_m (ignored rows:
- * not looked at, taken as 0); lse as ultima_hsamp_cross_entropy left it.
+/* Its gradients. grad_m is the loss's gradient with respect to loss_m; lse as
+ * ultima_hsamp_cross_entropy left it. An ignored row adds nothing, whatever its grad, lse
+ * and x hold.
  *   dz_mv = grad_m (exp(z_mv - lse_m) - [v = t_m]) (with a soft cap: times 1 - (z_mv / c)^2)
  *   d_x = dz W,   d_weight = dz^T x  (accumulate: added to what d_weight holds)
  * The logits are made again, a piece of the vocabulary at a time; dz is rounded to
  * x's type before the two products (half precision: grad / max |grad| stands in for
  * grad there, and dz / grad is scaled by 2^15, so that no probability above 2^-39
- * is lost), whose sums are float. Rows whose lse is NaN have NaN gradients. */
+ * is lost; an infinite grad makes all gradients NaN), whose sums are float. Rows whose
+ * lse is NaN have NaN gradients. No output overlaps an input, the workspace or the
+ * other output. */
 typedef struct ultima_hsamp_cross_entropy_grad_args {
     int32_t rows;               /* as in ultima_hsamp_cross_entropy_args, to target */
     int32_t in_dim;
@@ -665,7 +670,9 @@ typedef struct ultima_hsamp_cross_entropy_grad_args {
 } ultima_hsamp_cross_entropy_grad_args;
 
 /* Bytes of workspace ultima_hsamp_cross_entropy_grad needs (-1 for invalid sizes): a
- * piece of dz and float sums of d_x, 0.1 to 0.5 GB at large sizes whatever the vocabulary. */
+ * piece of dz (128 MB at most up to 2^18 rows), float sums of d_x, a copy of x, a piece of
+ * the weight (256 MB at most up to in_dim 2^19): 0.1 to 0.6 GB at common sizes, whatever
+ * the vocabulary. */
 int64_t ultima_hsamp_cross_entropy_grad_work_bytes(int32_t rows, int32_t in_dim, int32_t vocab);
 
 /* As ultima_hsamp_cross_entropy; the same call gives the same bits every time. */
@@ -674,7 +681,7 @@ int ultima_hsamp_cross_entropy_grad(const ultima_hsamp_cross_entropy_grad_args* 
 /* ---- Embedding -----------------------------------------------------------------
  * out_i = scale * table[id_i]: the sampled tokens' rows of the (tied) vocabulary
  * matrix, the next step's input. An id outside [0, vocab) (an ended slot's -1) gives
- * a row of zeros. */
+ * a row of zeros. The output overlaps no input (nor in the other calls here). */
 typedef struct ultima_hsamp_embed_args {
     int32_t tokens;             /* N >= 1 */
     int32_t width;              /* H >= 1 */

@@ -233,6 +233,29 @@ def test_infinite_and_nan_logits_stay_in_their_row(hs, M):
     assert torch.all(torch.isnan(out["loss"])) and torch.all(torch.isnan(out["lse"]))
 
 
+@pytest.mark.parametrize("M, K", [(5, 72), (40, 65), (300, 72)])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_ignored_rows_reach_nobody(hs, M, K, dtype):
+    """Rows of a padded batch hold anything: the same bits as with zeros there."""
+    import torch
+    x, w, t, grad = inputs(12, M, K, 700, dtype, ignored=0.0)
+    t[::4], t[2::4] = -1, 700
+    pad = torch.zeros(M, dtype=torch.bool, device="cuda")
+    pad[::2] = True
+    x[pad], grad[pad] = 0, 0
+    lse = hs.cross_entropy(x, w, t)["lse"]
+    want = hs.cross_entropy_grad(x, w, t, lse, grad)
+    for junk in (float("nan"), float("inf"), 60000.0):
+        x2, grad2 = x.clone(), grad.clone()
+        x2[pad], grad2[pad] = junk, junk
+        out = hs.cross_entropy(x2, w, t)
+        got = hs.cross_entropy_grad(x2, w, t, out["lse"], grad2)
+        torch.cuda.synchronize()
+        assert torch.equal(out["lse"][~pad], lse[~pad]) and not out["loss"][pad].any()
+        for k in ("d_x", "d_weight"):
+            assert torch.equal(got[k], want[k]), (k, junk)
+
+
 def test_all_rows_ignored(hs):
     import torch
     for dtype in ("bfloat16", "float16"):

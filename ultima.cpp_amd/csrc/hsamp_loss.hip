@@ -291,14 +291,17 @@ __global__ __launch_bounds__(1024) void k_top_grad(const float* grad, const int3
 }
 
 // Rows laid out for the products: eight columns a piece, the last one filled up with zeros.
-__global__ __launch_bounds__(256) void k_lay_out(const uint16_t* from, int64_t stride, int64_t rows, int columns, uint16_t* to, int pieces) {
+// target: rows that do not count are zeros (whatever they hold, an infinity times dz = 0 too).
+__global__ __launch_bounds__(256) void k_lay_out(const uint16_t* from, int64_t stride, int64_t rows, int columns, uint16_t* to, int pieces,
+                                                 const int32_t* target, int vocab) {
     const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t r = k / pieces;
     const int c = (int)(k % pieces) * 8;
     if (r >= rows) return;
     const uint16_t* p = from + r * stride + c;
     u32x4 v = {};
-    if (c + 8 <= columns) {
+    if (target != nullptr && (target[r] < 0 || target[r] >= vocab)) {
+    } else if (c + 8 <= columns) {
         v = load16(p);
     } else {
 #pragma unroll
@@ -505,19 +508,21 @@ hipError_t launch_grads(const ultima_hsamp_cross_entropy_grad_args& a, hipStream
     uint16_t* dz = reinterpret_cast<uint16_t*>(work + at.dz);
     float* parts = reinterpret_cast<float*>(work + at.parts);
     if (!BF) hipLaunchKernelGGL(k_top_grad, dim3(1), dim3(1024), 0, s, a.grad, a.target, a.rows, a.vocab, top);
-    // operands at other addresses than whole 16 bytes are laid out first
+    // operands at other addresses than whole 16 bytes are laid out first, and x for d_weight
+    // (1 row 3 us more, 4096 rows of 4096 13 of 12000)
     const auto odd = [&](const void* q, int64_t stride) {
         return a.in_dim % 8 != 0 || reinterpret_cast<uintptr_t>(q) % 16 != 0 || stride % 8 != 0 || stride > 1 << 20;
     };
-    const auto lay_out = [&](const uint16_t* from, int64_t stride, int64_t rows, uint16_t* to) {
+    const auto lay_out = [&](const uint16_t* from, int64_t stride, int64_t rows, uint16_t* to, const int32_t* target) {
         const int pieces = (int)(p.columns / 8);
-        hipLaunchKernelGGL(k_lay_out, dim3((uint32_t)((rows * pieces + 255) / 256)), dim3(256), 0, s, from, stride, rows, a.in_dim, to, pieces);
+        hipLaunchKernelGGL(k_lay_out, dim3((uint32_t)((rows * pieces + 255) / 256)), dim3(256), 0, s, from, stride, rows, a.in_dim, to, pieces, target,
+                           a.vocab);
     };
     const uint16_t* x = static_cast<const uint16_t*>(a.x);
     int64_t x_stride = a.x_stride;
-    if (odd(a.x, a.x_stride)) {
+    if (a.d_weight != nullptr || odd(a.x, a.x_stride)) {
         uint16_t* to = reinterpret_cast<uint16_t*>(work + at.x);
-        lay_out(x, x_stride, a.rows, to);
+        lay_out(x, x_stride, a.rows, to, a.target);
         x = to, x_stride = p.columns;
     }
     const bool odd_weight = odd(a.weight, a.weight_stride);
@@ -529,13 +534,13 @@ hipError_t launch_grads(const ultima_hsamp_cross_entropy_grad_args& a, hipStream
         int64_t w_stride = a.weight_stride;
         if (odd_weight) {
             uint16_t* to = reinterpret_cast<uint16_t*>(work + at.weight);
-            lay_out(w, w_stride, width, to);
+            lay_out(w, w_stride, width, to, nullptr);
             w = to, w_stride = p.columns;
         }
         LossArgs l = loss_args(a.rows, (int)p.columns, width, x, x_stride, w, w_stride, a.target, a.softcap);
         l.vocab = a.vocab, l.first = (int)first;
         l.lse = a.lse, l.grad = a.grad, l.top_grad = top, l.dz = dz, l.dz_stride = p.width;
-        hipError_t e = launch_product<LossGrad<BF>>(l, s);
+        hipError_t e = launch_product<LossGrad<BF>, true>(l, s);
         if (e != hipSuccess) return e;
         if (a.d_x != nullptr) {
             GradArgs g = {};

@@ -211,9 +211,9 @@ __device__ __forceinline__ void finish_eight(const typename Op::Args& a, int g, 
 
 // A wave's 16 TM rows by 16 TN columns of sums, out through its own 16 PU rows of LDS, so
 // that every lane finishes eight neighbouring columns. What is done with a row's sums
-// comes four rows at a time (their residuals in the air meanwhile), not unrolled over all
-// of them: code that runs once comes from beyond the instruction cache (256 x 256 tiles
-// with every activation in every unrolled copy: 12.4 us a tile of 126).
+// comes four rows at a time (their residuals in the air meanwhile) and by its activation,
+// not unrolled over all of them with every activation in every copy: 150 KB of code that
+// run once a tile (12.4 us for one of 256 x 256; 6 to 8 so).
 // Row r's piece p of four floats stands at p ^ r % (4 TN): a store's 16 rows lie in
 // different banks.
 template <class Op, int ACT, int TN, int TM, int PU, class Sum, class Scalar>
@@ -341,16 +341,12 @@ struct RowsOfK {
 // step for each wave, whose sums meet in LDS at the end.
 //
 // Few rows: W's stream bounds it (one row of 4096 x 4096 8.3 us, 4.0 TB/s with the
-// launch and the ramp in it; four groups of 64 rows 29 us, 134 MB at 4.6 TB/s): hence
-// narrow tiles, whose waves share K instead of columns, and many loads in the air.
-// Many: per stage the loads to LDS and the LDS reads beside the products: hence the
-// widest tile that the accumulators allow, whose operands are read least often
-// (4096 rows of 4096 x 16384 462 us, 1190 TFLOP/s, where 8192 cubed reaches 1215 to
-// 1415 in the library, by card and clock; with bias, tanh and residual 533). Of its 1350
-// MB from memory x is most: an XCD's 32 tiles in the air are all 16 of the rows by 2 of
-// the columns, so each reads x four times (8 x 4 x 34 MB), the weight and the residual
-// (134 MB each) come once. 320 rows of 4096 x 151936: 440 us (with the soft cap in float
-// 463), 905 TFLOP/s: 194 MB are written, and two and a half tiles of rows need 160 of 128.
+// launch and the ramp in it; four groups of 64 rows 29 us, 134 MB at 4.6 TB/s; of bytes 15
+// us): hence narrow tiles, whose waves share K instead of columns, and many loads in the
+// air. Many: per stage the loads to LDS and the LDS reads beside the products: hence wide
+// tiles, whose operands are read least often; k_linear_wide from 256 x 256. 320 rows of
+// 4096 x 151936: 440 us (with the soft cap in float 463), 905 TFLOP/s: 194 MB are written,
+// and two and a half tiles of rows need 160 of 128; of bytes 246.
 // ANY: rows at any element's address, a last piece of less than eight columns
 // (loads to LDS take neither): one stage in registers, two in LDS.
 // Op: the element types and instruction (Element, Sum, mfma), the arguments (Args: rows,
@@ -605,20 +601,6 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear_tile(typename Op::
 #endif
 }
 
-// 256 x 256 tiles by eight waves of 128 x 64, for calls of many rows: a block to a CU goes
-// from tile to tile, the next one's first two stages in the air under the last one's
-// epilogue. An operand's rows are rows of the tile (128 bytes of k a stage, as above), or k
-// (kTurnX, kTurnW: 64 rows of 256 columns a stage, which the reads turn).
-//
-// Bound by the matrix pipe and by the power that it takes: a stage takes 2500 cycles where
-// the products alone take 2048, and the clock falls to 1.5 - 1.7 GHz (a library product runs
-// 2400 at 1.7: 8192 cubed 1518 TFLOP/s). 4096 rows of 151936 x 4096 with the softmax's
-// statistics 1360 TFLOP/s; 8-bit 4096 x 4096 x 16384 2330 TOP/s (a library's 2130).
-// Measured and not kept: four waves of 128 x 128 (two thirds of the LDS reads; 3070 cycles a
-// stage: nobody issues products while the only wave of a SIMD issues loads; rows of k alike),
-// stores straight from the registers (32 bytes of a row each: 2 to 9 in a hundred slower),
-// loads in one go after the wait (466 against 445 us), the products of a half stage in one
-// run behind its reads (460 against 445).
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // Four rows of sixteen columns, read by sixteen lanes (lane i: row i / 4, columns
@@ -632,6 +614,25 @@ __device__ __forceinline__ uint64_t read_turned(const uint16_t* p) {
 #endif
 }
 
+// Tiles of 256 x 256 by eight waves of 128 x 64 (TM = 8), for calls of many rows: a block
+// to a CU goes from tile to tile, the next one's first two stages in the air under the last
+// one's epilogue. Or of 128 x 128 by eight of 64 x 32 (TM = 4), two blocks to a CU. An
+// operand's rows are rows of the tile (128 bytes of k a stage, as above), or k (kTurnX,
+// kTurnW: 64 rows of the tile's width a stage, which the reads turn; in LDS the sixteen
+// columns b of row k stand at b ^ (k % 4 + 4 (k / 8 % 2)), so that the eight rows of 32
+// bytes that a read takes at a time lie in different banks).
+//
+// Bound by the matrix pipe and by the power that it takes: a stage takes 2450 to 2560
+// cycles where the products alone take 2048, and the clock falls to 1.45 - 1.7 GHz (a
+// library product runs 2400 at 1.7: 8192 cubed 1518 TFLOP/s); then 6 to 12 us of epilogue
+// to 105 of loop at K = 4096. 4096 rows of 151936 x 4096 with the softmax's statistics
+// 1368 TFLOP/s, the gradients of that 1273; 8-bit 4096 x 4096 x 16384 2340 TOP/s (a
+// library's 2130).
+// Measured and not kept: four waves of 128 x 128, the sums in accumulation registers (two
+// thirds of the LDS reads, 12212 against 12033 us of gradients), stores straight from the
+// registers (32 bytes of a row each: 2 to 9 in a hundred slower), loads in one go after the
+// wait (466 against 445 us), the products of a half stage in one run behind its reads (460
+// against 445), a block to a tile (2 in a hundred slower).
 template <class Op, int TM, int TN>
 __global__ __launch_bounds__(512, TM == 8 ? 2 : 4) void k_linear_wide(typename Op::Args a, int tiles_m, int tiles_n) {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -864,18 +865,20 @@ int columns_of(const typename Op::Args& a) {
     return whole_pieces<Op>(a) ? kForms[f].bn : f < 6 ? any[f] : 128;
 }
 
-template <class Op>
+// WHOLE: the caller has laid its operands out.
+template <class Op, bool WHOLE = false>
 hipError_t launch_product(const typename Op::Args& a, hipStream_t s) {
     const int f = choose(a);
-    if (!whole_pieces<Op>(a)) switch (f) {
-            case 0: return launch_tile<Op, true, 1, 1, 8, 1, 1, 2>(a, s);
-            case 1: return launch_tile<Op, true, 1, 1, 8, 2, 2, 2>(a, s);
-            case 2:
-            case 3: return launch_tile<Op, true, 1, 2, 4, 4, 1, 2>(a, s);
-            case 4:
-            case 5: return launch_tile<Op, true, 2, 2, 2, 2, 2, 2>(a, s);
-            default: return launch_tile<Op, true, 2, 4, 1, 4, 2, 2>(a, s);
-        }
+    if constexpr (!WHOLE)
+        if (!whole_pieces<Op>(a)) switch (f) {
+                case 0: return launch_tile<Op, true, 1, 1, 8, 1, 1, 2>(a, s);
+                case 1: return launch_tile<Op, true, 1, 1, 8, 2, 2, 2>(a, s);
+                case 2:
+                case 3: return launch_tile<Op, true, 1, 2, 4, 4, 1, 2>(a, s);
+                case 4:
+                case 5: return launch_tile<Op, true, 2, 2, 2, 2, 2, 2>(a, s);
+                default: return launch_tile<Op, true, 2, 4, 1, 4, 2, 2>(a, s);
+            }
     switch (f) {
         case 0: return launch_tile<Op, false, 1, 1, 4, 1, 1, 8>(a, s);
         case 1: return launch_tile<Op, false, 1, 1, 4, 2, 2, 4>(a, s);
