@@ -111,6 +111,24 @@ def test_embed_grad(hs, N, H, V, skew):
         compare(more, d, ids, V, -2.0, old)
 
 
+@pytest.mark.parametrize("V,H,out", [(1000, 1, "bfloat16"), (29, 4519, "float16"), (999, 131, "bfloat16"), (4099, 16, "float32"),
+                                     (65537, 1027, "float32"), (150_001, 1001, "bfloat16")])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_embed_grad_clears_its_table_alone(hs, V, H, out, offset):
+    """Few tokens, rows one behind the other, at any element's address: zeros up to the last
+    element and not one further."""
+    import torch
+    dt = getattr(torch, out)
+    buf = torch.full((offset + V * H + 64,), 77.0, dtype=dt, device="cuda")
+    table = buf[offset:offset + V * H].view(V, H)
+    ids = torch.tensor([V - 1, -1, 0, V - 1], dtype=torch.int32, device="cuda")
+    d = torch.ones((4, H), dtype=dt, device="cuda")
+    hs.embed_grad(d, ids, V, out=table)
+    torch.cuda.synchronize()
+    assert torch.all(buf[:offset] == 77.0) and torch.all(buf[offset + V * H:] == 77.0)
+    assert torch.all(table[0] == 1) and torch.all(table[-1] == 2) and not table[1:-1].any()
+
+
 def test_embed_grad_many_tokens(hs):
     """Chunks of more than 64 positions; a vocabulary of more ids than blocks of a thousand."""
     import torch

@@ -78,16 +78,40 @@ struct Sorted {
     int32_t* start;      // [vocab + 1] where an id's positions begin
     int32_t* order;      // [tokens] the positions
 };
+//
+// Then it writes the zeros of its ids without tokens, which bound most calls. A table of at
+// least four rows to a token whose rows lie one behind the other is cleared as a whole by
+// blocks beside the sort, which that hides (32768 tokens of 4096 columns, us, by its own
+// blocks / as a whole: 151936 rows 320 / 335, of which the usual few ids take most 343 / 317,
+// 32768 rows 138 / 162; 700 of 1002 floats, 50257 rows 38 / 34).
 constexpr int kWaves = 16, kRange = 1024;      // waves of a block; ids of one, at most
+struct Zeros {
+    char* out;                       // null: none
+    int64_t stride;                  // bytes between rows
+    int bytes, lanes;                // of a row; a power of two that write one, sixteen each at a time
+    int64_t all;                     // bytes of the table, or 0: the rows without tokens
+    int piece;                       // of them that a block clears
+};
 
 int ranges_of(int vocab) { return std::max((vocab + kRange - 1) / kRange, std::min(256, (vocab + 63) / 64)); }
 
-__global__ __launch_bounds__(64 * kWaves) void k_sort_ids(const int32_t* ids, int tokens, int vocab, int range, Sorted out) {
+__global__ __launch_bounds__(64 * kWaves) void k_sort_ids(const int32_t* ids, int tokens, int vocab, int range, int sorts, Sorted out, Zeros zeros) {
     constexpr int U = 8;
+    struct __attribute__((packed, aligned(2))) Sixteen { uint32_t v[4]; };
     struct Four { int v[4]; };              // (at any token)
     __shared__ int at[kWaves * kRange];     // a wave's tokens of an id, then where its next one goes
     __shared__ int below[kWaves], sums[kWaves];
+    __shared__ uint64_t none[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if ((int)blockIdx.x >= sorts) {
+        const int64_t first = ((int64_t)blockIdx.x - sorts) * zeros.piece;
+        const int n = (int)min((int64_t)zeros.piece, zeros.all - first), whole = n & ~15;
+        char* p = zeros.out + first;
+#pragma unroll 4
+        for (int c = tid * 16; c < whole; c += 16 * 64 * kWaves) *reinterpret_cast<Sixteen*>(p + c) = Sixteen{};
+        if (whole + 2 * tid < n) *reinterpret_cast<uint16_t*>(p + whole + 2 * tid) = 0;
+        return;
+    }
     const int lo = blockIdx.x * range, hi = min(vocab, lo + range);
     const int64_t per = ((int64_t)tokens + 256 * kWaves - 1) / (256 * kWaves) * 256;   // of one wave
     const int first = (int)min((int64_t)tokens, wave * per), last = (int)min((int64_t)tokens, (wave + 1) * per);
@@ -133,6 +157,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_sort_ids(const int32_t* ids, in
     // a thread per id: its tokens, those of the ids before it, of the waves before
     int count = 0;
     for (int w = 0; w < kWaves; ++w) count += at[w * kRange + tid];
+    const uint64_t without = __ballot(count == 0);
+    if (lane == 0) none[wave] = without;
     int scan = count;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -172,6 +198,15 @@ __global__ __launch_bounds__(64 * kWaves) void k_sort_ids(const int32_t* ids, in
         if (mine) out.order[begin + rank] = k;
         if (mine && rank == more - 1) *next = begin + more;
     });
+    if (zeros.out == nullptr || zeros.all != 0) return;
+    const int rows = 64 / zeros.lanes, l = lane % zeros.lanes, whole = zeros.bytes & ~15;
+    for (int r = wave * rows + lane / zeros.lanes; r < hi - lo; r += kWaves * rows) {
+        if ((none[r / 64] >> (r % 64) & 1) == 0) continue;
+        char* p = zeros.out + (lo + r) * zeros.stride;
+#pragma unroll 4
+        for (int c = l * 16; c < whole; c += 16 * zeros.lanes) *reinterpret_cast<Sixteen*>(p + c) = Sixteen{};
+        for (int c = whole + 2 * l; c < zeros.bytes; c += 2 * zeros.lanes) *reinterpret_cast<uint16_t*>(p + c) = 0;
+    }
 }
 
 // The sums. The sorted positions are cut into chunks, a block per chunk and 2048 columns,
@@ -180,7 +215,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_sort_ids(const int32_t* ids, in
 // most two to a chunk (of the id that came in, of the one that goes on), for the launch
 // after it.
 // A chunk has 32 positions, or 8 where that few blocks would leave most CUs idle.
-constexpr int kChunk = 32, kEmpty = 16;      // positions of a chunk, at most; ids of a block of the others
+constexpr int kChunk = 32;      // positions of a chunk, at most
 int chunk_of(int tokens) { return tokens <= 8192 ? 8 : kChunk; }
 
 __device__ __forceinline__ int64_t padded(int width) { return (width + N - 1) / N * N; }
@@ -238,32 +273,10 @@ __global__ __launch_bounds__(256) void k_embed_sums(ultima_hsamp_embed_grad_args
 }
 
 // The ids that cross borders, by the chunk that they end in: the sum of the chunk that they
-// began in, then of the ones they go through, eight in the air at a time. The blocks behind
-// these write the rows of ids without tokens, a wave to a row, and hide them.
+// began in, then of the ones they go through, eight in the air at a time.
 template <class O>
-__global__ __launch_bounds__(256) void k_embed_join(ultima_hsamp_embed_grad_args a, Sorted s, const float* partial, int chunk, int joins, int slices) {
+__global__ __launch_bounds__(256) void k_embed_join(ultima_hsamp_embed_grad_args a, Sorted s, const float* partial, int chunk, int slices) {
     constexpr int U = 8;
-    if ((int)blockIdx.x >= joins) {
-        struct __attribute__((packed, aligned(sizeof(O)))) Sixteen { uint32_t v[4]; };
-        constexpr int E = 16 / sizeof(O);
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int64_t id0 = (int64_t)(blockIdx.x - joins) * kEmpty;
-        const int begins = lane <= kEmpty && id0 + lane <= a.vocab ? s.start[id0 + lane] : 0, ends = __shfl_down(begins, 1);
-        const uint64_t empty = __ballot(lane < kEmpty && id0 + lane < a.vocab && begins == ends);
-#pragma unroll
-        for (int k = 0; k < kEmpty / 4; ++k) {
-            if ((empty >> (4 * k + wave) & 1) == 0) continue;
-            O* row = static_cast<O*>(a.out) + (id0 + 4 * k + wave) * a.out_stride;
-            for (int c = lane * E; c < a.width; c += 64 * E) {
-                if (c + E <= a.width) {
-                    *reinterpret_cast<Sixteen*>(row + c) = Sixteen{};
-                } else {
-                    for (int e = c; e < a.width; ++e) row[e] = (O)0.0f;
-                }
-            }
-        }
-        return;
-    }
     const int c = (blockIdx.x % slices * 256 + threadIdx.x) * N, left = a.width - c;
     const int at = blockIdx.x / slices + 1, first = at * chunk;
     if (first >= s.start[a.vocab]) return;
@@ -292,14 +305,19 @@ hipError_t launch_grad(const ultima_hsamp_embed_grad_args& a, hipStream_t s) {
     char* work = static_cast<char*>(a.work);
     const Sorted sorted = {reinterpret_cast<int32_t*>(work), reinterpret_cast<int32_t*>(work + up16(4 * ((int64_t)a.vocab + 1)))};
     float* partial = reinterpret_cast<float*>(work + up16(4 * ((int64_t)a.vocab + 1)) + up16(4 * (int64_t)a.tokens));
-    const int blocks = ranges_of(a.vocab), range = (a.vocab + blocks - 1) / blocks;
-    hipLaunchKernelGGL(k_sort_ids, dim3((a.vocab + range - 1) / range), dim3(64 * kWaves), 0, s, a.ids, a.tokens, a.vocab, range, sorted);
+    const int ranges = ranges_of(a.vocab), range = (a.vocab + ranges - 1) / ranges, sorts = (a.vocab + range - 1) / range;
+    Zeros zeros = {a.accumulate ? nullptr : static_cast<char*>(a.out), (int64_t)(a.out_stride * sizeof(O)), (int)(a.width * sizeof(O)), 1, 0, 1};
+    if (zeros.out != nullptr && a.out_stride == a.width && a.tokens <= a.vocab / 4) zeros.all = a.vocab * zeros.stride;
+    // (a store a thread where the table passes the last cache: 2.5 GB 449 us, sixteen 469; else
+    // sixteen: 200 MB 34 us, one 36; beyond 32 GB a launch would count too many threads)
+    zeros.piece = zeros.all > (int64_t)1 << 28 && zeros.all <= (int64_t)1 << 35 ? 16384 : 262144;
+    while (zeros.lanes < 64 && zeros.lanes * 16 < zeros.bytes) zeros.lanes *= 2;
+    hipLaunchKernelGGL(k_sort_ids, dim3((uint32_t)(sorts + (zeros.all + zeros.piece - 1) / zeros.piece)), dim3(64 * kWaves), 0, s, a.ids, a.tokens, a.vocab, range,
+                       sorts, sorted, zeros);
     const int chunk = chunk_of(a.tokens), chunks = (a.tokens + chunk - 1) / chunk, slices = (a.width + 256 * N - 1) / (256 * N);
-    const int empty = a.accumulate ? 0 : (a.vocab + kEmpty - 1) / kEmpty;
-    const int joins = (chunks - 1) * slices;
     hipLaunchKernelGGL((k_embed_sums<T, O>), dim3(chunks * slices), dim3(256), 0, s, a, sorted, partial, chunk, slices);
-    if (joins + empty > 0)
-        hipLaunchKernelGGL((k_embed_join<O>), dim3(joins + empty), dim3(256), 0, s, a, sorted, (const float*)partial, chunk, joins, slices);
+    if (chunks > 1)
+        hipLaunchKernelGGL((k_embed_join<O>), dim3((chunks - 1) * slices), dim3(256), 0, s, a, sorted, (const float*)partial, chunk, slices);
     return hipGetLastError();
 }
 
