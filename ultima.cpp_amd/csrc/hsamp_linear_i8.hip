@@ -61,7 +61,8 @@ struct LinearI8 : RowsOfK<ultima_hsamp_linear_i8_args, int8_t> {
 };
 
 // A row's largest magnitude, then its values in steps of a 127th of it. Bound by the
-// row's read and write; a block keeps up to 8192 values in registers between the two.
+// row's read and write (4096 rows of 4096 in 16 bits: 17 us) and for few rows by its two
+// dependent steps (3.8); a block keeps up to 8192 values in registers between the two.
 // Magnitudes are compared as whole numbers (infinities and NaN above all others).
 template <class T>
 __global__ __launch_bounds__(256) void k_quantize_rows(ultima_hsamp_quantize_args a) {

@@ -6,6 +6,12 @@
 // Gradients, a piece of the vocabulary at a time: the logits again, whose tiles store
 // dz = grad (exp(z - lse) - [v = t]) in 16 bits (the piece stays in the caches),
 // then d_x += dz W and d_weight = dz^T x.
+//
+// One row is bound by the weight's stream (4096 x 151936 198 us, 6.3 TB/s), many by the
+// products (4096 rows 3.73 ms; the gradients 12.0, of a piece of 16384 ids the logits with
+// their dz 425 us, d_x 400, d_weight 432), few rows of small matrices by what goes to memory
+// between the launches (301 of 1002 x 50257, odd addresses: weight laid out 38, dz
+// 61, d_x 71 and 11, d_weight 73).
 #include "hsamp_product.h"
 
 namespace hsamp {

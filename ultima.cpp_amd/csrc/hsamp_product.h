@@ -622,17 +622,20 @@ __device__ __forceinline__ uint64_t read_turned(const uint16_t* p) {
 // columns b of row k stand at b ^ (k % 4 + 4 (k / 8 % 2)), so that the eight rows of 32
 // bytes that a read takes at a time lie in different banks).
 //
-// Bound by the matrix pipe and by the power that it takes: a stage takes 2450 to 2560
-// cycles where the products alone take 2048, and the clock falls to 1.45 - 1.7 GHz (a
-// library product runs 2400 at 1.7: 8192 cubed 1518 TFLOP/s); then 6 to 12 us of epilogue
-// to 105 of loop at K = 4096. 4096 rows of 151936 x 4096 with the softmax's statistics
-// 1368 TFLOP/s, the gradients of that 1273; 8-bit 4096 x 4096 x 16384 2340 TOP/s (a
-// library's 2130).
-// Measured and not kept: four waves of 128 x 128, the sums in accumulation registers (two
-// thirds of the LDS reads, 12212 against 12033 us of gradients), stores straight from the
-// registers (32 bytes of a row each: 2 to 9 in a hundred slower), loads in one go after the
-// wait (466 against 445 us), the products of a half stage in one run behind its reads (460
-// against 445), a block to a tile (2 in a hundred slower).
+// Bound by the matrix pipe (2048 cycles of a stage's 2450 to 2560, at 1.45 - 1.7 GHz where
+// calls follow each other; a library product 2400 at 1.7: 8192 cubed 1518 TFLOP/s), by the
+// operands' way (with every block reading the same two tiles the gradients below take 11.2
+// ms, linear's 4096 rows 390 us) and by 6 to 12 us of epilogue to 105 of loop at K = 4096.
+// 4096 rows of 151936 x 4096 with the softmax's statistics 3.73 ms, 1367 TFLOP/s; their
+// gradients 12.0 ms, 1270; 4096 x 4096 x 16384 449 us, 8-bit 234 (2350 TOP/s; a library's
+// 2130).
+// Measured and not kept, us against those: four waves of 128 x 128, the sums in
+// accumulation registers (two thirds of the LDS reads; 12212, 8-bit 248), stores straight
+// from the registers (32 bytes of a row each; 2 to 9 in a hundred slower), loads in one go
+// after the wait (466), two at a time in the first half of the products (12500), the
+// products of a half stage in one run behind its reads (460), a block to a tile (2 in a
+// hundred slower), a word of each line read two stages ahead by one of the blocks that
+// share it (445; loss 3930, 8-bit 251).
 template <class Op, int TM, int TN>
 __global__ __launch_bounds__(512, TM == 8 ? 2 : 4) void k_linear_wide(typename Op::Args a, int tiles_m, int tiles_n) {
 #ifdef __HIP_DEVICE_COMPILE__
