@@ -651,9 +651,15 @@ __global__ __launch_bounds__(512, TM == 8 ? 2 : 4) void k_linear_wide(typename O
     __shared__ __attribute__((aligned(16))) uint16_t sm[4 * HALF + Op::kWideLds * TN / 2];      // two stages, what the epilogue takes
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g = blockIdx.z, K = Op::depth(a, g);
-    const int total = tiles_m * tiles_n, per = total / 8, more = total % 8;
-    const int xcd = blockIdx.x % 8, from = xcd * per + min(xcd, more), here = per + (xcd < more);
+    // A group's tiles are runs for the eight XCDs; sums over parts of k (groups of one product)
+    // keep a part to one XCD, or to 8 / groups, whose L2s then read its operands once.
+    const int line = blockIdx.z * gridDim.x + blockIdx.x, xcd = line % 8;
+    int g = blockIdx.z, run = xcd, runs = 8, k = blockIdx.x / 8, step = gridDim.x / 8;
+    if (Op::kTurnW && gridDim.z % 8 == 0) g = line / 8 / gridDim.x * 8 + xcd, run = 0, runs = 1, k = line / 8 % gridDim.x, step = gridDim.x;
+    else if (Op::kTurnW && 8 % gridDim.z == 0) g = xcd % gridDim.z, run = xcd / gridDim.z, runs = 8 / gridDim.z, k = line / 8, step *= gridDim.z;
+    const int K = Op::depth(a, g);
+    const int total = tiles_m * tiles_n, per = total / runs, more = total % runs;
+    const int from = run * per + min(run, more), here = per + (run < more);
     const int S = (K + BK - 1) / BK, s0 = (int)((int64_t)xcd * S / 8);
     const int wm = wave % 2 * (16 * TM), wn = wave / 2 * (16 * TN);
 
@@ -727,7 +733,6 @@ __global__ __launch_bounds__(512, TM == 8 ? 2 : 4) void k_linear_wide(typename O
     };
 
     Place p;
-    int k = blockIdx.x / 8;
     if (k >= here) return;
     place(p, from + k);
     issue(p, 0, all);
@@ -768,7 +773,7 @@ __global__ __launch_bounds__(512, TM == 8 ? 2 : 4) void k_linear_wide(typename O
         }
         wait();
         const int m0 = p.m0, n0 = p.n0;
-        k += gridDim.x / 8;
+        k += step;
         if (k < here) {
             place(p, from + k);
             issue(p, 0, all);
