@@ -161,6 +161,14 @@ def test_blocks_per_cu(hs, M, K, N, G):
     one(hs, M + K, G, M, K, N, "bf16", ACTS[(M + K) % 6], "f32")
 
 
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype,out", [("bf16", "same"), ("bf16", "f32"), ("f16", "same"), ("f16", "f32")])
+@pytest.mark.parametrize("M,K,N,G", [(100, 80, 34_002, None), (384, 400, 16_500, None), (128, 1040, 9000, 5)])
+def test_one_and_a_half_to_two_tiles_a_cu(hs, M, K, N, G, act, dtype, out):
+    """Tiles of 128 x 128, two of them to a CU."""
+    one(hs, M + K, G, M, K, N, dtype, act, out)
+
+
 @pytest.mark.parametrize("M,K,N", [(1, 4096, 96), (7, 130, 50), (64, 513, 257), (130, 528, 300), (300, 1024, 520)])
 @pytest.mark.parametrize("pad,offset", [(1, 0), (0, 1), (3, 5), (16, 0), (16, 16), (8, 8)])
 def test_strides_and_alignment(hs, M, K, N, pad, offset):

@@ -166,6 +166,13 @@ def test_pieces_of_the_vocabulary(hs, M, K, V):
         one(hs, M + 1, M, K, V, "float16", 0.0, out_f32=False)
 
 
+@pytest.mark.parametrize("M,K,V", [(100, 72, 34_000), (128, 200, 50_257), (384, 64, 16_500), (500, 128, 15_000), (70, 320, 66_001)])
+@pytest.mark.parametrize("dtype,cap", [("bfloat16", 0.0), ("bfloat16", 30.0), ("float16", 0.0), ("float16", 30.0)])
+def test_one_and_a_half_to_two_tiles_a_cu(hs, M, K, V, dtype, cap):
+    """Tiles of 128 x 128, two of them to a CU, edges of rows and of the vocabulary."""
+    one(hs, M + K, M, K, V, dtype, cap)
+
+
 def test_many_rows(hs):
     one(hs, 3, 9000, 72, 17_000, "bfloat16", 0.0)
 

@@ -156,10 +156,10 @@ struct LossRows : RowsOfK<LossArgs, uint16_t> {
         }
         join_columns<BM, WN, 64 * WM * WN>(a, m0, n0 / BN, parts);
     }
-    // Of two by 16 / TN waves, sixteen rows at a time.
+    // Of two by four waves, sixteen rows at a time.
     template <int ACT, int TN, int TM>
     static __device__ __forceinline__ void wide_statistics(const Args& a, int m0, int n0, const Sum (&acc)[TN][TM], uint16_t* lds) {
-        constexpr int BM = 32 * TM, BN = 256, WN = 16 / TN;
+        constexpr int BM = 32 * TM, BN = 64 * TN, WN = 4;
         const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
         float2* parts = reinterpret_cast<float2*>(lds);
 #pragma unroll 1

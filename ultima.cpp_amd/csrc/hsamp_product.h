@@ -805,12 +805,13 @@ struct Form {
 constexpr Form kForms[] = {
     {16, 16, 2, {8, 12}}, {32, 32, 2, {13, 25}}, {64, 16, 1, {14.5f, 0}}, {64, 32, 1, {15.5f, 0}}, {64, 64, 2, {32, 39}},
     {64, 64, 1, {24, 0}}, {128, 128, 1, {44, 0}}, {160, 128, 2, {62, 84}}, {256, 256, 1, {112, 0}},
+    {128, 128, 2, {50, 75}},
 };
 // The same in 8 bits (K = 4096, half the bytes): 64 x 16 rows 64: 8.5 us; 64 x 32 rows 128:
 // 8.4; 64 x 64 rows 256: 24.7, rows 512: 26.9, by 16 waves rows 256: 11.0, rows 512: 20.9;
 // 128 x 128 rows 512: 18.8, 1024: 22.4; 160 x 128 rows 320 of 16384: 28.4, 2048: 41.8;
-// 256 x 256 rows 2048 of 8192: 61.6.
-constexpr float kBytes[][2] = {{6, 8}, {7, 13.5f}, {8.5f, 0}, {8.4f, 0}, {24.7f, 27}, {11, 0}, {21, 0}, {28, 42}, {60, 0}};
+// 256 x 256 rows 2048 of 8192: 61.6; 128 x 128 going from tile to tile rows 256: 26.8, 512: 39.9.
+constexpr float kBytes[][2] = {{6, 8}, {7, 13.5f}, {8.5f, 0}, {8.4f, 0}, {24.7f, 27}, {11, 0}, {21, 0}, {28, 42}, {60, 0}, {25, 39}};
 
 // Blocks of one group.
 template <class Args>
@@ -819,14 +820,18 @@ int64_t blocks_of(const Form& f, const Args& a) {
 }
 
 // Up to 32 rows: the narrowest form that holds them (bound by W's stream at any
-// width). More: the form whose rounds over the 256 CUs cost least.
+// width). More: the form whose rounds over the 256 CUs cost least. The last one (128 x 128 by
+// k_linear_wide) takes calls of one and a half to two rounds of the same tile by k_linear_tile:
+// the loss of 384 rows of 4096 x 16384 59 for 69 us, 512 69 for 79, 100 rows of 256 x 150000
+// 31 for 39, 8-bit 100 rows of 4096 x 50257 36 for 41; not linear, which keeps its forms and bits.
 template <class Args>
 int choose(const Args& a) {
     constexpr bool bytes = std::is_same_v<decltype(a.x), const int8_t*>;
+    constexpr int forms = (int)(sizeof(kForms) / sizeof(kForms[0])) - std::is_same_v<Args, ultima_hsamp_linear_args>;
     if (a.rows <= 32) return a.rows <= 16 ? 0 : 1;
     int best = 0;
     float least = 0;
-    for (int f = 2; f < (int)(sizeof(kForms) / sizeof(kForms[0])); ++f) {
+    for (int f = 2; f < forms; ++f) {
         const Form& v = kForms[f];
         const int64_t blocks = blocks_of(v, a) * a.groups;
         const int64_t round = 256 * v.blocks, rest = blocks % round;
@@ -896,7 +901,10 @@ hipError_t launch_product(const typename Op::Args& a, hipStream_t s) {
         case 5: return launch_tile<Op, false, 2, 2, 4, 2, 2, 4>(a, s);
         case 6: return launch_tile<Op, false, 2, 4, 1, 4, 2, 4>(a, s);
         case 7: return launch_tile<Op, false, 2, 4, 1, 5, 2, 2>(a, s);
-        default: return launch_wide<Op>(a, s);
+        case 8: return launch_wide<Op>(a, s);
+        default:
+            if constexpr (Op::kBand > 0) return launch_wide<Op, 4, 2>(a, s);      // (choose: linear never)
+            else return hipErrorInvalidValue;
     }
 }
 
