@@ -11,7 +11,7 @@
 // products (4096 rows 3.73 ms; the gradients 12.0, of a piece of 16384 ids the logits with
 // their dz 425 us, d_x 400, d_weight 432), few rows of small matrices by what goes to memory
 // between the launches (301 of 1002 x 50257, odd addresses: weight laid out 38, dz
-// 61, d_x 71 and 11, d_weight 73).
+// 61, d_x 52 and 6, d_weight 73).
 #include "hsamp_product.h"
 
 namespace hsamp {
